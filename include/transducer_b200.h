@@ -310,6 +310,79 @@ int tb200_peer_close(void* slots);
 int tb200_loss_sum_exchange(const float* lossSum, void* const* peerSlots, int rank, int world,
                             unsigned seq, float* total, unsigned timeoutUs);
 
+/* ---- operators on single lattice nodes -------------------------------------
+ * The reference works on whole lattices only: what follows has no counterpart there.
+ *
+ * Node n < N of utterance b is frame frames[b,n] and label position positions[b,n] (int, [B, N]);
+ * an index outside [0, maxT) resp. [0, maxU) (-1, say) means that there is no node, and nothing is
+ * read for it.  Nodes may come in any order and more than once.  The scores of a node are
+ * z[v] = E[b, frame, v] + P[b, position, v], one addition in fp32; words are masked by -inf or by any
+ * low number, and +inf and NaN are no scores (they make the results of their node NaN, or no word,
+ * and leave the other nodes alone).
+ * bf16 = 1: emissions, predictions and their gradients are bfloat16 instead of float.  Any alphabet
+ * size and alignment is taken; rows that are 16-byte aligned and whole multiples of 16 bytes are
+ * faster.  eStrideB, eStrideT, pStrideB, pStrideU: distances, in elements and not negative, between
+ * utterances and between frames resp. positions; words lie next to each other.  batchSize * nodes
+ * must be below 2^31 - 1, other sizes are limited by memory. */
+
+/* The k best words of every node (1 <= k <= 256, k <= V), the greater score first and of equal ones
+ * the lower word first: words int [B, N, k], logits [B, N, k] = z / temperature.  rest [B, N] (may be
+ * NULL): log sum of exp(z / temperature) over all other words, -inf if there are none.  Where there
+ * is no node: words -1, logits and rest -inf. */
+int tb200_top_words(const void* emissions, const void* predictions, int bf16, long long eStrideB,
+                    long long eStrideT, long long pStrideB, long long pStrideU, const int* frames,
+                    const int* positions, int* words, float* logits, float* rest, int batchSize,
+                    int maxInputLength, int maxLabelLength, int alphabetSize, int nodes, int k,
+                    double temperature);
+
+/* A word of every node, drawn with the given numbers, uniforms [B, N] in [0, 1).  In this order:
+ * w_v = exp((z_v - max z) / temperature); only the topK best words stay (0: all; the order of
+ * tb200_top_words); of them only the shortest prefix with at least the share topP of their weight
+ * (0 < topP <= 1; 1: all); of them only those with w_v >= minP (0 <= minP <= 1).  The word is the
+ * first, in the order of the alphabet, up to which (included) the weights that stay add up to more
+ * than uniforms[b,n] of their sum; logProbs [B, N] is the logarithm of its share of that sum.
+ * temperature = 0: the best word, logProbs 0.  Which word is taken is decided as in 64-bit
+ * arithmetic.  Where there is no node: word -1, logProbs 0; where every word is masked: -1, -inf;
+ * where a score is NaN or +inf: -1, NaN.  A number outside [0, 1) is taken as the nearest in it
+ * (NaN: as the greatest). */
+int tb200_sample_words(const void* emissions, const void* predictions, int bf16, long long eStrideB,
+                       long long eStrideT, long long pStrideB, long long pStrideU, const int* frames,
+                       const int* positions, const float* uniforms, int* words, float* logProbs,
+                       int batchSize, int maxInputLength, int maxLabelLength, int alphabetSize,
+                       int nodes, double temperature, int topK, double topP, double minP);
+
+/* Distillation from a teacher's recorded best words.  words int [B, N, K] (1 <= K <= 256; a word
+ * outside [0, V) is ignored, equal words of a node add up) and logits [B, N, K] as from
+ * tb200_top_words on the teacher's scores at the same temperature; rest [B, N], or NULL.  The
+ * teacher's distribution is softmax over logits[b,n,:] and, where given, rest[b,n], the weight of all
+ * words that are not listed.  costs [B, N] = its Kullback-Leibler divergence to the student's
+ * softmax(z / temperature), whose words that are not listed are one outcome if rest is given.  0
+ * where there is no node or the record has no weight; +inf where the student masks a word that the
+ * teacher does not (the gradient is then its limit).
+ * saved: what the backward call needs, tb200_distill_saved_bytes(), or NULL if none follows.  With
+ * rest the alphabet is limited to 2^20 words.
+ * The backward call writes egrads [B, maxT, V] and pgrads [B, maxU, V] whole and contiguous (either
+ * may be NULL): the gradients of sum weights[b,n] costs[b,n].  They are added up in the nodes' order,
+ * in fp32, and rounded once: the bits are the same from run to run. */
+size_t tb200_distill_saved_bytes(int batchSize, int nodes, int K);
+int tb200_distill_forward(const void* emissions, const void* predictions, int bf16,
+                          long long eStrideB, long long eStrideT, long long pStrideB,
+                          long long pStrideU, const int* frames, const int* positions,
+                          const int* words, const float* logits, const float* rest, float* costs,
+                          void* saved, size_t savedBytes, int batchSize, int maxInputLength,
+                          int maxLabelLength, int alphabetSize, int nodes, int K,
+                          double temperature);
+size_t tb200_distill_backward_workspace_bytes(int batchSize, int maxInputLength,
+                                              int maxLabelLength);
+int tb200_distill_backward(const void* emissions, const void* predictions, int bf16,
+                           long long eStrideB, long long eStrideT, long long pStrideB,
+                           long long pStrideU, const int* frames, const int* positions,
+                           const int* words, const void* saved, size_t savedBytes,
+                           const float* weights, void* egrads, void* pgrads, int batchSize,
+                           int maxInputLength, int maxLabelLength, int alphabetSize, int nodes,
+                           int K, int hasRest, double temperature, void* workspace,
+                           size_t workspaceBytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,10 +7,12 @@
 // ValueError (invalid argument) or RuntimeError (CUDA), as pybind11 maps the
 // reference's std::invalid_argument / std::runtime_error.
 #include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
 
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 
 #include "../../include/transducer.h"
 #include "../../include/transducer_b200.h"
@@ -181,6 +183,60 @@ PYBIND11_MODULE(_transducer, m) {
         "emissions"_a, "predictions"_a, "input_lengths"_a, "label_lengths"_a, "labels"_a,
         "batch_size"_a, "max_input_length"_a, "max_label_length"_a, "alphabet_size"_a,
         "blank"_a, "workspace"_a, "workspace_bytes"_a);
+
+  // ---- operators on single lattice nodes ---------------------------------------------
+  // `scores`: (emissions, predictions, bf16, their strides by utterance and by frame resp. position)
+  using Scores = std::tuple<addr, addr, bool, long long, long long, long long, long long>;
+  using Sizes = std::tuple<int, int, int, int, int>;   // B, T, U, V, N
+  m.def("top_words",
+        [](const Scores& s, addr frames, addr positions, addr words, addr logits, addr rest, const Sizes& n, int k,
+           double temperature) {
+          check(tb200_top_words(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)), std::get<2>(s),
+                                std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s),
+                                at<const int>(frames), at<const int>(positions), at<int>(words), at<float>(logits),
+                                at<float>(rest), std::get<0>(n), std::get<1>(n), std::get<2>(n), std::get<3>(n),
+                                std::get<4>(n), k, temperature));
+        },
+        "scores"_a, "frames"_a, "positions"_a, "words"_a, "logits"_a, "rest"_a, "sizes"_a, "k"_a, "temperature"_a);
+  m.def("sample_words",
+        [](const Scores& s, addr frames, addr positions, addr uniforms, addr words, addr log_probs, const Sizes& n,
+           double temperature, int top_k, double top_p, double min_p) {
+          check(tb200_sample_words(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)), std::get<2>(s),
+                                   std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s),
+                                   at<const int>(frames), at<const int>(positions), at<const float>(uniforms),
+                                   at<int>(words), at<float>(log_probs), std::get<0>(n), std::get<1>(n),
+                                   std::get<2>(n), std::get<3>(n), std::get<4>(n), temperature, top_k, top_p, min_p));
+        },
+        "scores"_a, "frames"_a, "positions"_a, "uniforms"_a, "words"_a, "log_probs"_a, "sizes"_a, "temperature"_a,
+        "top_k"_a, "top_p"_a, "min_p"_a);
+  m.def("distill_saved_bytes", &tb200_distill_saved_bytes);
+  m.def("distill_backward_workspace_bytes", &tb200_distill_backward_workspace_bytes);
+  m.def("distill_forward",
+        [](const Scores& s, addr frames, addr positions, addr words, addr logits, addr rest, addr costs, addr saved,
+           size_t saved_bytes, const Sizes& n, int k, double temperature) {
+          check(tb200_distill_forward(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)), std::get<2>(s),
+                                      std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s),
+                                      at<const int>(frames), at<const int>(positions), at<const int>(words),
+                                      at<const float>(logits), at<const float>(rest), at<float>(costs),
+                                      at<void>(saved), saved_bytes, std::get<0>(n), std::get<1>(n), std::get<2>(n),
+                                      std::get<3>(n), std::get<4>(n), k, temperature));
+        },
+        "scores"_a, "frames"_a, "positions"_a, "words"_a, "logits"_a, "rest"_a, "costs"_a, "saved"_a,
+        "saved_bytes"_a, "sizes"_a, "k"_a, "temperature"_a);
+  m.def("distill_backward",
+        [](const Scores& s, addr frames, addr positions, addr words, addr saved, size_t saved_bytes, addr weights,
+           addr egrads, addr pgrads, const Sizes& n, int k, bool has_rest, double temperature, addr ws,
+           size_t ws_bytes) {
+          check(tb200_distill_backward(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)),
+                                       std::get<2>(s), std::get<3>(s), std::get<4>(s), std::get<5>(s),
+                                       std::get<6>(s), at<const int>(frames), at<const int>(positions),
+                                       at<const int>(words), at<const void>(saved), saved_bytes,
+                                       at<const float>(weights), at<void>(egrads), at<void>(pgrads),
+                                       std::get<0>(n), std::get<1>(n), std::get<2>(n), std::get<3>(n),
+                                       std::get<4>(n), k, has_rest, temperature, at<void>(ws), ws_bytes));
+        },
+        "scores"_a, "frames"_a, "positions"_a, "words"_a, "saved"_a, "saved_bytes"_a, "weights"_a, "egrads"_a,
+        "pgrads"_a, "sizes"_a, "k"_a, "has_rest"_a, "temperature"_a, "workspace"_a, "workspace_bytes"_a);
 
   // ---- device status (bounded waits that ran out) -----------------------------------
   // Returns the code of tb200_check_status (0, or 5 = a kernel gave up) without throwing, so the

@@ -250,4 +250,50 @@ void launch_pgrad_simt(const float* E, const float* rowRef, const float* W, int 
                        const int* inLens, const int* labLens, Dims d,
                        cudaStream_t stream);
 
+// ---- node_words.cu, node_distill.cu ------------------------------------------
+// Operators on single lattice nodes: node n of utterance b is frame frames[b,n] and label position
+// positions[b,n] (int [B,N]); an index outside [0, T) x [0, U) means that there is no node.  Rows of E
+// and P have words next to each other; the other strides are in elements.
+struct NodeArgs {
+  const void *E, *P;
+  i64 eStrideB, eStrideT, pStrideB, pStrideU;
+  const int *frames, *positions;
+  int B, T, U, V, N;
+  int dtype = kDtypeF32;
+};
+
+constexpr int kMaxListedWords = 256;   // longest list of words per node
+// Largest vocabulary of a distillation with the rest's weight: a bit per word in shared memory.
+constexpr int kDistillMaxBits = 1 << 20;
+
+// Whether every row can be moved in 16-byte vectors.
+bool node_rows_aligned(const NodeArgs& a);
+
+// words/logits [B,N,k], rest [B,N]: see tb200_top_words.
+void launch_top_words(const NodeArgs& a, int* words, float* logits, float* rest, int k, double temperature,
+                      cudaStream_t stream);
+// words, logProbs [B,N]: see tb200_sample_words.
+struct SampleRule {
+  double temperature;
+  int topK;      // 0: all words
+  double topP;   // 1: all words
+  double minP;   // 0: all words
+};
+void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, float* logProbs,
+                         SampleRule rule, cudaStream_t stream);
+
+// What the forward call leaves for the backward call, per node and per listed word.
+struct DistillSaved {
+  float4* node;   // [B*N] m, L, A, sign: the gradient of a listed word is 2^((z-m) log2e/temperature - L) - q,
+                  // of the others sign * 2^((z-m) log2e/temperature - A)
+  float* q;       // [B*N*K] the teacher's share of a listed word; -1: to be ignored
+};
+void launch_distill_forward(const NodeArgs& a, const int* words, const float* logits, const float* rest,
+                            float* costs, DistillSaved saved, int K, double temperature,
+                            cudaStream_t stream);
+// spans: 2 (B*T + B*U) ints.  egrads [B,T,V], pgrads [B,U,V] of the inputs' type, written whole.
+void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved saved, const float* weights,
+                             void* egrads, void* pgrads, int K, bool hasRest, double temperature, int* spans,
+                             cudaStream_t stream);
+
 }  // namespace tb200

@@ -1,0 +1,144 @@
+// C ABI of the operators on single lattice nodes (include/transducer_b200.h, last part).
+#include <cmath>
+#include <string>
+
+#include "../../include/transducer_b200.h"
+#include "api_internal.h"
+#include "kernels.h"
+
+namespace tb200 {
+namespace {
+
+template <typename F>
+int guarded(F&& body) {
+  try {
+    body();
+    return kOk;
+  } catch (const CudaError& e) {
+    return api_fail(kErrCuda, e.what());
+  } catch (const std::invalid_argument& e) {
+    return api_fail(kErrInvalidArgument, e.what());
+  } catch (const std::exception& e) {
+    return api_fail(kErrCuda, e.what());
+  }
+}
+
+void check(bool ok, const char* what) {
+  if (!ok) throw std::invalid_argument(what);
+}
+
+NodeArgs node_args(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
+                   long long pStrideB, long long pStrideU, const int* frames, const int* positions, int B,
+                   int maxT, int maxU, int V, int N) {
+  check(B >= 0 && maxT >= 0 && maxU >= 0 && N >= 0 && V > 0,
+        "negative batch/length/number of nodes or non-positive alphabet size");
+  check(eStrideB >= 0 && eStrideT >= 0 && pStrideB >= 0 && pStrideU >= 0, "negative stride");
+  check((long long)B * N < 0x7fffffffLL, "too many nodes (batchSize * nodes must be below 2^31 - 1)");
+  return NodeArgs{E, P, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT, maxU, V, N,
+                  bf16 ? kDtypeBf16 : kDtypeF32};
+}
+
+void check_listed(int K) {
+  check(K >= 1 && K <= kMaxListedWords, "the number of listed words must be between 1 and 256");
+}
+void check_temperature(double t) {
+  check(t > 0.0 && std::isfinite(1.0f / (float)t) && (float)t > 0.0f, "temperature must be positive");
+}
+
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+DistillSaved distill_saved(void* p, int B, int N) {
+  DistillSaved s;
+  s.node = static_cast<float4*>(p);
+  s.q = p ? reinterpret_cast<float*>(static_cast<char*>(p) + round256(sizeof(float4) * (size_t)B * N)) : nullptr;
+  return s;
+}
+
+void need(size_t have, size_t want, const void* p, const char* what) {
+  if (want > 0 && (p == nullptr || have < want))
+    throw std::invalid_argument(std::string(what) + " too small: need " + std::to_string(want) + " bytes, got " +
+                                std::to_string(have));
+}
+
+}  // namespace
+}  // namespace tb200
+
+using namespace tb200;
+
+extern "C" {
+
+int tb200_top_words(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
+                    long long pStrideB, long long pStrideU, const int* frames, const int* positions, int* words,
+                    float* logits, float* rest, int B, int maxT, int maxU, int V, int N, int k,
+                    double temperature) {
+  return guarded([&] {
+    const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
+                                 maxU, V, N);
+    check_listed(k);
+    check(k <= V, "the number of listed words must not exceed the alphabet size");
+    check_temperature(temperature);
+    launch_top_words(a, words, logits, rest, k, temperature, api_stream());
+  });
+}
+
+int tb200_sample_words(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
+                       long long pStrideB, long long pStrideU, const int* frames, const int* positions,
+                       const float* uniforms, int* words, float* logProbs, int B, int maxT, int maxU, int V, int N,
+                       double temperature, int topK, double topP, double minP) {
+  return guarded([&] {
+    const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
+                                 maxU, V, N);
+    if (!(temperature == 0.0)) check_temperature(temperature);
+    check(topK >= 0, "top_k must not be negative");
+    check(topP > 0.0 && topP <= 1.0, "top_p must be above 0 and at most 1");
+    check(minP >= 0.0 && minP <= 1.0, "min_p must be between 0 and 1");
+    launch_sample_words(a, uniforms, words, logProbs, SampleRule{temperature, topK, topP, minP}, api_stream());
+  });
+}
+
+size_t tb200_distill_saved_bytes(int B, int N, int K) {
+  if (B <= 0 || N <= 0 || K <= 0) return 0;
+  const size_t nodes = (size_t)B * N;
+  return round256(sizeof(float4) * nodes) + round256(sizeof(float) * nodes * K);
+}
+
+int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
+                          long long pStrideB, long long pStrideU, const int* frames, const int* positions,
+                          const int* words, const float* logits, const float* rest, float* costs, void* saved,
+                          size_t savedBytes, int B, int maxT, int maxU, int V, int N, int K,
+                          double temperature) {
+  return guarded([&] {
+    const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
+                                 maxU, V, N);
+    check_listed(K);
+    check_temperature(temperature);
+    check(!rest || V <= kDistillMaxBits, "the alphabet must not exceed 2^20 words where the rest's weight is given");
+    if (saved) need(savedBytes, tb200_distill_saved_bytes(B, N, K), saved, "saved state");
+    launch_distill_forward(a, words, logits, rest, costs, distill_saved(saved, B, N), K, temperature,
+                           api_stream());
+  });
+}
+
+size_t tb200_distill_backward_workspace_bytes(int B, int maxT, int maxU) {
+  if (B <= 0 || maxT < 0 || maxU < 0) return 0;
+  return round256(2 * sizeof(int) * (size_t)B * ((size_t)maxT + maxU));
+}
+
+int tb200_distill_backward(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
+                           long long pStrideB, long long pStrideU, const int* frames, const int* positions,
+                           const int* words, const void* saved, size_t savedBytes, const float* weights,
+                           void* egrads, void* pgrads, int B, int maxT, int maxU, int V, int N, int K,
+                           int hasRest, double temperature, void* workspace, size_t workspaceBytes) {
+  return guarded([&] {
+    const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
+                                 maxU, V, N);
+    check_listed(K);
+    check_temperature(temperature);
+    need(savedBytes, tb200_distill_saved_bytes(B, N, K), saved, "saved state");
+    need(workspaceBytes, tb200_distill_backward_workspace_bytes(B, maxT, maxU), workspace, "workspace");
+    launch_distill_backward(a, words, distill_saved(const_cast<void*>(saved), B, N), weights, egrads, pgrads, K,
+                            hasRest != 0, temperature, static_cast<int*>(workspace), api_stream());
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,127 @@
+// Rows of scores at single lattice nodes, shared by the node kernels (node_words.cu,
+// node_distill.cu).  Node n of utterance b is frame frames[b,n] and label position
+// positions[b,n]; its scores are E[b,frame,v] + P[b,position,v], one addition in fp32.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace tb200 {
+
+// Words of a row held by a group of G threads: thread `tid` has the vectors tid, tid + G, ... of VEC
+// words each.  VEC words are 16 bytes where every row starts on a 16-byte boundary, else 1.
+template <typename TIn>
+constexpr int kVecWords = 16 / (int)sizeof(TIn);
+
+template <int VEC>
+struct Words {
+  float x[VEC];
+};
+template <int VEC>
+__device__ __forceinline__ Words<VEC> load_words(const float* p) {
+  Words<VEC> w;
+  if constexpr (VEC == 4) {
+    const float4 r = *reinterpret_cast<const float4*>(p);
+    w.x[0] = r.x, w.x[1] = r.y, w.x[2] = r.z, w.x[3] = r.w;
+  } else {
+    w.x[0] = *p;
+  }
+  return w;
+}
+template <int VEC>
+__device__ __forceinline__ Words<VEC> load_words(const bf16* p) {
+  Words<VEC> w;
+  if constexpr (VEC == 8) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    const unsigned u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w.x[2 * i] = __uint_as_float(u[i] << 16);
+      w.x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  } else {
+    w.x[0] = to_f32(*p);
+  }
+  return w;
+}
+template <int VEC>
+__device__ __forceinline__ void store_words(float* p, const float* x) {
+  if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  else *p = x[0];
+}
+template <int VEC>
+__device__ __forceinline__ void store_words(bf16* p, const float* x) {
+  if constexpr (VEC == 8) {
+    unsigned u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+    from_f32(*p, x[0]);
+  }
+}
+
+// The scores of one node.
+template <typename TIn>
+struct NodeScores {
+  const TIn *e, *p;
+  bool here;
+};
+template <typename TIn>
+__device__ __forceinline__ NodeScores<TIn> node_scores(const NodeArgs& a, i64 node) {
+  const i64 b = node / a.N;
+  const int t = a.frames[node], u = a.positions[node];
+  NodeScores<TIn> s;
+  s.here = (unsigned)t < (unsigned)a.T && (unsigned)u < (unsigned)a.U;
+  s.e = static_cast<const TIn*>(a.E) + b * a.eStrideB + (s.here ? t : 0) * a.eStrideT;
+  s.p = static_cast<const TIn*>(a.P) + b * a.pStrideB + (s.here ? u : 0) * a.pStrideU;
+  return s;
+}
+
+// Sums and maxima over a group of G threads (a warp, or the CTA): every thread gets the result, and
+// its bits do not depend on anything but the values.  `scratch`: two sets of 32 places in shared
+// memory, used in turn, so that one barrier per reduction is enough.
+template <int G>
+struct Group {
+  int tid;
+  double* scratch;   // [2][32], of the CTA; unused by a warp
+  int turn = 0;
+  __device__ __forceinline__ Group(int tid_, double* scratch_) : tid(tid_), scratch(scratch_) {}
+
+  __device__ __forceinline__ void sync() const {
+    if constexpr (G == 32) __syncwarp();
+    else __syncthreads();
+  }
+  template <typename T, typename Op>
+  __device__ __forceinline__ T reduce(T v, Op op) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (G > 32) {
+      T* s = reinterpret_cast<T*>(scratch + 32 * turn);
+      turn ^= 1;
+      if ((tid & 31) == 0) s[tid >> 5] = v;
+      __syncthreads();
+      v = s[0];
+#pragma unroll
+      for (int w = 1; w < G / 32; ++w) v = op(v, s[w]);
+    }
+    return v;
+  }
+  template <typename T>
+  __device__ __forceinline__ T sum(T v) { return reduce(v, [](T a, T b) { return a + b; }); }
+  template <typename T>
+  __device__ __forceinline__ T max(T v) { return reduce(v, [](T a, T b) { return a < b ? b : a; }); }
+};
+
+// Order-preserving integer of a score: NaN above everything, -0 as +0; 0 is below every score.
+__device__ __forceinline__ unsigned score_key(float z) {
+  if (z != z) return 0xffffffffu;
+  const unsigned u = __float_as_uint(z + 0.0f);
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_score(unsigned k) {
+  return __uint_as_float(k ^ ((unsigned)((int)~k >> 31) | 0x80000000u));
+}
+
+}  // namespace tb200
