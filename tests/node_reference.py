@@ -52,10 +52,9 @@ def sample_words(z, here, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
         stays &= ws >= min_p
         w = torch.zeros_like(w).scatter(-1, at, ws * stays)
         upto = w.cumsum(-1)
-        u = uniforms.cpu().double().nan_to_num(nan=1.0).clamp(0.0, 1.0)[..., None]
-        words = (upto <= u * upto[..., -1:]).sum(-1)
-        last = V - 1 - (w.flip(-1) > 0).int().argmax(-1)
-        words = torch.minimum(words, last)
+        # (outside [0, 1): the nearest 32-bit number in it)
+        u = uniforms.cpu().double().nan_to_num(nan=1.0).clamp(0.0, 1.0 - 2.0 ** -24)[..., None]
+        words = (upto <= u * upto[..., -1:]).sum(-1).clamp(max=V - 1)
         log_probs = (w.gather(-1, words[..., None]) / upto[..., -1:]).log()[..., 0]
     words = words.int()
     masked = m[..., 0] == -torch.inf

@@ -250,7 +250,7 @@ void launch_pgrad_simt(const float* E, const float* rowRef, const float* W, int 
                        const int* inLens, const int* labLens, Dims d,
                        cudaStream_t stream);
 
-// ---- node_words.cu, node_distill.cu ------------------------------------------
+// ---- node_top.cu, node_sample.cu, node_distill.cu ------------------------------------------
 // Operators on single lattice nodes: node n of utterance b is frame frames[b,n] and label position
 // positions[b,n] (int [B,N]); an index outside [0, T) x [0, U) means that there is no node.  Rows of E
 // and P have words next to each other; the other strides are in elements.

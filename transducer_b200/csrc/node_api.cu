@@ -42,7 +42,8 @@ void check_listed(int K) {
   check(K >= 1 && K <= kMaxListedWords, "the number of listed words must be between 1 and 256");
 }
 void check_temperature(double t) {
-  check(t > 0.0 && std::isfinite(1.0f / (float)t) && (float)t > 0.0f, "temperature must be positive");
+  // (its reciprocal is used in 32 bits)
+  check(t > 0.0 && std::isfinite((float)(1.4426950408889634 / t)), "temperature must be positive");
 }
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }

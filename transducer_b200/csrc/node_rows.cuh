@@ -1,4 +1,4 @@
-// Rows of scores at single lattice nodes, shared by the node kernels (node_words.cu,
+// Rows of scores at single lattice nodes, shared by the node kernels (node_top.cu, node_sample.cu,
 // node_distill.cu).  Node n of utterance b is frame frames[b,n] and label position
 // positions[b,n]; its scores are E[b,frame,v] + P[b,position,v], one addition in fp32.
 #pragma once
@@ -8,11 +8,7 @@
 
 namespace tb200 {
 
-// Words of a row held by a group of G threads: thread `tid` has the vectors tid, tid + G, ... of VEC
-// words each.  VEC words are 16 bytes where every row starts on a 16-byte boundary, else 1.
-template <typename TIn>
-constexpr int kVecWords = 16 / (int)sizeof(TIn);
-
+// Words are moved VEC at a time: 16 bytes where every row starts on a 16-byte boundary, else one word.
 template <int VEC>
 struct Words {
   float x[VEC];
@@ -84,34 +80,60 @@ __device__ __forceinline__ NodeScores<TIn> node_scores(const NodeArgs& a, i64 no
 // memory, used in turn, so that one barrier per reduction is enough.
 template <int G>
 struct Group {
-  int tid;
+  static constexpr int kWarps = G / 32;
+  int tid, lane, warp;
   double* scratch;   // [2][32], of the CTA; unused by a warp
   int turn = 0;
-  __device__ __forceinline__ Group(int tid_, double* scratch_) : tid(tid_), scratch(scratch_) {}
+  __device__ __forceinline__ Group(int tid_, double* scratch_)
+      : tid(tid_), lane(tid_ & 31), warp(tid_ >> 5), scratch(scratch_) {}
 
   __device__ __forceinline__ void sync() const {
     if constexpr (G == 32) __syncwarp();
     else __syncthreads();
   }
+  // The warps' values v (the same in all lanes of a warp) in the order of the warps: lane i gets that
+  // of warp i % kWarps.
+  template <typename T>
+  __device__ __forceinline__ T exchange(T v) {
+    if constexpr (G > 32) {
+      T* s = reinterpret_cast<T*>(scratch + 32 * turn);
+      turn ^= 1;
+      if (lane == 0) s[warp] = v;
+      __syncthreads();
+      v = s[lane % kWarps];
+    }
+    return v;
+  }
   template <typename T, typename Op>
   __device__ __forceinline__ T reduce(T v, Op op) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return across(v, op);
+  }
+  __device__ __forceinline__ float sum(float v) { return reduce(v, [](float a, float b) { return a + b; }); }
+  __device__ __forceinline__ double sum(double v) { return reduce(v, [](double a, double b) { return a + b; }); }
+  __device__ __forceinline__ int sum(int v) {
+    return across(__reduce_add_sync(0xffffffffu, v), [](int a, int b) { return a + b; });
+  }
+  __device__ __forceinline__ float max(float v) { return reduce(v, [](float a, float b) { return fmaxf(a, b); }); }
+  __device__ __forceinline__ int max(int v) {
+    return across(__reduce_max_sync(0xffffffffu, v), [](int a, int b) { return a < b ? b : a; });
+  }
+  __device__ __forceinline__ unsigned max(unsigned v) {
+    return across(__reduce_max_sync(0xffffffffu, v), [](unsigned a, unsigned b) { return a < b ? b : a; });
+  }
+  __device__ __forceinline__ unsigned min(unsigned v) { return ~max(~v); }
+
+ private:
+  template <typename T, typename Op>
+  __device__ __forceinline__ T across(T v, Op op) {
     if constexpr (G > 32) {
-      T* s = reinterpret_cast<T*>(scratch + 32 * turn);
-      turn ^= 1;
-      if ((tid & 31) == 0) s[tid >> 5] = v;
-      __syncthreads();
-      v = s[0];
+      v = exchange(v);
 #pragma unroll
-      for (int w = 1; w < G / 32; ++w) v = op(v, s[w]);
+      for (int o = kWarps / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
     }
     return v;
   }
-  template <typename T>
-  __device__ __forceinline__ T sum(T v) { return reduce(v, [](T a, T b) { return a + b; }); }
-  template <typename T>
-  __device__ __forceinline__ T max(T v) { return reduce(v, [](T a, T b) { return a < b ? b : a; }); }
 };
 
 // Order-preserving integer of a score: NaN above everything, -0 as +0; 0 is below every score.

@@ -1,0 +1,602 @@
+// A word drawn from a lattice node's distribution.
+//
+// Weights are 2^x in 32 bits, x = (z - m) log2(e) / temperature.  They decide where they are sure to:
+// the difference from the maximum m is rounded, the factor is, their product is (2^-24 of x each), and
+// ex2 is good to 2^-22, so that a weight is off by at most 2^-24 * 2.1 |x| + 2^-22 of itself, and any sum
+// of weights by 2^-24 * 2.1 sum w |x| + 2^-22 sum w, both sums over the row; with ten roundings of the
+// sum itself (a thread's part is added up in 32 bits, parts are in 64) that is `unsure` below.  Where a
+// comparison is closer than that the sums are formed anew from memory with exponentials in 64 bits.
+#include <algorithm>
+#include <cfloat>
+
+#include "node_select.cuh"
+#include "profile.h"
+
+namespace tb200 {
+namespace {
+
+// exp((z - m) scale) in 64 bits.
+struct ExactWeight {
+  float m;
+  double scale;
+  __device__ __forceinline__ double operator()(float z) const { return exp(((double)z - (double)m) * scale); }
+};
+
+// The first words of the order, among those that `all` keeps, that have the share topP of their weight.
+template <typename TIn, int VEC, int G>
+__device__ __noinline__ Cut general_share(NodeScores<TIn> s, int V, Group<G> g, Cut all, ExactWeight weight,
+                                          double topP) {
+  auto mass = [&](auto pick) {
+    double c = 0.0;
+    each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) {
+      const unsigned u = score_key(z);
+      if (all.keeps(u, v) && pick(u)) c += weight(z);
+    });
+    return g.sum(c);
+  };
+  const double share = topP * mass([](unsigned) { return true; });
+  Cut cut;
+  // the word that reaches the share: its key, then, among equal ones, its index
+  cut.key = max(all.key, largest_key([&](unsigned x) { return mass([&](unsigned u) { return u >= x; }) >= share; }));
+  const double above = mass([&](unsigned u) { return u > cut.key; }), one = weight(key_score(cut.key));
+  cut.last = smallest_index(V, [&](int y) {
+    int c = 0;
+    each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) {
+      c += score_key(z) == cut.key && v <= y && all.keeps(cut.key, v) ? 1 : 0;
+    });
+    c = g.sum(c);
+    return c > 0 && above + c * one >= share;
+  });
+  if (cut.key == all.key) cut.last = min(cut.last, all.last);
+  return cut;
+}
+
+constexpr double kUnsureSlope = 2.1 * 0x1p-24, kUnsureSum = 0x1p-22 + 10 * 0x1p-24;
+constexpr int kNear = 64;          // words about a cut that are listed
+constexpr float kAbove = 2.0f;     // above every weight
+constexpr int kResidentBytes = 220 * 1024;   // of shared memory for a row's weights, beside the lists
+
+struct Weight {
+  float m, c;
+  __device__ __forceinline__ float exponent(float z) const { return __fmul_rn(__fsub_rn(z, m), c); }
+  __device__ __forceinline__ float operator()(float z) const { return ex2(exponent(z)); }
+};
+
+// Which words stay: those of weight hi and above, and of those between lo and hi the ones before the cut;
+// in any case those of minP and above (`exact` decides where that is close).
+struct Keep {
+  float lo = FLT_MIN, hi = FLT_MIN;
+  Cut cut{0u, 0x7fffffff};
+  double minP = 0.0;
+  ExactWeight exact;
+  __device__ __forceinline__ bool operator()(float w, float z, int v) const {
+    if (w < lo || (w < hi && !cut.keeps(z, v))) return false;
+    if (w >= sure()) return true;
+    return w >= (float)minP * 0.9999f && exact(z) >= minP;
+  }
+  __device__ __forceinline__ float sure() const { return (float)minP * 1.0001f; }   // of minP, whatever the rounding
+};
+
+// Sums over the words that stay, in 64 bits from memory: of all of them, and of those of weight `from` and above.
+struct ExactSums {
+  double all, above;
+};
+template <typename TIn, int VEC, int G>
+__device__ __noinline__ ExactSums exact_sums(NodeScores<TIn> s, int V, Group<G> g, Keep keep, Weight weight,
+                                             float from) {
+  double all = 0.0, above = 0.0;
+  each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) {
+    const float w = weight(z);
+    if (!keep(w, z, v)) return;
+    const double x = keep.exact(z);
+    all += x;
+    if (w >= from) above += x;
+  });
+  return {g.sum(all), g.sum(above)};
+}
+
+// The word that `u` picks among those that stay, in 64 bits from memory.
+template <typename TIn, int VEC, int G>
+__device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group<G> g, Keep keep,
+                                        Weight weight, float u, int* word, float* logProb) {
+  const Place<TIn, VEC, G, 0> at(s, V, seg, g.warp, g.lane);
+  auto kept = [&](float z, int v) { return keep(weight(z), z, v) ? keep.exact(z) : 0.0; };
+  double part = 0.0;
+#pragma unroll 1
+  for (int v = at.word(0); v < at.end; v += 32 * VEC) {
+    float z[VEC];
+    at.load(v, z);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) part += kept(z[i], v + i);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  part = g.exchange(part);
+  double upto = part;
+#pragma unroll
+  for (int o = 1; o < Group<G>::kWarps; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (g.lane >= o) upto += x;
+  }
+  const double total = __shfl_sync(0xffffffffu, upto, Group<G>::kWarps - 1);
+  const double target = (double)u * total;
+  const unsigned past = __ballot_sync(0xffffffffu, upto > target && g.lane < Group<G>::kWarps);
+  // (the last warp with words that stay, should rounding let none pass)
+  const unsigned some = __ballot_sync(0xffffffffu, part > 0.0 && g.lane < Group<G>::kWarps);
+  const int pick = past ? __ffs(past) - 1 : 31 - __clz(some);
+  if (g.warp != pick) return;
+  double before = __shfl_sync(0xffffffffu, upto - part, pick), weightOf = 0.0;
+  int found = -1;   // the first word past the target, or (rounding) the last one that stays
+#pragma unroll 1
+  for (int j = 0; at.first + j * 32 * VEC < at.end; ++j) {
+    const int v = at.word(j);
+    float z[VEC];
+    double w[VEC], sum = 0.0;
+    if (v < at.end) at.load(v, z);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      w[i] = v < at.end ? kept(z[i], v + i) : 0.0;
+      sum += w[i];
+    }
+    double scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, scan, o);
+      if (g.lane >= o) scan += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, sum > 0.0 && before + scan > target);
+    const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
+    if (any) {
+      int word = -1;
+      double weightHere = 0.0, c = before + (scan - sum);
+      bool over = false;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        c += w[i];
+        if (w[i] > 0.0 && !over) word = v + i, weightHere = w[i], over = c > target;
+      }
+      const int owner = hit ? __ffs(hit) - 1 : 31 - __clz(any);
+      found = __shfl_sync(0xffffffffu, word, owner);
+      weightOf = __shfl_sync(0xffffffffu, weightHere, owner);
+    }
+    if (hit) break;
+    before += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  if (g.lane == 0) *word = found, *logProb = (float)log(weightOf / total);
+}
+
+// The row's weights lie in shared memory (RESIDENT; 227 KB hold 57,000 words), each thread goes through the
+// same ones in every pass; longer rows are read again instead.  In registers they were no faster to go
+// through and left room for a quarter of the threads.
+template <typename TIn, int VEC, int G, bool RESIDENT>
+__global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
+    NodeArgs a, const float* __restrict__ uniforms, int* __restrict__ words, float* __restrict__ logProbs,
+    SampleRule rule, int seg) {
+  constexpr int kRows = kCta<G> / G, kPass = RESIDENT ? 4 : VEC;   // words a thread takes at a time
+  extern __shared__ __align__(16) float weights[];
+  __shared__ double scratch[64];
+  __shared__ Entry listAll[kRows][kNear], sortedAll[kRows][kNear];
+  __shared__ int filledAll[kRows];
+  __shared__ int sureAll[kRows];
+  const int sub = threadIdx.x / G, tid = threadIdx.x % G;
+  const i64 node = (i64)blockIdx.x * kRows + sub;
+  if (node >= (i64)a.B * a.N) return;
+  Entry *list = listAll[sub], *sorted = sortedAll[sub];
+  int *filled = &filledAll[sub], *sure = &sureAll[sub];
+  auto answer = [&](int word, float logProb) {
+    if (tid == 0) words[node] = word, logProbs[node] = logProb;
+  };
+  const NodeScores<TIn> s = node_scores<TIn>(a, node);
+  if (!s.here) return answer(-1, 0.0f);
+  Group<G> g(tid, scratch);
+  const Place<TIn, VEC, G, 0> at(s, a.V, seg, g.warp, g.lane);
+  float* const w = weights + sub * seg * Group<G>::kWarps + at.first;   // the warp's words; scores at first
+  const float nan = __int_as_float(0x7fffffff);
+  float m = neg_inf();
+#pragma unroll 4
+  for (int o = g.lane * VEC; o < (RESIDENT ? seg : at.end - at.first); o += 32 * VEC) {
+    float x[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
+    if (at.first + o < at.end) at.load(at.first + o, x);
+    if constexpr (RESIDENT) {
+      if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4)
+          *reinterpret_cast<float4*>(w + o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      } else {
+        w[o] = x[0];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[i]);
+  }
+  __syncwarp();
+  m = g.max(m);
+  if (m == neg_inf() || rule.temperature == 0.0) {
+    // every word is masked, or the first of the greatest scores is asked for
+    int broken = 0, firstBest = 0x7fffffff;
+    each_score<TIn, VEC, G>(s, a.V, tid, [&](float z, int v) {
+      if (z != z) broken = 1;
+      if (z == m && v < firstBest) firstBest = v;
+    });
+    broken = g.max(broken);
+    firstBest = (int)g.min((unsigned)firstBest);
+    if (broken || m == pos_inf()) return answer(-1, nan);
+    return m == neg_inf() ? answer(-1, neg_inf()) : answer(firstBest, 0.0f);
+  }
+  const Weight weight{m, (float)(1.4426950408889634 / rule.temperature)};
+  Keep keep;
+  keep.exact = ExactWeight{m, 1.0 / rule.temperature};
+  // f(weights, first word) for kPass words at a time: weights of 0 for those that do not stay, as far as
+  // `keep` says it so far
+  auto each = [&](auto f) {
+    if constexpr (RESIDENT) {
+#pragma unroll 2
+      for (int o = g.lane * 4; o < seg; o += 128) {
+        const float4 q = *reinterpret_cast<const float4*>(w + o);
+        const float y[4] = {q.x, q.y, q.z, q.w};
+        f(y, at.first + o);
+      }
+    } else {
+#pragma unroll 1
+      for (int o = g.lane * VEC; at.first + o < at.end; o += 32 * VEC) {
+        float x[VEC], y[VEC];
+        at.load(at.first + o, x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          y[i] = weight(x[i]);
+          if (!(keep(y[i], x[i], at.first + o + i) || y[i] != y[i])) y[i] = 0.0f;
+        }
+        f(y, at.first + o);
+      }
+    }
+  };
+  // f(word, place) for those of this thread's words whose weight is in [from, below): few of them
+  auto each_between = [&](float from, float below, auto f) {
+    each([&](const float (&y)[kPass], int v) {
+      unsigned in = 0;
+#pragma unroll
+      for (int i = 0; i < kPass; ++i) in |= y[i] >= from && y[i] < below ? 1u << i : 0u;
+#pragma unroll 1
+      for (; in; in &= in - 1) f(v + __ffs(in) - 1);
+    });
+  };
+  auto apply = [&] {   // `keep` has changed
+    if constexpr (RESIDENT) {
+      const float tested = fmaxf(keep.hi, keep.sure());
+#pragma unroll 2
+      for (int o = g.lane * 4; o < seg; o += 128) {
+        const float4 q = *reinterpret_cast<const float4*>(w + o);
+        float y[4] = {q.x, q.y, q.z, q.w};
+        unsigned test = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (y[i] < keep.lo) y[i] = 0.0f;
+          else if (y[i] < tested) test |= 1u << i;
+        }
+#pragma unroll 1
+        for (; test; test &= test - 1) {
+          const int i = __ffs(test) - 1, v = at.first + o + i;
+          const float z = at.score(v), x = weight(z);
+          if (!keep(x, z, v)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (k == i) y[k] = 0.0f;
+          }
+        }
+        *reinterpret_cast<float4*>(w + o) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+    }
+  };
+  // The weights, and their first moments: of |x| for the bound on what is unsure, of x^2 for a first guess.
+  double part = 0.0;
+  float slope = 0.0f, square = 0.0f;
+  auto moments = [&](float x, float y) {
+    const float b = fmaxf(x, -200.0f), c = b * y;
+    slope -= c;
+    square += c * b;
+  };
+  if constexpr (RESIDENT) {
+#pragma unroll 2
+    for (int o = g.lane * 4; o < seg; o += 128) {
+      const float4 q = *reinterpret_cast<const float4*>(w + o);
+      const float z[4] = {q.x, q.y, q.z, q.w};
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = weight.exponent(z[i]);
+        y[i] = ex2(x);
+        moments(x, y[i]);
+      }
+      *reinterpret_cast<float4*>(w + o) = make_float4(y[0], y[1], y[2], y[3]);
+      part += (double)((y[0] + y[1]) + (y[2] + y[3]));
+    }
+  } else {
+#pragma unroll 1
+    for (int o = g.lane * VEC; at.first + o < at.end; o += 32 * VEC) {
+      float x[VEC];
+      at.load(at.first + o, x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float e = weight.exponent(x[i]), y = ex2(e);
+        moments(e, y);
+        part += (double)y;
+      }
+    }
+  }
+  double total = g.sum(part);
+  if (total != total) return answer(-1, nan);
+  slope = g.sum(slope);
+  const double unsure = 1.01 * kUnsureSlope * slope + kUnsureSum * total;
+  // this thread's part of the sum, a few weights at a time in 32 bits
+  auto part_of = [&] {
+    double sum = 0.0;
+    each([&](const float (&y)[kPass], int) {
+      float few = y[0];
+#pragma unroll
+      for (int i = 1; i < kPass; ++i) few += y[i];
+      sum += (double)few;
+    });
+    return sum;
+  };
+
+  // The first words of the order with a count of k, or a weight of topP * total.  False: that is all.
+  // A threshold that fewer reach and one that enough reach are brought together until at most kNear words
+  // lie between them.  Weights add up to about a logistic function of the exponent (log-counts are about
+  // linear): that gives the next threshold, a little past the target towards the farther end, so that
+  // the two close in from both sides; the first is that of a normal distribution.  4 to 5 rounds for
+  // topP = 0.9 and 10000 words, 11 with the weights themselves taken for linear.
+  auto find_cut = [&](auto by_weight, int k, float guess) {
+    constexpr bool kByWeight = decltype(by_weight)::value;
+    double target = kByWeight ? rule.topP * total : (double)k;
+    auto measure = [&](float t, double& sum, int& n) {
+      double part = 0.0;
+      int c = 0;
+      each([&](const float (&y)[kPass], int) {
+        float few = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPass; ++i)
+          if (y[i] >= t) {
+            few += y[i];
+            ++c;
+          }
+        if (kByWeight) part += (double)few;
+      });
+      n = g.sum(c);
+      sum = kByWeight ? g.sum(part) : (double)n;
+    };
+    float lo = FLT_MIN, hi = kAbove, t = guess;
+    double vLo = 0.0, vHi = 0.0;
+    int nLo = 0, nHi = 0, stuck = 0;
+    bool done = false;
+    Cut cut;
+    const float floor = (float)(1e-5 * total);
+    auto level = [&](double v) {
+      return kByWeight ? __log2f(fmaxf((float)v, 0.25f)) - __log2f(fmaxf((float)(total - v), floor))
+                       : -__log2f(fmaxf((float)v, 0.5f));
+    };
+#pragma unroll 1
+    for (int round = 0; round < 64 && !done; ++round) {
+      double v;
+      int n;
+      measure(t, v, n);
+      const int had = nLo - nHi;
+      if (v >= target) lo = t, vLo = v, nLo = n;
+      else hi = t, vHi = v, nHi = n;
+      if (nLo == 0) {   // nothing is known from below yet
+        if (!kByWeight && t == FLT_MIN) return false;   // there are no more words than that
+        if (t == FLT_MIN) break;
+        t = round == 0 && t > 1e-9f ? t * 1e-3f : FLT_MIN;
+        continue;
+      }
+      const int c = nLo - nHi;
+      if (c > kNear) {
+        stuck = had > 0 && c > had / 2 ? stuck + 1 : 0;
+        const float xl = __log2f(lo), xh = fminf(__log2f(hi), 0.1f), l = level(vLo), h = level(vHi);
+        float f = (l - level(target)) / (l - h);
+        const float past = 0.3f * kNear / (float)c;
+        f = stuck >= 2 ? 0.5f : f < 0.5f ? f + past : f - past;
+        f = fminf(fmaxf(f, 0.01f), 0.99f);
+        t = ex2(xl + f * (xh - xl));
+        if (!(t > lo && t < hi)) t = __uint_as_float((__float_as_uint(lo) + __float_as_uint(hi)) / 2);
+        if (!(t > lo && t < hi)) break;
+        continue;
+      }
+      g.sync();
+      if (tid == 0) *filled = 0;
+      g.sync();
+      each_between(lo, hi, [&](int v) { list[atomicAdd(filled, 1)] = entry_of(at.score(v), v); });
+      g.sync();
+      for (int i = tid; i < c; i += G) {
+        const Entry mine = list[i];
+        sorted[entries_before(list, c, mine)] = mine;
+      }
+      g.sync();
+      int kept = k - nHi;
+      bool enough = true;
+      if (kByWeight) {
+        // every warp for itself: lane i has entries 2 i and 2 i + 1
+        const int i0 = 2 * g.lane, i1 = i0 + 1;
+        const double w0 = i0 < c ? keep.exact(key_score(entry_key(sorted[i0]))) : 0.0;
+        const double w1 = i1 < c ? keep.exact(key_score(entry_key(sorted[i1]))) : 0.0;
+        double upto = w0 + w1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (g.lane >= o) upto += x;
+        }
+        double above = vHi;
+        // whether the sum up to a word is too close to the target to tell
+        const double d0 = above + (upto - w1) - target, d1 = above + upto - target;
+        const bool close = (g.lane == 0 && fabs(above - target) <= unsure) || (i0 < c && fabs(d0) <= unsure) ||
+                           (i1 < c && fabs(d1) <= unsure);
+        if (__any_sync(0xffffffffu, close)) {
+          const ExactSums sums = exact_sums<TIn, VEC, G>(s, a.V, g, keep, weight, hi);
+          g.sync();
+          above = sums.above;
+          target = rule.topP * sums.all;
+        }
+        // the words whose predecessors have not reached the target
+        const unsigned b0 = __ballot_sync(0xffffffffu, i0 < c && above + (upto - w1 - w0) < target);
+        const unsigned b1 = __ballot_sync(0xffffffffu, i1 < c && above + (upto - w1) < target);
+        kept = __popc(b0) + __popc(b1);
+        enough = above + __shfl_sync(0xffffffffu, upto, 31) >= target;
+      }
+      // (32-bit weights of different scores may come out in the wrong order by a rounding: not so the
+      // cut's and those beyond the thresholds)
+      float y = 0.0f;
+      if (kept > 0) {
+        const Entry last = sorted[kept - 1];
+        cut = Cut{entry_key(last), entry_word(last)};
+        y = weight(key_score(cut.key));
+      }
+      if (hi < kAbove && (kept == 0 || y * 1.000004f >= hi)) t = hi * 1.00003f;
+      else if (lo > FLT_MIN && (!enough || y * 0.999996f < lo)) t = fmaxf(lo * 0.99997f, FLT_MIN);
+      else if (kept > 0 && enough) done = true;
+      else break;
+    }
+    if (!done) {
+      cut = kByWeight ? general_share<TIn, VEC, G>(s, a.V, g, keep.cut, keep.exact, rule.topP)
+                      : general_first_k<TIn, VEC, G>(s, a.V, g, k);
+      g.sync();
+      lo = FLT_MIN;
+      hi = kAbove;
+    }
+    keep.lo = lo;
+    keep.hi = hi;
+    keep.cut = cut;
+    apply();
+    return true;
+  };
+  if (rule.topK > 0 && rule.topK < a.V && find_cut(std::false_type{}, rule.topK, 0x1p-8f) && rule.topP < 1.0)
+    total = g.sum(part_of());
+  if (rule.topP < 1.0) {
+    const float mean = -slope / (float)total, deviation = sqrtf(fmaxf(g.sum(square) / (float)total - mean * mean, 0.0f));
+    const float p = (float)rule.topP, odds = 0.55f * (__log2f(p) - __log2f(1.0f - p)) * 0.6931472f;
+    find_cut(std::true_type{}, 0, fmaxf(ex2(fminf(mean - odds * deviation, -0.05f)), 0.25f * (1.0f - p) / (float)a.V));
+  }
+  if (rule.minP > 0.0) {
+    keep.minP = rule.minP;
+    keep.lo = fmaxf(keep.lo, (float)rule.minP * 0.9999f);
+    apply();
+  }
+
+  // the draw: the warp, its vectors, the word
+  float u = uniforms[node];
+  u = u < 0.0f ? 0.0f : u < 1.0f ? u : 0.99999994f;
+  part = part_of();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  double own = g.exchange(part), upto = own;
+#pragma unroll
+  for (int o = 1; o < Group<G>::kWarps; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (g.lane >= o) upto += x;
+  }
+  total = __shfl_sync(0xffffffffu, upto, Group<G>::kWarps - 1);
+  const double target = (double)u * total;
+  const unsigned past = __ballot_sync(0xffffffffu, upto > target && g.lane < Group<G>::kWarps);
+  const int pick = past ? __ffs(past) - 1 : Group<G>::kWarps - 1;
+  if (g.warp == pick) {
+    double before = __shfl_sync(0xffffffffu, upto - own, pick);
+    int found = -1;
+    bool certain = false;
+#pragma unroll 1
+    for (int o = g.lane * kPass; found < 0 && at.first + o - g.lane * kPass < at.end; o += 32 * kPass) {
+      const int v = at.first + o;
+      float y[kPass], upTo[kPass];
+      if constexpr (RESIDENT) {
+        float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (o < seg) q = *reinterpret_cast<const float4*>(w + o);
+        y[0] = q.x, y[1] = q.y, y[2] = q.z, y[3] = q.w;
+      } else {
+        float x[VEC];
+        if (v < at.end) at.load(v, x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          y[i] = v < at.end ? weight(x[i]) : 0.0f;
+          if (v < at.end && !keep(y[i], x[i], v + i)) y[i] = 0.0f;
+        }
+      }
+      upTo[0] = y[0];
+#pragma unroll
+      for (int i = 1; i < kPass; ++i) upTo[i] = upTo[i - 1] + y[i];
+      const double sum = upTo[kPass - 1];
+      double scan = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, scan, d);
+        if (g.lane >= d) scan += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + scan > target);
+      if (hit) {
+        const int owner = __ffs(hit) - 1;
+        const double start = before + (scan - sum);
+        double b = start;
+        int word = -1;
+        bool clear = false;
+#pragma unroll
+        for (int i = 0; i < kPass; ++i) {
+          const double after = start + (double)upTo[i];
+          if (word < 0 && after > target) {
+            word = v + i;
+            clear = y[i] > 0.0f && target - b > unsure && after - target > unsure;
+          }
+          b = after;
+        }
+        found = __shfl_sync(0xffffffffu, word, owner);
+        certain = __shfl_sync(0xffffffffu, clear ? 1 : 0, owner) && found >= 0;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (g.lane == 0) {
+      *sure = certain;
+      if (certain) words[node] = found, logProbs[node] = (float)log(keep.exact(at.score(found)) / total);
+    }
+  }
+  g.sync();
+  if (*sure) return;
+  exact_draw<TIn, VEC, G>(s, a.V, seg, g, keep, weight, u, words + node, logProbs + node);
+}
+
+}  // namespace
+
+// Whether words can be moved 16 bytes at a time: every row starts on a 16-byte boundary and has whole
+// vectors.
+bool node_rows_aligned(const NodeArgs& a) {
+  const int size = a.dtype == kDtypeBf16 ? 2 : 4;
+  const i64 bytes[] = {(i64)reinterpret_cast<uintptr_t>(a.E), (i64)reinterpret_cast<uintptr_t>(a.P),
+                       a.eStrideB * size, a.eStrideT * size, a.pStrideB * size, a.pStrideU * size,
+                       (i64)a.V * size};
+  return std::all_of(std::begin(bytes), std::end(bytes), [](i64 x) { return x % 16 == 0; });
+}
+
+void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, float* logProbs,
+                         SampleRule rule, cudaStream_t stream) {
+  const i64 nodes = (i64)a.B * a.N;
+  if (nodes == 0) return;
+  with_type(a, [&](auto type, auto vec) {
+    using TIn = decltype(type);
+    auto launch = [&](auto group, auto resident) {
+      constexpr int G = decltype(group)::value, rows = kCta<G> / G;
+      auto kernel = sample_words_kernel<TIn, decltype(vec)::value, G, decltype(resident)::value>;
+      const int seg = (int)round_up64(div_up(a.V, G / 32), 32);
+      const int smem = decltype(resident)::value ? rows * seg * (G / 32) * (int)sizeof(float) : 0;
+      if (smem > 32 * 1024) allow_dyn_smem(kernel, kResidentBytes);
+      ScopedKernel prof("sample_words", stream);
+      kernel<<<(unsigned)div_up64(nodes, rows), kCta<G>, smem, stream>>>(a, uniforms, words, logProbs, rule, seg);
+      TB200_CHECK_LAUNCH();
+    };
+    using std::integral_constant;
+    if (a.V <= 1024) launch(integral_constant<int, 32>{}, std::true_type{});
+    else if (a.V <= 4096) launch(integral_constant<int, 128>{}, std::true_type{});
+    else if (a.V <= 16384) launch(integral_constant<int, 256>{}, std::true_type{});
+    else if (round_up64(div_up(a.V, 32), 32) * 32 * 4 <= kResidentBytes)
+      launch(integral_constant<int, 1024>{}, std::true_type{});
+    else launch(integral_constant<int, 1024>{}, std::false_type{});
+  });
+}
+
+}  // namespace tb200

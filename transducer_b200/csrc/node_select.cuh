@@ -1,0 +1,167 @@
+// What node_top.cu (the best words of a lattice node) and node_sample.cu (a word drawn from a node's
+// distribution) share.
+//
+// A row of scores is read once and stays in the registers of a group of threads (a warp for short rows,
+// a CTA for long ones; rows beyond a CTA's registers are read again for every pass).  What both
+// operators then need is a cut in the order of the words: the first k of them, or the first whose
+// weights reach a share.  Sorting is never needed for that: thresholds on the scores are tried, one
+// count (or sum of weights) over the registers each, until the few words about the cut can be put
+// in a list, where each finds its place by comparing itself with the others.
+#pragma once
+
+#include <type_traits>
+
+#include "node_rows.cuh"
+
+namespace tb200 {
+
+// Which words of a row a thread has: warp w has the words from w * seg on, as far as the next warp's,
+// and its lanes take vectors of VEC words in turn.  So the warps' parts follow each other in the order
+// of the alphabet, and so do the vectors of a warp.  EPT words at most in a thread (0: any number).
+template <typename TIn, int VEC, int G, int EPT>
+struct Place {
+  static_assert(EPT % VEC == 0 || EPT == 0);
+  NodeScores<TIn> s;
+  int first, end, lane;   // the warp's words
+  __device__ __forceinline__ Place(const NodeScores<TIn>& scores, int V, int seg, int warp, int lane_)
+      : s(scores), first(warp * seg), end(min(V, first + seg)), lane(lane_) {}
+  __device__ __forceinline__ int word(int j) const { return first + (j * 32 + lane) * VEC; }
+  __device__ __forceinline__ void load(int v, float (&z)[VEC]) const {
+    const Words<VEC> e = load_words<VEC>(s.e + v), p = load_words<VEC>(s.p + v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) z[i] = e.x[i] + p.x[i];
+  }
+  __device__ __forceinline__ float score(int v) const { return to_f32(s.e[v]) + to_f32(s.p[v]); }
+};
+
+// ---- the general way, from memory: one pass over the row per bit searched --------------------
+// For rows where the words about a cut are too many for a list (equal scores), and for NaN.  These
+// functions have a copy of the group: the caller's next reduction comes after a barrier.
+
+// Words are ordered by score, the greater first, equal ones by index, the lower first.  A cut is a
+// prefix of that order: the words above `key`, and those at `key` up to `last`.
+struct Cut {
+  unsigned key;
+  int last;
+  __device__ __forceinline__ bool keeps(unsigned k, int v) const { return k > key || (k == key && v <= last); }
+  __device__ __forceinline__ bool keeps(float z, int v) const { return keeps(score_key(z), v); }
+};
+
+template <typename TIn, int VEC, int G, typename F>
+__device__ __forceinline__ void each_score(const NodeScores<TIn>& s, int V, int tid, F f) {
+#pragma unroll 1
+  for (int v = tid * VEC; v < V; v += G * VEC) {
+    const Words<VEC> e = load_words<VEC>(s.e + v), p = load_words<VEC>(s.p + v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f(e.x[i] + p.x[i], v + i);
+  }
+}
+
+// The largest key x for which reaches(x) holds (a property that holds for 0 and for fewer and fewer
+// words from there on).
+template <typename F>
+__device__ __forceinline__ unsigned largest_key(F reaches) {
+  unsigned x = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned t = x | (1u << bit);
+    if (reaches(t)) x = t;
+  }
+  return x;
+}
+// The smallest index y in [0, V) for which reaches(y) holds, V - 1 if it never does.
+template <typename F>
+__device__ __forceinline__ int smallest_index(int V, F reaches) {
+  int lo = 0, hi = V - 1;
+#pragma unroll 1
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (reaches(mid)) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// The k first words of the order (0 < k <= V).
+template <typename TIn, int VEC, int G>
+__device__ __noinline__ Cut general_first_k(NodeScores<TIn> s, int V, Group<G> g, int k) {
+  auto count = [&](auto pick) {
+    int c = 0;
+    each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) { c += pick(score_key(z), v) ? 1 : 0; });
+    return g.sum(c);
+  };
+  Cut cut;
+  cut.key = largest_key([&](unsigned x) { return count([&](unsigned u, int) { return u >= x; }) >= k; });
+  const int above = count([&](unsigned u, int) { return u > cut.key; });
+  cut.last = smallest_index(V, [&](int y) {
+    return count([&](unsigned u, int v) { return u == cut.key && v <= y; }) >= k - above;
+  });
+  return cut;
+}
+
+// ---- groups and lists -------------------------------------------------------------------------
+
+constexpr int kWarpRows = 8;   // rows per CTA where a warp has a row
+template <int G>
+constexpr int kCta = G == 32 ? 32 * kWarpRows : G;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+using Entry = unsigned long long;   // a word and its score: greater for words that come first
+__device__ __forceinline__ Entry entry_of(float z, int v) {
+  return ((Entry)score_key(z) << 32) | (0xffffffffu - (unsigned)v);
+}
+__device__ __forceinline__ int entry_word(Entry e) { return (int)(0xffffffffu - (unsigned)e); }
+__device__ __forceinline__ unsigned entry_key(Entry e) { return (unsigned)(e >> 32); }
+
+// How many of the c entries of `list` come before `mine`.
+__device__ __forceinline__ int entries_before(const Entry* list, int c, Entry mine) {
+  int n = 0;
+#pragma unroll 4
+  for (int j = 0; j < c; ++j) n += list[j] > mine ? 1 : 0;
+  return n;
+}
+
+// ---- launches ---------------------------------------------------------------------------------
+
+// Group and words per thread for rows of V words: a warp has up to 1024, larger groups 16 to 32 a thread,
+// 1024 threads and more words are read again for every pass.
+template <typename F>
+void with_group(int V, F launch) {
+  auto go = [&](auto group, auto ept) { launch(group, ept, (int)round_up64(div_up(V, group / 32), 32)); };
+  auto fits = [&](int group, int ept) { return round_up64(div_up(V, group / 32), 32) <= 32 * ept; };
+  using std::integral_constant;
+#define TB200_GROUP(G, EPT) \
+  if (fits(G, EPT)) return go(integral_constant<int, G>{}, integral_constant<int, EPT>{})
+  TB200_GROUP(32, 8);
+  TB200_GROUP(32, 16);
+  TB200_GROUP(32, 32);
+  TB200_GROUP(128, 16);
+  TB200_GROUP(128, 32);
+  TB200_GROUP(256, 24);
+  TB200_GROUP(256, 32);
+  TB200_GROUP(512, 24);
+  TB200_GROUP(512, 32);
+  TB200_GROUP(1024, 24);
+  TB200_GROUP(1024, 32);
+#undef TB200_GROUP
+  go(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
+}
+
+template <typename F>
+void with_type(const NodeArgs& a, F launch) {
+  const bool wide = node_rows_aligned(a);
+  if (a.dtype == kDtypeBf16) {
+    if (wide) launch(bf16{}, std::integral_constant<int, 8>{});
+    else launch(bf16{}, std::integral_constant<int, 1>{});
+  } else {
+    if (wide) launch(float{}, std::integral_constant<int, 4>{});
+    else launch(float{}, std::integral_constant<int, 1>{});
+  }
+}
+
+}  // namespace tb200

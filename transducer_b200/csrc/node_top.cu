@@ -1,0 +1,225 @@
+// The best words of a lattice node.
+#include "node_select.cuh"
+#include "profile.h"
+
+namespace tb200 {
+namespace {
+
+template <typename TIn, int VEC, int G>
+__device__ __noinline__ void general_top_words(NodeScores<TIn> s, int V, Group<G> g, Entry* list, int* filled,
+                                               int* words, float* logits, float* rest, int k, float scale) {
+  const Cut cut = general_first_k<TIn, VEC, G>(s, V, g, k);
+  g.sync();
+  if (g.tid == 0) *filled = 0;
+  g.sync();
+  each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) {
+    if (cut.keeps(z, v)) list[atomicAdd(filled, 1)] = entry_of(z, v);
+  });
+  g.sync();
+  for (int i = g.tid; i < k; i += G) {
+    const Entry mine = list[i];
+    const int place = entries_before(list, k, mine);
+    words[place] = entry_word(mine);
+    logits[place] = key_score(entry_key(mine)) * scale;
+  }
+  if (!rest) return;
+  float m = neg_inf();
+  each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) {
+    if (!cut.keeps(z, v)) m = fmaxf(m, z);
+  });
+  m = g.max(m);
+  float sum = 0.0f;
+  if (m > neg_inf() && m < pos_inf())
+    each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) {
+      if (!cut.keeps(z, v)) sum += expf((z - m) * scale);
+    });
+  sum = g.sum(sum);
+  if (g.tid == 0) *rest = m > neg_inf() && m < pos_inf() ? m * scale + logf(sum) : m;
+}
+
+constexpr int kListed = 512;   // entries of a row's list; kMaxListedWords of them are asked for at most
+
+// The k best words.  Every thread takes the maxima of four subsets of its words; a threshold that k of the
+// G * 4 maxima reach (k of the G threads' maxima where k is small) is one that k words reach, and hardly more
+// than k do: 33 of 10000 words for k = 32 and 512 threads.
+template <typename TIn, int VEC, int G, int EPT>
+__global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __restrict__ words,
+                                                            float* __restrict__ logits,
+                                                            float* __restrict__ rest, int k, int seg, float scale) {
+  constexpr int kRows = kCta<G> / G;
+  __shared__ double scratch[64];
+  __shared__ Entry listAll[kRows][kListed];
+  __shared__ int filledAll[kRows];
+  __shared__ Entry edgeAll[kRows][2];   // the last word of the k, and the next one (0: not in the list)
+  const int sub = threadIdx.x / G, tid = threadIdx.x % G;
+  const i64 node = (i64)blockIdx.x * kRows + sub;
+  if (node >= (i64)a.B * a.N) return;
+  Entry *list = listAll[sub], *edge = edgeAll[sub];
+  int* filled = &filledAll[sub];
+  words += node * k;
+  logits += node * k;
+  if (rest) rest += node;
+  const NodeScores<TIn> s = node_scores<TIn>(a, node);
+  if (!s.here) {
+    for (int i = tid; i < k; i += G) words[i] = -1, logits[i] = neg_inf();
+    if (rest && tid == 0) *rest = neg_inf();
+    return;
+  }
+  Group<G> g(tid, scratch);
+  const Place<TIn, VEC, G, EPT> at(s, a.V, seg, g.warp, g.lane);
+  float z[EPT > 0 ? EPT : 1];
+  auto each = [&](auto f) {   // f(score, word) for each of this thread's words
+    if constexpr (EPT > 0) {
+#pragma unroll
+      for (int j = 0; j < EPT / VEC; ++j) {
+        const int v = at.word(j);
+        if (v < at.end)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f(z[j * VEC + i], v + i);
+      }
+    } else {
+#pragma unroll 1
+      for (int v = at.word(0); v < at.end; v += 32 * VEC) {
+        float x[VEC];
+        at.load(v, x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f(x[i], v + i);
+      }
+    }
+  };
+  // (subset v % 4 of the thread's words with vectors, (v / 32) % 4 without)
+  float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+  if constexpr (EPT > 0) {
+#pragma unroll
+    for (int j = 0; j < EPT / VEC; ++j) {
+      const int v = at.word(j);
+      float x[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
+      if (v < at.end) at.load(v, x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[j * VEC + i] = x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) top[i % 4] = fmaxf(top[i % 4], z[i]);
+  } else {
+    each([&](float x, int v) {
+      const int i = VEC > 1 ? v % 4 : (v - at.first) / 32 % 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q == i) top[q] = fmaxf(top[q], x);
+    });
+  }
+  unsigned key[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) key[q] = at.word(VEC > 1 ? 0 : q) < at.end ? score_key(top[q]) : 0u;
+  const unsigned best = max(max(key[0], key[1]), max(key[2], key[3]));
+  // (16 words in a thread's maximum, or a quarter of its words in one of four)
+  const bool one = G > 32 && k <= G / 4;
+  auto reach = [&](unsigned t) {
+    if (G > 32 && one) return __syncthreads_count(best >= t);
+    return g.sum((key[0] >= t) + (key[1] >= t) + (key[2] >= t) + (key[3] >= t));
+  };
+  unsigned hi = g.max(best), lo = 1;
+  int reached = reach(1);
+  if (reached >= k) {
+    lo = g.min(one ? (best ? best : ~0u)
+                   : min(min(key[0] ? key[0] : ~0u, key[1] ? key[1] : ~0u), min(key[2] ? key[2] : ~0u, key[3] ? key[3] : ~0u)));
+    hi = hi + 1;
+#pragma unroll 1
+    while (hi - lo > 1 && reached > k + max(k / 8, 4)) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      const int n = reach(mid);
+      if (n >= k) lo = mid, reached = n;
+      else hi = mid;
+    }
+  }
+  if (tid == 0) *filled = 0, edge[0] = edge[1] = 0;
+  g.sync();
+  const unsigned lowest = score_key(neg_inf());
+  const float bound = key_score(max(lo, lowest));
+  auto append = [&](float x, int v) {
+    const int i = atomicAdd(filled, 1);
+    if (i < kListed) list[i] = entry_of(x, v);
+  };
+  if (best >= lo || lo <= lowest) {
+    if constexpr (EPT > 0) {
+      unsigned in = 0;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) in |= z[i] >= bound ? 1u << i : 0u;
+#pragma unroll 1
+      for (; in; in &= in - 1) {
+        const int i = __ffs(in) - 1, v = at.word(i / VEC) + i % VEC;
+        if (v < at.end) append(at.score(v), v);
+      }
+    } else {
+      each([&](float x, int v) {
+        if (x >= bound) append(x, v);
+      });
+    }
+  }
+  g.sync();
+  const int c = *filled;
+  auto general = [&] { general_top_words<TIn, VEC, G>(s, a.V, g, list, filled, words, logits, rest, k, scale); };
+  if (c > kListed || c < k) return general();   // (fewer than k: some are NaN)
+#pragma unroll 1
+  for (int i = tid; i < c; i += G) {
+    const Entry mine = list[i];
+    const int place = entries_before(list, c, mine);
+    if (place < k) {
+      words[place] = entry_word(mine);
+      logits[place] = key_score(entry_key(mine)) * scale;
+    }
+    if (place == k - 1) edge[0] = mine;
+    if (place == k) edge[1] = mine;
+  }
+  g.sync();
+  // the others' weights, relative to the last listed word's; of the words with its score those that are
+  // left out are in the list
+  const float last = key_score(entry_key(edge[0]));
+  int ties = 0;
+  if (edge[1] >> 32 == edge[0] >> 32) {
+    for (int i = tid; i < c; i += G) ties += list[i] < edge[0] && list[i] >> 32 == edge[0] >> 32 ? 1 : 0;
+    ties = g.sum(ties);
+  }
+  const float scale2 = scale * 1.4426950408889634f;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  int turn = 0;
+  each([&](float x, int) {
+    sum[turn++ % 4] += x >= last ? 0.0f : ex2((x - last) * scale2);   // (NaN comes through)
+  });
+  float all = g.sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (all != all) return general();
+  if (!rest) return;
+  all += (float)ties;
+  float ref = last;
+  if (!(all > 1e-25f)) {   // the others are far below: relative to their own maximum
+    ref = neg_inf();
+    each([&](float x, int) { ref = x < last ? fmaxf(ref, x) : ref; });
+    ref = g.max(ref);
+    all = 0.0f;
+    if (ref > neg_inf()) each([&](float x, int) { all += x < last ? ex2((x - ref) * scale2) : 0.0f; });
+    all = g.sum(all);
+  }
+  if (tid == 0) *rest = fabsf(ref) < pos_inf() ? ref * scale + logf(all) : ref;
+}
+
+}  // namespace
+
+void launch_top_words(const NodeArgs& a, int* words, float* logits, float* rest, int k, double temperature,
+                      cudaStream_t stream) {
+  const i64 nodes = (i64)a.B * a.N;
+  if (nodes == 0) return;
+  with_type(a, [&](auto type, auto vec) {
+    using TIn = decltype(type);
+    with_group(a.V, [&](auto group, auto ept, int seg) {
+      constexpr int G = group, rows = kCta<G> / G;
+      ScopedKernel prof("top_words", stream);
+      top_words_kernel<TIn, vec, G, ept><<<(unsigned)div_up64(nodes, rows), kCta<G>, 0, stream>>>(
+          a, words, logits, rest, k, seg, (float)(1.0 / temperature));
+      TB200_CHECK_LAUNCH();
+    });
+  });
+}
+
+}  // namespace tb200
