@@ -157,7 +157,7 @@ def test_c_abi_refusals():
         assert forward(**bad) == 1, bad
     assert forward(B=0) == 0
 
-    need = lib.tb200_distill_backward_workspace_bytes(2, 5, 3)
+    need = lib.tb200_distill_backward_workspace_bytes(2, 5, 3, 8, 4)
     assert need >= 2 * 8 * 8
 
     def backward(saved=some, saved_bytes=saved, ws=some, ws_bytes=need, B=2):
@@ -173,7 +173,9 @@ def test_workspaces_do_not_grow_for_smaller_calls():
     for f, sizes in ((lib.tb200_distill_saved_bytes, [(B, 40, 8) for B in range(30)]),
                      (lib.tb200_distill_saved_bytes, [(3, N, 8) for N in range(300)]),
                      (lib.tb200_distill_saved_bytes, [(3, 40, K) for K in range(1, 257)]),
-                     (lib.tb200_distill_backward_workspace_bytes, [(3, T, 9) for T in range(300)]),
-                     (lib.tb200_distill_backward_workspace_bytes, [(3, 9, U) for U in range(300)])):
+                     *((lib.tb200_distill_backward_workspace_bytes, sizes) for sizes in (
+                         [(B, 300, 40, 600, 340) for B in range(120)], [(3, T, 9, 700, 400) for T in range(900)],
+                         [(3, 9, U, 1000, 90) for U in range(300)], [(2, 90, 9, V, 99) for V in range(1, 9000, 7)],
+                         [(2, 30, 9, 600, N) for N in range(900)]))):
         got = [f(*s) for s in sizes]
         assert got == sorted(got)

@@ -291,9 +291,10 @@ struct DistillSaved {
 void launch_distill_forward(const NodeArgs& a, const int* words, const float* logits, const float* rest,
                             float* costs, DistillSaved saved, int K, double temperature,
                             cudaStream_t stream);
-// spans: 2 (B*T + B*U) ints.  egrads [B,T,V], pgrads [B,U,V] of the inputs' type, written whole.
+// egrads [B,T,V], pgrads [B,U,V] of the inputs' type, written whole; either may be null.
+size_t distill_backward_workspace_bytes(int B, int T, int U, int V, int N);
 void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved saved, const float* weights,
-                             void* egrads, void* pgrads, int K, bool hasRest, double temperature, int* spans,
-                             cudaStream_t stream);
+                             void* egrads, void* pgrads, int K, bool hasRest, double temperature,
+                             void* workspace, cudaStream_t stream);
 
 }  // namespace tb200

@@ -120,9 +120,8 @@ int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStr
   });
 }
 
-size_t tb200_distill_backward_workspace_bytes(int B, int maxT, int maxU) {
-  if (B <= 0 || maxT < 0 || maxU < 0) return 0;
-  return round256(2 * sizeof(int) * (size_t)B * ((size_t)maxT + maxU));
+size_t tb200_distill_backward_workspace_bytes(int B, int maxT, int maxU, int V, int N) {
+  return distill_backward_workspace_bytes(B, maxT, maxU, V, N);
 }
 
 int tb200_distill_backward(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
@@ -136,9 +135,9 @@ int tb200_distill_backward(const void* E, const void* P, int bf16, long long eSt
     check_listed(K);
     check_temperature(temperature);
     need(savedBytes, tb200_distill_saved_bytes(B, N, K), saved, "saved state");
-    need(workspaceBytes, tb200_distill_backward_workspace_bytes(B, maxT, maxU), workspace, "workspace");
+    need(workspaceBytes, tb200_distill_backward_workspace_bytes(B, maxT, maxU, V, N), workspace, "workspace");
     launch_distill_backward(a, words, distill_saved(const_cast<void*>(saved), B, N), weights, egrads, pgrads, K,
-                            hasRest != 0, temperature, static_cast<int*>(workspace), api_stream());
+                            hasRest != 0, temperature, workspace, api_stream());
   });
 }
 

@@ -196,126 +196,6 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
   saved.node[node] = make_float4(all.m, L, A, sign);
 }
 
-// Where the nodes of each frame and each position lie among the N of their utterance: spans[row] =
-// (N - first, last + 1) for the B*T frames, then the B*U positions; zeros where there is none.
-__global__ void __launch_bounds__(256) node_spans_kernel(NodeArgs a, int2* __restrict__ spans) {
-  const i64 node = (i64)blockIdx.x * 256 + threadIdx.x;
-  if (node >= (i64)a.B * a.N) return;
-  const int t = a.frames[node], u = a.positions[node];
-  if ((unsigned)t >= (unsigned)a.T || (unsigned)u >= (unsigned)a.U) return;
-  const i64 b = node / a.N;
-  const int n = (int)(node - b * a.N);
-  int2* f = spans + b * a.T + t;
-  int2* p = spans + (i64)a.B * a.T + b * a.U + u;
-  atomicMax(&f->x, a.N - n);
-  atomicMax(&f->y, n + 1);
-  atomicMax(&p->x, a.N - n);
-  atomicMax(&p->y, n + 1);
-}
-
-// Gradients of the rows of E (FRAMES) or P: one warp per row and tile of 32 * VEC * NV words, which
-// goes through the row's nodes in their order.
-template <typename TIn, int VEC, int NV, bool REST, bool FRAMES>
-__global__ void __launch_bounds__(256) distill_rows_kernel(NodeArgs a, const int* __restrict__ words,
-                                                           DistillSaved saved,
-                                                           const float* __restrict__ weights,
-                                                           TIn* __restrict__ grads,
-                                                           const int2* __restrict__ spans, int K, int tiles,
-                                                           float scale, float scale2) {
-  constexpr int kTile = 32 * VEC * NV, kOwn = VEC * NV;
-  const int lane = threadIdx.x & 31;
-  const i64 task = (i64)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int perUtt = FRAMES ? a.T : a.U;
-  const i64 row = task / tiles;
-  if (row >= (i64)a.B * perUtt) return;
-  const int tile0 = (int)(task - row * tiles) * kTile;
-  const i64 b = row / perUtt;
-  const int own = (int)(row - b * perUtt);
-  const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
-  const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
-  const TIn* mine = FRAMES ? E + own * a.eStrideT : P + own * a.pStrideU;
-  float acc[kOwn], own_x[kOwn];
-#pragma unroll
-  for (int i = 0; i < kOwn; ++i) acc[i] = 0.0f, own_x[i] = 0.0f;
-  const int2 span = spans[(FRAMES ? 0 : (i64)a.B * a.T) + row];
-  const int* ownIdx = (FRAMES ? a.frames : a.positions) + b * a.N;
-  const int* otherIdx = (FRAMES ? a.positions : a.frames) + b * a.N;
-  const int others = FRAMES ? a.U : a.T;
-  if (span.y > 0) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int v = tile0 + (j * 32 + lane) * VEC;
-      if (v < a.V) {
-        const Words<VEC> x = load_words<VEC>(mine + v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) own_x[j * VEC + i] = x.x[i];
-      }
-    }
-    for (int n0 = a.N - span.x; n0 < span.y; n0 += 32) {
-      const int nl = n0 + lane;
-      int other = -1;
-      if (nl < span.y && ownIdx[nl] == own) other = otherIdx[nl];
-      unsigned todo = __ballot_sync(0xffffffffu, (unsigned)other < (unsigned)others);
-      while (todo) {
-        const int bit = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const i64 node = b * a.N + n0 + bit;
-        const i64 o = __shfl_sync(0xffffffffu, other, bit);
-        const TIn* theirs = FRAMES ? P + o * a.pStrideU : E + o * a.eStrideT;
-        const float4 of = saved.node[node];
-        const float w = weights[node] * scale;
-        // the listed words of this tile: the teacher's shares are subtracted by the lanes that have them
-        unsigned listed = 0;
-        for (int k0 = 0; k0 < K; k0 += 32) {
-          int v = -1;
-          float q = -1.0f;
-          if (k0 + lane < K) {
-            v = words[node * K + k0 + lane] - tile0;
-            q = saved.q[node * K + k0 + lane];
-          }
-          unsigned hits = __ballot_sync(0xffffffffu, (unsigned)v < (unsigned)kTile && !(q < 0.0f));
-          while (hits) {
-            const int k = __ffs(hits) - 1;
-            hits &= hits - 1;
-            const int at = __shfl_sync(0xffffffffu, v, k);
-            const float share = w * __shfl_sync(0xffffffffu, q, k);
-            if (at / VEC % 32 == lane) {
-              const int slot = at / (32 * VEC) * VEC + at % VEC;
-              listed |= 1u << slot;
-#pragma unroll
-              for (int i = 0; i < kOwn; ++i)
-                if (i == slot) acc[i] -= share;
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int v = tile0 + (j * 32 + lane) * VEC;
-          if (v < a.V) {
-            const Words<VEC> x = load_words<VEC>(theirs + v);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float z = own_x[j * VEC + i] + x.x[i] - of.x;
-              if constexpr (REST) {
-                const bool in = listed >> (j * VEC + i) & 1;
-                acc[j * VEC + i] += w * (in ? 1.0f : of.w) * ex2(fmaf(z, scale2, in ? -of.y : -of.z));
-              } else {
-                acc[j * VEC + i] += w * ex2(fmaf(z, scale2, -of.y));
-              }
-            }
-          }
-        }
-      }
-    }
-  }
-  grads += row * a.V;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = tile0 + (j * 32 + lane) * VEC;
-    if (v < a.V) store_words<VEC>(grads + v, acc + j * VEC);
-  }
-}
-
 template <typename F>
 void with_type(int dtype, bool wide, F launch) {
   if (dtype == kDtypeBf16) {
@@ -356,39 +236,6 @@ void launch_distill_forward(const NodeArgs& a, const int* words, const float* lo
       if (a.V <= 1024) launch(std::integral_constant<int, 32>{});
       else if (a.V <= 4096) launch(std::integral_constant<int, 128>{});
       else launch(std::integral_constant<int, 256>{});
-    });
-  });
-}
-
-void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved saved, const float* weights,
-                             void* egrads, void* pgrads, int K, bool hasRest, double temperature, int* spans,
-                             cudaStream_t stream) {
-  const i64 frameRows = (i64)a.B * a.T, posRows = (i64)a.B * a.U, nodes = (i64)a.B * a.N;
-  if (frameRows + posRows == 0) return;
-  TB200_CUDA_CHECK(cudaMemsetAsync(spans, 0, sizeof(int2) * (frameRows + posRows), stream));
-  int2* sp = reinterpret_cast<int2*>(spans);
-  if (nodes > 0) {
-    ScopedKernel prof("node_spans", stream);
-    node_spans_kernel<<<(unsigned)div_up64(nodes, 256), 256, 0, stream>>>(a, sp);
-    TB200_CHECK_LAUNCH();
-  }
-  const float scale = (float)(1.0 / temperature), scale2 = (float)(1.4426950408889634 / temperature);
-  const bool wide = node_rows_aligned(a) && reinterpret_cast<uintptr_t>(egrads) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(pgrads) % 16 == 0;
-  with_type(a.dtype, wide, [&](auto type, auto vec) {
-    using TIn = decltype(type);
-    with_flag(hasRest, [&](auto has_rest) {
-      constexpr int VEC = vec, NV = 16 / VEC;
-      const int tiles = div_up(a.V, 32 * VEC * NV);
-      auto rows = [&](auto frames, i64 n, void* grads, const char* name) {
-        if (n == 0 || grads == nullptr) return;
-        ScopedKernel prof(name, stream);
-        distill_rows_kernel<TIn, VEC, NV, has_rest, frames><<<(unsigned)div_up64(n * tiles, 8), 256, 0, stream>>>(
-            a, words, saved, weights, static_cast<TIn*>(grads), sp, K, tiles, scale, scale2);
-        TB200_CHECK_LAUNCH();
-      };
-      rows(std::true_type{}, frameRows, egrads, "distill_egrads");
-      rows(std::false_type{}, posRows, pgrads, "distill_pgrads");
     });
   });
 }

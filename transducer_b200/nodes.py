@@ -198,7 +198,7 @@ class NodeDistillation(torch.autograd.Function):
                 torch.empty(x.shape, device=device, dtype=x.dtype) if need else None
                 for x, need in zip((emissions, predictions), ctx.needs_input_grad))
             scores, sizes = _describe(emissions, predictions, frames)
-            nbytes = _transducer.distill_backward_workspace_bytes(*sizes[:3])
+            nbytes = _transducer.distill_backward_workspace_bytes(*sizes)
             ws = _workspace(nbytes, device)
             _transducer.distill_backward(
                 scores, frames.data_ptr(), positions.data_ptr(), words.data_ptr(),
