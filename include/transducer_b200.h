@@ -381,7 +381,7 @@ int tb200_distill_backward(const void* emissions, const void* predictions, int b
                            const int* words, const void* saved, size_t savedBytes,
                            const float* weights, void* egrads, void* pgrads, int batchSize,
                            int maxInputLength, int maxLabelLength, int alphabetSize, int nodes,
-                           int K, int hasRest, double temperature, void* workspace,
+                           int K, double temperature, void* workspace,
                            size_t workspaceBytes);
 
 #ifdef __cplusplus

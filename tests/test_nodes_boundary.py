@@ -162,7 +162,7 @@ def test_c_abi_refusals():
 
     def backward(saved=some, saved_bytes=saved, ws=some, ws_bytes=need, B=2):
         return lib.tb200_distill_backward(None, None, 0, *strides, None, None, None, saved, saved_bytes, None, None,
-                                          None, B, 5, 3, 8, 4, 3, 0, 1.0, ws, ws_bytes)
+                                          None, B, 5, 3, 8, 4, 3, 1.0, ws, ws_bytes)
 
     for bad in (dict(saved=None), dict(saved_bytes=saved - 1), dict(ws=None), dict(ws_bytes=need - 1)):
         assert backward(**bad) == 1, bad

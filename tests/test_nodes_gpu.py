@@ -184,6 +184,20 @@ def test_distillation_long_groups(V, B, T, U, N, kind, with_rest):
     check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.0, g, 5)
 
 
+@pytest.mark.parametrize("V", [30, 64, 1025])
+@pytest.mark.parametrize("gap", [10, 100])
+def test_distillation_paths_with_gaps(V, gap):
+    """Paths of very different lengths, with runs of places that hold no node and frames without any."""
+    E, P, frames, positions, g = make(4, 500, 6, V, 620, seed=V + gap, kind="path", holes=False)
+    frames[0, 60:] = -1           # 60 of 500 frames have nodes
+    frames[1] = -1                # none has
+    frames[2, 200:200 + gap] = -1
+    frames[3, :400] = -1          # the first frames have none
+    frames[3, 500:500 + gap] = -1
+    words, logits, rest = teacher(E, P, frames, positions, 5, g)
+    check_distill(E, P, frames, positions, words, logits, rest, 1.0, g, 5)
+
+
 @pytest.mark.parametrize("V", [30, 512, 1025, 5000])
 @pytest.mark.parametrize("with_rest", [False, True])
 def test_distillation_odd_records(V, with_rest):

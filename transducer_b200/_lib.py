@@ -71,7 +71,7 @@ SIGNATURES = {
     "tb200_distill_saved_bytes": (_z, [_i] * 3),
     "tb200_distill_forward": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 7 + [_z] + [_i] * 6 + [_d]),
     "tb200_distill_backward_workspace_bytes": (_z, [_i] * 5),
-    "tb200_distill_backward": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 4 + [_z] + [_p] * 3 + [_i] * 7
+    "tb200_distill_backward": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 4 + [_z] + [_p] * 3 + [_i] * 6
                                + [_d, _p, _z]),
     "tb200_loss_sum_exchange": (_i, [_p, _p, _i, _i, ctypes.c_uint, _p, ctypes.c_uint]),
 }

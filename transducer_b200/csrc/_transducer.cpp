@@ -225,7 +225,7 @@ PYBIND11_MODULE(_transducer, m) {
         "saved_bytes"_a, "sizes"_a, "k"_a, "temperature"_a);
   m.def("distill_backward",
         [](const Scores& s, addr frames, addr positions, addr words, addr saved, size_t saved_bytes, addr weights,
-           addr egrads, addr pgrads, const Sizes& n, int k, bool has_rest, double temperature, addr ws,
+           addr egrads, addr pgrads, const Sizes& n, int k, double temperature, addr ws,
            size_t ws_bytes) {
           check(tb200_distill_backward(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)),
                                        std::get<2>(s), std::get<3>(s), std::get<4>(s), std::get<5>(s),
@@ -233,10 +233,10 @@ PYBIND11_MODULE(_transducer, m) {
                                        at<const int>(words), at<const void>(saved), saved_bytes,
                                        at<const float>(weights), at<void>(egrads), at<void>(pgrads),
                                        std::get<0>(n), std::get<1>(n), std::get<2>(n), std::get<3>(n),
-                                       std::get<4>(n), k, has_rest, temperature, at<void>(ws), ws_bytes));
+                                       std::get<4>(n), k, temperature, at<void>(ws), ws_bytes));
         },
         "scores"_a, "frames"_a, "positions"_a, "words"_a, "saved"_a, "saved_bytes"_a, "weights"_a, "egrads"_a,
-        "pgrads"_a, "sizes"_a, "k"_a, "has_rest"_a, "temperature"_a, "workspace"_a, "workspace_bytes"_a);
+        "pgrads"_a, "sizes"_a, "k"_a, "temperature"_a, "workspace"_a, "workspace_bytes"_a);
 
   // ---- device status (bounded waits that ran out) -----------------------------------
   // Returns the code of tb200_check_status (0, or 5 = a kernel gave up) without throwing, so the

@@ -282,19 +282,21 @@ struct SampleRule {
 void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, float* logProbs,
                          SampleRule rule, cudaStream_t stream);
 
-// What the forward call leaves for the backward call, per node and per listed word.
+// What the forward call leaves for the backward call, per node and per listed word: with x = (z - m) log2e /
+// temperature the gradient of a word is sign * 2^(x - A), less `share` for a listed one.  Where sign is +-2
+// that would not do for the listed words: theirs is 2^(x - L) less `share`, the others' +-1 * 2^(x - A).
 struct DistillSaved {
-  float4* node;   // [B*N] m, L, A, sign: the gradient of a listed word is 2^((z-m) log2e/temperature - L) - q,
-                  // of the others sign * 2^((z-m) log2e/temperature - A)
-  float* q;       // [B*N*K] the teacher's share of a listed word; -1: to be ignored
+  float4* node;   // [B*N] m, A, sign, L
+  float* share;   // [B*N*K]; kNoShare: the word is to be ignored
 };
+constexpr float kNoShare = 3e38f;
 void launch_distill_forward(const NodeArgs& a, const int* words, const float* logits, const float* rest,
                             float* costs, DistillSaved saved, int K, double temperature,
                             cudaStream_t stream);
 // egrads [B,T,V], pgrads [B,U,V] of the inputs' type, written whole; either may be null.
 size_t distill_backward_workspace_bytes(int B, int T, int U, int V, int N);
 void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved saved, const float* weights,
-                             void* egrads, void* pgrads, int K, bool hasRest, double temperature,
+                             void* egrads, void* pgrads, int K, double temperature,
                              void* workspace, cudaStream_t stream);
 
 }  // namespace tb200

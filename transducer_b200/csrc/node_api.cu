@@ -51,7 +51,7 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 DistillSaved distill_saved(void* p, int B, int N) {
   DistillSaved s;
   s.node = static_cast<float4*>(p);
-  s.q = p ? reinterpret_cast<float*>(static_cast<char*>(p) + round256(sizeof(float4) * (size_t)B * N)) : nullptr;
+  s.share = p ? reinterpret_cast<float*>(static_cast<char*>(p) + round256(sizeof(float4) * (size_t)B * N)) : nullptr;
   return s;
 }
 
@@ -128,7 +128,7 @@ int tb200_distill_backward(const void* E, const void* P, int bf16, long long eSt
                            long long pStrideB, long long pStrideU, const int* frames, const int* positions,
                            const int* words, const void* saved, size_t savedBytes, const float* weights,
                            void* egrads, void* pgrads, int B, int maxT, int maxU, int V, int N, int K,
-                           int hasRest, double temperature, void* workspace, size_t workspaceBytes) {
+                           double temperature, void* workspace, size_t workspaceBytes) {
   return guarded([&] {
     const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
                                  maxU, V, N);
@@ -137,7 +137,7 @@ int tb200_distill_backward(const void* E, const void* P, int bf16, long long eSt
     need(savedBytes, tb200_distill_saved_bytes(B, N, K), saved, "saved state");
     need(workspaceBytes, tb200_distill_backward_workspace_bytes(B, maxT, maxU, V, N), workspace, "workspace");
     launch_distill_backward(a, words, distill_saved(const_cast<void*>(saved), B, N), weights, egrads, pgrads, K,
-                            hasRest != 0, temperature, workspace, api_stream());
+                            temperature, workspace, api_stream());
   });
 }
 

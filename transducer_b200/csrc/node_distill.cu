@@ -17,13 +17,8 @@
 namespace tb200 {
 namespace {
 
+constexpr int kForwardBytes = 150 * 1024;   // of shared memory: 2^20 bits, 256 words of a record and more
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Running maximum of the scores and sum of 2^((score - maximum) scale2).  The maximum is subtracted
 // before the scaling, so that scores as low as the type's lowest number still have a softmax.
@@ -38,8 +33,10 @@ struct RunningSum {
       s *= ex2((m - top) * scale2);
       m = top;
     }
+    float sum[2] = {s, 0.0f};
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += ex2((z[i] - m) * scale2);
+    for (int i = 0; i < N; ++i) sum[i % 2] += ex2((z[i] - m) * scale2);
+    s = sum[0] + sum[1];
   }
   __device__ __forceinline__ void add(RunningSum o, float scale2) {
     const float top = fmaxf(m, o.m);
@@ -58,142 +55,171 @@ struct RunningSum {
   }
 };
 
-constexpr int kWarpRows = 8;
-template <int G>
-constexpr int kCta = G == 32 ? 32 * kWarpRows : G;
+// A word of the teacher's record.
+struct Listed {
+  int word;      // -1: outside the vocabulary
+  float share;   // of the teacher's distribution; kNoShare: the word is ignored, or an earlier place has its share
+  float z;       // the student's score
+};
 
-// One group of G threads per node.  Dynamic shared memory: a bit per word and node, set for listed ones.
+constexpr int kWarpNodes = 8;   // nodes per CTA where a warp has a node
+template <int G>
+constexpr int kCta = G == 32 ? 32 * kWarpNodes : G;
+
+// One group of G threads per node.  Dynamic shared memory, per node: its record, K Listed; with REST a bit per word
+// of the vocabulary, set for listed ones.
 template <typename TIn, int VEC, int G, bool REST>
 __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
     NodeArgs a, const int* __restrict__ words, const float* __restrict__ logits,
     const float* __restrict__ rest, float* __restrict__ costs, DistillSaved saved, int K, float scale2) {
-  constexpr int kRows = kCta<G> / G;
-  extern __shared__ unsigned bits_all[];
+  constexpr int kNodes = kCta<G> / G, kTurn = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;   // vectors of a row at a time
+  extern __shared__ __align__(16) unsigned char memory[];
   __shared__ double scratch[64];
-  __shared__ int wordAll[kRows][kMaxListedWords];
-  __shared__ float shareAll[kRows][kMaxListedWords];
   const int sub = threadIdx.x / G, tid = threadIdx.x % G;
-  const i64 node = (i64)blockIdx.x * kRows + sub;
+  const i64 node = (i64)blockIdx.x * kNodes + sub;
   if (node >= (i64)a.B * a.N) return;
+  const int bitWords = (a.V + 31) / 32;
+  Listed* const record = reinterpret_cast<Listed*>(memory) + sub * K;
+  unsigned* const bits = reinterpret_cast<unsigned*>(memory + kNodes * K * sizeof(Listed)) + sub * bitWords;
+  float* const savedShare = saved.share ? saved.share + node * K : nullptr;
   const NodeScores<TIn> s = node_scores<TIn>(a, node);
-  int* word = wordAll[sub];
-  float* share = shareAll[sub];
-  words += node * K;
-  logits += node * K;
-  float* q = saved.q ? saved.q + node * K : nullptr;
   if (!s.here) {
     if (tid == 0) costs[node] = 0.0f;
-    if (q) {
-      for (int k = tid; k < K; k += G) q[k] = -1.0f;
-      if (tid == 0) saved.node[node] = make_float4(0.0f, pos_inf(), pos_inf(), 1.0f);
+    if (savedShare) {
+      for (int k = tid; k < K; k += G) savedShare[k] = kNoShare;
+      if (tid == 0) saved.node[node] = make_float4(0.0f, pos_inf(), 1.0f, pos_inf());
     }
     return;
   }
   Group<G> g(tid, scratch);
   // the teacher's shares
-  const float l_rest = REST ? rest[node] : neg_inf();
-  float top = l_rest;
+  const float lRest = REST ? rest[node] : neg_inf();
+  float top = lRest;
   for (int k = tid; k < K; k += G) {
-    const int v = words[k];
-    const bool there = (unsigned)v < (unsigned)a.V;
-    const float l = there ? logits[k] : neg_inf();
-    word[k] = there ? v : -1;
-    share[k] = l;
-    top = fmaxf(top, l);
+    Listed x{words[node * K + k], logits[node * K + k], neg_inf()};
+    if ((unsigned)x.word >= (unsigned)a.V) x.word = -1, x.share = neg_inf();
+    else x.z = to_f32(s.e[x.word]) + to_f32(s.p[x.word]);
+    record[k] = x;
+    top = fmaxf(top, x.share);
   }
-  unsigned* bits = bits_all;
-  if constexpr (REST) {
-    const int n = (a.V + 31) / 32;
-    bits += sub * n;
-    for (int i = tid; i < n; i += G) bits[i] = 0;
-  }
+  if constexpr (REST)
+    for (int i = tid; i < bitWords; i += G) bits[i] = 0;
   top = g.max(top);
   float sum = 0.0f;
   for (int k = tid; k < K; k += G) {
-    share[k] = share[k] == neg_inf() ? 0.0f : expf(share[k] - top);
-    sum += share[k];
+    const float l = record[k].share, x = l == neg_inf() ? 0.0f : expf(l - top);
+    record[k].share = x;
+    sum += x;
   }
-  float r = REST && l_rest != neg_inf() ? expf(l_rest - top) : 0.0f;
+  float r = REST && lRest != neg_inf() ? expf(lRest - top) : 0.0f;
   sum = g.sum(sum) + r;
   g.sync();
-  const bool empty = top == neg_inf();   // the record lists nothing: cost and gradient are 0
+  const bool empty = top == neg_inf();   // the record has no weight: cost and gradient are 0
   const float one = empty ? 0.0f : 1.0f / sum;
   r *= one;
-  // a word that is listed more than once: the first place has all its shares
-  for (int k = tid; k < K; k += G) {
-    const int v = word[k];
-    float all = 0.0f;
-    bool first = v >= 0;
-    if (first)
-      for (int j = 0; j < K; ++j)
-        if (word[j] == v) {
-          first = first && j >= k;
-          all += share[j];
-        }
-    if (q) q[k] = first ? all * one : -1.0f;
-    if constexpr (REST)
-      if (first) atomicOr(&bits[v >> 5], 1u << (v & 31));
+  // A word that is listed more than once: its first place has all its shares.  Then its bit.
+  bool twice = false;
+  if (G == 32 && K <= 32) {
+    const int v = tid < K ? record[tid].word : -1 - tid;
+    twice = (__match_any_sync(0xffffffffu, v) & ~(1u << tid)) != 0 && v >= 0;
+  } else {
+    for (int k = tid; k < K; k += G) {
+      const int v = record[k].word;
+      for (int j = 0; j < K; ++j) twice |= v >= 0 && j != k && record[j].word == v;
+    }
   }
-  if constexpr (REST) g.sync();
+  const bool repeated = g.max(twice ? 1 : 0) != 0;
+  float all[kMaxListedWords / G > 0 ? kMaxListedWords / G : 1];   // of this thread's words
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(all) / sizeof(float)); ++i) {
+    const int k = tid + i * G;
+    if (k >= K) break;
+    const int v = record[k].word;
+    all[i] = v < 0 ? kNoShare : record[k].share * one;
+    if (repeated && v >= 0) {
+      float x = 0.0f;
+      bool first = true;
+      for (int j = 0; j < K; ++j)
+        if (record[j].word == v) {
+          first = first && j >= k;
+          x += record[j].share;
+        }
+      all[i] = first ? x * one : kNoShare;
+    }
+    if constexpr (REST)
+      if (all[i] != kNoShare) atomicOr(&bits[v >> 5], 1u << (v & 31));
+  }
+  if (repeated) g.sync();   // (everybody has read the record)
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(all) / sizeof(float)); ++i) {
+    const int k = tid + i * G;
+    if (k < K) record[k].share = all[i];
+  }
+  g.sync();
   // the student's sums: of the words that are not listed (all words, without REST), and of all
   RunningSum others;
-  for (int v = tid * VEC; v < a.V; v += G * VEC) {
-    const Words<VEC> e = load_words<VEC>(s.e + v), p = load_words<VEC>(s.p + v);
-    unsigned listed = 0;
-    if constexpr (REST) listed = bits[v >> 5] >> (v & 31);
-    float z[VEC];
+  for (int v0 = tid * VEC; v0 < a.V; v0 += G * VEC * kTurn) {
+    RawWords<TIn, VEC> e[kTurn], p[kTurn];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      z[i] = e.x[i] + p.x[i];
-      if constexpr (REST) z[i] = listed >> i & 1 ? neg_inf() : z[i];
+    for (int j = 0; j < kTurn; ++j) {
+      const int v = v0 + j * G * VEC;
+      if (v < a.V) e[j].load(s.e + v), p[j].load(s.p + v);
+    }
+    float z[VEC * kTurn];
+#pragma unroll
+    for (int j = 0; j < kTurn; ++j) {
+      const int v = v0 + j * G * VEC;
+      const Words<VEC> x = e[j].words(), y = p[j].words();
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[j * VEC + i] = v < a.V ? x.x[i] + y.x[i] : neg_inf();
+      if constexpr (REST) {
+        const unsigned listed = v < a.V ? bits[v >> 5] >> (v & 31) & ((1u << VEC) - 1) : 0u;
+        if (listed) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (listed >> i & 1) z[j * VEC + i] = neg_inf();
+        }
+      }
     }
     others.add(z, scale2);
   }
   others.join(g, scale2);
-  RunningSum all = others;
+  RunningSum full = others;
   if constexpr (REST) {
     RunningSum mine;
     for (int k = tid; k < K; k += G) {
-      const int v = word[k];
-      bool first = v >= 0;
-      for (int j = 0; first && j < k; ++j) first = word[j] != v;
-      const float z[1] = {first ? to_f32(s.e[v]) + to_f32(s.p[v]) : neg_inf()};
+      const float z[1] = {record[k].share != kNoShare ? record[k].z : neg_inf()};
       mine.add(z, scale2);
     }
     mine.join(g, scale2);
-    all.add(mine, scale2);
+    full.add(mine, scale2);
   }
-  const float all2 = all.log2sum(all.m, scale2), other2 = others.log2sum(all.m, scale2);
+  const float all2 = full.log2sum(full.m, scale2), other2 = others.log2sum(full.m, scale2);
+  // what of the gradient a listed word shares with the others
+  float logRatio = neg_inf();   // of r to the student's weight of the others
+  if (REST && r > 0.0f && other2 != neg_inf()) logRatio = logf(r) - (other2 - all2) * kLn2;
+  const bool apart = logRatio > kLn2;   // (more than 2: listed words would be differences of large numbers)
+  const float ratio = apart ? 0.0f : expf(logRatio);
   float cost = 0.0f;
   for (int k = tid; k < K; k += G) {
-    const int v = word[k];
-    float mass = 0.0f;
-    bool first = v >= 0;
-    if (first)
-      for (int j = 0; j < K; ++j)
-        if (word[j] == v) {
-          first = first && j >= k;
-          mass += share[j];
-        }
-    const float qk = mass * one;
-    if (!first || qk == 0.0f) continue;
-    const float z = to_f32(s.e[v]) + to_f32(s.p[v]);
-    cost += qk * (logf(qk) - (z == neg_inf() ? z : ((z - all.m) * scale2 - all2) * kLn2));
+    const float q = record[k].share, z = record[k].z;
+    const float logP = z == neg_inf() ? z : ((z - full.m) * scale2 - all2) * kLn2;
+    if (q != kNoShare && q != 0.0f) cost += q * (logf(q) - logP);
+    if (savedShare) savedShare[k] = q == kNoShare ? q : q - ratio * (z == neg_inf() ? 0.0f : expf(logP));
   }
   cost = g.sum(cost);
   if (tid != 0) return;
   if (REST && r != 0.0f) cost += r * (logf(r) - (other2 == neg_inf() ? other2 : (other2 - all2) * kLn2));
   costs[node] = cost;
-  if (!q) return;
+  if (!savedShare) return;
   // (an empty record has no gradient, and a student without any word left has p = 0)
   const float L = empty || all2 == neg_inf() ? pos_inf() : all2;
   float A = L, sign = 1.0f;
-  if (REST && r > 0.0f && other2 != neg_inf()) {
-    const float d = logf(r) - (other2 - all2) * kLn2;   // log(r / rho)
-    sign = d > 0.0f ? -1.0f : 1.0f;
-    A = L - (fmaxf(d, 0.0f) + log1pf(-expf(-fabsf(d)))) * kLog2e;
+  if (logRatio != neg_inf()) {
+    sign = apart ? -2.0f : logRatio > 0.0f ? -1.0f : 1.0f;
+    A = L - (fmaxf(logRatio, 0.0f) + log1pf(-expf(-fabsf(logRatio)))) * kLog2e;
   }
-  saved.node[node] = make_float4(all.m, L, A, sign);
+  saved.node[node] = make_float4(full.m, A, sign, L);
 }
 
 template <typename F>
@@ -226,15 +252,15 @@ void launch_distill_forward(const NodeArgs& a, const int* words, const float* lo
       auto launch = [&](auto group) {
         constexpr int G = group, rows = kCta<G> / G;
         auto kernel = distill_forward_kernel<TIn, vec, G, has_rest>;
-        const int smem = has_rest ? rows * div_up(a.V, 32) * 4 : 0;
-        if (smem > 48 * 1024) allow_dyn_smem(kernel, kDistillMaxBits / 8);
+        const int smem = rows * (K * (int)sizeof(Listed) + (has_rest ? div_up(a.V, 32) * 4 : 0));
+        if (smem > 40 * 1024) allow_dyn_smem(kernel, kForwardBytes);
         ScopedKernel prof("distill_forward", stream);
         kernel<<<(unsigned)div_up64(nodes, rows), kCta<G>, smem, stream>>>(a, words, logits, rest, costs, saved,
                                                                          K, scale2);
         TB200_CHECK_LAUNCH();
       };
-      if (a.V <= 1024) launch(std::integral_constant<int, 32>{});
-      else if (a.V <= 4096) launch(std::integral_constant<int, 128>{});
+      // a warp per node where there are warps enough to fill the chip and their shared memory is small
+      if (a.V <= 1024 || (nodes >= 148 * 16 && a.V <= 65536)) launch(std::integral_constant<int, 32>{});
       else launch(std::integral_constant<int, 256>{});
     });
   });

@@ -1,5 +1,6 @@
 // Gradients of the distillation costs (node_distill.cu has the formulas): sums over the nodes on each
-// frame, and on each position, of w (p_v - q_v) for listed words and w sign 2^(x - A) for the others.
+// frame, and on each position, of w sign 2^(x - A), x = (z - m) log2e / temperature, less w share for
+// listed words (DistillSaved).
 //
 // A warp has a tile of 32 * COLS words and goes through nodes in their order, so that sums have the same
 // bits from run to run.  Two ways:
@@ -18,14 +19,9 @@
 namespace tb200 {
 namespace {
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-constexpr int kWarps = 8;         // per CTA
-constexpr int kTarget = 148 * 24;  // warps that fill the chip
+constexpr int kWarps = 4;       // per CTA
+constexpr int kPathWarps = 2;   // of the path kernel
+constexpr int kTarget = 148 * 60;  // warps that fill the chip
 constexpr int kLookBack = 64;      // places without a node that a path may have between two nodes
 
 struct GradArgs {
@@ -38,7 +34,8 @@ struct GradArgs {
   int2* spans;        // of the B * T frames, then the B * U positions: (N - first node, last node + 1), or 0
   int* offPath;       // [B] 1: the nodes are not a path
   int* segUsed;       // [B, segs] 1: a segment has nodes
-  float* partial;     // of paths [B, segs, 2, V], or of other nodes [splits, rows, V] of E, then of P
+  float* partial;     // of paths [B, segs, 2, V]
+  float* rowPartial;  // of other nodes [splits, rows, V] of E, then of P
   int segFrames, segs, tiles, eSplits, pSplits;
 };
 
@@ -61,162 +58,240 @@ __global__ void __launch_bounds__(256) node_spans_kernel(NodeArgs a, GradArgs k)
   k.segUsed[b * k.segs + t / k.segFrames] = 1;
   int back = 1;
   while (back <= n && back <= kLookBack && !valid(node - back)) ++back;
-  if (back > n) return;
+  if (back > n) return;   // (the first node)
   if (back > kLookBack || a.frames[node - back] > t || a.positions[node - back] > u) k.offPath[b] = 1;
 }
 
-// A warp's tile: 32 * COLS words in vectors of VEC, lane by lane.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from),
+               "n"(BYTES)
+               : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// A warp's tile: 32 * COLS words, vector j of a lane being the words (j * 32 + lane) * VEC and on.
 template <typename TIn, int VEC, int COLS>
 struct Tile {
   static constexpr int NV = COLS / VEC;
+  using Row = RawWords<TIn, VEC>[NV];
   int first, V, lane;
-  __device__ __forceinline__ int word(int j) const { return first + (j * 32 + lane) * VEC; }
-  __device__ __forceinline__ void load(const TIn* row, float (&x)[COLS]) const {
+  __device__ __forceinline__ int place(int j) const { return (j * 32 + lane) * VEC; }   // in the tile
+  __device__ __forceinline__ bool in(int j) const { return first + place(j) < V; }
+  __device__ __forceinline__ void load(const TIn* row, Row& x) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      Words<VEC> q;
+      x[j].clear();
+      if (in(j)) x[j].load(row + first + place(j));
+    }
+  }
+  // to shared memory: each lane its own words
+  __device__ __forceinline__ void fetch(const TIn* row, TIn* slot) const {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) q.x[i] = 0.0f;
-      if (word(j) < V) q = load_words<VEC>(row + word(j));
+    for (int j = 0; j < NV; ++j)
+      if (in(j)) {
+        if constexpr (VEC * sizeof(TIn) >= 4) copy_async<VEC * sizeof(TIn)>(slot + place(j), row + first + place(j));
+        else slot[place(j)] = row[first + place(j)];   // (too small for an asynchronous copy)
+      }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int j, const float* x) const {   // vector j
+    if (!in(j)) return;
+    if constexpr (std::is_same<T, TIn>::value) {
+      store_words<VEC>(row + first + place(j), x);
+    } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[j * VEC + i] = q.x[i];
+      for (int i = 0; i < VEC; ++i) row[first + place(j) + i] = x[i];
     }
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, const float (&x)[COLS]) const {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (word(j) < V) {
-        if constexpr (std::is_same<T, TIn>::value) {
-          store_words<VEC>(row + word(j), x + j * VEC);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) row[word(j) + i] = x[j * VEC + i];
-        }
-      }
+    for (int j = 0; j < NV; ++j) store(row, j, x + j * VEC);
   }
 };
 
-// The listed words' shares are subtracted in shared memory (`sub`, a number per word of the tile in the order
-// of memory), by the lanes that read the record, and join the sums when a row is finished.
-template <int VEC, int COLS>
-__device__ __forceinline__ void take_shares(float* sub, int lane, float (&acc)[COLS]) {
+// VEC floats of shared memory.
+template <int VEC>
+__device__ __forceinline__ void read_floats(const float* p, float (&x)[VEC]) {
 #pragma unroll
-  for (int j = 0; j < COLS / VEC; ++j) {
-    float* p = sub + (j * 32 + lane) * VEC;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      acc[j * VEC + i] += p[i];
-      p[i] = 0.0f;
-    }
-  }
-  __syncwarp();
-}
-
-// sums += the node's gradients, for one or both sides.
-template <int VEC, int COLS, bool REST, bool BOTH>
-__device__ __forceinline__ void add_node(const float (&e)[COLS], const float (&p)[COLS], float4 of, float w,
-                                         float scale2, unsigned listed, float (&accA)[COLS], float (&accB)[COLS]) {
-  const float ws = w * of.w;
-#pragma unroll
-  for (int i = 0; i < COLS; ++i) {
-    const float z = e[i] + p[i] - of.x;
-    float g;
-    if constexpr (REST) {
-      const bool in = listed >> i & 1;
-      g = (in ? w : ws) * ex2(fmaf(z, scale2, in ? -of.y : -of.z));
+  for (int i = 0; i < VEC; i += VEC > 1 ? 4 : 1) {
+    if constexpr (VEC > 1) {
+      const float4 q = *reinterpret_cast<const float4*>(p + i);
+      x[i] = q.x, x[i + 1] = q.y, x[i + 2] = q.z, x[i + 3] = q.w;
     } else {
-      g = w * ex2(fmaf(z, scale2, -of.y));
+      x[i] = p[i];
     }
-    accA[i] += g;
-    if constexpr (BOTH) accB[i] += g;
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void write_floats(float* p, const float (&x)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i += VEC > 1 ? 4 : 1) {
+    if constexpr (VEC > 1) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    else p[i] = x[i];
   }
 }
 
-// The listed words of a node that lie in the tile: subtracted from subA (and subB), marked in `marks`.
-template <int VEC, int COLS, bool REST, bool BOTH>
-__device__ __forceinline__ unsigned add_record(const GradArgs& k, i64 node, float w, int tileFirst, int lane,
-                                               float* subA, float* subB, unsigned* marks) {
-  bool any = false;
-  for (int k0 = 0; k0 < k.K; k0 += 32) {
-    int v = -1;
-    float q = -1.0f;
-    if (k0 + lane < k.K) {
-      v = k.words[node * k.K + k0 + lane] - tileFirst;
-      q = k.saved.q[node * k.K + k0 + lane];
-    }
-    const bool hit = (unsigned)v < (unsigned)(32 * COLS) && !(q < 0.0f);
-    if (hit) {
-      subA[v] -= w * q;
-      if (BOTH) subB[v] -= w * q;
-      if (REST) atomicOr(&marks[v / VEC % 32], 1u << (v / (32 * VEC) * VEC + v % VEC));
-    }
-    any |= hit;
+// What is saved of a node, made ready for its words' gradients.
+struct Terms {
+  float m, A, L, w, ws, scale2;
+  bool apart;   // the listed words have a normaliser of their own
+  __device__ __forceinline__ Terms(float4 of, float weight, const GradArgs& k)
+      : m(of.x), A(of.y), L(of.w), w(weight * k.scale), ws(of.z > 0.0f ? w : -w), scale2(k.scale2),
+        apart(fabsf(of.z) > 1.5f) {}
+  __device__ __forceinline__ float others(float z) const { return ws * ex2(fmaf(z - m, scale2, -A)); }
+  __device__ __forceinline__ float word(float z, bool listed) const {
+    return listed ? w * ex2(fmaf(z - m, scale2, -L)) : others(z);
   }
-  unsigned mine = 0;
-  if (REST && __any_sync(0xffffffffu, any)) {
-    __syncwarp();
-    mine = marks[lane];
-    marks[lane] = 0;
+  // gradients of a vector; bit i of `listed`: whether word i is (of use where it is a case apart)
+  template <int VEC>
+  __device__ __forceinline__ void vector(const Words<VEC>& e, const Words<VEC>& p, unsigned listed,
+                                         float (&g)[VEC]) const {
+    if (!apart) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[i] = others(e.x[i] + p.x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[i] = word(e.x[i] + p.x[i], listed >> i & 1);
+    }
+  }
+};
+
+// A node's number, and 32 words of its record, one in each lane.
+struct Record {
+  i64 node;
+  int v;
+  float share;
+  __device__ __forceinline__ void load(const GradArgs& k, i64 node_, int from, int lane) {
+    node = node_;
+    v = -1;
+    share = kNoShare;
+    if (from + lane < k.K) {
+      v = k.words[node * k.K + from + lane];
+      share = k.saved.share[node * k.K + from + lane];
+    }
+  }
+  // whether the lane's word is one of the tile's, and its place there
+  template <int WORDS>
+  __device__ __forceinline__ bool hits(int tileFirst, int& at) const {
+    at = v - tileFirst;
+    return v >= 0 && (unsigned)at < (unsigned)WORDS && share != kNoShare;
+  }
+};
+
+// The listed words of a node that lie in the tile: their shares are subtracted in shared memory, `sub`, by the lanes
+// that read the record; each lane gets a bit for each of its own words.
+template <int VEC, int COLS>
+__device__ __forceinline__ unsigned add_record(const GradArgs& k, Record r, float w, int tileFirst, int lane, float* sub,
+                                               unsigned* marks) {
+  for (int k0 = 0;;) {
+    int at;
+    if (r.hits<32 * COLS>(tileFirst, at)) {
+      sub[at] -= w * r.share;
+      atomicOr(&marks[at / VEC % 32], 1u << (at / (32 * VEC) * VEC + at % VEC));
+    }
+    k0 += 32;
+    if (k0 >= k.K) break;
+    r.load(k, r.node, k0, lane);
   }
   __syncwarp();
+  const unsigned mine = marks[lane];
+  if (mine) marks[lane] = 0;
   return mine;
 }
+// The same for sums in registers, for few nodes.
+template <int VEC, int COLS>
+__device__ __forceinline__ void add_record_to(const GradArgs& k, Record r, float w, int tileFirst, int lane,
+                                              float (&acc)[COLS]) {
+  for (int k0 = 0;;) {
+    int at;
+    unsigned todo = __ballot_sync(0xffffffffu, r.hits<32 * COLS>(tileFirst, at));
+#pragma unroll 1
+    for (; todo; todo &= todo - 1) {
+      const int i = __ffs(todo) - 1, place = __shfl_sync(0xffffffffu, at, i);
+      const float share = w * __shfl_sync(0xffffffffu, r.share, i);
+      const int slot = place / VEC % 32 == lane ? place / (32 * VEC) * VEC + place % VEC : -1;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+        if (c == slot) acc[c] -= share;
+    }
+    k0 += 32;
+    if (k0 >= k.K) break;
+    r.load(k, r.node, k0, lane);
+  }
+}
 
-template <typename TIn, int VEC, int COLS, bool REST>
-__global__ void __launch_bounds__(kWarps * 32) distill_path_kernel(NodeArgs a, GradArgs k) {
-  __shared__ __align__(16) float subAll[kWarps][2][32 * COLS];
-  __shared__ unsigned marksAll[kWarps][32];
+// A node as its warp comes to it.
+struct Step {
+  float4 of;
+  float weight;
+  int t, u, n;
+};
+constexpr int kSteps = 64;    // in shared memory
+constexpr int kAhead = 2;     // rows of E that are on their way
+template <typename TIn, int COLS>
+struct __align__(16) PathMemory {   // of a warp
+  TIn rows[kAhead + 1][32 * COLS];
+  float sub[32 * COLS];
+  Step steps[kSteps];
+  unsigned marks[32];
+};
+// Words per lane: 64 bytes of a row (two rows of sums and one of P in registers for bf16 would be too many).
+template <typename TIn>
+constexpr int kCols = sizeof(TIn) == 2 ? 24 : 16;
+
+// Per node and 64 bytes of a lane's row about 9 instructions a word and 130 besides.  The sums for P are in registers;
+// a frame's gradients are written when its last node comes by, and wait in `sub` until then.
+template <typename TIn, int VEC>
+__global__ void __launch_bounds__(kPathWarps * 32, 8) distill_path_kernel(NodeArgs a, GradArgs k) {
+  constexpr int COLS = kCols<TIn>, NV = COLS / VEC;
+  extern __shared__ __align__(16) unsigned char memory[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float *subE = subAll[warp][0], *subP = subAll[warp][1];
-  unsigned* marks = marksAll[warp];
-  const i64 task = (i64)blockIdx.x * kWarps + warp;
+  auto& mem = reinterpret_cast<PathMemory<TIn, COLS>*>(memory)[warp];
+  const i64 task = (i64)blockIdx.x * kPathWarps + warp;
   const i64 bs = task / k.tiles;
   const int b = (int)(bs / k.segs), seg = (int)(bs - (i64)b * k.segs);
   if (b >= a.B || k.offPath[b]) return;
-  for (int i = lane; i < 32 * COLS; i += 32) subE[i] = subP[i] = 0.0f;
-  marks[lane] = 0;
+  for (int i = lane; i < 32 * COLS; i += 32) mem.sub[i] = 0.0f;
+  mem.marks[lane] = 0;
   __syncwarp();
-  const Tile<TIn, VEC, COLS> tile{(int)(task - bs * k.tiles) * 32 * COLS, a.V, lane};
+  using T = Tile<TIn, VEC, COLS>;
+  const T tile{(int)(task - bs * k.tiles) * 32 * COLS, a.V, lane};
   const int t0 = seg * k.segFrames, t1 = min(t0 + k.segFrames, a.T);
   const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
   const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
   TIn* dE = k.egrads ? static_cast<TIn*>(k.egrads) + (i64)b * a.T * a.V : nullptr;
   TIn* dP = k.pgrads ? static_cast<TIn*>(k.pgrads) + (i64)b * a.U * a.V : nullptr;
-  const int2* frameSpans = k.spans + (i64)b * a.T;
-  const int2* posSpans = k.spans + (i64)a.B * a.T + (i64)b * a.U;
-  const int* frames = a.frames + (i64)b * a.N;
-  const int* positions = a.positions + (i64)b * a.N;
   // the segment's nodes
   int n0 = 0x7fffffff, n1 = 0;
   for (int t = t0 + lane; t < t1; t += 32) {
-    const int2 s = frameSpans[t];
+    const int2 s = k.spans[(i64)b * a.T + t];
     if (s.y > 0) n0 = min(n0, a.N - s.x), n1 = max(n1, s.y);
   }
   n0 = __reduce_min_sync(0xffffffffu, n0);
   n1 = __reduce_max_sync(0xffffffffu, n1);
-  float e[COLS], p[COLS], accE[COLS], accP[COLS];
+  if (n1 == 0) n0 = 0;   // (none: nothing is read below)
+  typename T::Row p;
+  float accP[COLS];
 #pragma unroll
-  for (int i = 0; i < COLS; ++i) accE[i] = accP[i] = 0.0f;
-  int curT = -1, curU = -1, nextRow = t0;   // frames below nextRow are written
-  auto finish_frame = [&] {   // writes the current frame, and zeros for those before it that have no nodes
-    take_shares<VEC>(subE, lane, accE);
-    if (dE) tile.store(dE + (i64)curT * a.V, accE);
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) accE[i] = 0.0f;
-    nextRow = curT + 1;
-  };
-  auto zeros_to = [&](int t) {
-    float zero[COLS];
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) zero[i] = 0.0f;
+  for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
+  int curU = -1, nextRow = t0;   // frames below nextRow are written
+  auto zeros_to = [&](int t) {   // zeros for the frames without nodes before t
+    const float zero[VEC] = {};
     for (; nextRow < t; ++nextRow)
-      if (dE) tile.store(dE + (i64)nextRow * a.V, zero);
+      if (dE)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) tile.store(dE + (i64)nextRow * a.V, j, zero);
   };
   auto finish_position = [&] {
-    take_shares<VEC>(subP, lane, accP);
     if (dP) {
-      const int2 s = posSpans[curU];
+      const int2 s = k.spans[(i64)a.B * a.T + (i64)b * a.U + curU];
+      const int* frames = a.frames + (i64)b * a.N;
       const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
       if (from == to) tile.store(dP + (i64)curU * a.V, accP);
       else tile.store(k.partial + (((i64)b * k.segs + seg) * 2 + (from == seg ? 1 : 0)) * a.V, accP);
@@ -224,57 +299,145 @@ __global__ void __launch_bounds__(kWarps * 32) distill_path_kernel(NodeArgs a, G
 #pragma unroll
     for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
   };
-  for (int nb = n0; nb < n1; nb += 32) {
-    const int n = nb + lane;
-    int t = -1, u = -1;
-    float4 of = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float w = 0.0f;
-    if (n < n1) {
-      t = frames[n], u = positions[n];
-      if ((unsigned)t >= (unsigned)a.T || (unsigned)u >= (unsigned)a.U) t = -1;
-      of = k.saved.node[(i64)b * a.N + n];
-      w = k.weights[(i64)b * a.N + n] * k.scale;
-    }
-    unsigned todo = __ballot_sync(0xffffffffu, t >= 0);
-    while (todo) {
-      const int bit = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const int nt = __shfl_sync(0xffffffffu, t, bit), nu = __shfl_sync(0xffffffffu, u, bit);
-      if (nt != curT) {
-        if (curT >= 0) finish_frame();
-        zeros_to(nt);
-        curT = nt;
-        tile.load(E + nt * a.eStrideT, e);
+  // The steps: appended 32 places at a time, rows fetched kAhead steps ahead; a group of copies per step.
+  int appended = 0, base = n0, written = 0;
+  auto append_to = [&](int want) {
+    while (appended < want && base < n1) {
+      Step x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -1, -1, base + lane};
+      if (x.n < n1) {
+        const i64 node = (i64)b * a.N + x.n;
+        x.t = a.frames[node], x.u = a.positions[node];
+        x.of = k.saved.node[node];
+        x.weight = k.weights[node];
       }
-      if (nu != curU) {
-        if (curU >= 0) finish_position();
-        curU = nu;
-        tile.load(P + nu * a.pStrideU, p);
-      }
-      float4 f;
-      f.x = __shfl_sync(0xffffffffu, of.x, bit);
-      f.y = __shfl_sync(0xffffffffu, of.y, bit);
-      f.z = __shfl_sync(0xffffffffu, of.z, bit);
-      f.w = __shfl_sync(0xffffffffu, of.w, bit);
-      const float fw = __shfl_sync(0xffffffffu, w, bit);
-      const unsigned listed =
-          add_record<VEC, COLS, REST, true>(k, (i64)b * a.N + nb + bit, fw, tile.first, lane, subE, subP, marks);
-      add_node<VEC, COLS, REST, true>(e, p, f, fw, k.scale2, listed, accE, accP);
+      const bool here = (unsigned)x.t < (unsigned)a.T && (unsigned)x.u < (unsigned)a.U;
+      const unsigned all = __ballot_sync(0xffffffffu, here);
+      if (here) mem.steps[(appended + __popc(all & ((1u << lane) - 1))) % kSteps] = x;
+      appended += __popc(all);
+      base += 32;
+      __syncwarp();
     }
+  };
+  auto fetch_row = [&](int i) {   // of step i, if it is another than the one before
+    if (i < appended) {
+      const int t = mem.steps[i % kSteps].t;
+      if (i == 0 || mem.steps[(i - 1) % kSteps].t != t) {
+        tile.fetch(E + t * a.eStrideT, mem.rows[written]);
+        written = written == kAhead ? 0 : written + 1;
+      }
+    }
+    commit_copies();
+  };
+  append_to(kAhead + 1);
+  for (int i = 0; i < kAhead; ++i) fetch_row(i);
+  Record record;
+  if (appended > 0) record.load(k, (i64)b * a.N + mem.steps[0].n, 0, lane);
+  int slot = kAhead, curT = -1;
+  for (int i = 0; i < appended; ++i) {
+    append_to(i + kAhead + 1);
+    fetch_row(i + kAhead);
+    const Record mine = record;
+    const Step step = mem.steps[i % kSteps];
+    int nextT = -1;
+    if (i + 1 < appended) {
+      record.load(k, (i64)b * a.N + mem.steps[(i + 1) % kSteps].n, 0, lane);
+      nextT = mem.steps[(i + 1) % kSteps].t;
+    }
+    const bool more = step.t == nextT, alone = !more && step.t != curT;   // nodes of the frame to come; none but this
+    if (step.t != curT) {
+      curT = step.t;
+      slot = slot == kAhead ? 0 : slot + 1;
+      zeros_to(curT);
+      nextRow = curT + 1;
+    }
+    if (step.u != curU) {
+      if (curU >= 0) finish_position();
+      curU = step.u;
+      tile.load(P + curU * a.pStrideU, p);
+    }
+    const Terms terms(step.of, step.weight, k);
+    const unsigned listed = add_record<VEC, COLS>(k, mine, terms.w, tile.first, lane, mem.sub, mem.marks);
+    if (!alone) add_record_to<VEC, COLS>(k, mine, terms.w, tile.first, lane, accP);
+    __syncwarp();
+    wait_copies<kAhead>();
+    TIn* out = dE ? dE + (i64)curT * a.V : nullptr;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      RawWords<TIn, VEC> e;
+      e.clear();
+      if (tile.in(j)) e.load(&mem.rows[slot][tile.place(j)]);
+      float* sub = &mem.sub[tile.place(j)];
+      const unsigned here = listed >> (j * VEC) & ((1u << VEC) - 1);
+      float g[VEC];
+      terms.vector(e.words(), p[j].words(), here, g);
+      if (alone) {
+        if (here) {   // the shares join the gradient, of both sides
+          float s[VEC];
+          const float zero[VEC] = {};
+          read_floats<VEC>(sub, s);
+          write_floats<VEC>(sub, zero);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) g[i] += s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) accP[j * VEC + i] += g[i];
+        if (out) tile.store(out, j, g);
+      } else {
+        float s[VEC];
+        const float zero[VEC] = {};
+        read_floats<VEC>(sub, s);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          accP[j * VEC + i] += g[i];
+          s[i] += g[i];
+        }
+        if (more) {
+          write_floats<VEC>(sub, s);
+        } else {
+          write_floats<VEC>(sub, zero);
+          if (out) tile.store(out, j, s);
+        }
+      }
+    }
+    __syncwarp();
   }
-  if (curT >= 0) finish_frame();
   zeros_to(t1);
   if (curU >= 0) finish_position();
 }
 
+// 32 places of an utterance's nodes in a warp's shared memory.
+struct Batch {
+  float4 of[32];     // DistillSaved::node
+  float weight[32];
+  int t[32], u[32];
+  // lane by lane; places from `end` on have no node
+  __device__ __forceinline__ void fetch(const NodeArgs& a, const GradArgs& k, int b, int base, int end, int lane) {
+    const i64 node = (i64)b * a.N + base + lane;
+    if (base + lane < end) {
+      copy_async<16>(&of[lane], k.saved.node + node);
+      copy_async<4>(&weight[lane], k.weights + node);
+      copy_async<4>(&t[lane], a.frames + node);
+      copy_async<4>(&u[lane], a.positions + node);
+    } else {
+      t[lane] = -1;
+    }
+  }
+  __device__ __forceinline__ bool here(const NodeArgs& a, int lane) const {
+    return (unsigned)t[lane] < (unsigned)a.T && (unsigned)u[lane] < (unsigned)a.U;
+  }
+};
+
 // Rows of either gradient of utterances whose nodes are not a path.  Tasks: (row, split, tile) of E, then of P.
-template <typename TIn, int VEC, int COLS, bool REST>
-__global__ void __launch_bounds__(kWarps * 32) distill_rows_kernel(NodeArgs a, GradArgs k) {
+template <typename TIn, int VEC>
+__global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a, GradArgs k) {
+  constexpr int COLS = kCols<TIn>, NV = COLS / VEC;
   __shared__ __align__(16) float subAll[kWarps][32 * COLS];
   __shared__ unsigned marksAll[kWarps][32];
+  __shared__ Batch batchAll[kWarps][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* sub = subAll[warp];
   unsigned* marks = marksAll[warp];
+  Batch* const batch = batchAll[warp];
   for (int i = lane; i < 32 * COLS; i += 32) sub[i] = 0.0f;
   marks[lane] = 0;
   __syncwarp();
@@ -289,116 +452,168 @@ __global__ void __launch_bounds__(kWarps * 32) distill_rows_kernel(NodeArgs a, G
       const int splits = ofFrames ? k.eSplits : k.pSplits;
       const int own = (int)(r / (splits * k.tiles)), rem = (int)(r - (i64)own * splits * k.tiles);
       const int split = rem / k.tiles;
-      const Tile<TIn, VEC, COLS> tile{(rem - split * k.tiles) * 32 * COLS, a.V, lane};
+      using T = Tile<TIn, VEC, COLS>;
+      const T tile{(rem - split * k.tiles) * 32 * COLS, a.V, lane};
       const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
       const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
       const int2 span = k.spans[ofFrames ? (i64)b * a.T + own : (i64)a.B * a.T + (i64)b * a.U + own];
-      const int* ownIdx = (ofFrames ? a.frames : a.positions) + (i64)b * a.N;
-      const int* otherIdx = (ofFrames ? a.positions : a.frames) + (i64)b * a.N;
-      const unsigned others = ofFrames ? a.U : a.T;
       const TIn* otherRows = ofFrames ? P : E;
       const i64 otherStride = ofFrames ? a.pStrideU : a.eStrideT;
-      float mine[COLS], acc[COLS];
+      typename T::Row mine, theirs, next;
+      float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
       const int first = a.N - span.x, count = span.y > 0 ? span.y - first : 0;
       const int n0 = first + (int)((i64)count * split / splits), n1 = first + (int)((i64)count * (split + 1) / splits);
       if (n0 < n1) tile.load(ofFrames ? E + own * a.eStrideT : P + own * a.pStrideU, mine);
-      for (int nb = n0; nb < n1; nb += 32) {
-        const int n = nb + lane;
-        int o = -1;
-        float4 of = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float w = 0.0f;
-        if (n < n1 && ownIdx[n] == own) {
-          o = otherIdx[n];
-          of = k.saved.node[(i64)b * a.N + n];
-          w = k.weights[(i64)b * a.N + n] * k.scale;
+      // the next node's row and record are on their way while a node is added up
+      Record record;
+      auto fetch = [&](const Batch& x, int base, int at) {
+        tile.load(otherRows + (ofFrames ? x.u[at] : x.t[at]) * otherStride, next);
+        record.load(k, (i64)b * a.N + base + at, 0, lane);
+      };
+      auto advance = [&](Batch& x, int& base) {   // to the next 32 places from `base` on with a node of this row
+        for (;; base += 32) {
+          x.fetch(a, k, b, base, n1, lane);
+          commit_copies();
+          wait_copies<0>();
+          __syncwarp();
+          const unsigned some =
+              __ballot_sync(0xffffffffu, x.here(a, lane) && (ofFrames ? x.t[lane] : x.u[lane]) == own);
+          if (some || base + 32 >= n1) return some;
+          __syncwarp();
         }
-        unsigned todo = __ballot_sync(0xffffffffu, (unsigned)o < others);
+      };
+      int now = 0, base = n0, baseThen;
+      unsigned todo = n0 < n1 ? advance(batch[0], base) : 0, todoThen = 0;
+      if (todo) fetch(batch[0], base, __ffs(todo) - 1);
+      for (; todo; now ^= 1, base = baseThen, todo = todoThen) {
+        const Batch& here = batch[now];
+        Batch& then = batch[now ^ 1];
+        baseThen = base + 32;
+        todoThen = baseThen < n1 ? advance(then, baseThen) : 0;
         while (todo) {
           const int bit = __ffs(todo) - 1;
           todo &= todo - 1;
-          float theirs[COLS];
-          tile.load(otherRows + __shfl_sync(0xffffffffu, o, bit) * otherStride, theirs);
-          float4 f;
-          f.x = __shfl_sync(0xffffffffu, of.x, bit);
-          f.y = __shfl_sync(0xffffffffu, of.y, bit);
-          f.z = __shfl_sync(0xffffffffu, of.z, bit);
-          f.w = __shfl_sync(0xffffffffu, of.w, bit);
-          const float fw = __shfl_sync(0xffffffffu, w, bit);
-          const unsigned listed =
-              add_record<VEC, COLS, REST, false>(k, (i64)b * a.N + nb + bit, fw, tile.first, lane, sub, sub, marks);
-          add_node<VEC, COLS, REST, false>(mine, theirs, f, fw, k.scale2, listed, acc, acc);
+          const Record theirRecord = record;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) theirs[j] = next[j];
+          if (todo) fetch(here, base, __ffs(todo) - 1);
+          else if (todoThen) fetch(then, baseThen, __ffs(todoThen) - 1);
+          const Terms terms(here.of[bit], here.weight[bit], k);
+          const unsigned listed = add_record<VEC, COLS>(k, theirRecord, terms.w, tile.first, lane, sub, marks);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            float g[VEC];
+            terms.vector(theirs[j].words(), mine[j].words(), listed >> (j * VEC), g);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[j * VEC + i] += g[i];
+          }
+          __syncwarp();
         }
+        __syncwarp();   // (everybody is done with `here`, which is filled next)
       }
-      take_shares<VEC>(sub, lane, acc);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {   // the shares
+        float s[VEC];
+        const float zero[VEC] = {};
+        read_floats<VEC>(sub + tile.place(j), s);
+        write_floats<VEC>(sub + tile.place(j), zero);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[j * VEC + i] += s[i];
+      }
+      __syncwarp();
       const i64 row = ofFrames ? (i64)b * a.T + own : (i64)b * a.U + own;
       if (splits == 1) {
         tile.store(static_cast<TIn*>(ofFrames ? k.egrads : k.pgrads) + row * a.V, acc);
       } else {
         const i64 rows = (i64)a.B * (ofFrames ? a.T : a.U);
-        float* part = k.partial + (ofFrames || k.eSplits == 1 ? 0 : (i64)k.eSplits * a.B * a.T * a.V);
+        float* part = k.rowPartial + (ofFrames || k.eSplits == 1 ? 0 : (i64)k.eSplits * a.B * a.T * a.V);
         tile.store(part + (split * rows + row) * a.V, acc);
       }
     }
   }
 }
 
-// Rows that are added up from partial ones, and rows of P without nodes on a path.  One CTA per row.
+// Rows that are added up from partial ones, and rows of P without nodes on a path.  A warp looks at `group` rows
+// (up to 32), one in each lane, and adds up 128 words of those that ask for it.
+constexpr int kJoinWords = 128;
 template <typename TIn>
-__global__ void __launch_bounds__(256) distill_join_kernel(NodeArgs a, GradArgs k, int eRows) {
-  i64 row = blockIdx.x;
+__global__ void __launch_bounds__(kWarps * 32) distill_join_kernel(NodeArgs a, GradArgs k, int eRows, int rows,
+                                                                   int group, int chunks) {
+  const int lane = threadIdx.x & 31;
+  const i64 task = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int first = (int)(task / chunks) * group, chunk = (int)(task - (task / chunks) * chunks);
+  if (first >= rows) return;
+  // this lane's row: where its partial rows are, and how many (-1: it is written already)
+  int row = first + lane, count = -1;
   const bool ofFrames = row < eRows;
   if (!ofFrames) row -= eRows;
-  const int per = ofFrames ? a.T : a.U;
-  const int b = (int)(row / per);
-  const float* part = k.partial;
-  i64 stride = a.V;
-  int count = 0;
-  const int* used = nullptr;
-  if (k.offPath[b]) {
-    count = ofFrames ? k.eSplits : k.pSplits;
-    if (count == 1) return;
-    const i64 rows = (i64)a.B * per;
-    if (!ofFrames && k.eSplits > 1) part += (i64)k.eSplits * a.B * a.T * a.V;
-    part += row * a.V;
-    stride = rows * a.V;
-  } else {
-    if (ofFrames) return;
-    const int2 s = k.spans[(i64)a.B * a.T + row];
-    if (s.y > 0) {
-      const int* frames = a.frames + (i64)b * a.N;
-      const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
-      if (from == to) return;
-      // the part of the first segment is in its second place, the others' in their first
-      part += (((i64)b * k.segs + from) * 2 + 1) * a.V;
-      count = to - from + 1;
-      used = k.segUsed + (i64)b * k.segs + from;
-    }
-  }
-  TIn* out = static_cast<TIn*>(ofFrames ? k.egrads : k.pgrads) + row * a.V;
-  for (int v = threadIdx.x; v < a.V; v += 256) {
-    float sum = 0.0f;
-    for (int c = 0; c < count; ++c) {
-      if (used) {
-        if (used[c]) sum += part[c == 0 ? v : (2 * c - 1) * stride + v];
+  i64 at = 0, stride = 0;   // of k.partial, or (of nodes off a path) of k.rowPartial
+  int used = -1;            // first entry of segUsed
+  if (lane < group && first + lane < rows) {
+    const int per = ofFrames ? a.T : a.U;
+    const int b = row / per;
+    if (k.offPath[b]) {
+      const int splits = ofFrames ? k.eSplits : k.pSplits;
+      if (splits > 1) {
+        count = splits;
+        at = (!ofFrames && k.eSplits > 1 ? (i64)k.eSplits * a.B * a.T : 0) + row;
+        stride = (i64)a.B * per;
+      }
+    } else if (!ofFrames) {
+      const int2 s = k.spans[(i64)a.B * a.T + row];
+      if (s.y == 0) {
+        count = 0;
       } else {
-        sum += part[c * stride + v];
+        const int* frames = a.frames + (i64)b * a.N;
+        const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
+        if (from != to) {   // the part of the first segment is in its second place, the others' in their first
+          count = to - from + 1;
+          used = b * k.segs + from;
+          at = (i64)used * 2;
+          stride = 2;
+        }
       }
     }
-    from_f32(out[v], sum);
+  }
+  for (unsigned todo = __ballot_sync(0xffffffffu, count >= 0); todo; todo &= todo - 1) {
+    const int i = __ffs(todo) - 1;
+    const int n = __shfl_sync(0xffffffffu, count, i), u = __shfl_sync(0xffffffffu, used, i);
+    const i64 from = __shfl_sync(0xffffffffu, at, i), step = __shfl_sync(0xffffffffu, stride, i);
+    const bool e = __shfl_sync(0xffffffffu, ofFrames ? 1 : 0, i);
+    const i64 to = __shfl_sync(0xffffffffu, row, i);
+    const float* part = (u < 0 ? k.rowPartial : k.partial) + from * a.V;
+    float sum[kJoinWords / 32] = {};
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+      const float* p = part + (u >= 0 && c == 0 ? 1 : c * step) * a.V;
+      const bool there = u < 0 || k.segUsed[u + c];   // (a segment without nodes has left nothing)
+#pragma unroll
+      for (int j = 0; j < kJoinWords / 32; ++j) {
+        const int v = chunk * kJoinWords + j * 32 + lane;
+        if (v < a.V && there) sum[j] += p[v];
+      }
+    }
+    TIn* out = static_cast<TIn*>(e ? k.egrads : k.pgrads) + to * a.V;
+#pragma unroll
+    for (int j = 0; j < kJoinWords / 32; ++j) {
+      const int v = chunk * kJoinWords + j * 32 + lane;
+      if (v < a.V) from_f32(out[v], sum[j]);
+    }
   }
 }
 
-constexpr int kCols = 16, kLeastFrames = 16, kLeastNodes = 8;
+constexpr int kLeastFrames = 16, kLeastNodes = 8, kTileWords = 1024;   // (the largest tile)
 
 struct Plan {
   int tiles, segFrames, segs, eSplits, pSplits;
   size_t spanBytes;
 };
-Plan plan_of(int B, int T, int U, int V, int N) {
+Plan plan_of(int B, int T, int U, int V, int N, int dtype) {
   Plan p{};
-  p.tiles = div_up(V, 32 * kCols);
+  p.tiles = div_up(V, 32 * (dtype == kDtypeBf16 ? kCols<bf16> : kCols<float>));
   // segments of at least 16 frames, as many as fill the chip
   const i64 want = std::max<i64>(1, kTarget / std::max<i64>(1, (i64)B * p.tiles));
   p.segFrames = (int)std::max<i64>(kLeastFrames, div_up64(std::max(T, 1), want));
@@ -413,27 +628,31 @@ Plan plan_of(int B, int T, int U, int V, int N) {
   return p;
 }
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+// Of the paths' partial rows: the segments of all utterances are max(B, kTarget / tiles) at most, and a
+// tile is kTileWords words at most.  (A bound on what the plan takes, so that no smaller call needs more.)
+size_t path_floats(int B, int T, int V) {
+  const size_t leastSegs = div_up(std::max(T, 1), kLeastFrames);
+  return 2 * std::min(B * leastSegs * V, std::max((size_t)B * V, (size_t)kTarget * kTileWords));
+}
 
 }  // namespace
 
 size_t distill_backward_workspace_bytes(int B, int T, int U, int V, int N) {
   if (B <= 0 || T < 0 || U < 0 || V <= 0 || N < 0) return 0;
-  // Bounds on what the plan takes, so that no smaller call needs more than a larger one: the segments of all
-  // utterances are max(B, kTarget / tiles) at most and a tile is 32 * kCols words; the splits of a side
-  // fill kTarget tiles at most.
-  const size_t leastSegs = div_up(std::max(T, 1), kLeastFrames), full = (size_t)kTarget * 32 * kCols;
-  const size_t path = 2 * std::min(B * leastSegs * V, std::max((size_t)B * V, full));
+  // (the splits of a side fill kTarget tiles at most)
+  const size_t leastSegs = div_up(std::max(T, 1), kLeastFrames), full = (size_t)kTarget * kTileWords;
+  const size_t path = path_floats(B, T, V);
   const size_t rows = 2 * std::min((size_t)N / kLeastNodes * B * V, full);
   return round256(sizeof(int) * ((size_t)B * (2 * ((size_t)T + U) + 1 + leastSegs))) +
-         round256(sizeof(float) * std::max(path, rows));
+         round256(sizeof(float) * path) + round256(sizeof(float) * rows);
 }
 
 void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved saved, const float* weights,
-                             void* egrads, void* pgrads, int K, bool hasRest, double temperature,
+                             void* egrads, void* pgrads, int K, double temperature,
                              void* workspace, cudaStream_t stream) {
   const i64 frameRows = egrads ? (i64)a.B * a.T : 0, posRows = pgrads ? (i64)a.B * a.U : 0, nodes = (i64)a.B * a.N;
   if (frameRows + posRows == 0) return;
-  const Plan p = plan_of(a.B, a.T, a.U, a.V, a.N);
+  const Plan p = plan_of(a.B, a.T, a.U, a.V, a.N, a.dtype);
   GradArgs k{};
   k.words = words;
   k.saved = saved;
@@ -447,6 +666,7 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
   k.offPath = reinterpret_cast<int*>(k.spans + (i64)a.B * ((i64)a.T + a.U));
   k.segUsed = k.offPath + a.B;
   k.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(p.spanBytes));
+  k.rowPartial = k.partial + round256(sizeof(float) * path_floats(a.B, a.T, a.V)) / sizeof(float);
   k.segFrames = p.segFrames;
   k.segs = p.segs;
   k.tiles = p.tiles;
@@ -460,41 +680,41 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
   }
   const bool wide = node_rows_aligned(a) && reinterpret_cast<uintptr_t>(egrads) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(pgrads) % 16 == 0;
-  auto run = [&](auto type, auto vec, auto rest) {
+  auto run = [&](auto type, auto vec) {
     using TIn = decltype(type);
     constexpr int VEC = decltype(vec)::value;
-    constexpr bool REST = decltype(rest)::value;
     {
       ScopedKernel prof("distill_path", stream);
       const i64 tasks = (i64)a.B * p.segs * p.tiles;
-      distill_path_kernel<TIn, VEC, kCols, REST><<<(unsigned)div_up64(tasks, kWarps), kWarps * 32, 0, stream>>>(a, k);
+      constexpr int smem = kPathWarps * (int)sizeof(PathMemory<TIn, kCols<TIn>>);
+      allow_dyn_smem(distill_path_kernel<TIn, VEC>, smem);
+      distill_path_kernel<TIn, VEC><<<(unsigned)div_up64(tasks, kPathWarps), kPathWarps * 32, smem, stream>>>(a, k);
       TB200_CHECK_LAUNCH();
     }
     if (nodes > 1) {   // (a single node is a path)
       ScopedKernel prof("distill_rows", stream);
       const i64 tasks = ((i64)a.T * p.eSplits + (i64)a.U * p.pSplits) * p.tiles;
       const i64 ctas = std::min<i64>(div_up64(tasks, kWarps), 148 * 6);
-      distill_rows_kernel<TIn, VEC, kCols, REST><<<(unsigned)ctas, kWarps * 32, 0, stream>>>(a, k);
+      distill_rows_kernel<TIn, VEC><<<(unsigned)ctas, kWarps * 32, 0, stream>>>(a, k);
       TB200_CHECK_LAUNCH();
     }
     const i64 eRows = p.eSplits > 1 ? frameRows : 0;
     if (eRows + posRows > 0) {
       ScopedKernel prof("distill_join", stream);
-      distill_join_kernel<TIn><<<(unsigned)(eRows + posRows), 256, 0, stream>>>(a, k, (int)eRows);
+      const i64 rows = eRows + posRows, chunks = div_up(a.V, kJoinWords);
+      const i64 group = std::min<i64>(32, std::max<i64>(1, rows * chunks / 8192));
+      distill_join_kernel<TIn><<<(unsigned)div_up64(div_up64(rows, group) * chunks, kWarps), kWarps * 32, 0, stream>>>(
+          a, k, (int)eRows, (int)rows, (int)group, (int)chunks);
       TB200_CHECK_LAUNCH();
     }
   };
-  auto with_rest = [&](auto type, auto vec) {
-    if (hasRest) run(type, vec, std::true_type{});
-    else run(type, vec, std::false_type{});
-  };
   using std::integral_constant;
   if (a.dtype == kDtypeBf16) {
-    if (wide) with_rest(bf16{}, integral_constant<int, 8>{});
-    else with_rest(bf16{}, integral_constant<int, 1>{});
+    if (wide) run(bf16{}, integral_constant<int, 8>{});
+    else run(bf16{}, integral_constant<int, 1>{});
   } else {
-    if (wide) with_rest(float{}, integral_constant<int, 4>{});
-    else with_rest(float{}, integral_constant<int, 1>{});
+    if (wide) run(float{}, integral_constant<int, 4>{});
+    else run(float{}, integral_constant<int, 1>{});
   }
 }
 

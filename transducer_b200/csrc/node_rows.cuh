@@ -3,6 +3,8 @@
 // positions[b,n]; its scores are E[b,frame,v] + P[b,position,v], one addition in fp32.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -13,32 +15,37 @@ template <int VEC>
 struct Words {
   float x[VEC];
 };
-template <int VEC>
-__device__ __forceinline__ Words<VEC> load_words(const float* p) {
-  Words<VEC> w;
-  if constexpr (VEC == 4) {
-    const float4 r = *reinterpret_cast<const float4*>(p);
-    w.x[0] = r.x, w.x[1] = r.y, w.x[2] = r.z, w.x[3] = r.w;
-  } else {
-    w.x[0] = *p;
-  }
-  return w;
-}
-template <int VEC>
-__device__ __forceinline__ Words<VEC> load_words(const bf16* p) {
-  Words<VEC> w;
-  if constexpr (VEC == 8) {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
-    const unsigned u[4] = {r.x, r.y, r.z, r.w};
+// ... and in storage form, as they come.
+template <typename TIn, int VEC>
+struct RawWords {
+  static_assert(VEC == 1 || VEC * sizeof(TIn) == 16);
+  std::conditional_t<VEC == 1, TIn, uint4> bits;
+  __device__ __forceinline__ void load(const TIn* p) { bits = *reinterpret_cast<const decltype(bits)*>(p); }
+  __device__ __forceinline__ void clear() { bits = {}; }
+  __device__ __forceinline__ Words<VEC> words() const {
+    Words<VEC> w;
+    if constexpr (VEC == 1) {
+      w.x[0] = to_f32(bits);
+    } else {
+      const unsigned u[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w.x[2 * i] = __uint_as_float(u[i] << 16);
-      w.x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (VEC == 4) {
+          w.x[i] = __uint_as_float(u[i]);
+        } else {
+          w.x[2 * i] = __uint_as_float(u[i] << 16);
+          w.x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+      }
     }
-  } else {
-    w.x[0] = to_f32(*p);
+    return w;
   }
-  return w;
+};
+template <int VEC, typename TIn>
+__device__ __forceinline__ Words<VEC> load_words(const TIn* p) {
+  RawWords<TIn, VEC> r;
+  r.load(p);
+  return r.words();
 }
 template <int VEC>
 __device__ __forceinline__ void store_words(float* p, const float* x) {
@@ -56,6 +63,12 @@ __device__ __forceinline__ void store_words(bf16* p, const float* x) {
   } else {
     from_f32(*p, x[0]);
   }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // The scores of one node.

@@ -105,12 +105,6 @@ constexpr int kWarpRows = 8;   // rows per CTA where a warp has a row
 template <int G>
 constexpr int kCta = G == 32 ? 32 * kWarpRows : G;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 using Entry = unsigned long long;   // a word and its score: greater for words that come first
 __device__ __forceinline__ Entry entry_of(float z, int v) {
   return ((Entry)score_key(z) << 32) | (0xffffffffu - (unsigned)v);

@@ -184,7 +184,7 @@ class NodeDistillation(torch.autograd.Function):
                 saved.data_ptr() if save else 0, nbytes, sizes, K, temperature)
         if save:
             ctx.save_for_backward(emissions, predictions, frames, positions, words, saved)
-            ctx.temperature, ctx.has_rest = temperature, rest is not None
+            ctx.temperature = temperature
         return costs
 
     @staticmethod
@@ -204,7 +204,7 @@ class NodeDistillation(torch.autograd.Function):
                 scores, frames.data_ptr(), positions.data_ptr(), words.data_ptr(),
                 saved.data_ptr(), saved.numel(), deltas.data_ptr(),
                 0 if egrads is None else egrads.data_ptr(),
-                0 if pgrads is None else pgrads.data_ptr(), sizes, words.shape[2], ctx.has_rest,
+                0 if pgrads is None else pgrads.data_ptr(), sizes, words.shape[2],
                 ctx.temperature, ws.data_ptr(), nbytes)
         return (egrads, pgrads) + (None,) * 7
 
