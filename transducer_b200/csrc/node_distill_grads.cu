@@ -139,56 +139,56 @@ __device__ __forceinline__ void write_floats(float* p, const float (&x)[VEC]) {
 
 // What is saved of a node, made ready for its words' gradients.
 struct Terms {
-  float m, A, L, w, ws, scale2;
-  bool apart;   // the listed words have a normaliser of their own
-  __device__ __forceinline__ Terms(float4 of, float weight, const GradArgs& k)
-      : m(of.x), A(of.y), L(of.w), w(weight * k.scale), ws(of.z > 0.0f ? w : -w), scale2(k.scale2),
-        apart(fabsf(of.z) > 1.5f) {}
-  __device__ __forceinline__ float others(float z) const { return ws * ex2(fmaf(z - m, scale2, -A)); }
-  __device__ __forceinline__ float word(float z, bool listed) const {
-    return listed ? w * ex2(fmaf(z - m, scale2, -L)) : others(z);
+  float m, A, L, w, ws;   // ws: w with the others' sign
+  bool apart;             // the listed words have a normaliser of their own
+  __device__ __forceinline__ static Terms of(float4 saved, float w) {
+    return Terms{saved.x, saved.y, saved.w, w, saved.z > 0.0f ? w : -w, fabsf(saved.z) > 1.5f};
   }
+  __device__ __forceinline__ float others(float z, float scale2) const { return ws * ex2(fmaf(z - m, scale2, -A)); }
   // gradients of a vector; bit i of `listed`: whether word i is (of use where it is a case apart)
   template <int VEC>
-  __device__ __forceinline__ void vector(const Words<VEC>& e, const Words<VEC>& p, unsigned listed,
+  __device__ __forceinline__ void vector(const Words<VEC>& e, const Words<VEC>& p, unsigned listed, float scale2,
                                          float (&g)[VEC]) const {
     if (!apart) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = others(e.x[i] + p.x[i]);
+      for (int i = 0; i < VEC; ++i) g[i] = others(e.x[i] + p.x[i], scale2);
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = word(e.x[i] + p.x[i], listed >> i & 1);
+      for (int i = 0; i < VEC; ++i) {
+        const bool in = listed >> i & 1;
+        g[i] = (in ? w : ws) * ex2(fmaf(e.x[i] + p.x[i] - m, scale2, in ? -L : -A));
+      }
     }
   }
 };
 
 // A node's number, and 32 words of its record, one in each lane.
 struct Record {
-  i64 node;
+  i64 at;   // of the record's first word among all
   int v;
   float share;
-  __device__ __forceinline__ void load(const GradArgs& k, i64 node_, int from, int lane) {
-    node = node_;
+  __device__ __forceinline__ void load(const GradArgs& k, i64 at_, int from, int lane) {
+    at = at_;
     v = -1;
     share = kNoShare;
     if (from + lane < k.K) {
-      v = k.words[node * k.K + from + lane];
-      share = k.saved.share[node * k.K + from + lane];
+      v = k.words[at + from + lane];
+      share = k.saved.share[at + from + lane];
     }
   }
   // whether the lane's word is one of the tile's, and its place there
   template <int WORDS>
-  __device__ __forceinline__ bool hits(int tileFirst, int& at) const {
-    at = v - tileFirst;
-    return v >= 0 && (unsigned)at < (unsigned)WORDS && share != kNoShare;
+  __device__ __forceinline__ bool hits(int tileFirst, int& place) const {
+    place = v - tileFirst;
+    return v >= 0 && (unsigned)place < (unsigned)WORDS && share != kNoShare;
   }
 };
 
 // The listed words of a node that lie in the tile: their shares are subtracted in shared memory, `sub`, by the lanes
-// that read the record; each lane gets a bit for each of its own words.
+// that read the record, and `marks` gets a bit for each word of a lane.
 template <int VEC, int COLS>
-__device__ __forceinline__ unsigned add_record(const GradArgs& k, Record r, float w, int tileFirst, int lane, float* sub,
-                                               unsigned* marks) {
+__device__ __forceinline__ void add_record(const GradArgs& k, Record r, float w, int tileFirst, int lane, float* sub,
+                                           unsigned* marks) {
   for (int k0 = 0;;) {
     int at;
     if (r.hits<32 * COLS>(tileFirst, at)) {
@@ -197,12 +197,8 @@ __device__ __forceinline__ unsigned add_record(const GradArgs& k, Record r, floa
     }
     k0 += 32;
     if (k0 >= k.K) break;
-    r.load(k, r.node, k0, lane);
+    r.load(k, r.at, k0, lane);
   }
-  __syncwarp();
-  const unsigned mine = marks[lane];
-  if (mine) marks[lane] = 0;
-  return mine;
 }
 // The same for sums in registers, for few nodes.
 template <int VEC, int COLS>
@@ -222,37 +218,37 @@ __device__ __forceinline__ void add_record_to(const GradArgs& k, Record r, float
     }
     k0 += 32;
     if (k0 >= k.K) break;
-    r.load(k, r.node, k0, lane);
+    r.load(k, r.at, k0, lane);
   }
 }
 
-// A node as its warp comes to it.
-struct Step {
-  float4 of;
-  float weight;
-  int t, u, n;
+// A node as its warp comes to it: all that can be known beforehand, made for 32 nodes at a time by a lane each.
+struct __align__(16) Step {
+  Terms terms;
+  int flags, u;
+  i64 row, out, record;   // from the utterance's first: the frame's row of E and of dE; the node's record
 };
+constexpr int kNewFrame = 1, kMoreOfFrame = 2, kNewPosition = 4;   // another than the node's before; not the last node
 constexpr int kSteps = 64;    // in shared memory
-constexpr int kAhead = 2;     // rows of E that are on their way
-template <typename TIn, int COLS>
+constexpr int kAhead = 3;     // rows of E that are on their way
+constexpr int kCols = 16;     // words per lane
+template <typename TIn>
 struct __align__(16) PathMemory {   // of a warp
-  TIn rows[kAhead + 1][32 * COLS];
-  float sub[32 * COLS];
+  TIn rows[kAhead + 1][32 * kCols];
+  float sub[32 * kCols];
   Step steps[kSteps];
   unsigned marks[32];
 };
-// Words per lane: 64 bytes of a row (two rows of sums and one of P in registers for bf16 would be too many).
-template <typename TIn>
-constexpr int kCols = sizeof(TIn) == 2 ? 24 : 16;
 
-// Per node and 64 bytes of a lane's row about 9 instructions a word and 130 besides.  The sums for P are in registers;
-// a frame's gradients are written when its last node comes by, and wait in `sub` until then.
+// The sums for P are in registers; a frame's gradients are written when its last node comes by, and wait in `sub`
+// until then.
 template <typename TIn, int VEC>
-__global__ void __launch_bounds__(kPathWarps * 32, 8) distill_path_kernel(NodeArgs a, GradArgs k) {
-  constexpr int COLS = kCols<TIn>, NV = COLS / VEC;
+__global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
+    distill_path_kernel(NodeArgs a, GradArgs k) {
+  constexpr int COLS = kCols, NV = COLS / VEC;
   extern __shared__ __align__(16) unsigned char memory[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto& mem = reinterpret_cast<PathMemory<TIn, COLS>*>(memory)[warp];
+  auto& mem = reinterpret_cast<PathMemory<TIn>*>(memory)[warp];
   const i64 task = (i64)blockIdx.x * kPathWarps + warp;
   const i64 bs = task / k.tiles;
   const int b = (int)(bs / k.segs), seg = (int)(bs - (i64)b * k.segs);
@@ -262,138 +258,149 @@ __global__ void __launch_bounds__(kPathWarps * 32, 8) distill_path_kernel(NodeAr
   __syncwarp();
   using T = Tile<TIn, VEC, COLS>;
   const T tile{(int)(task - bs * k.tiles) * 32 * COLS, a.V, lane};
+  const int vectors = min(NV, div_up(a.V - tile.first, 32 * VEC));   // that have words of the row
   const int t0 = seg * k.segFrames, t1 = min(t0 + k.segFrames, a.T);
   const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
   const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
   TIn* dE = k.egrads ? static_cast<TIn*>(k.egrads) + (i64)b * a.T * a.V : nullptr;
-  TIn* dP = k.pgrads ? static_cast<TIn*>(k.pgrads) + (i64)b * a.U * a.V : nullptr;
   // the segment's nodes
   int n0 = 0x7fffffff, n1 = 0;
-  for (int t = t0 + lane; t < t1; t += 32) {
-    const int2 s = k.spans[(i64)b * a.T + t];
-    if (s.y > 0) n0 = min(n0, a.N - s.x), n1 = max(n1, s.y);
+  for (int tb = t0; tb < t1; tb += 32) {
+    const int t = tb + lane;
+    const int2 s = t < t1 ? k.spans[(i64)b * a.T + t] : make_int2(0, 1);
+    if (t < t1 && s.y > 0) n0 = min(n0, a.N - s.x), n1 = max(n1, s.y);
+    const float zero[VEC] = {};   // for frames without nodes
+    for (unsigned none = __ballot_sync(0xffffffffu, s.y == 0); dE && none; none &= none - 1)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) tile.store(dE + (i64)(tb + __ffs(none) - 1) * a.V, j, zero);
   }
   n0 = __reduce_min_sync(0xffffffffu, n0);
   n1 = __reduce_max_sync(0xffffffffu, n1);
-  if (n1 == 0) n0 = 0;   // (none: nothing is read below)
+  if (n1 == 0) return;
   typename T::Row p;
   float accP[COLS];
 #pragma unroll
   for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
-  int curU = -1, nextRow = t0;   // frames below nextRow are written
-  auto zeros_to = [&](int t) {   // zeros for the frames without nodes before t
-    const float zero[VEC] = {};
-    for (; nextRow < t; ++nextRow)
-      if (dE)
-#pragma unroll
-        for (int j = 0; j < NV; ++j) tile.store(dE + (i64)nextRow * a.V, j, zero);
-  };
+  int curU = -1;
   auto finish_position = [&] {
-    if (dP) {
+    if (k.pgrads) {
       const int2 s = k.spans[(i64)a.B * a.T + (i64)b * a.U + curU];
       const int* frames = a.frames + (i64)b * a.N;
       const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
-      if (from == to) tile.store(dP + (i64)curU * a.V, accP);
+      if (from == to) tile.store(static_cast<TIn*>(k.pgrads) + ((i64)b * a.U + curU) * a.V, accP);
       else tile.store(k.partial + (((i64)b * k.segs + seg) * 2 + (from == seg ? 1 : 0)) * a.V, accP);
     }
 #pragma unroll
     for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
   };
-  // The steps: appended 32 places at a time, rows fetched kAhead steps ahead; a group of copies per step.
-  int appended = 0, base = n0, written = 0;
+  int appended = 0, base = n0, lastT = -1, lastU = -1;
   auto append_to = [&](int want) {
     while (appended < want && base < n1) {
-      Step x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -1, -1, base + lane};
-      if (x.n < n1) {
-        const i64 node = (i64)b * a.N + x.n;
-        x.t = a.frames[node], x.u = a.positions[node];
-        x.of = k.saved.node[node];
-        x.weight = k.weights[node];
+      Step x;
+      int t = -1;
+      x.u = -1;
+      const int n = base + lane;
+      if (n < n1) {
+        const i64 node = (i64)b * a.N + n;
+        t = a.frames[node], x.u = a.positions[node];
+        x.terms = Terms::of(k.saved.node[node], k.weights[node] * k.scale);
+        x.row = t * a.eStrideT;
+        x.out = (i64)t * a.V;
+        x.record = node * k.K;
       }
-      const bool here = (unsigned)x.t < (unsigned)a.T && (unsigned)x.u < (unsigned)a.U;
-      const unsigned all = __ballot_sync(0xffffffffu, here);
-      if (here) mem.steps[(appended + __popc(all & ((1u << lane) - 1))) % kSteps] = x;
+      const bool here = (unsigned)t < (unsigned)a.T && (unsigned)x.u < (unsigned)a.U;
+      const unsigned all = __ballot_sync(0xffffffffu, here), before = all & ((1u << lane) - 1), after = all & ~before & ~(1u << lane);
+      const int tBefore = __shfl_sync(0xffffffffu, t, before ? 31 - __clz(before) : 0);
+      const int uBefore = __shfl_sync(0xffffffffu, x.u, before ? 31 - __clz(before) : 0);
+      const int tAfter = __shfl_sync(0xffffffffu, t, after ? __ffs(after) - 1 : 0);
+      x.flags = (t != (before ? tBefore : lastT) ? kNewFrame : 0) | (x.u != (before ? uBefore : lastU) ? kNewPosition : 0) |
+                (after && t == tAfter ? kMoreOfFrame : 0);
+      if (here) {
+        mem.steps[(appended + __popc(before)) % kSteps] = x;
+        if (!before && appended > 0 && t == lastT) mem.steps[(appended - 1) % kSteps].flags |= kMoreOfFrame;
+      }
+      if (all) {
+        lastT = __shfl_sync(0xffffffffu, t, 31 - __clz(all));
+        lastU = __shfl_sync(0xffffffffu, x.u, 31 - __clz(all));
+      }
       appended += __popc(all);
       base += 32;
       __syncwarp();
     }
   };
-  auto fetch_row = [&](int i) {   // of step i, if it is another than the one before
+  int ringTo = 0;
+  auto fetch_row = [&](int i) {   // of step i, if it is another than the one before; a group of copies per step
     if (i < appended) {
-      const int t = mem.steps[i % kSteps].t;
-      if (i == 0 || mem.steps[(i - 1) % kSteps].t != t) {
-        tile.fetch(E + t * a.eStrideT, mem.rows[written]);
-        written = written == kAhead ? 0 : written + 1;
+      const Step& x = mem.steps[i % kSteps];
+      if (x.flags & kNewFrame) {
+        tile.fetch(E + x.row, mem.rows[ringTo]);
+        ringTo = (ringTo + 1) & kAhead;
       }
     }
     commit_copies();
   };
   append_to(kAhead + 1);
   for (int i = 0; i < kAhead; ++i) fetch_row(i);
-  Record record;
-  if (appended > 0) record.load(k, (i64)b * a.N + mem.steps[0].n, 0, lane);
-  int slot = kAhead, curT = -1;
+  Record next;
+  next.load(k, mem.steps[0].record, 0, lane);
+  int slot = kAhead;
   for (int i = 0; i < appended; ++i) {
-    append_to(i + kAhead + 1);
+    append_to(i + kAhead + 2);
     fetch_row(i + kAhead);
-    const Record mine = record;
-    const Step step = mem.steps[i % kSteps];
-    int nextT = -1;
-    if (i + 1 < appended) {
-      record.load(k, (i64)b * a.N + mem.steps[(i + 1) % kSteps].n, 0, lane);
-      nextT = mem.steps[(i + 1) % kSteps].t;
-    }
-    const bool more = step.t == nextT, alone = !more && step.t != curT;   // nodes of the frame to come; none but this
-    if (step.t != curT) {
-      curT = step.t;
-      slot = slot == kAhead ? 0 : slot + 1;
-      zeros_to(curT);
-      nextRow = curT + 1;
-    }
-    if (step.u != curU) {
+    const Record record = next;
+    if (i + 1 < appended) next.load(k, mem.steps[(i + 1) % kSteps].record, 0, lane);
+    const Step& step = mem.steps[i % kSteps];
+    const Terms terms = step.terms;
+    const int flags = step.flags;
+    if (flags & kNewPosition) {
       if (curU >= 0) finish_position();
       curU = step.u;
       tile.load(P + curU * a.pStrideU, p);
     }
-    const Terms terms(step.of, step.weight, k);
-    const unsigned listed = add_record<VEC, COLS>(k, mine, terms.w, tile.first, lane, mem.sub, mem.marks);
-    if (!alone) add_record_to<VEC, COLS>(k, mine, terms.w, tile.first, lane, accP);
+    if (flags & kNewFrame) slot = (slot + 1) & kAhead;
+    const bool alone = (flags & (kNewFrame | kMoreOfFrame)) == kNewFrame;   // on its frame
+    add_record<VEC, COLS>(k, record, terms.w, tile.first, lane, mem.sub, mem.marks);
+    if (!alone) add_record_to<VEC, COLS>(k, record, terms.w, tile.first, lane, accP);
     __syncwarp();
+    const unsigned listed = mem.marks[lane];
+    if (listed) mem.marks[lane] = 0;
     wait_copies<kAhead>();
-    TIn* out = dE ? dE + (i64)curT * a.V : nullptr;
+    const TIn* row = mem.rows[slot];
+    TIn* out = dE ? dE + step.out : nullptr;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (NV > 4 && j >= vectors) break;
       RawWords<TIn, VEC> e;
       e.clear();
-      if (tile.in(j)) e.load(&mem.rows[slot][tile.place(j)]);
-      float* sub = &mem.sub[tile.place(j)];
+      if (tile.in(j)) e.load(row + tile.place(j));
       const unsigned here = listed >> (j * VEC) & ((1u << VEC) - 1);
       float g[VEC];
-      terms.vector(e.words(), p[j].words(), here, g);
+      terms.vector(e.words(), p[j].words(), here, k.scale2, g);
+      float* sub = &mem.sub[tile.place(j)];
       if (alone) {
-        if (here) {   // the shares join the gradient, of both sides
+        if (here) {   // the shares join the gradients, of both sides
           float s[VEC];
           const float zero[VEC] = {};
           read_floats<VEC>(sub, s);
           write_floats<VEC>(sub, zero);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) g[i] += s[i];
+          for (int c = 0; c < VEC; ++c) g[c] += s[c];
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) accP[j * VEC + i] += g[i];
+        for (int c = 0; c < VEC; ++c) accP[j * VEC + c] += g[c];
         if (out) tile.store(out, j, g);
       } else {
         float s[VEC];
-        const float zero[VEC] = {};
         read_floats<VEC>(sub, s);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          accP[j * VEC + i] += g[i];
-          s[i] += g[i];
+        for (int c = 0; c < VEC; ++c) {
+          accP[j * VEC + c] += g[c];
+          s[c] += g[c];
         }
-        if (more) {
+        if (flags & kMoreOfFrame) {
           write_floats<VEC>(sub, s);
         } else {
+          const float zero[VEC] = {};
           write_floats<VEC>(sub, zero);
           if (out) tile.store(out, j, s);
         }
@@ -401,8 +408,7 @@ __global__ void __launch_bounds__(kPathWarps * 32, 8) distill_path_kernel(NodeAr
     }
     __syncwarp();
   }
-  zeros_to(t1);
-  if (curU >= 0) finish_position();
+  finish_position();
 }
 
 // 32 places of an utterance's nodes in a warp's shared memory.
@@ -430,7 +436,7 @@ struct Batch {
 // Rows of either gradient of utterances whose nodes are not a path.  Tasks: (row, split, tile) of E, then of P.
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a, GradArgs k) {
-  constexpr int COLS = kCols<TIn>, NV = COLS / VEC;
+  constexpr int COLS = kCols, NV = COLS / VEC;
   __shared__ __align__(16) float subAll[kWarps][32 * COLS];
   __shared__ unsigned marksAll[kWarps][32];
   __shared__ Batch batchAll[kWarps][2];
@@ -470,7 +476,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
       Record record;
       auto fetch = [&](const Batch& x, int base, int at) {
         tile.load(otherRows + (ofFrames ? x.u[at] : x.t[at]) * otherStride, next);
-        record.load(k, (i64)b * a.N + base + at, 0, lane);
+        record.load(k, ((i64)b * a.N + base + at) * k.K, 0, lane);
       };
       auto advance = [&](Batch& x, int& base) {   // to the next 32 places from `base` on with a node of this row
         for (;; base += 32) {
@@ -500,12 +506,15 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
           for (int j = 0; j < NV; ++j) theirs[j] = next[j];
           if (todo) fetch(here, base, __ffs(todo) - 1);
           else if (todoThen) fetch(then, baseThen, __ffs(todoThen) - 1);
-          const Terms terms(here.of[bit], here.weight[bit], k);
-          const unsigned listed = add_record<VEC, COLS>(k, theirRecord, terms.w, tile.first, lane, sub, marks);
+          const Terms terms = Terms::of(here.of[bit], here.weight[bit] * k.scale);
+          add_record<VEC, COLS>(k, theirRecord, terms.w, tile.first, lane, sub, marks);
+          __syncwarp();
+          const unsigned listed = marks[lane];
+          marks[lane] = 0;
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
             float g[VEC];
-            terms.vector(theirs[j].words(), mine[j].words(), listed >> (j * VEC), g);
+            terms.vector(theirs[j].words(), mine[j].words(), listed >> (j * VEC), k.scale2, g);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[j * VEC + i] += g[i];
           }
@@ -605,15 +614,15 @@ __global__ void __launch_bounds__(kWarps * 32) distill_join_kernel(NodeArgs a, G
   }
 }
 
-constexpr int kLeastFrames = 16, kLeastNodes = 8, kTileWords = 1024;   // (the largest tile)
+constexpr int kLeastFrames = 16, kLeastNodes = 8, kTileWords = 32 * kCols;
 
 struct Plan {
   int tiles, segFrames, segs, eSplits, pSplits;
   size_t spanBytes;
 };
-Plan plan_of(int B, int T, int U, int V, int N, int dtype) {
+Plan plan_of(int B, int T, int U, int V, int N) {
   Plan p{};
-  p.tiles = div_up(V, 32 * (dtype == kDtypeBf16 ? kCols<bf16> : kCols<float>));
+  p.tiles = div_up(V, kTileWords);
   // segments of at least 16 frames, as many as fill the chip
   const i64 want = std::max<i64>(1, kTarget / std::max<i64>(1, (i64)B * p.tiles));
   p.segFrames = (int)std::max<i64>(kLeastFrames, div_up64(std::max(T, 1), want));
@@ -629,7 +638,7 @@ Plan plan_of(int B, int T, int U, int V, int N, int dtype) {
 }
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 // Of the paths' partial rows: the segments of all utterances are max(B, kTarget / tiles) at most, and a
-// tile is kTileWords words at most.  (A bound on what the plan takes, so that no smaller call needs more.)
+// tile is kTileWords words.  (A bound on what the plan takes, so that no smaller call needs more.)
 size_t path_floats(int B, int T, int V) {
   const size_t leastSegs = div_up(std::max(T, 1), kLeastFrames);
   return 2 * std::min(B * leastSegs * V, std::max((size_t)B * V, (size_t)kTarget * kTileWords));
@@ -652,7 +661,7 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
                              void* workspace, cudaStream_t stream) {
   const i64 frameRows = egrads ? (i64)a.B * a.T : 0, posRows = pgrads ? (i64)a.B * a.U : 0, nodes = (i64)a.B * a.N;
   if (frameRows + posRows == 0) return;
-  const Plan p = plan_of(a.B, a.T, a.U, a.V, a.N, a.dtype);
+  const Plan p = plan_of(a.B, a.T, a.U, a.V, a.N);
   GradArgs k{};
   k.words = words;
   k.saved = saved;
@@ -686,7 +695,7 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
     {
       ScopedKernel prof("distill_path", stream);
       const i64 tasks = (i64)a.B * p.segs * p.tiles;
-      constexpr int smem = kPathWarps * (int)sizeof(PathMemory<TIn, kCols<TIn>>);
+      constexpr int smem = kPathWarps * (int)sizeof(PathMemory<TIn>);
       allow_dyn_smem(distill_path_kernel<TIn, VEC>, smem);
       distill_path_kernel<TIn, VEC><<<(unsigned)div_up64(tasks, kPathWarps), kPathWarps * 32, smem, stream>>>(a, k);
       TB200_CHECK_LAUNCH();
