@@ -283,11 +283,12 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
                          SampleRule rule, cudaStream_t stream);
 
 // What the forward call leaves for the backward call, per node and per listed word: with x = (z - m) log2e /
-// temperature the gradient of a word is sign * 2^(x - A), less `share` for a listed one.  Where sign is +-2
-// that would not do for the listed words: theirs is 2^(x - L) less `share`, the others' +-1 * 2^(x - A).
+// temperature the gradient of a word is sign * 2^(x - A), less `share` for a listed one.  Where sign is -2 that
+// would be a difference of large numbers for the listed words: theirs is -share alone, the others' -2^(x - A).  The
+// listed words' whole gradients are kept too.
 struct DistillSaved {
-  float4* node;   // [B*N] m, A, sign, L
-  float* share;   // [B*N*K]; kNoShare: the word is to be ignored
+  float4* node;   // [B*N] m, A, sign, unused
+  float2* listed;   // [B*N*K] share (kNoShare: the word is to be ignored), gradient
 };
 constexpr float kNoShare = 3e38f;
 void launch_distill_forward(const NodeArgs& a, const int* words, const float* logits, const float* rest,

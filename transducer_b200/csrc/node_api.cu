@@ -51,7 +51,7 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 DistillSaved distill_saved(void* p, int B, int N) {
   DistillSaved s;
   s.node = static_cast<float4*>(p);
-  s.share = p ? reinterpret_cast<float*>(static_cast<char*>(p) + round256(sizeof(float4) * (size_t)B * N)) : nullptr;
+  s.listed = p ? reinterpret_cast<float2*>(static_cast<char*>(p) + round256(sizeof(float4) * (size_t)B * N)) : nullptr;
   return s;
 }
 
@@ -100,7 +100,7 @@ int tb200_sample_words(const void* E, const void* P, int bf16, long long eStride
 size_t tb200_distill_saved_bytes(int B, int N, int K) {
   if (B <= 0 || N <= 0 || K <= 0) return 0;
   const size_t nodes = (size_t)B * N;
-  return round256(sizeof(float4) * nodes) + round256(sizeof(float) * nodes * K);
+  return round256(sizeof(float4) * nodes) + round256(sizeof(float2) * nodes * K);
 }
 
 int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,

@@ -81,13 +81,13 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
   const int bitWords = (a.V + 31) / 32;
   Listed* const record = reinterpret_cast<Listed*>(memory) + sub * K;
   unsigned* const bits = reinterpret_cast<unsigned*>(memory + kNodes * K * sizeof(Listed)) + sub * bitWords;
-  float* const savedShare = saved.share ? saved.share + node * K : nullptr;
+  float2* const savedListed = saved.listed ? saved.listed + node * K : nullptr;
   const NodeScores<TIn> s = node_scores<TIn>(a, node);
   if (!s.here) {
     if (tid == 0) costs[node] = 0.0f;
-    if (savedShare) {
-      for (int k = tid; k < K; k += G) savedShare[k] = kNoShare;
-      if (tid == 0) saved.node[node] = make_float4(0.0f, pos_inf(), 1.0f, pos_inf());
+    if (savedListed) {
+      for (int k = tid; k < K; k += G) savedListed[k] = make_float2(kNoShare, 0.0f);
+      if (tid == 0) saved.node[node] = make_float4(0.0f, pos_inf(), 1.0f, 0.0f);
     }
     return;
   }
@@ -199,19 +199,22 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
   float logRatio = neg_inf();   // of r to the student's weight of the others
   if (REST && r > 0.0f && other2 != neg_inf()) logRatio = logf(r) - (other2 - all2) * kLn2;
   const bool apart = logRatio > kLn2;   // (more than 2: listed words would be differences of large numbers)
-  const float ratio = apart ? 0.0f : expf(logRatio);
+  const float ratio = apart ? 1.0f : expf(logRatio);
   float cost = 0.0f;
   for (int k = tid; k < K; k += G) {
     const float q = record[k].share, z = record[k].z;
     const float logP = z == neg_inf() ? z : ((z - full.m) * scale2 - all2) * kLn2;
     if (q != kNoShare && q != 0.0f) cost += q * (logf(q) - logP);
-    if (savedShare) savedShare[k] = q == kNoShare ? q : q - ratio * (z == neg_inf() ? 0.0f : expf(logP));
+    if (savedListed) {
+      const float p = z == neg_inf() || empty ? 0.0f : expf(logP);
+      savedListed[k] = q == kNoShare ? make_float2(q, 0.0f) : make_float2(q - ratio * p, p - q);
+    }
   }
   cost = g.sum(cost);
   if (tid != 0) return;
   if (REST && r != 0.0f) cost += r * (logf(r) - (other2 == neg_inf() ? other2 : (other2 - all2) * kLn2));
   costs[node] = cost;
-  if (!savedShare) return;
+  if (!savedListed) return;
   // (an empty record has no gradient, and a student without any word left has p = 0)
   const float L = empty || all2 == neg_inf() ? pos_inf() : all2;
   float A = L, sign = 1.0f;
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
     sign = apart ? -2.0f : logRatio > 0.0f ? -1.0f : 1.0f;
     A = L - (fmaxf(logRatio, 0.0f) + log1pf(-expf(-fabsf(logRatio)))) * kLog2e;
   }
-  saved.node[node] = make_float4(full.m, A, sign, L);
+  saved.node[node] = make_float4(full.m, A, sign, 0.0f);
 }
 
 template <typename F>

@@ -20,8 +20,8 @@ namespace tb200 {
 namespace {
 
 constexpr int kWarps = 4;       // per CTA
-constexpr int kPathWarps = 2;   // of the path kernel
-constexpr int kTarget = 148 * 60;  // warps that fill the chip
+constexpr int kPathWarps = 4;   // of the path kernel, at most
+constexpr int kTarget = 148 * 96;  // warps that fill the chip
 constexpr int kLookBack = 64;      // places without a node that a path may have between two nodes
 
 struct GradArgs {
@@ -39,34 +39,43 @@ struct GradArgs {
   int segFrames, segs, tiles, eSplits, pSplits;
 };
 
+// Of consecutive nodes on the same frame, or position, the first and the last one of a warp's 32 speak for all.
 __global__ void __launch_bounds__(256) node_spans_kernel(NodeArgs a, GradArgs k) {
   const i64 node = (i64)blockIdx.x * 256 + threadIdx.x;
-  if (node >= (i64)a.B * a.N) return;
+  const int lane = threadIdx.x & 31;
+  const bool in = node < (i64)a.B * a.N;
   auto valid = [&](i64 i) {
     return (unsigned)a.frames[i] < (unsigned)a.T && (unsigned)a.positions[i] < (unsigned)a.U;
   };
-  if (!valid(node)) return;
-  const int t = a.frames[node], u = a.positions[node];
-  const i64 b = node / a.N;
+  const bool here = in && valid(node);
+  const i64 b = here ? node / a.N : -1;
+  const int t = here ? a.frames[node] : -1, u = here ? a.positions[node] : -1;
+  const i64 frame = here ? b * a.T + t : -1, position = here ? (i64)a.B * a.T + b * a.U + u : -1;
+  const i64 frameUp = __shfl_up_sync(0xffffffffu, frame, 1), frameDown = __shfl_down_sync(0xffffffffu, frame, 1);
+  const i64 posUp = __shfl_up_sync(0xffffffffu, position, 1), posDown = __shfl_down_sync(0xffffffffu, position, 1);
+  if (!here) return;
   const int n = (int)(node - b * a.N);
-  int2* f = k.spans + b * a.T + t;
-  int2* p = k.spans + (i64)a.B * a.T + b * a.U + u;
-  atomicMax(&f->x, a.N - n);
-  atomicMax(&f->y, n + 1);
-  atomicMax(&p->x, a.N - n);
-  atomicMax(&p->y, n + 1);
-  k.segUsed[b * k.segs + t / k.segFrames] = 1;
+  if (lane == 0 || frameUp != frame) {
+    atomicMax(&k.spans[frame].x, a.N - n);
+    k.segUsed[b * k.segs + t / k.segFrames] = 1;
+  }
+  if (lane == 31 || frameDown != frame) atomicMax(&k.spans[frame].y, n + 1);
+  if (lane == 0 || posUp != position) atomicMax(&k.spans[position].x, a.N - n);
+  if (lane == 31 || posDown != position) atomicMax(&k.spans[position].y, n + 1);
   int back = 1;
   while (back <= n && back <= kLookBack && !valid(node - back)) ++back;
   if (back > n) return;   // (the first node)
   if (back > kLookBack || a.frames[node - back] > t || a.positions[node - back] > u) k.offPath[b] = 1;
 }
 
+// (16 bytes: past the L1, most of which is shared memory here)
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from),
-               "n"(BYTES)
-               : "memory");
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
@@ -101,11 +110,12 @@ struct Tile {
   template <typename T>
   __device__ __forceinline__ void store(T* row, int j, const float* x) const {   // vector j
     if (!in(j)) return;
+    row += first + place(j);
     if constexpr (std::is_same<T, TIn>::value) {
-      store_words<VEC>(row + first + place(j), x);
-    } else {
+      store_words<VEC>(row, x);
+    } else {   // fp32 sums of bf16 gradients
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) row[first + place(j) + i] = x[i];
+      for (int i = 0; i < VEC; i += VEC > 1 ? 4 : 1) store_words<(VEC > 1 ? 4 : 1)>(row + i, x + i);
     }
   }
   template <typename T>
@@ -139,26 +149,22 @@ __device__ __forceinline__ void write_floats(float* p, const float (&x)[VEC]) {
 
 // What is saved of a node, made ready for its words' gradients.
 struct Terms {
-  float m, A, L, w, ws;   // ws: w with the others' sign
-  bool apart;             // the listed words have a normaliser of their own
+  float m, A, w, ws;   // ws: w with the others' sign
+  bool apart;          // the listed words' gradients are their shares alone
   __device__ __forceinline__ static Terms of(float4 saved, float w) {
-    return Terms{saved.x, saved.y, saved.w, w, saved.z > 0.0f ? w : -w, fabsf(saved.z) > 1.5f};
+    return Terms{saved.x, saved.y, w, saved.z > 0.0f ? w : -w, fabsf(saved.z) > 1.5f};
   }
-  __device__ __forceinline__ float others(float z, float scale2) const { return ws * ex2(fmaf(z - m, scale2, -A)); }
-  // gradients of a vector; bit i of `listed`: whether word i is (of use where it is a case apart)
+  // gradients of a vector but for the shares; bit i of `listed`: whether word i is
   template <int VEC>
-  __device__ __forceinline__ void vector(const Words<VEC>& e, const Words<VEC>& p, unsigned listed, float scale2,
+  __device__ __forceinline__ void vector(Words<VEC> e, const Words<VEC>& p, unsigned listed, float scale2,
                                          float (&g)[VEC]) const {
-    if (!apart) {
+    if (apart && listed) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = others(e.x[i] + p.x[i], scale2);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const bool in = listed >> i & 1;
-        g[i] = (in ? w : ws) * ex2(fmaf(e.x[i] + p.x[i] - m, scale2, in ? -L : -A));
-      }
+      for (int i = 0; i < VEC; ++i)
+        if (listed >> i & 1) e.x[i] = neg_inf();
     }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) g[i] = ws * ex2(fmaf(e.x[i] + p.x[i] - m, scale2, -A));
   }
 };
 
@@ -166,33 +172,35 @@ struct Terms {
 struct Record {
   i64 at;   // of the record's first word among all
   int v;
-  float share;
+  float2 listed;   // share, gradient
   __device__ __forceinline__ void load(const GradArgs& k, i64 at_, int from, int lane) {
     at = at_;
     v = -1;
-    share = kNoShare;
+    listed = make_float2(kNoShare, 0.0f);
     if (from + lane < k.K) {
       v = k.words[at + from + lane];
-      share = k.saved.share[at + from + lane];
+      listed = k.saved.listed[at + from + lane];
     }
   }
   // whether the lane's word is one of the tile's, and its place there
   template <int WORDS>
   __device__ __forceinline__ bool hits(int tileFirst, int& place) const {
     place = v - tileFirst;
-    return v >= 0 && (unsigned)place < (unsigned)WORDS && share != kNoShare;
+    return v >= 0 && (unsigned)place < (unsigned)WORDS && listed.x != kNoShare;
   }
 };
 
-// The listed words of a node that lie in the tile: their shares are subtracted in shared memory, `sub`, by the lanes
-// that read the record, and `marks` gets a bit for each word of a lane.
+// The listed words of a node that lie in the tile: their shares are subtracted in shared memory, `subA` (and `subB`
+// if there is one), by the lanes that read the record, and `marks` gets a bit for each word of a lane.
 template <int VEC, int COLS>
-__device__ __forceinline__ void add_record(const GradArgs& k, Record r, float w, int tileFirst, int lane, float* sub,
-                                           unsigned* marks) {
+__device__ __forceinline__ void add_record(const GradArgs& k, Record r, float w, int tileFirst, float* subA, float* subB,
+                                           unsigned* marks, int lane) {
   for (int k0 = 0;;) {
     int at;
     if (r.hits<32 * COLS>(tileFirst, at)) {
-      sub[at] -= w * r.share;
+      const float x = w * r.listed.x;
+      subA[at] -= x;
+      if (subB) subB[at] -= x;
       atomicOr(&marks[at / VEC % 32], 1u << (at / (32 * VEC) * VEC + at % VEC));
     }
     k0 += 32;
@@ -200,68 +208,52 @@ __device__ __forceinline__ void add_record(const GradArgs& k, Record r, float w,
     r.load(k, r.at, k0, lane);
   }
 }
-// The same for sums in registers, for few nodes.
-template <int VEC, int COLS>
-__device__ __forceinline__ void add_record_to(const GradArgs& k, Record r, float w, int tileFirst, int lane,
-                                              float (&acc)[COLS]) {
-  for (int k0 = 0;;) {
-    int at;
-    unsigned todo = __ballot_sync(0xffffffffu, r.hits<32 * COLS>(tileFirst, at));
-#pragma unroll 1
-    for (; todo; todo &= todo - 1) {
-      const int i = __ffs(todo) - 1, place = __shfl_sync(0xffffffffu, at, i);
-      const float share = w * __shfl_sync(0xffffffffu, r.share, i);
-      const int slot = place / VEC % 32 == lane ? place / (32 * VEC) * VEC + place % VEC : -1;
-#pragma unroll
-      for (int c = 0; c < COLS; ++c)
-        if (c == slot) acc[c] -= share;
-    }
-    k0 += 32;
-    if (k0 >= k.K) break;
-    r.load(k, r.at, k0, lane);
-  }
-}
 
-// A node as its warp comes to it: all that can be known beforehand, made for 32 nodes at a time by a lane each.
+// A node as its CTA comes to it: all that can be known beforehand, made for 32 nodes at a time by a lane each.
 struct __align__(16) Step {
   Terms terms;
-  int flags, u;
+  int flags, u, unused;
   i64 row, out, record;   // from the utterance's first: the frame's row of E and of dE; the node's record
+  i64 target;             // of a new position: its row of dP, or -1 less its place among the partial rows
 };
 constexpr int kNewFrame = 1, kMoreOfFrame = 2, kNewPosition = 4;   // another than the node's before; not the last node
 constexpr int kSteps = 64;    // in shared memory
-constexpr int kAhead = 3;     // rows of E that are on their way
 constexpr int kCols = 16;     // words per lane
 template <typename TIn>
-struct __align__(16) PathMemory {   // of a warp
-  TIn rows[kAhead + 1][32 * kCols];
-  float sub[32 * kCols];
-  Step steps[kSteps];
+constexpr int kAhead = sizeof(TIn) == 2 ? 3 : 2;   // rows of E that are on their way
+template <typename TIn>
+struct __align__(16) PathWarp {
+  TIn rows[kAhead<TIn> + 1][32 * kCols];
+  TIn nextP[32 * kCols];   // the row of P of the next new position
+  float subE[32 * kCols], subP[32 * kCols];
   unsigned marks[32];
 };
+struct __align__(16) PathCta {
+  Step steps[kSteps];
+  int appended, base, lastT, lastU;
+};
 
-// The sums for P are in registers; a frame's gradients are written when its last node comes by, and wait in `sub`
-// until then.
+// A warp's tile: rows of E come through a ring in shared memory, the row of P in use and the sums for it are in registers,
+// a frame's gradients are written when its last node comes by and wait in `subE` until then.  The warps of a CTA go
+// along the same nodes.  Bound by instructions' latencies and issue: per node and tile about 130 besides 9 for each of the
+// 16 words of a lane, so that warps count, but not at the price of spilled registers: next to this much shared memory
+// the L1 does not hold them.
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
     distill_path_kernel(NodeArgs a, GradArgs k) {
-  constexpr int COLS = kCols, NV = COLS / VEC;
+  constexpr int COLS = kCols, NV = COLS / VEC, kA = kAhead<TIn>;
   extern __shared__ __align__(16) unsigned char memory[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto& mem = reinterpret_cast<PathMemory<TIn>*>(memory)[warp];
-  const i64 task = (i64)blockIdx.x * kPathWarps + warp;
-  const i64 bs = task / k.tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  PathCta& cta = *reinterpret_cast<PathCta*>(memory);
+  PathWarp<TIn>& mem = reinterpret_cast<PathWarp<TIn>*>(memory + sizeof(PathCta))[warp];
+  const int groups = (k.tiles + warps - 1) / warps;   // of tiles
+  const i64 bs = blockIdx.x / groups;
   const int b = (int)(bs / k.segs), seg = (int)(bs - (i64)b * k.segs);
-  if (b >= a.B || k.offPath[b]) return;
-  for (int i = lane; i < 32 * COLS; i += 32) mem.sub[i] = 0.0f;
-  mem.marks[lane] = 0;
-  __syncwarp();
+  if (k.offPath[b]) return;
   using T = Tile<TIn, VEC, COLS>;
-  const T tile{(int)(task - bs * k.tiles) * 32 * COLS, a.V, lane};
-  const int vectors = min(NV, div_up(a.V - tile.first, 32 * VEC));   // that have words of the row
+  const T tile{((int)(blockIdx.x - bs * groups) * warps + warp) * 32 * COLS, a.V, lane};
   const int t0 = seg * k.segFrames, t1 = min(t0 + k.segFrames, a.T);
   const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
-  const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
   TIn* dE = k.egrads ? static_cast<TIn*>(k.egrads) + (i64)b * a.T * a.V : nullptr;
   // the segment's nodes
   int n0 = 0x7fffffff, n1 = 0;
@@ -276,26 +268,16 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
   }
   n0 = __reduce_min_sync(0xffffffffu, n0);
   n1 = __reduce_max_sync(0xffffffffu, n1);
-  if (n1 == 0) return;
-  typename T::Row p;
-  float accP[COLS];
-#pragma unroll
-  for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
-  int curU = -1;
-  auto finish_position = [&] {
-    if (k.pgrads) {
-      const int2 s = k.spans[(i64)a.B * a.T + (i64)b * a.U + curU];
-      const int* frames = a.frames + (i64)b * a.N;
-      const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
-      if (from == to) tile.store(static_cast<TIn*>(k.pgrads) + ((i64)b * a.U + curU) * a.V, accP);
-      else tile.store(k.partial + (((i64)b * k.segs + seg) * 2 + (from == seg ? 1 : 0)) * a.V, accP);
-    }
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
-  };
-  int appended = 0, base = n0, lastT = -1, lastU = -1;
-  auto append_to = [&](int want) {
-    while (appended < want && base < n1) {
+  if (n1 == 0) return;   // (the same for all warps)
+  for (int i = lane; i < 32 * COLS; i += 32) mem.subE[i] = mem.subP[i] = 0.0f;
+  mem.marks[lane] = 0;
+  if (threadIdx.x == 0) cta.appended = 0, cta.base = n0, cta.lastT = cta.lastU = -1;
+  auto append = [&] {   // the next 32 places with a node, by one warp
+    int base = cta.base;
+    const int appended = cta.appended, lastT = cta.lastT, lastU = cta.lastU;
+    __syncwarp();
+    unsigned all = 0;
+    for (; !all && base < n1; base += 32) {
       Step x;
       int t = -1;
       x.u = -1;
@@ -309,102 +291,166 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
         x.record = node * k.K;
       }
       const bool here = (unsigned)t < (unsigned)a.T && (unsigned)x.u < (unsigned)a.U;
-      const unsigned all = __ballot_sync(0xffffffffu, here), before = all & ((1u << lane) - 1), after = all & ~before & ~(1u << lane);
+      all = __ballot_sync(0xffffffffu, here);
+      const unsigned before = all & ((1u << lane) - 1), after = all & ~before & ~(1u << lane);
       const int tBefore = __shfl_sync(0xffffffffu, t, before ? 31 - __clz(before) : 0);
       const int uBefore = __shfl_sync(0xffffffffu, x.u, before ? 31 - __clz(before) : 0);
       const int tAfter = __shfl_sync(0xffffffffu, t, after ? __ffs(after) - 1 : 0);
-      x.flags = (t != (before ? tBefore : lastT) ? kNewFrame : 0) | (x.u != (before ? uBefore : lastU) ? kNewPosition : 0) |
-                (after && t == tAfter ? kMoreOfFrame : 0);
+      x.flags = (t != (before ? tBefore : lastT) ? kNewFrame : 0) |
+                (x.u != (before ? uBefore : lastU) ? kNewPosition : 0) | (after && t == tAfter ? kMoreOfFrame : 0);
+      if (here && (x.flags & kNewPosition) && k.pgrads) {
+        const int2 s = k.spans[(i64)a.B * a.T + (i64)b * a.U + x.u];
+        const int* frames = a.frames + (i64)b * a.N;
+        const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
+        x.target = from == to ? (i64)x.u * a.V : -1 - (((i64)b * k.segs + seg) * 2 + (from == seg ? 1 : 0)) * a.V;
+      }
       if (here) {
-        mem.steps[(appended + __popc(before)) % kSteps] = x;
-        if (!before && appended > 0 && t == lastT) mem.steps[(appended - 1) % kSteps].flags |= kMoreOfFrame;
+        cta.steps[(appended + __popc(before)) % kSteps] = x;
+        if (!before && appended > 0 && t == lastT) cta.steps[(appended - 1) % kSteps].flags |= kMoreOfFrame;
+        if (!after) cta.lastT = t, cta.lastU = x.u;
       }
-      if (all) {
-        lastT = __shfl_sync(0xffffffffu, t, 31 - __clz(all));
-        lastU = __shfl_sync(0xffffffffu, x.u, 31 - __clz(all));
-      }
-      appended += __popc(all);
-      base += 32;
-      __syncwarp();
     }
+    if (lane == 0) cta.appended = appended + __popc(all), cta.base = base;
+  };
+  __syncthreads();
+  if (warp == 0) append();
+  __syncthreads();
+  int appended = cta.appended;
+  bool more = cta.base < n1;
+  typename T::Row p;
+  float accP[COLS];
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
+  i64 target = 0;   // of the position in use
+  auto finish_position = [&] {
+    if (k.pgrads) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {   // the shares
+        float s[VEC];
+        const float zero[VEC] = {};
+        read_floats<VEC>(mem.subP + tile.place(j), s);
+        write_floats<VEC>(mem.subP + tile.place(j), zero);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) accP[j * VEC + i] += s[i];
+      }
+      if (target >= 0) tile.store(static_cast<TIn*>(k.pgrads) + (i64)b * a.U * a.V + target, accP);
+      else tile.store(k.partial + (-1 - target), accP);
+    }
+#pragma unroll
+    for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
   };
   int ringTo = 0;
+  const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
+  int stepP = -1;   // whose row of P is in nextP, or on its way there
   auto fetch_row = [&](int i) {   // of step i, if it is another than the one before; a group of copies per step
     if (i < appended) {
-      const Step& x = mem.steps[i % kSteps];
+      const Step& x = cta.steps[i % kSteps];
       if (x.flags & kNewFrame) {
         tile.fetch(E + x.row, mem.rows[ringTo]);
-        ringTo = (ringTo + 1) & kAhead;
+        ringTo = ringTo == kA ? 0 : ringTo + 1;
+      }
+      if ((x.flags & kNewPosition) && stepP < 0) {
+        tile.fetch(P + x.u * a.pStrideU, mem.nextP);
+        stepP = i;
       }
     }
     commit_copies();
   };
-  append_to(kAhead + 1);
-  for (int i = 0; i < kAhead; ++i) fetch_row(i);
   Record next;
-  next.load(k, mem.steps[0].record, 0, lane);
-  int slot = kAhead;
+  int slot = kA;
   for (int i = 0; i < appended; ++i) {
-    append_to(i + kAhead + 2);
-    fetch_row(i + kAhead);
+    while (more && appended < i + kA + 2) {
+      __syncthreads();   // (everybody is here: the steps before are free)
+      if (warp == 0) append();
+      __syncthreads();
+      appended = cta.appended;
+      more = cta.base < n1;
+    }
+    if (i == 0) {
+      for (int j = 0; j < kA; ++j) fetch_row(j);
+      next.load(k, cta.steps[0].record, 0, lane);
+    }
+    fetch_row(i + kA);
     const Record record = next;
-    if (i + 1 < appended) next.load(k, mem.steps[(i + 1) % kSteps].record, 0, lane);
-    const Step& step = mem.steps[i % kSteps];
+    if (i + 1 < appended) next.load(k, cta.steps[(i + 1) % kSteps].record, 0, lane);
+    const Step& step = cta.steps[i % kSteps];
     const Terms terms = step.terms;
     const int flags = step.flags;
     if (flags & kNewPosition) {
-      if (curU >= 0) finish_position();
-      curU = step.u;
-      tile.load(P + curU * a.pStrideU, p);
+      if (i > 0) finish_position();
+      target = step.target;
+      if (stepP == i) {
+        wait_copies<kA>();
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          p[j].clear();
+          if (tile.in(j)) p[j].load(mem.nextP + tile.place(j));
+        }
+        stepP = -1;
+      } else {
+        tile.load(P + step.u * a.pStrideU, p);
+      }
     }
-    if (flags & kNewFrame) slot = (slot + 1) & kAhead;
-    const bool alone = (flags & (kNewFrame | kMoreOfFrame)) == kNewFrame;   // on its frame
-    add_record<VEC, COLS>(k, record, terms.w, tile.first, lane, mem.sub, mem.marks);
-    if (!alone) add_record_to<VEC, COLS>(k, record, terms.w, tile.first, lane, accP);
+    if (flags & kNewFrame) slot = slot == kA ? 0 : slot + 1;
+    const TIn* row = mem.rows[slot];
+    TIn* out = dE + step.out;
+    const bool whole = (flags & (kNewFrame | kMoreOfFrame)) == kNewFrame;   // the frame's only node
+    if (whole && !terms.apart) {
+      wait_copies<kA>();
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        RawWords<TIn, VEC> e;
+        e.clear();
+        if (tile.in(j)) e.load(row + tile.place(j));
+        float g[VEC];
+        terms.vector(e.words(), p[j].words(), 0u, k.scale2, g);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) accP[j * VEC + c] += g[c];
+        if (dE) tile.store(out, j, g);
+      }
+      __syncwarp();
+      // the listed words' gradients take the place of what has been stored for them
+      Record r = record;
+      for (int k0 = 0;;) {
+        int at;
+        if (r.template hits<32 * COLS>(tile.first, at)) {
+          if (dE) from_f32(out[tile.first + at], terms.w * r.listed.y);
+          mem.subP[at] -= terms.w * r.listed.x;
+        }
+        k0 += 32;
+        if (k0 >= k.K) break;
+        r.load(k, r.at, k0, lane);
+      }
+      __syncwarp();
+      continue;
+    }
+    add_record<VEC, COLS>(k, record, terms.w, tile.first, mem.subE, mem.subP, mem.marks, lane);
     __syncwarp();
     const unsigned listed = mem.marks[lane];
     if (listed) mem.marks[lane] = 0;
-    wait_copies<kAhead>();
-    const TIn* row = mem.rows[slot];
-    TIn* out = dE ? dE + step.out : nullptr;
+    wait_copies<kA>();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (NV > 4 && j >= vectors) break;
+      if (!tile.in(j)) break;
       RawWords<TIn, VEC> e;
-      e.clear();
-      if (tile.in(j)) e.load(row + tile.place(j));
+      e.load(row + tile.place(j));
       const unsigned here = listed >> (j * VEC) & ((1u << VEC) - 1);
       float g[VEC];
       terms.vector(e.words(), p[j].words(), here, k.scale2, g);
-      float* sub = &mem.sub[tile.place(j)];
-      if (alone) {
-        if (here) {   // the shares join the gradients, of both sides
-          float s[VEC];
-          const float zero[VEC] = {};
-          read_floats<VEC>(sub, s);
-          write_floats<VEC>(sub, zero);
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) g[c] += s[c];
-        }
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) accP[j * VEC + c] += g[c];
-        if (out) tile.store(out, j, g);
-      } else {
+      for (int c = 0; c < VEC; ++c) accP[j * VEC + c] += g[c];
+      if (!whole || here) {   // what waits there joins the gradient
         float s[VEC];
+        float* sub = mem.subE + tile.place(j);
         read_floats<VEC>(sub, s);
 #pragma unroll
         for (int c = 0; c < VEC; ++c) {
-          accP[j * VEC + c] += g[c];
-          s[c] += g[c];
+          g[c] += s[c];
+          s[c] = flags & kMoreOfFrame ? g[c] : 0.0f;
         }
-        if (flags & kMoreOfFrame) {
-          write_floats<VEC>(sub, s);
-        } else {
-          const float zero[VEC] = {};
-          write_floats<VEC>(sub, zero);
-          if (out) tile.store(out, j, s);
-        }
+        write_floats<VEC>(sub, s);
       }
+      if (dE && !(flags & kMoreOfFrame)) tile.store(out, j, g);
     }
     __syncwarp();
   }
@@ -507,7 +553,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
           if (todo) fetch(here, base, __ffs(todo) - 1);
           else if (todoThen) fetch(then, baseThen, __ffs(todoThen) - 1);
           const Terms terms = Terms::of(here.of[bit], here.weight[bit] * k.scale);
-          add_record<VEC, COLS>(k, theirRecord, terms.w, tile.first, lane, sub, marks);
+          add_record<VEC, COLS>(k, theirRecord, terms.w, tile.first, sub, nullptr, marks, lane);
           __syncwarp();
           const unsigned listed = marks[lane];
           marks[lane] = 0;
@@ -694,10 +740,13 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
     constexpr int VEC = decltype(vec)::value;
     {
       ScopedKernel prof("distill_path", stream);
-      const i64 tasks = (i64)a.B * p.segs * p.tiles;
-      constexpr int smem = kPathWarps * (int)sizeof(PathMemory<TIn>);
-      allow_dyn_smem(distill_path_kernel<TIn, VEC>, smem);
-      distill_path_kernel<TIn, VEC><<<(unsigned)div_up64(tasks, kPathWarps), kPathWarps * 32, smem, stream>>>(a, k);
+      int warps = kPathWarps;   // with the fewest that have no tile
+      for (int w = kPathWarps - 1; w > 0; --w)
+        if (div_up(p.tiles, w) * w < div_up(p.tiles, warps) * warps) warps = w;
+      const int smem = (int)sizeof(PathCta) + warps * (int)sizeof(PathWarp<TIn>);
+      allow_dyn_smem(distill_path_kernel<TIn, VEC>, (int)sizeof(PathCta) + kPathWarps * (int)sizeof(PathWarp<TIn>));
+      distill_path_kernel<TIn, VEC><<<(unsigned)((i64)a.B * p.segs * div_up(p.tiles, warps)), warps * 32, smem, stream>>>(
+          a, k);
       TB200_CHECK_LAUNCH();
     }
     if (nodes > 1) {   // (a single node is a path)
