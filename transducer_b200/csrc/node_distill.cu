@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
     const float* __restrict__ rest, float* __restrict__ costs, DistillSaved saved, int K, float scale2) {
   constexpr int kNodes = kCta<G> / G, kTurn = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;   // vectors of a row at a time
   extern __shared__ __align__(16) unsigned char memory[];
-  __shared__ double scratch[64];
+  __shared__ double2 scratch[64];
   const int sub = threadIdx.x / G, tid = threadIdx.x % G;
   const i64 node = (i64)blockIdx.x * kNodes + sub;
   if (node >= (i64)a.B * a.N) return;

@@ -89,15 +89,15 @@ __device__ __forceinline__ NodeScores<TIn> node_scores(const NodeArgs& a, i64 no
 }
 
 // Sums and maxima over a group of G threads (a warp, or the CTA): every thread gets the result, and
-// its bits do not depend on anything but the values.  `scratch`: two sets of 32 places in shared
-// memory, used in turn, so that one barrier per reduction is enough.
+// its bits do not depend on anything but the values.  `scratch`: two sets of 32 places of 16 bytes in
+// shared memory, used in turn, so that one barrier per reduction is enough.
 template <int G>
 struct Group {
   static constexpr int kWarps = G / 32;
   int tid, lane, warp;
-  double* scratch;   // [2][32], of the CTA; unused by a warp
+  double2* scratch;   // [2][32], of the CTA; unused by a warp
   int turn = 0;
-  __device__ __forceinline__ Group(int tid_, double* scratch_)
+  __device__ __forceinline__ Group(int tid_, double2* scratch_)
       : tid(tid_), lane(tid_ & 31), warp(tid_ >> 5), scratch(scratch_) {}
 
   __device__ __forceinline__ void sync() const {
@@ -125,6 +125,23 @@ struct Group {
   }
   __device__ __forceinline__ float sum(float v) { return reduce(v, [](float a, float b) { return a + b; }); }
   __device__ __forceinline__ double sum(double v) { return reduce(v, [](double a, double b) { return a + b; }); }
+  // two sums at once
+  __device__ __forceinline__ void sum(double& a, float& b) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if constexpr (G > 32) {
+      const double2 v = exchange(make_double2(a, (double)b));
+      a = v.x, b = (float)v.y;
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+      }
+    }
+  }
   __device__ __forceinline__ int sum(int v) {
     return across(__reduce_add_sync(0xffffffffu, v), [](int a, int b) { return a + b; });
   }

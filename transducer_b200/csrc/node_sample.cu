@@ -3,8 +3,8 @@
 // Weights are 2^x in 32 bits, x = (z - m) log2(e) / temperature.  They decide where they are sure to:
 // the difference from the maximum m is rounded, the factor is, their product is (2^-24 of x each), and
 // ex2 is good to 2^-22, so that a weight is off by at most 2^-24 * 2.1 |x| + 2^-22 of itself, and any sum
-// of weights by 2^-24 * 2.1 sum w |x| + 2^-22 sum w, both sums over the row; with ten roundings of the
-// sum itself (a thread's part is added up in 32 bits, parts are in 64) that is `unsure` below.  Where a
+// of weights by 2^-24 * 2.1 sum w |x| + 2^-22 sum w, both sums over the row; with twelve roundings
+// of the sum itself (a thread's part is eight sums in 32 bits, parts are in 64) that is `unsure` below.  Where a
 // comparison is closer than that the sums are formed anew from memory with exponentials in 64 bits.
 #include <algorithm>
 #include <cfloat>
@@ -51,7 +51,7 @@ __device__ __noinline__ Cut general_share(NodeScores<TIn> s, int V, Group<G> g, 
   return cut;
 }
 
-constexpr double kUnsureSlope = 2.1 * 0x1p-24, kUnsureSum = 0x1p-22 + 10 * 0x1p-24;
+constexpr double kUnsureSlope = 2.1 * 0x1p-24, kUnsureSum = 0x1p-22 + 12 * 0x1p-24;
 constexpr int kNear = 64;          // words about a cut that are listed
 constexpr float kAbove = 2.0f;     // above every weight
 constexpr int kResidentBytes = 220 * 1024;   // of shared memory for a row's weights, beside the lists
@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     NodeArgs a, const float* __restrict__ uniforms, int* __restrict__ words, float* __restrict__ logProbs,
     SampleRule rule, int seg) {
   constexpr int kRows = kCta<G> / G, kPass = RESIDENT ? 4 : VEC;   // words a thread takes at a time
-  extern __shared__ __align__(16) float weights[];
-  __shared__ double scratch[64];
+  extern __shared__ __align__(16) float weights[];   // a warp's part of a row: seg = 128 * trips words
+  __shared__ double2 scratch[64];
   __shared__ Entry listAll[kRows][kNear], sortedAll[kRows][kNear];
   __shared__ int filledAll[kRows];
   __shared__ int sureAll[kRows];
@@ -190,10 +190,12 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   if (!s.here) return answer(-1, 0.0f);
   Group<G> g(tid, scratch);
   const Place<TIn, VEC, G, 0> at(s, a.V, seg, g.warp, g.lane);
-  float* const w = weights + sub * seg * Group<G>::kWarps + at.first;   // the warp's words; scores at first
+  float* const row = weights + sub * seg * Group<G>::kWarps;   // (scores at first)
+  float* const w = row + at.first;                             // the warp's words
+  const int trips = seg / 128;
   const float nan = __int_as_float(0x7fffffff);
   float m = neg_inf();
-#pragma unroll 4
+#pragma unroll(VEC == 8 ? 3 : 5)
   for (int o = g.lane * VEC; o < (RESIDENT ? seg : at.end - at.first); o += 32 * VEC) {
     float x[VEC];
 #pragma unroll
@@ -232,11 +234,12 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   // `keep` says it so far
   auto each = [&](auto f) {
     if constexpr (RESIDENT) {
-#pragma unroll 2
-      for (int o = g.lane * 4; o < seg; o += 128) {
-        const float4 q = *reinterpret_cast<const float4*>(w + o);
-        const float y[4] = {q.x, q.y, q.z, q.w};
-        f(y, at.first + o);
+      const float4* q = reinterpret_cast<const float4*>(w) + g.lane;
+#pragma unroll 4
+      for (int j = 0; j < trips; ++j) {
+        const float4 x = q[32 * j];
+        const float y[4] = {x.x, x.y, x.z, x.w};
+        f(y, at.first + 128 * j + 4 * g.lane);
       }
     } else {
 #pragma unroll 1
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       }
     }
   };
-  // f(word, place) for those of this thread's words whose weight is in [from, below): few of them
+  // f(word) for those of this thread's words whose weight is in [from, below): few of them
   auto each_between = [&](float from, float below, auto f) {
     each([&](const float (&y)[kPass], int v) {
       unsigned in = 0;
@@ -262,84 +265,85 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       for (; in; in &= in - 1) f(v + __ffs(in) - 1);
     });
   };
-  auto apply = [&] {   // `keep` has changed
+  // The sum of this thread's words that stay, a few weights at a time in 32 bits; those below keep.lo become 0 (what
+  // else does not stay has been made 0), and those below keep.minP, of which a few are close to it.
+  auto apply = [&] {
+    double sum = 0.0;
     if constexpr (RESIDENT) {
-      const float tested = fmaxf(keep.hi, keep.sure());
+      const float lo = keep.lo, tested = keep.sure();
+      float4* q = reinterpret_cast<float4*>(w) + g.lane;
 #pragma unroll 2
-      for (int o = g.lane * 4; o < seg; o += 128) {
-        const float4 q = *reinterpret_cast<const float4*>(w + o);
-        float y[4] = {q.x, q.y, q.z, q.w};
-        unsigned test = 0;
+      for (int j = 0; j < trips; ++j) {
+        const float4 x = q[32 * j];
+        float y[4] = {x.x, x.y, x.z, x.w};
+        bool test = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (y[i] < keep.lo) y[i] = 0.0f;
-          else if (y[i] < tested) test |= 1u << i;
+          y[i] = y[i] < lo ? 0.0f : y[i];
+          test |= y[i] > 0.0f && y[i] < tested;
         }
-#pragma unroll 1
-        for (; test; test &= test - 1) {
-          const int i = __ffs(test) - 1, v = at.first + o + i;
-          const float z = at.score(v), x = weight(z);
-          if (!keep(x, z, v)) {
+        if (test) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (k == i) y[k] = 0.0f;
-          }
+          for (int i = 0; i < 4; ++i)
+            if (y[i] > 0.0f && y[i] < tested && keep.exact(at.score(at.first + 128 * j + 4 * g.lane + i)) < keep.minP)
+              y[i] = 0.0f;
         }
-        *reinterpret_cast<float4*>(w + o) = make_float4(y[0], y[1], y[2], y[3]);
+        q[32 * j] = make_float4(y[0], y[1], y[2], y[3]);
+        sum += (double)((y[0] + y[1]) + (y[2] + y[3]));
       }
+    } else {
+      each([&](const float (&y)[kPass], int) {
+#pragma unroll
+        for (int i = 0; i < kPass; ++i) sum += (double)y[i];
+      });
     }
+    return sum;
   };
   // The weights, and their first moments: of |x| for the bound on what is unsure, of x^2 for a first guess.
   double part = 0.0;
   float slope = 0.0f, square = 0.0f;
-  auto moments = [&](float x, float y) {
-    const float b = fmaxf(x, -200.0f), c = b * y;
-    slope -= c;
-    square += c * b;
-  };
-  if constexpr (RESIDENT) {
+  auto form = [&](auto guessed) {
+    auto moments = [&](float x, float y) {
+      const float b = fmaxf(x, -200.0f);
+      slope = fmaf(-b, y, slope);
+      if (decltype(guessed)::value) square = fmaf(b * b, y, square);
+    };
+    if constexpr (RESIDENT) {
+      float4* q = reinterpret_cast<float4*>(w) + g.lane;
 #pragma unroll 2
-    for (int o = g.lane * 4; o < seg; o += 128) {
-      const float4 q = *reinterpret_cast<const float4*>(w + o);
-      const float z[4] = {q.x, q.y, q.z, q.w};
-      float y[4];
+      for (int j = 0; j < trips; ++j) {
+        const float4 x = q[32 * j];
+        const float z[4] = {x.x, x.y, x.z, x.w};
+        float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = weight.exponent(z[i]);
-        y[i] = ex2(x);
-        moments(x, y[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float e = weight.exponent(z[i]);
+          y[i] = ex2(e);
+          moments(e, y[i]);
+        }
+        q[32 * j] = make_float4(y[0], y[1], y[2], y[3]);
+        part += (double)((y[0] + y[1]) + (y[2] + y[3]));
       }
-      *reinterpret_cast<float4*>(w + o) = make_float4(y[0], y[1], y[2], y[3]);
-      part += (double)((y[0] + y[1]) + (y[2] + y[3]));
-    }
-  } else {
+    } else {
 #pragma unroll 1
-    for (int o = g.lane * VEC; at.first + o < at.end; o += 32 * VEC) {
-      float x[VEC];
-      at.load(at.first + o, x);
+      for (int o = g.lane * VEC; at.first + o < at.end; o += 32 * VEC) {
+        float x[VEC];
+        at.load(at.first + o, x);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float e = weight.exponent(x[i]), y = ex2(e);
-        moments(e, y);
-        part += (double)y;
+        for (int i = 0; i < VEC; ++i) {
+          const float e = weight.exponent(x[i]), y = ex2(e);
+          moments(e, y);
+          part += (double)y;
+        }
       }
     }
-  }
-  double total = g.sum(part);
-  if (total != total) return answer(-1, nan);
-  slope = g.sum(slope);
-  const double unsure = 1.01 * kUnsureSlope * slope + kUnsureSum * total;
-  // this thread's part of the sum, a few weights at a time in 32 bits
-  auto part_of = [&] {
-    double sum = 0.0;
-    each([&](const float (&y)[kPass], int) {
-      float few = y[0];
-#pragma unroll
-      for (int i = 1; i < kPass; ++i) few += y[i];
-      sum += (double)few;
-    });
-    return sum;
   };
+  if (rule.topP < 1.0) form(std::true_type{});
+  else form(std::false_type{});
+  double total = part;
+  g.sum(total, slope);
+  if (total != total) return answer(-1, nan);
+  const double unsure = 1.01 * kUnsureSlope * slope + kUnsureSum * total;
 
   // The first words of the order with a count of k, or a weight of topP * total.  False: that is all.
   // A threshold that fewer reach and one that enough reach are brought together until at most kNear words
@@ -350,25 +354,45 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   auto find_cut = [&](auto by_weight, int k, float guess) {
     constexpr bool kByWeight = decltype(by_weight)::value;
     double target = kByWeight ? rule.topP * total : (double)k;
-    auto measure = [&](float t, double& sum, int& n) {
-      double part = 0.0;
-      int c = 0;
-      each([&](const float (&y)[kPass], int) {
-        float few = 0.0f;
+    auto measure = [&](float t) -> double {
+      if constexpr (!kByWeight) {
+        int c = 0;
+        each([&](const float (&y)[kPass], int) {
 #pragma unroll
-        for (int i = 0; i < kPass; ++i)
-          if (y[i] >= t) {
-            few += y[i];
-            ++c;
-          }
-        if (kByWeight) part += (double)few;
-      });
-      n = g.sum(c);
-      sum = kByWeight ? g.sum(part) : (double)n;
+          for (int i = 0; i < kPass; ++i) c += y[i] >= t ? 1 : 0;
+        });
+        return g.sum(c);
+      } else if constexpr (RESIDENT) {
+        float sum[8] = {};
+        const float4* q = reinterpret_cast<const float4*>(w) + g.lane;
+        auto add = [&](const float4& x, int i) {
+          if (x.x >= t) sum[i] += x.x;
+          if (x.y >= t) sum[i + 1] += x.y;
+          if (x.z >= t) sum[i + 2] += x.z;
+          if (x.w >= t) sum[i + 3] += x.w;
+        };
+        int j = 0;
+#pragma unroll 2
+        for (; j + 1 < trips; j += 2) {
+          const float4 x = q[32 * j], y = q[32 * j + 32];
+          add(x, 0);
+          add(y, 4);
+        }
+        if (j < trips) add(q[32 * j], 0);
+        return g.sum((double)(((sum[0] + sum[4]) + (sum[1] + sum[5])) + ((sum[2] + sum[6]) + (sum[3] + sum[7]))));
+      } else {
+        double sum = 0.0;
+        each([&](const float (&y)[kPass], int) {
+#pragma unroll
+          for (int i = 0; i < kPass; ++i)
+            if (y[i] >= t) sum += (double)y[i];
+        });
+        return g.sum(sum);
+      }
     };
-    float lo = FLT_MIN, hi = kAbove, t = guess;
+    float lo = FLT_MIN, hi = kAbove, t = guess, had = 3e38f;
     double vLo = 0.0, vHi = 0.0;
-    int nLo = 0, nHi = 0, stuck = 0;
+    int stuck = 0;
     bool done = false;
     Cut cut;
     const float floor = (float)(1e-5 * total);
@@ -376,26 +400,40 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       return kByWeight ? __log2f(fmaxf((float)v, 0.25f)) - __log2f(fmaxf((float)(total - v), floor))
                        : -__log2f(fmaxf((float)v, 0.5f));
     };
+    const float l_target = level(target);
 #pragma unroll 1
     for (int round = 0; round < 64 && !done; ++round) {
-      double v;
-      int n;
-      measure(t, v, n);
-      const int had = nLo - nHi;
-      if (v >= target) lo = t, vLo = v, nLo = n;
-      else hi = t, vHi = v, nHi = n;
-      if (nLo == 0) {   // nothing is known from below yet
+      const double v = measure(t);
+      if (v >= target) lo = t, vLo = v;
+      else hi = t, vHi = v;
+      if (vLo == 0.0) {   // nothing is known from below yet
         if (!kByWeight && t == FLT_MIN) return false;   // there are no more words than that
         if (t == FLT_MIN) break;
         t = round == 0 && t > 1e-9f ? t * 1e-3f : FLT_MIN;
         continue;
       }
-      const int c = nLo - nHi;
-      if (c > kNear) {
-        stuck = had > 0 && c > had / 2 ? stuck + 1 : 0;
+      // how many words lie between: known, or at most the weight over the lesser threshold
+      const float between = kByWeight ? (float)(vLo - vHi) / lo : (float)(vLo - vHi);
+      bool listed = between <= kNear;
+      int c = 0;
+      if (listed) {
+        g.sync();
+        if (tid == 0) *filled = 0;
+        g.sync();
+        each_between(lo, hi, [&](int v) {
+          const int i = atomicAdd(filled, 1);
+          if (i < kNear) list[i] = entry_of(at.score(v), v);
+        });
+        g.sync();
+        c = *filled;
+        listed = c <= kNear;   // (weights next to nothing may be more)
+      }
+      if (!listed) {
+        stuck = between > 0.5f * had ? stuck + 1 : 0;
+        had = between;
         const float xl = __log2f(lo), xh = fminf(__log2f(hi), 0.1f), l = level(vLo), h = level(vHi);
-        float f = (l - level(target)) / (l - h);
-        const float past = 0.3f * kNear / (float)c;
+        float f = (l - l_target) / (l - h);
+        const float past = 0.3f * kNear / fmaxf(between, (float)kNear);
         f = stuck >= 2 ? 0.5f : f < 0.5f ? f + past : f - past;
         f = fminf(fmaxf(f, 0.01f), 0.99f);
         t = ex2(xl + f * (xh - xl));
@@ -403,45 +441,54 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         if (!(t > lo && t < hi)) break;
         continue;
       }
-      g.sync();
-      if (tid == 0) *filled = 0;
-      g.sync();
-      each_between(lo, hi, [&](int v) { list[atomicAdd(filled, 1)] = entry_of(at.score(v), v); });
-      g.sync();
-      for (int i = tid; i < c; i += G) {
-        const Entry mine = list[i];
-        sorted[entries_before(list, c, mine)] = mine;
+      if constexpr (G >= 4 * kNear) {   // four threads per entry, each looking at every fourth of the others
+        const Entry mine = tid / 4 < c ? list[tid / 4] : ~0ull;
+        int place = 0;
+#pragma unroll 4
+        for (int i = tid % 4; i < c; i += 4) place += list[i] > mine ? 1 : 0;
+        place += __shfl_xor_sync(0xffffffffu, place, 1);
+        place += __shfl_xor_sync(0xffffffffu, place, 2);
+        if (tid % 4 == 0 && tid / 4 < c) sorted[place] = mine;
+      } else {
+        for (int i = tid; i < c; i += G) {
+          const Entry mine = list[i];
+          sorted[entries_before(list, c, mine)] = mine;
+        }
       }
       g.sync();
-      int kept = k - nHi;
+      int kept = k - (int)vHi;
       bool enough = true;
       if (kByWeight) {
-        // every warp for itself: lane i has entries 2 i and 2 i + 1
+        // by one warp: lane i has entries 2 i and 2 i + 1.  In 32 bits, or, where the sum up to a word is too close
+        // to the target to tell, in 64 bits from memory.
         const int i0 = 2 * g.lane, i1 = i0 + 1;
-        const double w0 = i0 < c ? keep.exact(key_score(entry_key(sorted[i0]))) : 0.0;
-        const double w1 = i1 < c ? keep.exact(key_score(entry_key(sorted[i1]))) : 0.0;
-        double upto = w0 + w1;
+        auto judge = [&](double above, double share, double w0, double w1, double margin) {
+          double upto = w0 + w1;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double x = __shfl_up_sync(0xffffffffu, upto, o);
-          if (g.lane >= o) upto += x;
-        }
-        double above = vHi;
-        // whether the sum up to a word is too close to the target to tell
-        const double d0 = above + (upto - w1) - target, d1 = above + upto - target;
-        const bool close = (g.lane == 0 && fabs(above - target) <= unsure) || (i0 < c && fabs(d0) <= unsure) ||
-                           (i1 < c && fabs(d1) <= unsure);
-        if (__any_sync(0xffffffffu, close)) {
+          for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (g.lane >= o) upto += x;
+          }
+          // the words whose predecessors have not reached the target
+          const double d0 = above + (upto - w1 - w0) - share, d1 = above + (upto - w1) - share;
+          const double end = above + __shfl_sync(0xffffffffu, upto, 31) - share;
+          const bool close = (i0 < c && fabs(d0) <= margin) || (i1 < c && fabs(d1) <= margin) || fabs(end) <= margin;
+          const unsigned b0 = __ballot_sync(0xffffffffu, i0 < c && d0 < 0.0), b1 = __ballot_sync(0xffffffffu, i1 < c && d1 < 0.0);
+          const bool any = __any_sync(0xffffffffu, close);
+          if (g.lane == 0) *filled = 4 * (__popc(b0) + __popc(b1)) + (end >= 0.0 ? 2 : 0) + (any ? 1 : 0);
+        };
+        auto score = [&](int i) { return i < c ? key_score(entry_key(sorted[i])) : neg_inf(); };
+        if (g.warp == 0) judge(vHi, target, (double)weight(score(i0)), (double)weight(score(i1)), unsure);
+        g.sync();
+        if (*filled & 1) {
           const ExactSums sums = exact_sums<TIn, VEC, G>(s, a.V, g, keep, weight, hi);
-          g.sync();
-          above = sums.above;
           target = rule.topP * sums.all;
+          g.sync();
+          if (g.warp == 0) judge(sums.above, target, keep.exact(score(i0)), keep.exact(score(i1)), -1.0);
+          g.sync();
         }
-        // the words whose predecessors have not reached the target
-        const unsigned b0 = __ballot_sync(0xffffffffu, i0 < c && above + (upto - w1 - w0) < target);
-        const unsigned b1 = __ballot_sync(0xffffffffu, i1 < c && above + (upto - w1) < target);
-        kept = __popc(b0) + __popc(b1);
-        enough = above + __shfl_sync(0xffffffffu, upto, 31) >= target;
+        kept = *filled >> 2;
+        enough = *filled & 2;
       }
       // (32-bit weights of different scores may come out in the wrong order by a rounding: not so the
       // cut's and those beyond the thresholds)
@@ -455,6 +502,9 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       else if (lo > FLT_MIN && (!enough || y * 0.999996f < lo)) t = fmaxf(lo * 0.99997f, FLT_MIN);
       else if (kept > 0 && enough) done = true;
       else break;
+      if constexpr (RESIDENT)   // what lies between and does not stay
+        if (done)
+          for (int i = kept + tid; i < c; i += G) row[entry_word(sorted[i])] = 0.0f;
     }
     if (!done) {
       cut = kByWeight ? general_share<TIn, VEC, G>(s, a.V, g, keep.cut, keep.exact, rule.topP)
@@ -462,30 +512,39 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       g.sync();
       lo = FLT_MIN;
       hi = kAbove;
+      if constexpr (RESIDENT)
+        each([&](const float (&)[kPass], int v) {
+          for (int i = 0; i < kPass; ++i)
+            if (v + i < a.V && !cut.keeps(at.score(v + i), v + i)) row[v + i] = 0.0f;
+        });
     }
+    g.sync();
     keep.lo = lo;
     keep.hi = hi;
     keep.cut = cut;
-    apply();
     return true;
   };
-  if (rule.topK > 0 && rule.topK < a.V && find_cut(std::false_type{}, rule.topK, 0x1p-8f) && rule.topP < 1.0)
-    total = g.sum(part_of());
+  bool cutAny = false;   // `keep` says something that has not been applied
+  if (rule.topK > 0 && rule.topK < a.V) {
+    cutAny = find_cut(std::false_type{}, rule.topK, 0x1p-8f);
+    if (cutAny && rule.topP < 1.0) total = g.sum(apply());
+  }
   if (rule.topP < 1.0) {
     const float mean = -slope / (float)total, deviation = sqrtf(fmaxf(g.sum(square) / (float)total - mean * mean, 0.0f));
     const float p = (float)rule.topP, odds = 0.55f * (__log2f(p) - __log2f(1.0f - p)) * 0.6931472f;
     find_cut(std::true_type{}, 0, fmaxf(ex2(fminf(mean - odds * deviation, -0.05f)), 0.25f * (1.0f - p) / (float)a.V));
+    cutAny = true;
   }
   if (rule.minP > 0.0) {
     keep.minP = rule.minP;
     keep.lo = fmaxf(keep.lo, (float)rule.minP * 0.9999f);
-    apply();
+    cutAny = true;
   }
 
   // the draw: the warp, its vectors, the word
   float u = uniforms[node];
   u = u < 0.0f ? 0.0f : u < 1.0f ? u : 0.99999994f;
-  part = part_of();
+  if (cutAny) part = apply();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
   double own = g.exchange(part), upto = own;
@@ -553,7 +612,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     }
     if (g.lane == 0) {
       *sure = certain;
-      if (certain) words[node] = found, logProbs[node] = (float)log(keep.exact(at.score(found)) / total);
+      if (certain) words[node] = found, logProbs[node] = (float)((double)(at.score(found) - m) * keep.exact.scale) - logf((float)total);
     }
   }
   g.sync();
@@ -582,7 +641,7 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
     auto launch = [&](auto group, auto resident) {
       constexpr int G = decltype(group)::value, rows = kCta<G> / G;
       auto kernel = sample_words_kernel<TIn, decltype(vec)::value, G, decltype(resident)::value>;
-      const int seg = (int)round_up64(div_up(a.V, G / 32), 32);
+      const int seg = (int)round_up64(div_up(a.V, G / 32), 128);
       const int smem = decltype(resident)::value ? rows * seg * (G / 32) * (int)sizeof(float) : 0;
       if (smem > 32 * 1024) allow_dyn_smem(kernel, kResidentBytes);
       ScopedKernel prof("sample_words", stream);
@@ -593,7 +652,7 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
     if (a.V <= 1024) launch(integral_constant<int, 32>{}, std::true_type{});
     else if (a.V <= 4096) launch(integral_constant<int, 128>{}, std::true_type{});
     else if (a.V <= 16384) launch(integral_constant<int, 256>{}, std::true_type{});
-    else if (round_up64(div_up(a.V, 32), 32) * 32 * 4 <= kResidentBytes)
+    else if (round_up64(div_up(a.V, 32), 128) * 32 * 4 <= kResidentBytes)
       launch(integral_constant<int, 1024>{}, std::true_type{});
     else launch(integral_constant<int, 1024>{}, std::false_type{});
   });

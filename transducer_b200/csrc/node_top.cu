@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __r
                                                             float* __restrict__ logits,
                                                             float* __restrict__ rest, int k, int seg, float scale) {
   constexpr int kRows = kCta<G> / G;
-  __shared__ double scratch[64];
+  __shared__ double2 scratch[64];
   __shared__ Entry listAll[kRows][kListed];
   __shared__ int filledAll[kRows];
   __shared__ Entry edgeAll[kRows][2];   // the last word of the k, and the next one (0: not in the list)
