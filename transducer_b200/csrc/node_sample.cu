@@ -3,9 +3,11 @@
 // Weights are 2^x in 32 bits, x = (z - m) log2(e) / temperature.  They decide where they are sure to:
 // the difference from the maximum m is rounded, the factor is, their product is (2^-24 of x each), and
 // ex2 is good to 2^-22, so that a weight is off by at most 2^-24 * 2.1 |x| + 2^-22 of itself, and any sum
-// of weights by 2^-24 * 2.1 sum w |x| + 2^-22 sum w, both sums over the row; with twelve roundings
-// of the sum itself (a thread's part is eight sums in 32 bits, parts are in 64) that is `unsure` below.  Where a
-// comparison is closer than that the sums are formed anew from memory with exponentials in 64 bits.
+// of weights by 2^-24 * 2.1 sum w |x| + 2^-22 sum w, both sums over the row (the former is log2 of the number of
+// words times the latter at most: the difference of the logarithm of the sum and the entropy).  With twenty roundings
+// of the sum itself (a thread has eight sums of up to nine weights, then come eleven steps; the row's whole and the
+// draw's sums are of fours in 32 bits and 64 bits from there) that is `unsure` below.  Where a comparison is closer than
+// that the sums are formed anew from memory with exponentials in 64 bits.
 #include <algorithm>
 #include <cfloat>
 
@@ -15,12 +17,34 @@
 namespace tb200 {
 namespace {
 
+// exp(x) for x <= 0 in 64 bits: 2^n times the Taylor series of exp(f) for |f| <= log(2) / 2, whose twelfth power
+// is below 2^-46 of it and whose 13th of 1e-15; 0 below exp(-700).  The library's own takes about twice the
+// instructions, and a row's 64-bit sums are nothing but these.
+__device__ __forceinline__ double exp64(double x) {
+  if (!(x > -700.0)) return x != x ? x : 0.0;
+  const double n = rint(x * 1.4426950408889634074);
+  // log(2) as its 32-bit rounding, n times which is exact, and the rest
+  const double f = fma(-n, -1.904654299957767878541823e-9, fma(-n, (double)0.69314718246459960937f, x));
+  constexpr double inverse[13] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
+                                  1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
+  double y = inverse[12];
+#pragma unroll
+  for (int i = 11; i >= 0; --i) y = fma(y, f, inverse[i]);
+  return __hiloint2double(__double2hiint(y) + ((int)n << 20), __double2loint(y));
+}
+
 // exp((z - m) scale) in 64 bits.
 struct ExactWeight {
   float m;
   double scale;
-  __device__ __forceinline__ double operator()(float z) const { return exp(((double)z - (double)m) * scale); }
+  __device__ __forceinline__ double operator()(float z) const { return exp64(((double)z - (double)m) * scale); }
 };
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // The first words of the order, among those that `all` keeps, that have the share topP of their weight.
 template <typename TIn, int VEC, int G>
@@ -51,7 +75,7 @@ __device__ __noinline__ Cut general_share(NodeScores<TIn> s, int V, Group<G> g, 
   return cut;
 }
 
-constexpr double kUnsureSlope = 2.1 * 0x1p-24, kUnsureSum = 0x1p-22 + 12 * 0x1p-24;
+constexpr double kUnsureSlope = 2.1 * 0x1p-24, kUnsureSum = 0x1p-22 + 20 * 0x1p-24;
 constexpr int kNear = 64;          // words about a cut that are listed
 constexpr float kAbove = 2.0f;     // above every weight
 constexpr int kResidentBytes = 220 * 1024;   // of shared memory for a row's weights, beside the lists
@@ -176,18 +200,21 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   extern __shared__ __align__(16) float weights[];   // a warp's part of a row: seg = 128 * trips words
   __shared__ double2 scratch[64];
   __shared__ Entry listAll[kRows][kNear], sortedAll[kRows][kNear];
+  __shared__ int nearAll[kRows][kNear];
   __shared__ int filledAll[kRows];
   __shared__ int sureAll[kRows];
   const int sub = threadIdx.x / G, tid = threadIdx.x % G;
   const i64 node = (i64)blockIdx.x * kRows + sub;
   if (node >= (i64)a.B * a.N) return;
   Entry *list = listAll[sub], *sorted = sortedAll[sub];
-  int *filled = &filledAll[sub], *sure = &sureAll[sub];
+  int *near = nearAll[sub], *filled = &filledAll[sub], *sure = &sureAll[sub];
   auto answer = [&](int word, float logProb) {
     if (tid == 0) words[node] = word, logProbs[node] = logProb;
   };
   const NodeScores<TIn> s = node_scores<TIn>(a, node);
   if (!s.here) return answer(-1, 0.0f);
+  float u = uniforms[node];
+  u = u < 0.0f ? 0.0f : u < 1.0f ? u : 0.99999994f;
   Group<G> g(tid, scratch);
   const Place<TIn, VEC, G, 0> at(s, a.V, seg, g.warp, g.lane);
   float* const row = weights + sub * seg * Group<G>::kWarps;   // (scores at first)
@@ -299,14 +326,16 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     }
     return sum;
   };
-  // The weights, and their first moments: of |x| for the bound on what is unsure, of x^2 for a first guess.
+  // The weights, and where a share of them is looked for their moments: of |x| for the bound on what is unsure,
+  // of x^2 for a first guess.
   double part = 0.0;
   float slope = 0.0f, square = 0.0f;
   auto form = [&](auto guessed) {
     auto moments = [&](float x, float y) {
+      if (!decltype(guessed)::value) return;
       const float b = fmaxf(x, -200.0f);
       slope = fmaf(-b, y, slope);
-      if (decltype(guessed)::value) square = fmaf(b * b, y, square);
+      square = fmaf(b * b, y, square);
     };
     if constexpr (RESIDENT) {
       float4* q = reinterpret_cast<float4*>(w) + g.lane;
@@ -341,7 +370,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   if (rule.topP < 1.0) form(std::true_type{});
   else form(std::false_type{});
   double total = part;
-  g.sum(total, slope);
+  if (rule.topP < 1.0) g.sum(total, slope);
+  else total = g.sum(total), slope = (float)total * lg2((float)a.V);   // (its bound)
   if (total != total) return answer(-1, nan);
   const double unsure = 1.01 * kUnsureSlope * slope + kUnsureSum * total;
 
@@ -354,14 +384,14 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   auto find_cut = [&](auto by_weight, int k, float guess) {
     constexpr bool kByWeight = decltype(by_weight)::value;
     double target = kByWeight ? rule.topP * total : (double)k;
-    auto measure = [&](float t) -> double {
+    auto measure = [&](float t) -> float {
       if constexpr (!kByWeight) {
         int c = 0;
         each([&](const float (&y)[kPass], int) {
 #pragma unroll
           for (int i = 0; i < kPass; ++i) c += y[i] >= t ? 1 : 0;
         });
-        return g.sum(c);
+        return (float)g.sum(c);
       } else if constexpr (RESIDENT) {
         float sum[8] = {};
         const float4* q = reinterpret_cast<const float4*>(w) + g.lane;
@@ -379,7 +409,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
           add(y, 4);
         }
         if (j < trips) add(q[32 * j], 0);
-        return g.sum((double)(((sum[0] + sum[4]) + (sum[1] + sum[5])) + ((sum[2] + sum[6]) + (sum[3] + sum[7]))));
+        return g.sum(((sum[0] + sum[4]) + (sum[1] + sum[5])) + ((sum[2] + sum[6]) + (sum[3] + sum[7])));
       } else {
         double sum = 0.0;
         each([&](const float (&y)[kPass], int) {
@@ -387,33 +417,34 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
           for (int i = 0; i < kPass; ++i)
             if (y[i] >= t) sum += (double)y[i];
         });
-        return g.sum(sum);
+        return (float)g.sum(sum);
       }
     };
-    float lo = FLT_MIN, hi = kAbove, t = guess, had = 3e38f;
-    double vLo = 0.0, vHi = 0.0;
+    const float floor = (float)(1e-5 * total), all = (float)total, want = (float)target;
+    auto level = [&](float v) {
+      return kByWeight ? lg2(fmaxf(v, 0.25f)) - lg2(fmaxf(all - v, floor)) : -lg2(fmaxf(v, 0.5f));
+    };
+    // thresholds, what has been measured there, their exponents and levels
+    float lo = FLT_MIN, hi = kAbove, vLo = 0.0f, vHi = 0.0f, xLo = -126.0f, xHi = 0.1f, lLo = 0.0f, lHi = level(0.0f);
+    float t = guess, x = lg2(guess), had = 3e38f;
+    const float lWant = level(want);
     int stuck = 0;
     bool done = false;
     Cut cut;
-    const float floor = (float)(1e-5 * total);
-    auto level = [&](double v) {
-      return kByWeight ? __log2f(fmaxf((float)v, 0.25f)) - __log2f(fmaxf((float)(total - v), floor))
-                       : -__log2f(fmaxf((float)v, 0.5f));
-    };
-    const float l_target = level(target);
 #pragma unroll 1
     for (int round = 0; round < 64 && !done; ++round) {
-      const double v = measure(t);
-      if (v >= target) lo = t, vLo = v;
-      else hi = t, vHi = v;
-      if (vLo == 0.0) {   // nothing is known from below yet
+      const float v = measure(t), l = level(v);
+      if (v >= want) lo = t, vLo = v, xLo = x, lLo = l;
+      else hi = t, vHi = v, xHi = x, lHi = l;
+      if (vLo == 0.0f) {   // nothing is known from below yet
         if (!kByWeight && t == FLT_MIN) return false;   // there are no more words than that
         if (t == FLT_MIN) break;
         t = round == 0 && t > 1e-9f ? t * 1e-3f : FLT_MIN;
+        x = lg2(t);
         continue;
       }
       // how many words lie between: known, or at most the weight over the lesser threshold
-      const float between = kByWeight ? (float)(vLo - vHi) / lo : (float)(vLo - vHi);
+      const float between = kByWeight ? __fdividef(vLo - vHi, lo) : vLo - vHi;
       bool listed = between <= kNear;
       int c = 0;
       if (listed) {
@@ -422,22 +453,29 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         g.sync();
         each_between(lo, hi, [&](int v) {
           const int i = atomicAdd(filled, 1);
-          if (i < kNear) list[i] = entry_of(at.score(v), v);
+          if (i < kNear) near[i] = v;
         });
         g.sync();
         c = *filled;
         listed = c <= kNear;   // (weights next to nothing may be more)
+        if (listed) {
+          for (int i = tid; i < c; i += G) list[i] = entry_of(at.score(near[i]), near[i]);
+          g.sync();
+        }
       }
       if (!listed) {
         stuck = between > 0.5f * had ? stuck + 1 : 0;
         had = between;
-        const float xl = __log2f(lo), xh = fminf(__log2f(hi), 0.1f), l = level(vLo), h = level(vHi);
-        float f = (l - l_target) / (l - h);
-        const float past = 0.3f * kNear / fmaxf(between, (float)kNear);
+        float f = __fdividef(lLo - lWant, lLo - lHi);
+        const float past = __fdividef(0.3f * kNear, fmaxf(between, (float)kNear));
         f = stuck >= 2 ? 0.5f : f < 0.5f ? f + past : f - past;
         f = fminf(fmaxf(f, 0.01f), 0.99f);
-        t = ex2(xl + f * (xh - xl));
-        if (!(t > lo && t < hi)) t = __uint_as_float((__float_as_uint(lo) + __float_as_uint(hi)) / 2);
+        x = xLo + f * (xHi - xLo);
+        t = ex2(x);
+        if (!(t > lo && t < hi)) {
+          t = __uint_as_float((__float_as_uint(lo) + __float_as_uint(hi)) / 2);
+          x = lg2(t);
+        }
         if (!(t > lo && t < hi)) break;
         continue;
       }
@@ -478,7 +516,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
           if (g.lane == 0) *filled = 4 * (__popc(b0) + __popc(b1)) + (end >= 0.0 ? 2 : 0) + (any ? 1 : 0);
         };
         auto score = [&](int i) { return i < c ? key_score(entry_key(sorted[i])) : neg_inf(); };
-        if (g.warp == 0) judge(vHi, target, (double)weight(score(i0)), (double)weight(score(i1)), unsure);
+        if (g.warp == 0) judge((double)vHi, target, (double)weight(score(i0)), (double)weight(score(i1)), unsure);
         g.sync();
         if (*filled & 1) {
           const ExactSums sums = exact_sums<TIn, VEC, G>(s, a.V, g, keep, weight, hi);
@@ -498,8 +536,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         cut = Cut{entry_key(last), entry_word(last)};
         y = weight(key_score(cut.key));
       }
-      if (hi < kAbove && (kept == 0 || y * 1.000004f >= hi)) t = hi * 1.00003f;
-      else if (lo > FLT_MIN && (!enough || y * 0.999996f < lo)) t = fmaxf(lo * 0.99997f, FLT_MIN);
+      if (hi < kAbove && (kept == 0 || y * 1.000004f >= hi)) t = hi * 1.00003f, x = xHi;
+      else if (lo > FLT_MIN && (!enough || y * 0.999996f < lo)) t = fmaxf(lo * 0.99997f, FLT_MIN), x = xLo;
       else if (kept > 0 && enough) done = true;
       else break;
       if constexpr (RESIDENT)   // what lies between and does not stay
@@ -530,8 +568,11 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     if (cutAny && rule.topP < 1.0) total = g.sum(apply());
   }
   if (rule.topP < 1.0) {
-    const float mean = -slope / (float)total, deviation = sqrtf(fmaxf(g.sum(square) / (float)total - mean * mean, 0.0f));
-    const float p = (float)rule.topP, odds = 0.55f * (__log2f(p) - __log2f(1.0f - p)) * 0.6931472f;
+    const float mean = __fdividef(-slope, (float)total);
+    const float spread2 = __fdividef(g.sum(square), (float)total) - mean * mean;
+    const float p = (float)rule.topP, odds = 0.55f * 0.6931472f * (lg2(p) - lg2(1.0f - p));
+    float deviation;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(deviation) : "f"(fmaxf(spread2, 0.0f)));
     find_cut(std::true_type{}, 0, fmaxf(ex2(fminf(mean - odds * deviation, -0.05f)), 0.25f * (1.0f - p) / (float)a.V));
     cutAny = true;
   }
@@ -542,8 +583,6 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   }
 
   // the draw: the warp, its vectors, the word
-  float u = uniforms[node];
-  u = u < 0.0f ? 0.0f : u < 1.0f ? u : 0.99999994f;
   if (cutAny) part = apply();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -561,6 +600,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     double before = __shfl_sync(0xffffffffu, upto - own, pick);
     int found = -1;
     bool certain = false;
+    float mine = 0.0f;
 #pragma unroll 1
     for (int o = g.lane * kPass; found < 0 && at.first + o - g.lane * kPass < at.end; o += 32 * kPass) {
       const int v = at.first + o;
@@ -600,11 +640,13 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
           const double after = start + (double)upTo[i];
           if (word < 0 && after > target) {
             word = v + i;
+            mine = y[i];
             clear = y[i] > 0.0f && target - b > unsure && after - target > unsure;
           }
           b = after;
         }
         found = __shfl_sync(0xffffffffu, word, owner);
+        mine = __shfl_sync(0xffffffffu, mine, owner);
         certain = __shfl_sync(0xffffffffu, clear ? 1 : 0, owner) && found >= 0;
         break;
       }
@@ -612,7 +654,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     }
     if (g.lane == 0) {
       *sure = certain;
-      if (certain) words[node] = found, logProbs[node] = (float)((double)(at.score(found) - m) * keep.exact.scale) - logf((float)total);
+      if (certain) words[node] = found, logProbs[node] = logf(mine / (float)total);
     }
   }
   g.sync();
