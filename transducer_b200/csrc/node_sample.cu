@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   const Place<TIn, VEC, G, 0> at(s, a.V, seg, g.warp, g.lane);
   float* const row = weights + sub * seg * Group<G>::kWarps;   // (scores at first)
   float* const w = row + at.first;                             // the warp's words
-  const int trips = seg / 128;
+  const int trips = seg / 128, own = g.lane * 4 * trips;   // a lane's words follow each other
   const float nan = __int_as_float(0x7fffffff);
   float m = neg_inf();
 #pragma unroll(VEC == 8 ? 3 : 5)
@@ -261,12 +261,12 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   // `keep` says it so far
   auto each = [&](auto f) {
     if constexpr (RESIDENT) {
-      const float4* q = reinterpret_cast<const float4*>(w) + g.lane;
+      const float4* q = reinterpret_cast<const float4*>(w + own);
 #pragma unroll 4
       for (int j = 0; j < trips; ++j) {
-        const float4 x = q[32 * j];
+        const float4 x = q[j];
         const float y[4] = {x.x, x.y, x.z, x.w};
-        f(y, at.first + 128 * j + 4 * g.lane);
+        f(y, at.first + own + 4 * j);
       }
     } else {
 #pragma unroll 1
@@ -298,10 +298,10 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     double sum = 0.0;
     if constexpr (RESIDENT) {
       const float lo = keep.lo, tested = keep.sure();
-      float4* q = reinterpret_cast<float4*>(w) + g.lane;
+      float4* q = reinterpret_cast<float4*>(w + own);
 #pragma unroll 2
       for (int j = 0; j < trips; ++j) {
-        const float4 x = q[32 * j];
+        const float4 x = q[j];
         float y[4] = {x.x, x.y, x.z, x.w};
         bool test = false;
 #pragma unroll
@@ -312,10 +312,10 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         if (test) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (y[i] > 0.0f && y[i] < tested && keep.exact(at.score(at.first + 128 * j + 4 * g.lane + i)) < keep.minP)
+            if (y[i] > 0.0f && y[i] < tested && keep.exact(at.score(at.first + own + 4 * j + i)) < keep.minP)
               y[i] = 0.0f;
         }
-        q[32 * j] = make_float4(y[0], y[1], y[2], y[3]);
+        q[j] = make_float4(y[0], y[1], y[2], y[3]);
         sum += (double)((y[0] + y[1]) + (y[2] + y[3]));
       }
     } else {
@@ -338,10 +338,10 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       square = fmaf(b * b, y, square);
     };
     if constexpr (RESIDENT) {
-      float4* q = reinterpret_cast<float4*>(w) + g.lane;
+      float4* q = reinterpret_cast<float4*>(w + own);
 #pragma unroll 2
       for (int j = 0; j < trips; ++j) {
-        const float4 x = q[32 * j];
+        const float4 x = q[j];
         const float z[4] = {x.x, x.y, x.z, x.w};
         float y[4];
 #pragma unroll
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
           y[i] = ex2(e);
           moments(e, y[i]);
         }
-        q[32 * j] = make_float4(y[0], y[1], y[2], y[3]);
+        q[j] = make_float4(y[0], y[1], y[2], y[3]);
         part += (double)((y[0] + y[1]) + (y[2] + y[3]));
       }
     } else {
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         return (float)g.sum(c);
       } else if constexpr (RESIDENT) {
         float sum[8] = {};
-        const float4* q = reinterpret_cast<const float4*>(w) + g.lane;
+        const float4* q = reinterpret_cast<const float4*>(w + own);
         auto add = [&](const float4& x, int i) {
           if (x.x >= t) sum[i] += x.x;
           if (x.y >= t) sum[i + 1] += x.y;
@@ -404,11 +404,11 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         int j = 0;
 #pragma unroll 2
         for (; j + 1 < trips; j += 2) {
-          const float4 x = q[32 * j], y = q[32 * j + 32];
+          const float4 x = q[j], y = q[j + 1];
           add(x, 0);
           add(y, 4);
         }
-        if (j < trips) add(q[32 * j], 0);
+        if (j < trips) add(q[j], 0);
         return g.sum(((sum[0] + sum[4]) + (sum[1] + sum[5])) + ((sum[2] + sum[6]) + (sum[3] + sum[7])));
       } else {
         double sum = 0.0;
@@ -426,6 +426,11 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     };
     // thresholds, what has been measured there, their exponents and levels
     float lo = FLT_MIN, hi = kAbove, vLo = 0.0f, vHi = 0.0f, xLo = -126.0f, xHi = 0.1f, lLo = 0.0f, lHi = level(0.0f);
+    if (kByWeight) {
+      // (the words below a quarter of (1 - topP) / V cannot be needed for the share)
+      lo = fmaxf(0.25f * (1.0f - (float)rule.topP) / (float)a.V, FLT_MIN), xLo = lg2(lo);
+      vLo = all * (1.0f - 0.25f * (1.0f - (float)rule.topP)), lLo = level(vLo);
+    }
     float t = guess, x = lg2(guess), had = 3e38f;
     const float lWant = level(want);
     int stuck = 0;
@@ -437,15 +442,14 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       if (v >= want) lo = t, vLo = v, xLo = x, lLo = l;
       else hi = t, vHi = v, xHi = x, lHi = l;
       if (vLo == 0.0f) {   // nothing is known from below yet
-        if (!kByWeight && t == FLT_MIN) return false;   // there are no more words than that
-        if (t == FLT_MIN) break;
+        if (t == FLT_MIN) return false;   // there are no more words than that
         t = round == 0 && t > 1e-9f ? t * 1e-3f : FLT_MIN;
         x = lg2(t);
         continue;
       }
       // how many words lie between: known, or at most the weight over the lesser threshold
       const float between = kByWeight ? __fdividef(vLo - vHi, lo) : vLo - vHi;
-      bool listed = between <= kNear;
+      bool listed = between <= (kByWeight ? 1.25f * kNear : (float)kNear);
       int c = 0;
       if (listed) {
         g.sync();
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     const float p = (float)rule.topP, odds = 0.55f * 0.6931472f * (lg2(p) - lg2(1.0f - p));
     float deviation;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(deviation) : "f"(fmaxf(spread2, 0.0f)));
-    find_cut(std::true_type{}, 0, fmaxf(ex2(fminf(mean - odds * deviation, -0.05f)), 0.25f * (1.0f - p) / (float)a.V));
+    find_cut(std::true_type{}, 0, fmaxf(ex2(fminf(mean - odds * deviation, -0.05f)), 0.5f * (1.0f - p) / (float)a.V));
     cutAny = true;
   }
   if (rule.minP > 0.0) {
@@ -584,73 +588,97 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
 
   // the draw: the warp, its vectors, the word
   if (cutAny) part = apply();
+  // sums up to and with each lane's words, then each warp's
+  double scan = part;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  double own = g.exchange(part), upto = own;
+  for (int d = 1; d < 32; d <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, scan, d);
+    if (g.lane >= d) scan += x;
+  }
+  const double whole = g.exchange(__shfl_sync(0xffffffffu, scan, 31));
+  double upto = whole;
 #pragma unroll
-  for (int o = 1; o < Group<G>::kWarps; o <<= 1) {
-    const double x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (g.lane >= o) upto += x;
+  for (int d = 1; d < Group<G>::kWarps; d <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, upto, d);
+    if (g.lane >= d) upto += x;
   }
   total = __shfl_sync(0xffffffffu, upto, Group<G>::kWarps - 1);
   const double target = (double)u * total;
   const unsigned past = __ballot_sync(0xffffffffu, upto > target && g.lane < Group<G>::kWarps);
   const int pick = past ? __ffs(past) - 1 : Group<G>::kWarps - 1;
   if (g.warp == pick) {
-    double before = __shfl_sync(0xffffffffu, upto - own, pick);
+    double before = __shfl_sync(0xffffffffu, upto - whole, pick);
     int found = -1;
     bool certain = false;
     float mine = 0.0f;
+    if constexpr (RESIDENT) {
+      const unsigned hit = __ballot_sync(0xffffffffu, before + scan > target);
+      if (hit && g.lane == __ffs(hit) - 1) {   // one of this lane's words
+        before += scan - part;
+        const float4* q = reinterpret_cast<const float4*>(w + own);
+#pragma unroll 2
+        for (int j = 0; j < trips && found < 0; ++j) {
+          const float4 x = q[j];
+          const float y[4] = {x.x, x.y, x.z, x.w};
+          float few = 0.0f;
+          double b = before;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            few += y[i];
+            const double after = before + (double)few;
+            if (found < 0 && after > target) {
+              found = at.first + own + 4 * j + i;
+              mine = y[i];
+              certain = y[i] > 0.0f && target - b > unsure && after - target > unsure;
+            }
+            b = after;
+          }
+          before = b;
+        }
+      }
+      const int owner = hit ? __ffs(hit) - 1 : 0;
+      found = __shfl_sync(0xffffffffu, found, owner);
+      mine = __shfl_sync(0xffffffffu, mine, owner);
+      certain = __shfl_sync(0xffffffffu, certain ? 1 : 0, owner);
+    } else {
 #pragma unroll 1
-    for (int o = g.lane * kPass; found < 0 && at.first + o - g.lane * kPass < at.end; o += 32 * kPass) {
-      const int v = at.first + o;
-      float y[kPass], upTo[kPass];
-      if constexpr (RESIDENT) {
-        float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (o < seg) q = *reinterpret_cast<const float4*>(w + o);
-        y[0] = q.x, y[1] = q.y, y[2] = q.z, y[3] = q.w;
-      } else {
-        float x[VEC];
+      for (int o = 0; found < 0 && at.first + o < at.end; o += 32 * VEC) {
+        const int v = at.first + o + g.lane * VEC;
+        float x[VEC], y[VEC];
+        double sum = 0.0;
         if (v < at.end) at.load(v, x);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           y[i] = v < at.end ? weight(x[i]) : 0.0f;
           if (v < at.end && !keep(y[i], x[i], v + i)) y[i] = 0.0f;
+          sum += (double)y[i];
         }
-      }
-      upTo[0] = y[0];
+        double upTo = sum;
 #pragma unroll
-      for (int i = 1; i < kPass; ++i) upTo[i] = upTo[i - 1] + y[i];
-      const double sum = upTo[kPass - 1];
-      double scan = sum;
+        for (int d = 1; d < 32; d <<= 1) {
+          const double z = __shfl_up_sync(0xffffffffu, upTo, d);
+          if (g.lane >= d) upTo += z;
+        }
+        if (const unsigned hit = __ballot_sync(0xffffffffu, before + upTo > target)) {
+          double b = before + (upTo - sum);
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double x = __shfl_up_sync(0xffffffffu, scan, d);
-        if (g.lane >= d) scan += x;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + scan > target);
-      if (hit) {
-        const int owner = __ffs(hit) - 1;
-        const double start = before + (scan - sum);
-        double b = start;
-        int word = -1;
-        bool clear = false;
-#pragma unroll
-        for (int i = 0; i < kPass; ++i) {
-          const double after = start + (double)upTo[i];
-          if (word < 0 && after > target) {
-            word = v + i;
-            mine = y[i];
-            clear = y[i] > 0.0f && target - b > unsure && after - target > unsure;
+          for (int i = 0; i < VEC; ++i) {
+            const double after = b + (double)y[i];
+            if (found < 0 && after > target) {
+              found = v + i;
+              mine = y[i];
+              certain = y[i] > 0.0f && target - b > unsure && after - target > unsure;
+            }
+            b = after;
           }
-          b = after;
+          const int owner = __ffs(hit) - 1;
+          found = __shfl_sync(0xffffffffu, found, owner);
+          mine = __shfl_sync(0xffffffffu, mine, owner);
+          certain = __shfl_sync(0xffffffffu, certain ? 1 : 0, owner);
+          break;
         }
-        found = __shfl_sync(0xffffffffu, word, owner);
-        mine = __shfl_sync(0xffffffffu, mine, owner);
-        certain = __shfl_sync(0xffffffffu, clear ? 1 : 0, owner) && found >= 0;
-        break;
+        before += __shfl_sync(0xffffffffu, upTo, 31);
       }
-      before += __shfl_sync(0xffffffffu, scan, 31);
     }
     if (g.lane == 0) {
       *sure = certain;
@@ -661,6 +689,10 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   if (*sure) return;
   exact_draw<TIn, VEC, G>(s, a.V, seg, g, keep, weight, u, words + node, logProbs + node);
 }
+
+// Words of each of so many warps: 128 for every four of a lane, an odd number of fours, so that the lanes' words, which
+// follow each other, are read from different banks.
+int words_of_warp(int V, int warps) { return 128 * (div_up(V, 128 * warps) | 1); }
 
 }  // namespace
 
@@ -683,9 +715,9 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
     auto launch = [&](auto group, auto resident) {
       constexpr int G = decltype(group)::value, rows = kCta<G> / G;
       auto kernel = sample_words_kernel<TIn, decltype(vec)::value, G, decltype(resident)::value>;
-      const int seg = (int)round_up64(div_up(a.V, G / 32), 128);
+      const int seg = words_of_warp(a.V, G / 32);
       const int smem = decltype(resident)::value ? rows * seg * (G / 32) * (int)sizeof(float) : 0;
-      if (smem > 32 * 1024) allow_dyn_smem(kernel, kResidentBytes);
+      if (smem > 32 * 1024) allow_dyn_smem(kernel, G == 32 ? 64 * 1024 : kResidentBytes);
       ScopedKernel prof("sample_words", stream);
       kernel<<<(unsigned)div_up64(nodes, rows), kCta<G>, smem, stream>>>(a, uniforms, words, logProbs, rule, seg);
       TB200_CHECK_LAUNCH();
@@ -694,7 +726,7 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
     if (a.V <= 1024) launch(integral_constant<int, 32>{}, std::true_type{});
     else if (a.V <= 4096) launch(integral_constant<int, 128>{}, std::true_type{});
     else if (a.V <= 16384) launch(integral_constant<int, 256>{}, std::true_type{});
-    else if (round_up64(div_up(a.V, 32), 128) * 32 * 4 <= kResidentBytes)
+    else if (words_of_warp(a.V, 32) * 32 * 4 <= kResidentBytes)
       launch(integral_constant<int, 1024>{}, std::true_type{});
     else launch(integral_constant<int, 1024>{}, std::false_type{});
   });
