@@ -78,7 +78,6 @@ __device__ __noinline__ Cut general_share(NodeScores<TIn> s, int V, Group<G> g, 
 constexpr double kUnsureSlope = 2.1 * 0x1p-24, kUnsureSum = 0x1p-22 + 20 * 0x1p-24;
 constexpr int kNear = 64;          // words about a cut that are listed
 constexpr float kAbove = 2.0f;     // above every weight
-constexpr int kResidentBytes = 220 * 1024;   // of shared memory for a row's weights, beside the lists
 
 struct Weight {
   float m, c;
@@ -123,11 +122,11 @@ __device__ __noinline__ ExactSums exact_sums(NodeScores<TIn> s, int V, Group<G> 
 template <typename TIn, int VEC, int G>
 __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group<G> g, Keep keep,
                                         Weight weight, float u, int* word, float* logProb) {
-  const Place<TIn, VEC, G, 0> at(s, V, seg, g.warp, g.lane);
+  const Place<TIn, VEC> at(s, V, seg, g.warp, g.lane);
   auto kept = [&](float z, int v) { return keep(weight(z), z, v) ? keep.exact(z) : 0.0; };
   double part = 0.0;
 #pragma unroll 1
-  for (int v = at.word(0); v < at.end; v += 32 * VEC) {
+  for (int v = at.first + g.lane * VEC; v < at.end; v += 32 * VEC) {
     float z[VEC];
     at.load(v, z);
 #pragma unroll
@@ -153,7 +152,7 @@ __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group
   int found = -1;   // the first word past the target, or (rounding) the last one that stays
 #pragma unroll 1
   for (int j = 0; at.first + j * 32 * VEC < at.end; ++j) {
-    const int v = at.word(j);
+    const int v = at.first + (j * 32 + g.lane) * VEC;
     float z[VEC];
     double w[VEC], sum = 0.0;
     if (v < at.end) at.load(v, z);
@@ -189,9 +188,7 @@ __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group
   if (g.lane == 0) *word = found, *logProb = (float)log(weightOf / total);
 }
 
-// The row's weights lie in shared memory (RESIDENT; 227 KB hold 57,000 words), each thread goes through the
-// same ones in every pass; longer rows are read again instead.  In registers they were no faster to go
-// through and left room for a quarter of the threads.
+// The row's weights take the scores' place in shared memory.
 template <typename TIn, int VEC, int G, bool RESIDENT>
 __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     NodeArgs a, const float* __restrict__ uniforms, int* __restrict__ words, float* __restrict__ logProbs,
@@ -216,31 +213,16 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   float u = uniforms[node];
   u = u < 0.0f ? 0.0f : u < 1.0f ? u : 0.99999994f;
   Group<G> g(tid, scratch);
-  const Place<TIn, VEC, G, 0> at(s, a.V, seg, g.warp, g.lane);
+  const Place<TIn, VEC> at(s, a.V, seg, g.warp, g.lane);
   float* const row = weights + sub * seg * Group<G>::kWarps;   // (scores at first)
   float* const w = row + at.first;                             // the warp's words
   const int trips = seg / 128, own = g.lane * 4 * trips;   // a lane's words follow each other
   const float nan = __int_as_float(0x7fffffff);
   float m = neg_inf();
-#pragma unroll(VEC == 8 ? 3 : 5)
-  for (int o = g.lane * VEC; o < (RESIDENT ? seg : at.end - at.first); o += 32 * VEC) {
-    float x[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
-    if (at.first + o < at.end) at.load(at.first + o, x);
-    if constexpr (RESIDENT) {
-      if constexpr (VEC % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < VEC; i += 4)
-          *reinterpret_cast<float4*>(w + o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-      } else {
-        w[o] = x[0];
-      }
-    }
+  bring_row<RESIDENT>(at, w, seg, [&](const float (&x)[VEC]) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[i]);
-  }
-  __syncwarp();
+  });
   m = g.max(m);
   if (m == neg_inf() || rule.temperature == 0.0) {
     // every word is masked, or the first of the greatest scores is asked for
@@ -690,10 +672,6 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   exact_draw<TIn, VEC, G>(s, a.V, seg, g, keep, weight, u, words + node, logProbs + node);
 }
 
-// Words of each of so many warps: 128 for every four of a lane, an odd number of fours, so that the lanes' words, which
-// follow each other, are read from different banks.
-int words_of_warp(int V, int warps) { return 128 * (div_up(V, 128 * warps) | 1); }
-
 }  // namespace
 
 // Whether words can be moved 16 bytes at a time: every row starts on a 16-byte boundary and has whole
@@ -712,7 +690,7 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
   if (nodes == 0) return;
   with_type(a, [&](auto type, auto vec) {
     using TIn = decltype(type);
-    auto launch = [&](auto group, auto resident) {
+    with_group(a.V, true, [&](auto group, auto resident) {
       constexpr int G = decltype(group)::value, rows = kCta<G> / G;
       auto kernel = sample_words_kernel<TIn, decltype(vec)::value, G, decltype(resident)::value>;
       const int seg = words_of_warp(a.V, G / 32);
@@ -721,14 +699,7 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
       ScopedKernel prof("sample_words", stream);
       kernel<<<(unsigned)div_up64(nodes, rows), kCta<G>, smem, stream>>>(a, uniforms, words, logProbs, rule, seg);
       TB200_CHECK_LAUNCH();
-    };
-    using std::integral_constant;
-    if (a.V <= 1024) launch(integral_constant<int, 32>{}, std::true_type{});
-    else if (a.V <= 4096) launch(integral_constant<int, 128>{}, std::true_type{});
-    else if (a.V <= 16384) launch(integral_constant<int, 256>{}, std::true_type{});
-    else if (words_of_warp(a.V, 32) * 32 * 4 <= kResidentBytes)
-      launch(integral_constant<int, 1024>{}, std::true_type{});
-    else launch(integral_constant<int, 1024>{}, std::false_type{});
+    });
   });
 }
 

@@ -1,12 +1,12 @@
 // What node_top.cu (the best words of a lattice node) and node_sample.cu (a word drawn from a node's
 // distribution) share.
 //
-// A row of scores is read once and stays in the registers of a group of threads (a warp for short rows,
-// a CTA for long ones; rows beyond a CTA's registers are read again for every pass).  What both
-// operators then need is a cut in the order of the words: the first k of them, or the first whose
-// weights reach a share.  Sorting is never needed for that: thresholds on the scores are tried, one
-// count (or sum of weights) over the registers each, until the few words about the cut can be put
-// in a list, where each finds its place by comparing itself with the others.
+// A row of scores is read once and stays in shared memory, seen by a group of threads (a warp for short rows, a CTA for
+// long ones; rows beyond that are read again for every pass).  What both operators then need is a cut in the order
+// of the words: the first k of them, or the first whose weights reach a share.  Sorting is never needed for that:
+// thresholds on the scores are tried until the few words about the cut can be put in a list, where each finds its
+// place by comparing itself with the others.  (In registers rows were no faster to go through, and left room for a
+// quarter of the threads.)
 #pragma once
 
 #include <type_traits>
@@ -17,15 +17,13 @@ namespace tb200 {
 
 // Which words of a row a thread has: warp w has the words from w * seg on, as far as the next warp's,
 // and its lanes take vectors of VEC words in turn.  So the warps' parts follow each other in the order
-// of the alphabet, and so do the vectors of a warp.  EPT words at most in a thread (0: any number).
-template <typename TIn, int VEC, int G, int EPT>
+// of the alphabet, and so do the vectors of a warp.
+template <typename TIn, int VEC>
 struct Place {
-  static_assert(EPT % VEC == 0 || EPT == 0);
   NodeScores<TIn> s;
   int first, end, lane;   // the warp's words
   __device__ __forceinline__ Place(const NodeScores<TIn>& scores, int V, int seg, int warp, int lane_)
       : s(scores), first(warp * seg), end(min(V, first + seg)), lane(lane_) {}
-  __device__ __forceinline__ int word(int j) const { return first + (j * 32 + lane) * VEC; }
   __device__ __forceinline__ void load(int v, float (&z)[VEC]) const {
     const Words<VEC> e = load_words<VEC>(s.e + v), p = load_words<VEC>(s.p + v);
 #pragma unroll
@@ -120,30 +118,50 @@ __device__ __forceinline__ int entries_before(const Entry* list, int c, Entry mi
   return n;
 }
 
+// ---- rows in shared memory ---------------------------------------------------------------------
+
+// A row's scores, fp32, in shared memory: warp w has seg words from w * seg on, and of these each lane seg / 32 that
+// follow each other, so that the lanes' words are in the order of the alphabet.  seg is 128 times an odd number: lanes
+// that read four of their words at a time then read from different banks.
+constexpr int kResidentBytes = 220 * 1024;   // for a row, beside the lists
+inline int words_of_warp(int V, int warps) { return 128 * (div_up(V, 128 * warps) | 1); }
+
+// The warp's scores from memory to `w` (words beyond the row: -inf); f(scores) for each vector as it comes by.  Without
+// RESIDENT only the latter.
+template <bool RESIDENT, typename TIn, int VEC, typename F>
+__device__ __forceinline__ void bring_row(const Place<TIn, VEC>& at, float* w, int seg, F f) {
+#pragma unroll(VEC == 8 ? 3 : 5)
+  for (int o = at.lane * VEC; o < (RESIDENT ? seg : at.end - at.first); o += 32 * VEC) {
+    float x[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
+    if (at.first + o < at.end) at.load(at.first + o, x);
+    if constexpr (RESIDENT) {
+      if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4)
+          *reinterpret_cast<float4*>(w + o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      } else {
+        w[o] = x[0];
+      }
+    }
+    f(x);
+  }
+  __syncwarp();
+}
+
 // ---- launches ---------------------------------------------------------------------------------
 
-// Group and words per thread for rows of V words: a warp has up to 1024, larger groups 16 to 32 a thread,
-// 1024 threads and more words are read again for every pass.
+// launch(group, resident): group sizes for rows of V words.  A warp has up to 1024, a CTA of 128 or 256 threads 32 to 64
+// words a thread; rows beyond shared memory are read again for every pass.
 template <typename F>
-void with_group(int V, F launch) {
-  auto go = [&](auto group, auto ept) { launch(group, ept, (int)round_up64(div_up(V, group / 32), 32)); };
-  auto fits = [&](int group, int ept) { return round_up64(div_up(V, group / 32), 32) <= 32 * ept; };
+void with_group(int V, bool warps, F launch) {
   using std::integral_constant;
-#define TB200_GROUP(G, EPT) \
-  if (fits(G, EPT)) return go(integral_constant<int, G>{}, integral_constant<int, EPT>{})
-  TB200_GROUP(32, 8);
-  TB200_GROUP(32, 16);
-  TB200_GROUP(32, 32);
-  TB200_GROUP(128, 16);
-  TB200_GROUP(128, 32);
-  TB200_GROUP(256, 24);
-  TB200_GROUP(256, 32);
-  TB200_GROUP(512, 24);
-  TB200_GROUP(512, 32);
-  TB200_GROUP(1024, 24);
-  TB200_GROUP(1024, 32);
-#undef TB200_GROUP
-  go(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
+  if (V <= 1024 && warps) launch(integral_constant<int, 32>{}, std::true_type{});
+  else if (V <= 4096) launch(integral_constant<int, 128>{}, std::true_type{});
+  else if (V <= 16384) launch(integral_constant<int, 256>{}, std::true_type{});
+  else if (words_of_warp(V, 32) * 32 * 4 <= kResidentBytes) launch(integral_constant<int, 1024>{}, std::true_type{});
+  else launch(integral_constant<int, 1024>{}, std::false_type{});
 }
 
 template <typename F>

@@ -37,16 +37,16 @@ __device__ __noinline__ void general_top_words(NodeScores<TIn> s, int V, Group<G
   if (g.tid == 0) *rest = m > neg_inf() && m < pos_inf() ? m * scale + logf(sum) : m;
 }
 
-constexpr int kListed = 512;   // entries of a row's list; kMaxListedWords of them are asked for at most
-
-// The k best words.  Every thread takes the maxima of four subsets of its words; a threshold that k of the
+// The k best words.  Every thread takes the maxima of four subsets of the words that it brings; a threshold that k of the
 // G * 4 maxima reach (k of the G threads' maxima where k is small) is one that k words reach, and hardly more
-// than k do: 33 of 10000 words for k = 32 and 512 threads.
-template <typename TIn, int VEC, int G, int EPT>
-__global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __restrict__ words,
-                                                            float* __restrict__ logits,
-                                                            float* __restrict__ rest, int k, int seg, float scale) {
-  constexpr int kRows = kCta<G> / G;
+// than k do: 34 of 10000 words for k = 32 and 256 threads.
+template <typename TIn, int VEC, int G, bool RESIDENT>
+__global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) top_words_kernel(NodeArgs a, int* __restrict__ words,
+                                                                            float* __restrict__ logits,
+                                                                            float* __restrict__ rest, int k, int seg,
+                                                                            float scale) {
+  constexpr int kRows = kCta<G> / G, kListed = G == 32 ? 256 : 512, kPass = RESIDENT ? 4 : VEC;
+  extern __shared__ __align__(16) float scores[];   // a warp's part of a row: seg = 128 * trips words
   __shared__ double2 scratch[64];
   __shared__ Entry listAll[kRows][kListed];
   __shared__ int filledAll[kRows];
@@ -66,55 +66,52 @@ __global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __r
     return;
   }
   Group<G> g(tid, scratch);
-  const Place<TIn, VEC, G, EPT> at(s, a.V, seg, g.warp, g.lane);
-  float z[EPT > 0 ? EPT : 1];
-  auto each = [&](auto f) {   // f(score, word) for each of this thread's words
-    if constexpr (EPT > 0) {
-#pragma unroll
-      for (int j = 0; j < EPT / VEC; ++j) {
-        const int v = at.word(j);
-        if (v < at.end)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) f(z[j * VEC + i], v + i);
+  const Place<TIn, VEC> at(s, a.V, seg, g.warp, g.lane);
+  float* const w = scores + sub * seg * Group<G>::kWarps + at.first;   // the warp's words
+  const int trips = seg / 128, own = g.lane * 4 * trips;
+  // f(scores, first word) for kPass of this thread's words at a time (words beyond the row: -inf)
+  auto each = [&](auto f) {
+    if constexpr (RESIDENT) {
+      const float4* q = reinterpret_cast<const float4*>(w + own);
+#pragma unroll 4
+      for (int j = 0; j < trips; ++j) {
+        const float4 x = q[j];
+        const float z[4] = {x.x, x.y, x.z, x.w};
+        f(z, at.first + own + 4 * j);
       }
     } else {
 #pragma unroll 1
-      for (int v = at.word(0); v < at.end; v += 32 * VEC) {
-        float x[VEC];
-        at.load(v, x);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f(x[i], v + i);
+      for (int v = at.first + g.lane * VEC; v < at.end; v += 32 * VEC) {
+        float z[VEC];
+        at.load(v, z);
+        f(z, v);
       }
     }
   };
-  // (subset v % 4 of the thread's words with vectors, (v / 32) % 4 without)
   float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
-  if constexpr (EPT > 0) {
+  bring_row<RESIDENT>(at, w, seg, [&](const float (&x)[VEC]) {
+    if constexpr (VEC > 1) {   // (the i-th words of the vectors)
 #pragma unroll
-    for (int j = 0; j < EPT / VEC; ++j) {
-      const int v = at.word(j);
-      float x[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
-      if (v < at.end) at.load(v, x);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) z[j * VEC + i] = x[i];
+      for (int i = 0; i < VEC; ++i) top[i % 4] = fmaxf(top[i % 4], x[i]);
+    } else {                   // (every fourth of the words)
+      const float oldest = fmaxf(top[3], x[0]);
+      top[3] = top[2], top[2] = top[1], top[1] = top[0], top[0] = oldest;
     }
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) top[i % 4] = fmaxf(top[i % 4], z[i]);
-  } else {
-    each([&](float x, int v) {
-      const int i = VEC > 1 ? v % 4 : (v - at.first) / 32 % 4;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (q == i) top[q] = fmaxf(top[q], x);
-    });
-  }
+  });
+  // (a thread that has brought no words, or fewer than four without vectors, has empty subsets)
+  const int mine = max(0, div_up(at.end - at.first - g.lane * VEC, 32 * VEC));
   unsigned key[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) key[q] = at.word(VEC > 1 ? 0 : q) < at.end ? score_key(top[q]) : 0u;
+  for (int q = 0; q < 4; ++q) key[q] = score_key(top[q]);
+  if (VEC > 1 ? mine == 0 : mine < 4) {
+    if constexpr (VEC > 1) {
+      key[0] = key[1] = key[2] = key[3] = 0u;
+    } else {   // (too few to tell which maxima are of words: all in one)
+      key[0] = mine > 0 ? max(max(key[0], key[1]), max(key[2], key[3])) : 0u;
+      key[1] = key[2] = key[3] = 0u;
+    }
+  }
   const unsigned best = max(max(key[0], key[1]), max(key[2], key[3]));
-  // (16 words in a thread's maximum, or a quarter of its words in one of four)
   const bool one = G > 32 && k <= G / 4;
   auto reach = [&](unsigned t) {
     if (G > 32 && one) return __syncthreads_count(best >= t);
@@ -142,22 +139,16 @@ __global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __r
     const int i = atomicAdd(filled, 1);
     if (i < kListed) list[i] = entry_of(x, v);
   };
-  if (best >= lo || lo <= lowest) {
-    if constexpr (EPT > 0) {
-      unsigned in = 0;
+  each([&](const float (&z)[kPass], int v) {
+    unsigned in = 0;
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) in |= z[i] >= bound ? 1u << i : 0u;
+    for (int i = 0; i < kPass; ++i) in |= z[i] >= bound ? 1u << i : 0u;
 #pragma unroll 1
-      for (; in; in &= in - 1) {
-        const int i = __ffs(in) - 1, v = at.word(i / VEC) + i % VEC;
-        if (v < at.end) append(at.score(v), v);
-      }
-    } else {
-      each([&](float x, int v) {
-        if (x >= bound) append(x, v);
-      });
+    for (; in; in &= in - 1) {
+      const int i = __ffs(in) - 1;
+      if (v + i < a.V) append(at.score(v + i), v + i);
     }
-  }
+  });
   g.sync();
   const int c = *filled;
   auto general = [&] { general_top_words<TIn, VEC, G>(s, a.V, g, list, filled, words, logits, rest, k, scale); };
@@ -184,9 +175,9 @@ __global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __r
   }
   const float scale2 = scale * 1.4426950408889634f;
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  int turn = 0;
-  each([&](float x, int) {
-    sum[turn++ % 4] += x >= last ? 0.0f : ex2((x - last) * scale2);   // (NaN comes through)
+  each([&](const float (&z)[kPass], int) {
+#pragma unroll
+    for (int i = 0; i < kPass; ++i) sum[i % 4] += z[i] >= last ? 0.0f : ex2((z[i] - last) * scale2);   // (NaN comes through)
   });
   float all = g.sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
   if (all != all) return general();
@@ -195,10 +186,17 @@ __global__ void __launch_bounds__(kCta<G>) top_words_kernel(NodeArgs a, int* __r
   float ref = last;
   if (!(all > 1e-25f)) {   // the others are far below: relative to their own maximum
     ref = neg_inf();
-    each([&](float x, int) { ref = x < last ? fmaxf(ref, x) : ref; });
+    each([&](const float (&z)[kPass], int) {
+#pragma unroll
+      for (int i = 0; i < kPass; ++i) ref = z[i] < last ? fmaxf(ref, z[i]) : ref;
+    });
     ref = g.max(ref);
     all = 0.0f;
-    if (ref > neg_inf()) each([&](float x, int) { all += x < last ? ex2((x - ref) * scale2) : 0.0f; });
+    if (ref > neg_inf())
+      each([&](const float (&z)[kPass], int) {
+#pragma unroll
+        for (int i = 0; i < kPass; ++i) all += z[i] < last ? ex2((z[i] - ref) * scale2) : 0.0f;
+      });
     all = g.sum(all);
   }
   if (tid == 0) *rest = fabsf(ref) < pos_inf() ? ref * scale + logf(all) : ref;
@@ -212,11 +210,16 @@ void launch_top_words(const NodeArgs& a, int* words, float* logits, float* rest,
   if (nodes == 0) return;
   with_type(a, [&](auto type, auto vec) {
     using TIn = decltype(type);
-    with_group(a.V, [&](auto group, auto ept, int seg) {
-      constexpr int G = group, rows = kCta<G> / G;
+    // (a warp's list holds 256 entries, and its 128 maxima tell the best 64 at most)
+    with_group(a.V, k <= 64, [&](auto group, auto resident) {
+      constexpr int G = decltype(group)::value, rows = kCta<G> / G;
+      auto kernel = top_words_kernel<TIn, decltype(vec)::value, G, decltype(resident)::value>;
+      const int seg = words_of_warp(a.V, G / 32);
+      const int smem = decltype(resident)::value ? rows * seg * (G / 32) * (int)sizeof(float) : 0;
+      if (smem > 24 * 1024) allow_dyn_smem(kernel, G == 32 ? 64 * 1024 : kResidentBytes);
       ScopedKernel prof("top_words", stream);
-      top_words_kernel<TIn, vec, G, ept><<<(unsigned)div_up64(nodes, rows), kCta<G>, 0, stream>>>(
-          a, words, logits, rest, k, seg, (float)(1.0 / temperature));
+      kernel<<<(unsigned)div_up64(nodes, rows), kCta<G>, smem, stream>>>(a, words, logits, rest, k, seg,
+                                                                        (float)(1.0 / temperature));
       TB200_CHECK_LAUNCH();
     });
   });
