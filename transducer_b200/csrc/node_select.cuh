@@ -130,22 +130,39 @@ inline int words_of_warp(int V, int warps) { return 128 * (div_up(V, 128 * warps
 // RESIDENT only the latter.
 template <bool RESIDENT, typename TIn, int VEC, typename F>
 __device__ __forceinline__ void bring_row(const Place<TIn, VEC>& at, float* w, int seg, F f) {
-#pragma unroll(VEC == 8 ? 3 : 5)
-  for (int o = at.lane * VEC; o < (RESIDENT ? seg : at.end - at.first); o += 32 * VEC) {
-    float x[VEC];
+  constexpr int kBatch = VEC == 1 ? 8 : VEC == 8 ? 3 : 4;   // vectors on their way at a time (more: spilled registers)
+  const int words = at.end - at.first, whole = RESIDENT ? seg : words;
+  for (int o = at.lane * VEC; o < whole; o += 32 * VEC * kBatch) {
+    RawWords<TIn, VEC> e[kBatch], p[kBatch];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
-    if (at.first + o < at.end) at.load(at.first + o, x);
-    if constexpr (RESIDENT) {
-      if constexpr (VEC % 4 == 0) {
+    for (int j = 0; j < kBatch; ++j) {
+      const int v = o + 32 * VEC * j;
+      if (v < words) e[j].load(at.s.e + at.first + v), p[j].load(at.s.p + at.first + v);
+    }
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4)
-          *reinterpret_cast<float4*>(w + o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-      } else {
-        w[o] = x[0];
+    for (int j = 0; j < kBatch; ++j) {
+      const int v = o + 32 * VEC * j;
+      float x[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = neg_inf();
+      if (v < words) {
+        const Words<VEC> y = e[j].words(), z = p[j].words();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[i] = y.x[i] + z.x[i];
+        f(x);
+      }
+      if constexpr (RESIDENT) {
+        if (v < whole) {
+          if constexpr (VEC % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4)
+              *reinterpret_cast<float4*>(w + v + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+          } else {
+            w[v] = x[0];
+          }
+        }
       }
     }
-    f(x);
   }
   __syncwarp();
 }

@@ -112,24 +112,58 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) top_words_kernel(Node
     }
   }
   const unsigned best = max(max(key[0], key[1]), max(key[2], key[3]));
-  const bool one = G > 32 && k <= G / 4;
-  auto reach = [&](unsigned t) {
-    if (G > 32 && one) return __syncthreads_count(best >= t);
-    return g.sum((key[0] >= t) + (key[1] >= t) + (key[2] >= t) + (key[3] >= t));
-  };
-  unsigned hi = g.max(best), lo = 1;
-  int reached = reach(1);
-  if (reached >= k) {
-    lo = g.min(one ? (best ? best : ~0u)
-                   : min(min(key[0] ? key[0] : ~0u, key[1] ? key[1] : ~0u), min(key[2] ? key[2] : ~0u, key[3] ? key[3] : ~0u)));
-    hi = hi + 1;
+  unsigned lo = 1;   // no threshold
+  // The least key of so many that k of them reach, and not many more than k (`reach` counts; all do from `least` on).
+  auto threshold = [&](unsigned least, unsigned most, int reached, auto reach) {
+    unsigned from = least, to = most + 1;
 #pragma unroll 1
-    while (hi - lo > 1 && reached > k + max(k / 8, 4)) {
-      const unsigned mid = lo + (hi - lo) / 2;
+    while (to - from > 1 && reached > k + max(k / 8, 4)) {
+      const unsigned mid = from + (to - from) / 2;
       const int n = reach(mid);
-      if (n >= k) lo = mid, reached = n;
-      else hi = mid;
+      if (n >= k) from = mid, reached = n;
+      else to = mid;
     }
+    return from;
+  };
+  constexpr int kKeys = G / 32;   // of the threads' maxima in each lane of a warp
+  if (G > 32 && G <= 256 && k <= G / 4) {   // by one warp, from the threads' maxima
+    unsigned* maxima = reinterpret_cast<unsigned*>(list);
+    maxima[tid] = best;
+    g.sync();
+    if (g.warp == 0) {
+      unsigned x[kKeys], least = ~0u, most = 0;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) {
+        x[i] = maxima[32 * i + g.lane];
+        least = min(least, x[i] ? x[i] : ~0u), most = max(most, x[i]);
+        n += x[i] ? 1 : 0;
+      }
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n >= k)
+        lo = threshold(__reduce_min_sync(0xffffffffu, least), __reduce_max_sync(0xffffffffu, most), n, [&](unsigned t) {
+          int c = 0;
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) c += x[i] >= t ? 1 : 0;
+          return __reduce_add_sync(0xffffffffu, c);
+        });
+      if (g.lane == 0) *filled = (int)lo;
+    }
+    g.sync();
+    lo = (unsigned)*filled;
+    g.sync();
+  } else {
+    const bool threads = G > 256 && k <= G / 4;   // (their maxima, too many for one warp)
+    auto reach = [&](unsigned t) {
+      if (G > 256 && threads) return __syncthreads_count(best >= t);
+      return g.sum((key[0] >= t) + (key[1] >= t) + (key[2] >= t) + (key[3] >= t));
+    };
+    auto least = [](unsigned x) { return x ? x : ~0u; };
+    const int n = reach(1);
+    const unsigned most = g.max(best);
+    if (n >= k)
+      lo = threshold(g.min(threads ? least(best) : min(min(least(key[0]), least(key[1])), min(least(key[2]), least(key[3])))),
+                     most, n, reach);
   }
   if (tid == 0) *filled = 0, edge[0] = edge[1] = 0;
   g.sync();
@@ -146,17 +180,24 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) top_words_kernel(Node
 #pragma unroll 1
     for (; in; in &= in - 1) {
       const int i = __ffs(in) - 1;
-      if (v + i < a.V) append(at.score(v + i), v + i);
+      if (v + i < a.V) append(RESIDENT ? w[v + i - at.first] : at.score(v + i), v + i);
     }
   });
   g.sync();
   const int c = *filled;
   auto general = [&] { general_top_words<TIn, VEC, G>(s, a.V, g, list, filled, words, logits, rest, k, scale); };
   if (c > kListed || c < k) return general();   // (fewer than k: some are NaN)
+  constexpr int kShare = G >= 128 ? 4 : 1;   // threads per entry, each looking at its part of the others
 #pragma unroll 1
-  for (int i = tid; i < c; i += G) {
-    const Entry mine = list[i];
-    const int place = entries_before(list, c, mine);
+  for (int i0 = 0; i0 < c; i0 += G / kShare) {
+    const int i = i0 + tid / kShare;
+    const Entry mine = i < c ? list[i] : 0;
+    int place = 0;
+#pragma unroll 4
+    for (int j = tid % kShare; j < c; j += kShare) place += list[j] > mine ? 1 : 0;
+#pragma unroll
+    for (int o = 1; o < kShare; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    if (tid % kShare != 0 || i >= c) continue;
     if (place < k) {
       words[place] = entry_word(mine);
       logits[place] = key_score(entry_key(mine)) * scale;
