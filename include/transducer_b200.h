@@ -325,6 +325,14 @@ int tb200_loss_sum_exchange(const float* lossSum, void* const* peerSlots, int ra
  * utterances and between frames resp. positions; words lie next to each other.  batchSize * nodes
  * must be below 2^31 - 1, other sizes are limited by memory. */
 
+/* What a checked call wants to know of its indices, for one kernel and one synchronisation of the
+ * calling thread's stream: the greatest frame, position and (words may be NULL) listed word, -1 if
+ * there is none, in most[3] (host memory).  scratch: tb200_node_summary_scratch_bytes() of device
+ * memory. */
+size_t tb200_node_summary_scratch_bytes(void);
+int tb200_node_summary(const int* frames, const int* positions, long long nodes, const int* words,
+                       long long wordCount, void* scratch, int* most);
+
 /* The k best words of every node (1 <= k <= 256, k <= V), the greater score first and of equal ones
  * the lower word first: words int [B, N, k], logits [B, N, k] = z / temperature.  rest [B, N] (may be
  * NULL): log sum of exp(z / temperature) over all other words, -inf if there are none.  Where there

@@ -322,6 +322,30 @@ def test_indices_beyond_the_tensors_are_no_nodes_when_not_validated():
                                rtol=1e-5, atol=1e-6)
 
 
+@pytest.mark.parametrize("N", [1, 7, 40000])
+def test_validated_indices(N):
+    """Each index beyond its tensor is refused, wherever it is, and the next call is not affected."""
+    E, P, frames, positions, g = make(2, 4, 3, 20, N, holes=False)
+    words, logits, _ = top_words(E, P, frames, positions, 2)
+    good = sample_words(E, P, frames, positions, torch.zeros(2, N).cuda())
+    criterion = NodeDistillationLoss()
+    for index, most, message in ((frames, 4, "Frame"), (positions, 3, "Position"), (words, 20, "Word")):
+        flat = index.view(-1)
+        for at in (0, flat.numel() // 2, flat.numel() - 1):
+            was = flat[at].item()
+            flat[at] = most
+            if index is not words:
+                with pytest.raises(ValueError, match=message + " index mismatch"):
+                    top_words(E, P, frames, positions, 2)
+                with pytest.raises(ValueError, match=message + " index mismatch"):
+                    sample_words(E, P, frames, positions, torch.zeros(2, N).cuda())
+            with pytest.raises(ValueError, match=message + " index mismatch"):
+                criterion(E, P, frames, positions, words, logits)
+            flat[at] = was
+    again = sample_words(E, P, frames, positions, torch.zeros(2, N).cuda())
+    assert all(torch.equal(a, b) for a, b in zip(good, again))
+
+
 def test_masked_places_are_not_read():
     """NaN in rows without nodes and in nodes that are not weighted by the record stay there."""
     E, P, frames, positions, g = make(2, 5, 3, 40, 7, holes=False)

@@ -66,6 +66,8 @@ SIGNATURES = {
     "tb200_peer_export": (_i, [_p, _p]),
     "tb200_peer_import": (_i, [_p, ctypes.POINTER(_p)]),
     "tb200_peer_close": (_i, [_p]),
+    "tb200_node_summary_scratch_bytes": (_z, []),
+    "tb200_node_summary": (_i, [_p] * 2 + [_l, _p, _l, _p, ctypes.POINTER(_i)]),
     "tb200_top_words": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 5 + [_i] * 6 + [_d]),
     "tb200_sample_words": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 5 + [_i] * 5 + [_d, _i, _d, _d]),
     "tb200_distill_saved_bytes": (_z, [_i] * 3),

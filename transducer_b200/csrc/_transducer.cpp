@@ -188,6 +188,16 @@ PYBIND11_MODULE(_transducer, m) {
   // `scores`: (emissions, predictions, bf16, their strides by utterance and by frame resp. position)
   using Scores = std::tuple<addr, addr, bool, long long, long long, long long, long long>;
   using Sizes = std::tuple<int, int, int, int, int>;   // B, T, U, V, N
+  m.attr("node_summary_scratch_bytes") = tb200_node_summary_scratch_bytes();
+  // (greatest frame, position, listed word), after one synchronisation
+  m.def("node_summary",
+        [](addr frames, addr positions, long long nodes, addr words, long long word_count, addr scratch) {
+          int most[3];
+          check(tb200_node_summary(at<const int>(frames), at<const int>(positions), nodes, at<const int>(words),
+                                   word_count, at<void>(scratch), most));
+          return py::make_tuple(most[0], most[1], most[2]);
+        },
+        "frames"_a, "positions"_a, "nodes"_a, "words"_a, "word_count"_a, "scratch"_a);
   m.def("top_words",
         [](const Scores& s, addr frames, addr positions, addr words, addr logits, addr rest, const Sizes& n, int k,
            double temperature) {

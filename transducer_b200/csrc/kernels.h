@@ -262,6 +262,11 @@ struct NodeArgs {
   int dtype = kDtypeF32;
 };
 
+// most[CTAs * 3]: the greatest frame, position and listed word (words may be null) that each CTA has seen.
+int node_summary_ctas(i64 nodes, i64 wordCount);
+void launch_node_summary(const int* frames, const int* positions, i64 nodes, const int* words, i64 wordCount,
+                         int* most, cudaStream_t stream);
+
 constexpr int kMaxListedWords = 256;   // longest list of words per node
 // Largest vocabulary of a distillation with the rest's weight: a bit per word in shared memory.
 constexpr int kDistillMaxBits = 1 << 20;

@@ -68,6 +68,24 @@ using namespace tb200;
 
 extern "C" {
 
+size_t tb200_node_summary_scratch_bytes(void) { return 64 * 3 * sizeof(int); }
+
+int tb200_node_summary(const int* frames, const int* positions, long long nodes, const int* words,
+                       long long wordCount, void* scratch, int* most) {
+  return guarded([&] {
+    check(nodes >= 0 && wordCount >= 0 && scratch && most, "null pointer or negative count");
+    int host[64 * 3];
+    const int ctas = node_summary_ctas(nodes, wordCount);
+    launch_node_summary(frames, positions, nodes, words, wordCount, static_cast<int*>(scratch), api_stream());
+    TB200_CUDA_CHECK(cudaMemcpyAsync(host, scratch, sizeof(int) * 3 * ctas, cudaMemcpyDeviceToHost, api_stream()));
+    TB200_CUDA_CHECK(cudaStreamSynchronize(api_stream()));
+    for (int k = 0; k < 3; ++k) {
+      most[k] = host[k];
+      for (int c = 1; c < ctas; ++c) most[k] = host[3 * c + k] > most[k] ? host[3 * c + k] : most[k];
+    }
+  });
+}
+
 int tb200_top_words(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
                     long long pStrideB, long long pStrideU, const int* frames, const int* positions, int* words,
                     float* logits, float* rest, int B, int maxT, int maxU, int V, int N, int k,

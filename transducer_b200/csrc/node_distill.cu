@@ -225,6 +225,27 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
   saved.node[node] = make_float4(full.m, A, sign, 0.0f);
 }
 
+// The greatest indices of a call, so that it can be refused: one CTA per 16384 of them, up to 64.
+__global__ void __launch_bounds__(512) node_summary_kernel(const int* __restrict__ frames,
+                                                           const int* __restrict__ positions, i64 nodes,
+                                                           const int* __restrict__ words, i64 wordCount,
+                                                           int* __restrict__ most) {
+  __shared__ double2 scratch[64];
+  Group<512> g(threadIdx.x, scratch);
+  const i64 first = (i64)blockIdx.x * 512 + threadIdx.x, step = (i64)gridDim.x * 512;
+  int frame = -1, position = -1, word = -1;
+  for (i64 i = first; i < nodes; i += step) frame = max(frame, frames[i]), position = max(position, positions[i]);
+#pragma unroll 8
+  for (i64 i = first; i < wordCount; i += step) word = max(word, words[i]);
+  frame = g.max(frame);
+  position = g.max(position);
+  word = g.max(word);
+  if (threadIdx.x == 0) {
+    int* mine = most + 3 * blockIdx.x;
+    mine[0] = frame, mine[1] = position, mine[2] = word;
+  }
+}
+
 template <typename F>
 void with_type(int dtype, bool wide, F launch) {
   if (dtype == kDtypeBf16) {
@@ -242,6 +263,18 @@ void with_flag(bool on, F launch) {
 }
 
 }  // namespace
+
+int node_summary_ctas(i64 nodes, i64 wordCount) {
+  return (int)std::min<i64>(64, std::max<i64>(1, (nodes + wordCount) / 16384));
+}
+
+void launch_node_summary(const int* frames, const int* positions, i64 nodes, const int* words, i64 wordCount,
+                         int* most, cudaStream_t stream) {
+  ScopedKernel prof("node_summary", stream);
+  node_summary_kernel<<<node_summary_ctas(nodes, wordCount), 512, 0, stream>>>(frames, positions, nodes, words,
+                                                                              words ? wordCount : 0, most);
+  TB200_CHECK_LAUNCH();
+}
 
 void launch_distill_forward(const NodeArgs& a, const int* words, const float* logits, const float* rest,
                             float* costs, DistillSaved saved, int K, double temperature,

@@ -17,7 +17,7 @@ CUDA tensors only, like `TransducerLoss`; the work is enqueued on torch's curren
 import torch
 
 from . import _transducer
-from .torch_binding import DeviceManager, _workspace, check_contiguous, check_dim, check_type
+from .torch_binding import _workspace, check_contiguous, check_dim, check_type
 
 MAX_LISTED_WORDS = 256
 
@@ -50,20 +50,43 @@ def certify_nodes(emissions, predictions, frames, positions):
 
 
 def certify_indices(emissions, predictions, frames, positions, words=None):
-    """That no frame, position or listed word lies beyond its tensor: reads the greatest back from
-    the device.  (The kernels themselves take such an index for none.)"""
+    """That no frame, position or listed word lies beyond its tensor: after the kernels are enqueued one
+    small kernel and one synchronisation tell the greatest.  (The kernels themselves take such an
+    index for none, so a call with too great ones may run before it is refused.)  Inside `OnDevice`."""
     if frames.numel() == 0:
         return
-    most = [frames.max(), positions.max()]
-    if words is not None:
-        most.append(words.max())
-    most = torch.stack(most).tolist()
-    if most[0] >= emissions.shape[1]:
+    scratch = torch.empty(_transducer.node_summary_scratch_bytes, dtype=torch.uint8,
+                          device=emissions.device)
+    frame, position, word = _transducer.node_summary(
+        frames.data_ptr(), positions.data_ptr(), frames.numel(),
+        0 if words is None else words.data_ptr(), 0 if words is None else words.numel(),
+        scratch.data_ptr())
+    if frame >= emissions.shape[1]:
         raise ValueError("Frame index mismatch")
-    if most[1] >= predictions.shape[1]:
+    if position >= predictions.shape[1]:
         raise ValueError("Position index mismatch")
-    if words is not None and most[2] >= emissions.shape[2]:
+    if word >= emissions.shape[2]:
         raise ValueError("Word index mismatch")
+
+
+class OnDevice(object):
+    """torch_binding.DeviceManager for calls that take a few microseconds: the device is switched only
+    where it is another one."""
+
+    def __init__(self, device):
+        if device.type != "cuda":
+            raise ValueError("transducer_b200 runs on CUDA tensors only (got %s)" % device)
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        _transducer.set_stream(torch._C._cuda_getCurrentRawStream(self.index))
+
+    def __exit__(self, exc_type, exc_value, traceback):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
 def check_device(first, *others):
@@ -91,7 +114,6 @@ def _describe(emissions, predictions, frames):
              e[0], e[1], p[0], p[1]), (B, T, predictions.shape[1], V, frames.shape[1]))
 
 
-@torch.no_grad()
 def top_words(emissions, predictions, frames, positions, k, temperature=1.0, validate_nodes=True):
     """The ``k`` best words of every node (at most 256): what a beam search extends, and what a
     teacher records for `NodeDistillationLoss`.
@@ -99,28 +121,27 @@ def top_words(emissions, predictions, frames, positions, k, temperature=1.0, val
     Returns words int32 [B, N, k] (the greater score first, of equal ones the lower word), their
     logits float32 [B, N, k] = scores / temperature, and rest float32 [B, N], the log-sum-exp of
     scores / temperature over all other words (-inf where there are none).  Where there is no node:
-    -1, -inf, -inf.  ``validate_nodes=False`` skips the check of the indices, which reads them back
-    from the device, so that the call only enqueues work."""
+    -1, -inf, -inf.  ``validate_nodes=False`` skips the check of the indices, which waits for the
+    kernels, so that the call only enqueues work."""
     certify_nodes(emissions, predictions, frames, positions)
     check_temperature(temperature)
     if not 1 <= k <= min(MAX_LISTED_WORDS, emissions.shape[2]):
         raise ValueError("k must be between 1 and min(%d, vocabulary)" % MAX_LISTED_WORDS)
-    if validate_nodes:
-        certify_indices(emissions, predictions, frames, positions)
     emissions, predictions = _rows(emissions), _rows(predictions)
     B, N = frames.shape
     device = emissions.device
-    with DeviceManager(device):
+    with OnDevice(device):
         words = torch.empty((B, N, k), device=device, dtype=torch.int32)
         logits = torch.empty((B, N, k), device=device, dtype=torch.float32)
         rest = torch.empty((B, N), device=device, dtype=torch.float32)
         scores, sizes = _describe(emissions, predictions, frames)
         _transducer.top_words(scores, frames.data_ptr(), positions.data_ptr(), words.data_ptr(),
                               logits.data_ptr(), rest.data_ptr(), sizes, k, temperature)
+        if validate_nodes:
+            certify_indices(emissions, predictions, frames, positions)
     return words, logits, rest
 
 
-@torch.no_grad()
 def sample_words(emissions, predictions, frames, positions, uniforms, temperature=1.0, top_k=0,
                  top_p=1.0, min_p=0.0, validate_nodes=True):
     """A word of every node, drawn with the numbers ``uniforms`` float32 [B, N] in [0, 1).
@@ -150,17 +171,17 @@ def sample_words(emissions, predictions, frames, positions, uniforms, temperatur
         raise ValueError("top_p must be above 0 and at most 1")
     if not 0.0 <= min_p <= 1.0:
         raise ValueError("min_p must be between 0 and 1")
-    if validate_nodes:
-        certify_indices(emissions, predictions, frames, positions)
     emissions, predictions = _rows(emissions), _rows(predictions)
     device = emissions.device
-    with DeviceManager(device):
+    with OnDevice(device):
         words = torch.empty(frames.shape, device=device, dtype=torch.int32)
         log_probs = torch.empty(frames.shape, device=device, dtype=torch.float32)
         scores, sizes = _describe(emissions, predictions, frames)
         _transducer.sample_words(scores, frames.data_ptr(), positions.data_ptr(),
                                  uniforms.data_ptr(), words.data_ptr(), log_probs.data_ptr(), sizes,
                                  temperature, min(top_k, sizes[3]), top_p, min_p)
+        if validate_nodes:
+            certify_indices(emissions, predictions, frames, positions)
     return words, log_probs
 
 
@@ -169,11 +190,11 @@ class NodeDistillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, emissions, predictions, frames, positions, words, logits, rest, temperature,
-                save):
+                save, validate_nodes):
         emissions, predictions = _rows(emissions), _rows(predictions)
         device = emissions.device
         K = words.shape[2]
-        with DeviceManager(device):
+        with OnDevice(device):
             costs = torch.empty(frames.shape, device=device, dtype=torch.float32)
             scores, sizes = _describe(emissions, predictions, frames)
             nbytes = _transducer.distill_saved_bytes(sizes[0], sizes[4], K) if save else 0
@@ -182,6 +203,8 @@ class NodeDistillation(torch.autograd.Function):
                 scores, frames.data_ptr(), positions.data_ptr(), words.data_ptr(),
                 logits.data_ptr(), 0 if rest is None else rest.data_ptr(), costs.data_ptr(),
                 saved.data_ptr() if save else 0, nbytes, sizes, K, temperature)
+            if validate_nodes:
+                certify_indices(emissions, predictions, frames, positions, words)
         if save:
             ctx.save_for_backward(emissions, predictions, frames, positions, words, saved)
             ctx.temperature = temperature
@@ -193,7 +216,7 @@ class NodeDistillation(torch.autograd.Function):
         emissions, predictions, frames, positions, words, saved = ctx.saved_tensors
         device = emissions.device
         deltas = deltas.to(torch.float32).contiguous()
-        with DeviceManager(device):
+        with OnDevice(device):
             egrads, pgrads = (
                 torch.empty(x.shape, device=device, dtype=x.dtype) if need else None
                 for x, need in zip((emissions, predictions), ctx.needs_input_grad))
@@ -206,7 +229,7 @@ class NodeDistillation(torch.autograd.Function):
                 0 if egrads is None else egrads.data_ptr(),
                 0 if pgrads is None else pgrads.data_ptr(), sizes, words.shape[2],
                 ctx.temperature, ws.data_ptr(), nbytes)
-        return (egrads, pgrads) + (None,) * 7
+        return (egrads, pgrads) + (None,) * 8
 
 
 class NodeDistillationLoss(torch.nn.Module):
@@ -220,8 +243,8 @@ class NodeDistillationLoss(torch.nn.Module):
     Arguments:
         temperature (float, optional): divides the student's scores.  The teacher's logits are taken
             as they are: `top_words` with the same temperature has divided them already.
-        validate_nodes (bool, optional): check that no index lies beyond its tensor (default; reads
-            three numbers back from the device, i.e. synchronises).  Pass False for a call that only
+        validate_nodes (bool, optional): check that no index lies beyond its tensor (default; waits
+            for the forward kernels and reads three numbers back).  Pass False for a call that only
             enqueues work and can be captured in a CUDA graph.
         reduction (str, optional): "none" (default), "sum" or "mean", the latter over the nodes
             that there are.
@@ -270,11 +293,9 @@ class NodeDistillationLoss(torch.nn.Module):
             if rest.shape != frames.shape:
                 raise ValueError("must have a rest per node.")
             check_device(emissions, rest)
-        if self.validate_nodes:
-            certify_indices(emissions, predictions, frames, positions, words)
         save = torch.is_grad_enabled() and (emissions.requires_grad or predictions.requires_grad)
         costs = NodeDistillation.apply(emissions, predictions, frames, positions, words, logits,
-                                       rest, self.temperature, save)
+                                       rest, self.temperature, save, self.validate_nodes)
         if self.reduction == "sum":
             return costs.sum()
         if self.reduction == "mean":
