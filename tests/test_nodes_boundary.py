@@ -142,8 +142,8 @@ def test_c_abi_refusals():
         assert sample(**bad) == 1, bad
     assert sample(B=0, temperature=0.0) == 0
 
-    saved = lib.tb200_distill_saved_bytes(2, 4, 3)
-    assert saved >= 2 * 4 * (16 + 12) and lib.tb200_distill_saved_bytes(0, 4, 3) == 0
+    saved = lib.tb200_distill_saved_bytes(2, 5, 3, 4, 3)
+    assert saved >= 2 * 4 * (16 + 12) and lib.tb200_distill_saved_bytes(0, 5, 3, 4, 3) == 0
     some = ctypes.c_void_p(256)
     most = (ctypes.c_int * 3)()
     assert lib.tb200_node_summary(None, None, -1, None, 0, some, most) == 1
@@ -159,7 +159,7 @@ def test_c_abi_refusals():
     assert forward(B=0) == 0
 
     need = lib.tb200_distill_backward_workspace_bytes(2, 5, 3, 8, 4)
-    assert need >= 2 * 8 * 8
+    assert need > 0
 
     def backward(saved=some, saved_bytes=saved, ws=some, ws_bytes=need, B=2):
         return lib.tb200_distill_backward(None, None, 0, *strides, None, None, None, saved, saved_bytes, None, None,
@@ -171,9 +171,10 @@ def test_c_abi_refusals():
 
 
 def test_workspaces_do_not_grow_for_smaller_calls():
-    for f, sizes in ((lib.tb200_distill_saved_bytes, [(B, 40, 8) for B in range(30)]),
-                     (lib.tb200_distill_saved_bytes, [(3, N, 8) for N in range(300)]),
-                     (lib.tb200_distill_saved_bytes, [(3, 40, K) for K in range(1, 257)]),
+    for f, sizes in ((lib.tb200_distill_saved_bytes, [(B, 50, 9, 40, 8) for B in range(30)]),
+                     (lib.tb200_distill_saved_bytes, [(3, 50, 9, N, 8) for N in range(300)]),
+                     (lib.tb200_distill_saved_bytes, [(3, 50, 9, 40, K) for K in range(1, 257)]),
+                     (lib.tb200_distill_saved_bytes, [(3, T, 9, 40, 8) for T in range(600)]),
                      *((lib.tb200_distill_backward_workspace_bytes, sizes) for sizes in (
                          [(B, 300, 40, 600, 340) for B in range(120)], [(3, T, 9, 700, 400) for T in range(900)],
                          [(3, 9, U, 1000, 90) for U in range(300)], [(2, 90, 9, V, 99) for V in range(1, 9000, 7)],

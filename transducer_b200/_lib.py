@@ -70,7 +70,7 @@ SIGNATURES = {
     "tb200_node_summary": (_i, [_p] * 2 + [_l, _p, _l, _p, ctypes.POINTER(_i)]),
     "tb200_top_words": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 5 + [_i] * 6 + [_d]),
     "tb200_sample_words": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 5 + [_i] * 5 + [_d, _i, _d, _d]),
-    "tb200_distill_saved_bytes": (_z, [_i] * 3),
+    "tb200_distill_saved_bytes": (_z, [_i] * 5),
     "tb200_distill_forward": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 7 + [_z] + [_i] * 6 + [_d]),
     "tb200_distill_backward_workspace_bytes": (_z, [_i] * 5),
     "tb200_distill_backward": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 4 + [_z] + [_p] * 3 + [_i] * 6

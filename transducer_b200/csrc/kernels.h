@@ -292,9 +292,16 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
 // would be a difference of large numbers for the listed words: theirs is -share alone, the others' -2^(x - A).  The
 // listed words' whole gradients are kept too.
 struct DistillSaved {
-  float4* node;   // [B*N] m, A, sign, unused
+  float4* node;     // [B*N] m, A, sign, unused
   float2* listed;   // [B*N*K] share (kNoShare: the word is to be ignored), gradient
+  // where the nodes lie, of each utterance's N
+  int2* spans;      // of the B * T frames, then the B * U positions: (N - first node, last node + 1), or 0
+  int* offPath;     // [B] 1: the nodes are not a path (frames and positions never go back from one to the next)
+  int* segUsed;     // [B, segs] 1: a segment of segFrames frames has nodes
+  int segFrames, segs;
 };
+size_t distill_saved_bytes(int B, int T, int U, int N, int K);
+DistillSaved distill_saved(void* p, int B, int T, int U, int V, int N, int K);
 constexpr float kNoShare = 3e38f;
 void launch_distill_forward(const NodeArgs& a, const int* words, const float* logits, const float* rest,
                             float* costs, DistillSaved saved, int K, double temperature,

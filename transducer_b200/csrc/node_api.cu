@@ -46,15 +46,6 @@ void check_temperature(double t) {
   check(t > 0.0 && std::isfinite((float)(1.4426950408889634 / t)), "temperature must be positive");
 }
 
-size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
-
-DistillSaved distill_saved(void* p, int B, int N) {
-  DistillSaved s;
-  s.node = static_cast<float4*>(p);
-  s.listed = p ? reinterpret_cast<float2*>(static_cast<char*>(p) + round256(sizeof(float4) * (size_t)B * N)) : nullptr;
-  return s;
-}
-
 void need(size_t have, size_t want, const void* p, const char* what) {
   if (want > 0 && (p == nullptr || have < want))
     throw std::invalid_argument(std::string(what) + " too small: need " + std::to_string(want) + " bytes, got " +
@@ -115,10 +106,8 @@ int tb200_sample_words(const void* E, const void* P, int bf16, long long eStride
   });
 }
 
-size_t tb200_distill_saved_bytes(int B, int N, int K) {
-  if (B <= 0 || N <= 0 || K <= 0) return 0;
-  const size_t nodes = (size_t)B * N;
-  return round256(sizeof(float4) * nodes) + round256(sizeof(float2) * nodes * K);
+size_t tb200_distill_saved_bytes(int B, int maxT, int maxU, int N, int K) {
+  return distill_saved_bytes(B, maxT, maxU, N, K);
 }
 
 int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
@@ -132,8 +121,8 @@ int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStr
     check_listed(K);
     check_temperature(temperature);
     check(!rest || V <= kDistillMaxBits, "the alphabet must not exceed 2^20 words where the rest's weight is given");
-    if (saved) need(savedBytes, tb200_distill_saved_bytes(B, N, K), saved, "saved state");
-    launch_distill_forward(a, words, logits, rest, costs, distill_saved(saved, B, N), K, temperature,
+    if (saved) need(savedBytes, distill_saved_bytes(B, maxT, maxU, N, K), saved, "saved state");
+    launch_distill_forward(a, words, logits, rest, costs, distill_saved(B > 0 ? saved : nullptr, B, maxT, maxU, V, N, K), K, temperature,
                            api_stream());
   });
 }
@@ -152,9 +141,9 @@ int tb200_distill_backward(const void* E, const void* P, int bf16, long long eSt
                                  maxU, V, N);
     check_listed(K);
     check_temperature(temperature);
-    need(savedBytes, tb200_distill_saved_bytes(B, N, K), saved, "saved state");
+    need(savedBytes, distill_saved_bytes(B, maxT, maxU, N, K), saved, "saved state");
     need(workspaceBytes, tb200_distill_backward_workspace_bytes(B, maxT, maxU, V, N), workspace, "workspace");
-    launch_distill_backward(a, words, distill_saved(const_cast<void*>(saved), B, N), weights, egrads, pgrads, K,
+    launch_distill_backward(a, words, distill_saved(const_cast<void*>(saved), B, maxT, maxU, V, N, K), weights, egrads, pgrads, K,
                             temperature, workspace, api_stream());
   });
 }

@@ -55,6 +55,32 @@ struct RunningSum {
   }
 };
 
+constexpr int kLookBack = 64;   // places without a node that a path may have between two nodes
+
+// Where a node lies: of consecutive nodes on the same frame, or position, the first and the last one speak for all.
+__device__ __forceinline__ void mark_spans(const NodeArgs& a, const DistillSaved& k, i64 node, int n, int t, int u,
+                                           int tBefore, int uBefore, int tAfter, int uAfter) {
+  auto valid = [&](int t, int u) { return (unsigned)t < (unsigned)a.T && (unsigned)u < (unsigned)a.U; };
+  const i64 b = (unsigned)(node - n) / (unsigned)a.N;
+  const bool before = valid(tBefore, uBefore), after = valid(tAfter, uAfter);
+  int2* frame = k.spans + b * a.T + t;
+  int2* position = k.spans + (i64)a.B * a.T + b * a.U + u;
+  if (!before || tBefore != t) {
+    atomicMax(&frame->x, a.N - n);
+    k.segUsed[b * k.segs + t / k.segFrames] = 1;
+  }
+  if (!after || tAfter != t) atomicMax(&frame->y, n + 1);
+  if (!before || uBefore != u) atomicMax(&position->x, a.N - n);
+  if (!after || uAfter != u) atomicMax(&position->y, n + 1);
+  if (!before) {
+    int back = 2;
+    while (back <= n && back <= kLookBack && !valid(a.frames[node - back], a.positions[node - back])) ++back;
+    if (back > n) return;   // (the first node)
+    tBefore = back > kLookBack ? a.T : a.frames[node - back], uBefore = a.positions[node - back];
+  }
+  if (tBefore > t || uBefore > u) k.offPath[b] = 1;
+}
+
 // A word of the teacher's record.
 struct Listed {
   int word;      // -1: outside the vocabulary
@@ -69,7 +95,7 @@ constexpr int kCta = G == 32 ? 32 * kWarpNodes : G;
 // One group of G threads per node.  Dynamic shared memory, per node: its record, K Listed; with REST a bit per word
 // of the vocabulary, set for listed ones.
 template <typename TIn, int VEC, int G, bool REST>
-__global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
+__global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCta<G>) distill_forward_kernel(
     NodeArgs a, const int* __restrict__ words, const float* __restrict__ logits,
     const float* __restrict__ rest, float* __restrict__ costs, DistillSaved saved, int K, float scale2) {
   constexpr int kNodes = kCta<G> / G, kTurn = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;   // vectors of a row at a time
@@ -91,6 +117,11 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
     }
     return;
   }
+  // (the nodes before and after: their frames and positions, wanted at the end)
+  const i64 beside = node + (tid < 2 ? -1 : 1);
+  const int n = (int)((unsigned)node % (unsigned)a.N);
+  int around = -1;
+  if (savedListed && tid < 4 && (tid < 2 ? n > 0 : n + 1 < a.N)) around = (tid & 1 ? a.positions : a.frames)[beside];
   Group<G> g(tid, scratch);
   // the teacher's shares
   const float lRest = REST ? rest[node] : neg_inf();
@@ -211,6 +242,9 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
     }
   }
   cost = g.sum(cost);
+  if (tid >= 32) return;
+  const int tBefore = __shfl_sync(0xffffffffu, around, 0), uBefore = __shfl_sync(0xffffffffu, around, 1);
+  const int tAfter = __shfl_sync(0xffffffffu, around, 2), uAfter = __shfl_sync(0xffffffffu, around, 3);
   if (tid != 0) return;
   if (REST && r != 0.0f) cost += r * (logf(r) - (other2 == neg_inf() ? other2 : (other2 - all2) * kLn2));
   costs[node] = cost;
@@ -223,6 +257,7 @@ __global__ void __launch_bounds__(kCta<G>) distill_forward_kernel(
     A = L - (fmaxf(logRatio, 0.0f) + log1pf(-expf(-fabsf(logRatio)))) * kLog2e;
   }
   saved.node[node] = make_float4(full.m, A, sign, 0.0f);
+  mark_spans(a, saved, node, n, s.t, s.u, tBefore, uBefore, tAfter, uAfter);
 }
 
 // The greatest indices of a call, so that it can be refused: one CTA per 16384 of them, up to 64.
@@ -280,6 +315,8 @@ void launch_distill_forward(const NodeArgs& a, const int* words, const float* lo
                             float* costs, DistillSaved saved, int K, double temperature,
                             cudaStream_t stream) {
   const i64 nodes = (i64)a.B * a.N;
+  if (saved.spans)
+    TB200_CUDA_CHECK(cudaMemsetAsync(saved.spans, 0, sizeof(int) * a.B * (2 * ((size_t)a.T + a.U) + 1 + saved.segs), stream));
   if (nodes == 0) return;
   const float scale2 = (float)(1.4426950408889634 / temperature);
   with_type(a.dtype, node_rows_aligned(a), [&](auto type, auto vec) {

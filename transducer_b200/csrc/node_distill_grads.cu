@@ -22,7 +22,6 @@ namespace {
 constexpr int kWarps = 4;       // per CTA
 constexpr int kPathWarps = 4;   // of the path kernel, at most
 constexpr int kTarget = 148 * 96;  // warps that fill the chip
-constexpr int kLookBack = 64;      // places without a node that a path may have between two nodes
 
 struct GradArgs {
   const int* words;
@@ -31,42 +30,10 @@ struct GradArgs {
   void *egrads, *pgrads;   // either may be null
   int K;
   float scale, scale2;
-  int2* spans;        // of the B * T frames, then the B * U positions: (N - first node, last node + 1), or 0
-  int* offPath;       // [B] 1: the nodes are not a path
-  int* segUsed;       // [B, segs] 1: a segment has nodes
   float* partial;     // of paths [B, segs, 2, V]
   float* rowPartial;  // of other nodes [splits, rows, V] of E, then of P
-  int segFrames, segs, tiles, eSplits, pSplits;
+  int tiles, eSplits, pSplits;
 };
-
-// Of consecutive nodes on the same frame, or position, the first and the last one of a warp's 32 speak for all.
-__global__ void __launch_bounds__(256) node_spans_kernel(NodeArgs a, GradArgs k) {
-  const i64 node = (i64)blockIdx.x * 256 + threadIdx.x;
-  const int lane = threadIdx.x & 31;
-  const bool in = node < (i64)a.B * a.N;
-  auto valid = [&](i64 i) {
-    return (unsigned)a.frames[i] < (unsigned)a.T && (unsigned)a.positions[i] < (unsigned)a.U;
-  };
-  const bool here = in && valid(node);
-  const i64 b = here ? node / a.N : -1;
-  const int t = here ? a.frames[node] : -1, u = here ? a.positions[node] : -1;
-  const i64 frame = here ? b * a.T + t : -1, position = here ? (i64)a.B * a.T + b * a.U + u : -1;
-  const i64 frameUp = __shfl_up_sync(0xffffffffu, frame, 1), frameDown = __shfl_down_sync(0xffffffffu, frame, 1);
-  const i64 posUp = __shfl_up_sync(0xffffffffu, position, 1), posDown = __shfl_down_sync(0xffffffffu, position, 1);
-  if (!here) return;
-  const int n = (int)(node - b * a.N);
-  if (lane == 0 || frameUp != frame) {
-    atomicMax(&k.spans[frame].x, a.N - n);
-    k.segUsed[b * k.segs + t / k.segFrames] = 1;
-  }
-  if (lane == 31 || frameDown != frame) atomicMax(&k.spans[frame].y, n + 1);
-  if (lane == 0 || posUp != position) atomicMax(&k.spans[position].x, a.N - n);
-  if (lane == 31 || posDown != position) atomicMax(&k.spans[position].y, n + 1);
-  int back = 1;
-  while (back <= n && back <= kLookBack && !valid(node - back)) ++back;
-  if (back > n) return;   // (the first node)
-  if (back > kLookBack || a.frames[node - back] > t || a.positions[node - back] > u) k.offPath[b] = 1;
-}
 
 // (16 bytes: past the L1, most of which is shared memory here)
 template <int BYTES>
@@ -248,18 +215,18 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
   PathWarp<TIn>& mem = reinterpret_cast<PathWarp<TIn>*>(memory + sizeof(PathCta))[warp];
   const int groups = (k.tiles + warps - 1) / warps;   // of tiles
   const i64 bs = blockIdx.x / groups;
-  const int b = (int)(bs / k.segs), seg = (int)(bs - (i64)b * k.segs);
-  if (k.offPath[b]) return;
+  const int b = (int)(bs / k.saved.segs), seg = (int)(bs - (i64)b * k.saved.segs);
+  if (k.saved.offPath[b]) return;
   using T = Tile<TIn, VEC, COLS>;
   const T tile{((int)(blockIdx.x - bs * groups) * warps + warp) * 32 * COLS, a.V, lane};
-  const int t0 = seg * k.segFrames, t1 = min(t0 + k.segFrames, a.T);
+  const int t0 = seg * k.saved.segFrames, t1 = min(t0 + k.saved.segFrames, a.T);
   const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
   TIn* dE = k.egrads ? static_cast<TIn*>(k.egrads) + (i64)b * a.T * a.V : nullptr;
   // the segment's nodes
   int n0 = 0x7fffffff, n1 = 0;
   for (int tb = t0; tb < t1; tb += 32) {
     const int t = tb + lane;
-    const int2 s = t < t1 ? k.spans[(i64)b * a.T + t] : make_int2(0, 1);
+    const int2 s = t < t1 ? k.saved.spans[(i64)b * a.T + t] : make_int2(0, 1);
     if (t < t1 && s.y > 0) n0 = min(n0, a.N - s.x), n1 = max(n1, s.y);
     const float zero[VEC] = {};   // for frames without nodes
     for (unsigned none = __ballot_sync(0xffffffffu, s.y == 0); dE && none; none &= none - 1)
@@ -299,10 +266,10 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
       x.flags = (t != (before ? tBefore : lastT) ? kNewFrame : 0) |
                 (x.u != (before ? uBefore : lastU) ? kNewPosition : 0) | (after && t == tAfter ? kMoreOfFrame : 0);
       if (here && (x.flags & kNewPosition) && k.pgrads) {
-        const int2 s = k.spans[(i64)a.B * a.T + (i64)b * a.U + x.u];
+        const int2 s = k.saved.spans[(i64)a.B * a.T + (i64)b * a.U + x.u];
         const int* frames = a.frames + (i64)b * a.N;
-        const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
-        x.target = from == to ? (i64)x.u * a.V : -1 - (((i64)b * k.segs + seg) * 2 + (from == seg ? 1 : 0)) * a.V;
+        const int from = frames[a.N - s.x] / k.saved.segFrames, to = frames[s.y - 1] / k.saved.segFrames;
+        x.target = from == to ? (i64)x.u * a.V : -1 - (((i64)b * k.saved.segs + seg) * 2 + (from == seg ? 1 : 0)) * a.V;
       }
       if (here) {
         cta.steps[(appended + __popc(before)) % kSteps] = x;
@@ -496,7 +463,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
   const i64 ePer = (i64)a.T * k.eSplits * k.tiles, pPer = (i64)a.U * k.pSplits * k.tiles;   // tasks of an utterance
   const i64 step = (i64)gridDim.x * kWarps;
   for (int b = 0; b < a.B; ++b) {
-    if (!k.offPath[b]) continue;
+    if (!k.saved.offPath[b]) continue;
     for (i64 task = (i64)blockIdx.x * kWarps + warp; task < ePer + pPer; task += step) {
       const bool ofFrames = task < ePer;
       if ((ofFrames ? k.egrads : k.pgrads) == nullptr) continue;
@@ -508,7 +475,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
       const T tile{(rem - split * k.tiles) * 32 * COLS, a.V, lane};
       const TIn* E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
       const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
-      const int2 span = k.spans[ofFrames ? (i64)b * a.T + own : (i64)a.B * a.T + (i64)b * a.U + own];
+      const int2 span = k.saved.spans[ofFrames ? (i64)b * a.T + own : (i64)a.B * a.T + (i64)b * a.U + own];
       const TIn* otherRows = ofFrames ? P : E;
       const i64 otherStride = ofFrames ? a.pStrideU : a.eStrideT;
       typename T::Row mine, theirs, next;
@@ -610,7 +577,7 @@ __global__ void __launch_bounds__(kWarps * 32) distill_join_kernel(NodeArgs a, G
   if (lane < group && first + lane < rows) {
     const int per = ofFrames ? a.T : a.U;
     const int b = row / per;
-    if (k.offPath[b]) {
+    if (k.saved.offPath[b]) {
       const int splits = ofFrames ? k.eSplits : k.pSplits;
       if (splits > 1) {
         count = splits;
@@ -618,15 +585,15 @@ __global__ void __launch_bounds__(kWarps * 32) distill_join_kernel(NodeArgs a, G
         stride = (i64)a.B * per;
       }
     } else if (!ofFrames) {
-      const int2 s = k.spans[(i64)a.B * a.T + row];
+      const int2 s = k.saved.spans[(i64)a.B * a.T + row];
       if (s.y == 0) {
         count = 0;
       } else {
         const int* frames = a.frames + (i64)b * a.N;
-        const int from = frames[a.N - s.x] / k.segFrames, to = frames[s.y - 1] / k.segFrames;
+        const int from = frames[a.N - s.x] / k.saved.segFrames, to = frames[s.y - 1] / k.saved.segFrames;
         if (from != to) {   // the part of the first segment is in its second place, the others' in their first
           count = to - from + 1;
-          used = b * k.segs + from;
+          used = b * k.saved.segs + from;
           at = (i64)used * 2;
           stride = 2;
         }
@@ -644,7 +611,7 @@ __global__ void __launch_bounds__(kWarps * 32) distill_join_kernel(NodeArgs a, G
 #pragma unroll 4
     for (int c = 0; c < n; ++c) {
       const float* p = part + (u >= 0 && c == 0 ? 1 : c * step) * a.V;
-      const bool there = u < 0 || k.segUsed[u + c];   // (a segment without nodes has left nothing)
+      const bool there = u < 0 || k.saved.segUsed[u + c];   // (a segment without nodes has left nothing)
 #pragma unroll
       for (int j = 0; j < kJoinWords / 32; ++j) {
         const int v = chunk * kJoinWords + j * 32 + lane;
@@ -664,7 +631,6 @@ constexpr int kLeastFrames = 16, kLeastNodes = 8, kTileWords = 32 * kCols;
 
 struct Plan {
   int tiles, segFrames, segs, eSplits, pSplits;
-  size_t spanBytes;
 };
 Plan plan_of(int B, int T, int U, int V, int N) {
   Plan p{};
@@ -679,7 +645,6 @@ Plan plan_of(int B, int T, int U, int V, int N) {
   };
   p.eSplits = splits(T);
   p.pSplits = splits(U);
-  p.spanBytes = sizeof(int) * ((size_t)B * (2 * ((size_t)T + U) + 1 + p.segs));
   return p;
 }
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -692,14 +657,34 @@ size_t path_floats(int B, int T, int V) {
 
 }  // namespace
 
+size_t distill_saved_bytes(int B, int T, int U, int N, int K) {
+  if (B <= 0 || T < 0 || U < 0 || N < 0 || K <= 0) return 0;
+  const size_t nodes = (size_t)B * N, segs = div_up(std::max(T, 1), kLeastFrames);
+  return round256(sizeof(float4) * nodes) + round256(sizeof(float2) * nodes * K) +
+         round256(sizeof(int) * B * (2 * ((size_t)T + U) + 1 + segs));
+}
+
+DistillSaved distill_saved(void* p, int B, int T, int U, int V, int N, int K) {
+  DistillSaved s{};
+  if (!p) return s;
+  const Plan plan = plan_of(B, T, U, V, N);
+  const size_t nodes = (size_t)B * N;
+  char* at = static_cast<char*>(p);
+  s.node = reinterpret_cast<float4*>(at);
+  s.listed = reinterpret_cast<float2*>(at += round256(sizeof(float4) * nodes));
+  s.spans = reinterpret_cast<int2*>(at + round256(sizeof(float2) * nodes * K));
+  s.offPath = reinterpret_cast<int*>(s.spans + (i64)B * ((i64)T + U));
+  s.segUsed = s.offPath + B;
+  s.segFrames = plan.segFrames;
+  s.segs = plan.segs;
+  return s;
+}
+
 size_t distill_backward_workspace_bytes(int B, int T, int U, int V, int N) {
   if (B <= 0 || T < 0 || U < 0 || V <= 0 || N < 0) return 0;
   // (the splits of a side fill kTarget tiles at most)
-  const size_t leastSegs = div_up(std::max(T, 1), kLeastFrames), full = (size_t)kTarget * kTileWords;
-  const size_t path = path_floats(B, T, V);
-  const size_t rows = 2 * std::min((size_t)N / kLeastNodes * B * V, full);
-  return round256(sizeof(int) * ((size_t)B * (2 * ((size_t)T + U) + 1 + leastSegs))) +
-         round256(sizeof(float) * path) + round256(sizeof(float) * rows);
+  const size_t rows = 2 * std::min((size_t)N / kLeastNodes * B * V, (size_t)kTarget * kTileWords);
+  return round256(sizeof(float) * path_floats(B, T, V)) + round256(sizeof(float) * rows);
 }
 
 void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved saved, const float* weights,
@@ -717,22 +702,11 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
   k.K = K;
   k.scale = (float)(1.0 / temperature);
   k.scale2 = (float)(1.4426950408889634 / temperature);
-  k.spans = static_cast<int2*>(workspace);
-  k.offPath = reinterpret_cast<int*>(k.spans + (i64)a.B * ((i64)a.T + a.U));
-  k.segUsed = k.offPath + a.B;
-  k.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(p.spanBytes));
+  k.partial = static_cast<float*>(workspace);
   k.rowPartial = k.partial + round256(sizeof(float) * path_floats(a.B, a.T, a.V)) / sizeof(float);
-  k.segFrames = p.segFrames;
-  k.segs = p.segs;
   k.tiles = p.tiles;
   k.eSplits = p.eSplits;
   k.pSplits = p.pSplits;
-  TB200_CUDA_CHECK(cudaMemsetAsync(workspace, 0, p.spanBytes, stream));
-  if (nodes > 0) {
-    ScopedKernel prof("node_spans", stream);
-    node_spans_kernel<<<(unsigned)div_up64(nodes, 256), 256, 0, stream>>>(a, k);
-    TB200_CHECK_LAUNCH();
-  }
   const bool wide = node_rows_aligned(a) && reinterpret_cast<uintptr_t>(egrads) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(pgrads) % 16 == 0;
   auto run = [&](auto type, auto vec) {

@@ -75,13 +75,15 @@ __device__ __forceinline__ float ex2(float x) {
 template <typename TIn>
 struct NodeScores {
   const TIn *e, *p;
+  int t, u;
   bool here;
 };
 template <typename TIn>
 __device__ __forceinline__ NodeScores<TIn> node_scores(const NodeArgs& a, i64 node) {
-  const i64 b = node / a.N;
+  const i64 b = (unsigned)node / (unsigned)a.N;   // (fewer than 2^31 nodes)
   const int t = a.frames[node], u = a.positions[node];
   NodeScores<TIn> s;
+  s.t = t, s.u = u;
   s.here = (unsigned)t < (unsigned)a.T && (unsigned)u < (unsigned)a.U;
   s.e = static_cast<const TIn*>(a.E) + b * a.eStrideB + (s.here ? t : 0) * a.eStrideT;
   s.p = static_cast<const TIn*>(a.P) + b * a.pStrideB + (s.here ? u : 0) * a.pStrideU;

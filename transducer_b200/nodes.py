@@ -197,7 +197,7 @@ class NodeDistillation(torch.autograd.Function):
         with OnDevice(device):
             costs = torch.empty(frames.shape, device=device, dtype=torch.float32)
             scores, sizes = _describe(emissions, predictions, frames)
-            nbytes = _transducer.distill_saved_bytes(sizes[0], sizes[4], K) if save else 0
+            nbytes = _transducer.distill_saved_bytes(*sizes[:3], sizes[4], K) if save else 0
             saved = _workspace(nbytes, device) if save else None
             _transducer.distill_forward(
                 scores, frames.data_ptr(), positions.data_ptr(), words.data_ptr(),
@@ -211,18 +211,17 @@ class NodeDistillation(torch.autograd.Function):
         return costs
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, deltas):
         emissions, predictions, frames, positions, words, saved = ctx.saved_tensors
         device = emissions.device
-        deltas = deltas.to(torch.float32).contiguous()
+        deltas = deltas.contiguous()
+        need_e, need_p = ctx.needs_input_grad[:2]
         with OnDevice(device):
-            egrads, pgrads = (
-                torch.empty(x.shape, device=device, dtype=x.dtype) if need else None
-                for x, need in zip((emissions, predictions), ctx.needs_input_grad))
+            egrads = torch.empty(emissions.shape, device=device, dtype=emissions.dtype) if need_e else None
+            pgrads = torch.empty(predictions.shape, device=device, dtype=predictions.dtype) if need_p else None
             scores, sizes = _describe(emissions, predictions, frames)
             nbytes = _transducer.distill_backward_workspace_bytes(*sizes)
-            ws = _workspace(nbytes, device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _transducer.distill_backward(
                 scores, frames.data_ptr(), positions.data_ptr(), words.data_ptr(),
                 saved.data_ptr(), saved.numel(), deltas.data_ptr(),
