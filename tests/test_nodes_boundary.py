@@ -61,7 +61,7 @@ def test_bad_k(k):
         top_words(*nodes(), k)
 
 
-@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), float("inf")])
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), float("inf"), 1e-40, 1e31])
 def test_bad_temperature(temperature):
     with pytest.raises(ValueError, match="temperature must be positive"):
         top_words(*nodes(), 2, temperature=temperature)
@@ -127,8 +127,9 @@ def test_c_abi_refusals():
                                    temperature)
 
     for bad in (dict(B=-1), dict(T=-1), dict(U=-1), dict(V=0), dict(N=-1), dict(k=0), dict(k=9), dict(k=257, V=400),
-                dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=1e-60),
-                dict(B=1 << 16, N=1 << 15), dict(strides=(-40, 8, 24, 8))):
+                dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=1e-60), dict(temperature=1e31),
+                dict(B=1 << 16, N=1 << 15), dict(B=1 << 16, T=1 << 15, N=0), dict(B=1 << 16, U=1 << 15, N=0),
+                dict(strides=(-40, 8, 24, 8))):
         assert top(**bad) == 1, bad
         assert lib.tb200_last_error()
     assert top(B=0) == 0 and top(N=0) == 0
@@ -165,7 +166,8 @@ def test_c_abi_refusals():
         return lib.tb200_distill_backward(None, None, 0, *strides, None, None, None, saved, saved_bytes, None, None,
                                           None, B, 5, 3, 8, 4, 3, 1.0, ws, ws_bytes)
 
-    for bad in (dict(saved=None), dict(saved_bytes=saved - 1), dict(ws=None), dict(ws_bytes=need - 1)):
+    odd = ctypes.c_void_p(264)
+    for bad in (dict(saved=None), dict(saved_bytes=saved - 1), dict(saved=odd), dict(ws=odd), dict(ws=None), dict(ws_bytes=need - 1)):
         assert backward(**bad) == 1, bad
     assert backward(B=0, saved_bytes=0) == 0
 

@@ -31,7 +31,7 @@ def make(B, T, U, V, N, dtype=torch.float32, seed=0, std=2.0, holes=True, kind="
 
 
 SIZES = [1, 2, 7, 8, 31, 33, 128, 255, 256, 257, 264, 1000, 1023, 1024, 1025, 1032, 4096, 4097, 4104, 10000,
-         16384, 16392, 32768, 32769, 40000]
+         16384, 16392, 32768, 32769, 40000, 60000, 60001]
 
 
 @pytest.mark.parametrize("V", SIZES)
@@ -51,7 +51,7 @@ def test_top_words(V, dtype, k):
     torch.testing.assert_close(rest.cpu().double(), r, rtol=64 * UNIT, atol=128 * UNIT)
 
 
-@pytest.mark.parametrize("V", [1, 40, 1025, 4096, 12000, 33000])
+@pytest.mark.parametrize("V", [1, 40, 1025, 4096, 12000, 33000, 60000])
 @pytest.mark.parametrize("k", [1, 3, 200])
 def test_top_words_of_equal_and_masked_scores(V, k):
     k = min(k, V)
@@ -71,6 +71,23 @@ def test_top_words_of_equal_and_masked_scores(V, k):
     assert torch.equal(words.cpu(), w)
     assert torch.equal(logits.cpu().double(), l)
     torch.testing.assert_close(rest.cpu().double(), r, rtol=64 * UNIT, atol=128 * UNIT)
+
+
+@pytest.mark.parametrize("V", [33, 1000, 5000, 60001])
+def test_top_words_of_broken_scores(V):
+    """NaN stands above everything and +inf above all numbers; the other nodes are what they were."""
+    E, P, frames, positions, g = make(2, 4, 2, V, 8, seed=V, holes=False)
+    clean = top_words(E, P, frames, positions, 9)
+    E[0, 1, V // 3], E[0, 1, V - 1], E[0, 2, 5], E[1, 3, 7] = math.nan, math.nan, math.inf, math.nan
+    E[1, 3, 8], E[1, 3, 20] = math.inf, -math.inf
+    words, logits, rest = top_words(E, P, frames, positions, 9)
+    z, here = ref.scores(E, P, frames, positions)
+    w, l, r = ref.top_words(z, here, 9)
+    assert torch.equal(words.cpu(), w)
+    torch.testing.assert_close(logits.cpu().double(), l, rtol=0, atol=0, equal_nan=True)
+    whole = z.isfinite().all(-1)
+    torch.testing.assert_close(rest.cpu().double()[whole], r[whole], rtol=64 * UNIT, atol=128 * UNIT)
+    assert torch.equal(rest[whole.cuda()], clean[2][whole.cuda()])
 
 
 def check_sample(E, P, frames, positions, uniforms, **rule):
@@ -98,7 +115,7 @@ def test_sample_words(V, dtype):
         check_sample(E, P, frames, positions, uniforms, **rule)
 
 
-@pytest.mark.parametrize("V", [3, 100, 1025, 5000, 20000, 33000])
+@pytest.mark.parametrize("V", [3, 100, 1025, 5000, 20000, 33000, 60000])
 def test_sample_words_of_equal_and_masked_scores(V):
     E, P, frames, positions, g = make(4, 4, 2, V, 40, seed=V, holes=False)
     E[0], P[0] = 0.0, 0.0
@@ -225,6 +242,56 @@ def test_distillation_odd_records(V, with_rest):
     E[1, 5, words[1, 2, 0].long()] = -math.inf
     E[1, 4] = torch.finfo(torch.float32).min
     check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.0, g, K)
+
+
+@pytest.mark.parametrize("with_rest", [False, True])
+@pytest.mark.parametrize("K", [33, 64, 100, 256])
+def test_distillation_long_records(K, with_rest):
+    """Records of several words per lane, some longer than the vocabulary, with words more than once."""
+    for V in (50, 300, 3001):
+        E, P, frames, positions, g = make(2, 20, 4, V, 24, seed=K, kind="path")
+        words = torch.randint(-1, V, (2, 24, K), generator=g).int().cuda()
+        logits = (2.0 * torch.randn(2, 24, K, generator=g)).cuda()
+        rest = torch.randn(2, 24, generator=g).cuda()
+        check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.5, g, K)
+
+
+def test_native_calls_without_optional_buffers():
+    """No rest from the best words, no state from the forward call, one gradient alone."""
+    from transducer_b200 import _transducer, nodes
+    E, P, frames, positions, g = make(2, 9, 4, 100, 12, kind="path")
+    words, logits, rest = top_words(E, P, frames, positions, 5)
+    costs = NodeDistillationLoss()(E.requires_grad_(True), P.requires_grad_(True), frames, positions, words,
+                                   logits + 0.3 * torch.randn(logits.shape, generator=g).cuda(), rest)
+    weights = torch.rand(2, 12, generator=g).cuda()
+    dE, dP = torch.autograd.grad(costs, (E, P), weights, retain_graph=True)
+    saved = costs.grad_fn.saved_tensors[-1]
+    with nodes.OnDevice(E.device):
+        scores, sizes = nodes._describe(E, P, frames)
+        at = frames.data_ptr(), positions.data_ptr()
+        w2, l2 = torch.empty_like(words), torch.empty_like(logits)
+        _transducer.top_words(scores, *at, w2.data_ptr(), l2.data_ptr(), 0, sizes, 5, 1.0)
+        assert torch.equal(w2, words) and torch.equal(l2, logits)
+        n = _transducer.distill_backward_workspace_bytes(*sizes)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        for which, want in ((0, dE), (1, dP)):
+            out = torch.full_like(want, math.nan)
+            to = (out.data_ptr(), 0) if which == 0 else (0, out.data_ptr())
+            _transducer.distill_backward(scores, *at, words.data_ptr(), saved.data_ptr(), saved.numel(),
+                                         weights.data_ptr(), *to, sizes, 5, 1.0, ws.data_ptr(), n)
+            assert torch.equal(out, want)
+
+
+def test_the_same_tensor_on_both_sides():
+    """Scores that are twice a row of one tensor: its gradient is both sides' together."""
+    E, _, frames, positions, g = make(2, 6, 6, 40, 9, holes=False)
+    words, logits, _ = teacher(E, E, frames, positions, 4, g)
+    E.requires_grad_(True)
+    other = E.detach().clone().requires_grad_(True)
+    criterion = NodeDistillationLoss()
+    both = torch.autograd.grad(criterion(E, E, frames, positions, words, logits).sum(), E)[0]
+    a, b = torch.autograd.grad(criterion(E, other, frames, positions, words, logits).sum(), (E, other))
+    torch.testing.assert_close(both, a + b, rtol=0, atol=0)
 
 
 def test_distillation_where_every_word_is_listed():

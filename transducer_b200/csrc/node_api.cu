@@ -34,6 +34,8 @@ NodeArgs node_args(const void* E, const void* P, int bf16, long long eStrideB, l
         "negative batch/length/number of nodes or non-positive alphabet size");
   check(eStrideB >= 0 && eStrideT >= 0 && pStrideB >= 0 && pStrideU >= 0, "negative stride");
   check((long long)B * N < 0x7fffffffLL, "too many nodes (batchSize * nodes must be below 2^31 - 1)");
+  check((long long)B * maxT < 0x7fffffffLL && (long long)B * maxU < 0x7fffffffLL,
+        "too many rows (batchSize * maxInputLength and batchSize * maxLabelLength must be below 2^31 - 1)");
   return NodeArgs{E, P, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT, maxU, V, N,
                   bf16 ? kDtypeBf16 : kDtypeF32};
 }
@@ -42,14 +44,17 @@ void check_listed(int K) {
   check(K >= 1 && K <= kMaxListedWords, "the number of listed words must be between 1 and 256");
 }
 void check_temperature(double t) {
-  // (its reciprocal is used in 32 bits)
-  check(t > 0.0 && std::isfinite((float)(1.4426950408889634 / t)), "temperature must be positive");
+  // (it and its reciprocal are used in 32 bits)
+  check(t > 0.0 && t <= 1e30 && std::isfinite((float)(1.4426950408889634 / t)),
+        "temperature must be positive, at least 1e-38 and at most 1e30");
 }
 
 void need(size_t have, size_t want, const void* p, const char* what) {
   if (want > 0 && (p == nullptr || have < want))
     throw std::invalid_argument(std::string(what) + " too small: need " + std::to_string(want) + " bytes, got " +
                                 std::to_string(have));
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+    throw std::invalid_argument(std::string(what) + " must be 16-byte aligned");
 }
 
 }  // namespace

@@ -96,9 +96,9 @@ def check_device(first, *others):
             raise ValueError("all inputs must be on the same device.")
 
 
-def check_temperature(temperature, least=0.0):
-    if not least < temperature < float("inf"):
-        raise ValueError("temperature must be positive")
+def check_temperature(temperature):
+    if not 1e-38 <= temperature <= 1e30:
+        raise ValueError("temperature must be positive, at least 1e-38 and at most 1e30")
 
 
 def _rows(scores):
