@@ -322,9 +322,10 @@ int tb200_loss_sum_exchange(const float* lossSum, void* const* peerSlots, int ra
  * bf16 = 1: emissions, predictions and their gradients are bfloat16 instead of float.  Any alphabet
  * size and alignment is taken; rows that are 16-byte aligned and whole multiples of 16 bytes are
  * faster.  eStrideB, eStrideT, pStrideB, pStrideU: distances, in elements and not negative, between
- * utterances and between frames resp. positions; words lie next to each other.  batchSize * nodes,
- * batchSize * maxInputLength and batchSize * maxLabelLength must be below 2^31 - 1.  temperature:
- * 1e-38 to 1e30.  Saved state and workspaces are 16-byte aligned. */
+ * utterances and between frames resp. positions; words lie next to each other.  batchSize * nodes
+ * is below 2^31 - 1, batchSize * maxInputLength and batchSize * maxLabelLength are 2^31 - 2^16 at
+ * most, the alphabet has up to 2^28 words.  temperature: 1e-38 to 1e30.  Saved state and workspaces
+ * are 16-byte aligned. */
 
 /* What a checked call wants to know of its indices, for one kernel and one synchronisation of the
  * calling thread's stream: the greatest frame, position and (words may be NULL) listed word, -1 if

@@ -128,7 +128,7 @@ def test_c_abi_refusals():
 
     for bad in (dict(B=-1), dict(T=-1), dict(U=-1), dict(V=0), dict(N=-1), dict(k=0), dict(k=9), dict(k=257, V=400),
                 dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=1e-60), dict(temperature=1e31),
-                dict(B=1 << 16, N=1 << 15), dict(B=1 << 16, T=1 << 15, N=0), dict(B=1 << 16, U=1 << 15, N=0),
+                dict(B=1 << 16, N=1 << 15), dict(B=1 << 16, T=1 << 15, N=0), dict(B=1 << 16, U=1 << 15, N=0), dict(V=(1 << 28) + 1),
                 dict(strides=(-40, 8, 24, 8))):
         assert top(**bad) == 1, bad
         assert lib.tb200_last_error()

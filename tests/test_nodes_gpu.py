@@ -282,6 +282,21 @@ def test_native_calls_without_optional_buffers():
             assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("which", [0, 1, (0, 1)])
+def test_second_derivatives_are_refused(which):
+    E, P, frames, positions, g = make(2, 6, 4, 40, 9, holes=False)
+    words, logits, rest = teacher(E, P, frames, positions, 4, g)
+    E.requires_grad_(True), P.requires_grad_(True)
+    leaves = [(E, P)[i] for i in (which if isinstance(which, tuple) else (which,))]
+    cost = NodeDistillationLoss(reduction="sum")(E, P, frames, positions, words, logits, rest)
+    plain = torch.autograd.grad(cost, leaves, retain_graph=True)
+    grads = torch.autograd.grad(cost, leaves, create_graph=True)
+    for a, b in zip(plain, grads):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (cost + sum(x.square().sum() for x in grads)).backward()
+
+
 def test_the_same_tensor_on_both_sides():
     """Scores that are twice a row of one tensor: its gradient is both sides' together."""
     E, _, frames, positions, g = make(2, 6, 6, 40, 9, holes=False)

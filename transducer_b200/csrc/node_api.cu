@@ -34,8 +34,9 @@ NodeArgs node_args(const void* E, const void* P, int bf16, long long eStrideB, l
         "negative batch/length/number of nodes or non-positive alphabet size");
   check(eStrideB >= 0 && eStrideT >= 0 && pStrideB >= 0 && pStrideU >= 0, "negative stride");
   check((long long)B * N < 0x7fffffffLL, "too many nodes (batchSize * nodes must be below 2^31 - 1)");
-  check((long long)B * maxT < 0x7fffffffLL && (long long)B * maxU < 0x7fffffffLL,
-        "too many rows (batchSize * maxInputLength and batchSize * maxLabelLength must be below 2^31 - 1)");
+  check((long long)B * maxT <= 0x7fff0000LL && (long long)B * maxU <= 0x7fff0000LL,
+        "too many rows (batchSize * maxInputLength and batchSize * maxLabelLength must be at most 2^31 - 2^16)");
+  check(V <= 1 << 28, "the alphabet must not exceed 2^28 words");
   return NodeArgs{E, P, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT, maxU, V, N,
                   bf16 ? kDtypeBf16 : kDtypeF32};
 }
@@ -127,8 +128,8 @@ int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStr
     check_temperature(temperature);
     check(!rest || V <= kDistillMaxBits, "the alphabet must not exceed 2^20 words where the rest's weight is given");
     if (saved) need(savedBytes, distill_saved_bytes(B, maxT, maxU, N, K), saved, "saved state");
-    launch_distill_forward(a, words, logits, rest, costs, distill_saved(B > 0 ? saved : nullptr, B, maxT, maxU, V, N, K), K, temperature,
-                           api_stream());
+    const DistillSaved state = distill_saved(B > 0 ? saved : nullptr, B, maxT, maxU, V, N, K);
+    launch_distill_forward(a, words, logits, rest, costs, state, K, temperature, api_stream());
   });
 }
 
@@ -148,8 +149,8 @@ int tb200_distill_backward(const void* E, const void* P, int bf16, long long eSt
     check_temperature(temperature);
     need(savedBytes, distill_saved_bytes(B, maxT, maxU, N, K), saved, "saved state");
     need(workspaceBytes, tb200_distill_backward_workspace_bytes(B, maxT, maxU, V, N), workspace, "workspace");
-    launch_distill_backward(a, words, distill_saved(const_cast<void*>(saved), B, maxT, maxU, V, N, K), weights, egrads, pgrads, K,
-                            temperature, workspace, api_stream());
+    const DistillSaved state = distill_saved(const_cast<void*>(saved), B, maxT, maxU, V, N, K);
+    launch_distill_backward(a, words, state, weights, egrads, pgrads, K, temperature, workspace, api_stream());
   });
 }
 

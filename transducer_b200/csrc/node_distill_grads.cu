@@ -21,7 +21,9 @@ namespace {
 
 constexpr int kWarps = 4;       // per CTA
 constexpr int kPathWarps = 4;   // of the path kernel, at most
-constexpr int kTarget = 148 * 96;  // warps that fill the chip
+// Warps that a launch is cut into where it can be: six times the 16 that an SM holds, so that the last ones to
+// finish leave little of the chip idle.
+constexpr int kTarget = 148 * 96;
 
 struct GradArgs {
   const int* words;
@@ -179,7 +181,7 @@ __device__ __forceinline__ void add_record(const GradArgs& k, Record r, float w,
 // A node as its CTA comes to it: all that can be known beforehand, made for 32 nodes at a time by a lane each.
 struct __align__(16) Step {
   Terms terms;
-  int flags, u, unused;
+  int flags, u;
   i64 row, out, record;   // from the utterance's first: the frame's row of E and of dE; the node's record
   i64 target;             // of a new position: its row of dP, or -1 less its place among the partial rows
 };

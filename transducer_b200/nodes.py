@@ -228,7 +228,21 @@ class NodeDistillation(torch.autograd.Function):
                 0 if egrads is None else egrads.data_ptr(),
                 0 if pgrads is None else pgrads.data_ptr(), sizes, words.shape[2],
                 ctx.temperature, ws.data_ptr(), nbytes)
+        if torch.is_grad_enabled():   # (somebody wants to differentiate these)
+            egrads, pgrads = Once.apply(egrads, pgrads, emissions, predictions, deltas)
         return (egrads, pgrads) + (None,) * 8
+
+
+class Once(torch.autograd.Function):
+    """Gradients that are not differentiable again: asking for it is an error, not 0."""
+
+    @staticmethod
+    def forward(ctx, egrads, pgrads, *what_they_depend_on):
+        return tuple(None if g is None else g.view_as(g) for g in (egrads, pgrads))
+
+    @staticmethod
+    def backward(ctx, *deltas):
+        raise RuntimeError("the distillation cost is differentiable once only")
 
 
 class NodeDistillationLoss(torch.nn.Module):
@@ -244,7 +258,9 @@ class NodeDistillationLoss(torch.nn.Module):
             as they are: `top_words` with the same temperature has divided them already.
         validate_nodes (bool, optional): check that no index lies beyond its tensor (default; waits
             for the forward kernels and reads three numbers back).  Pass False for a call that only
-            enqueues work and can be captured in a CUDA graph.
+            enqueues work and can be captured in a CUDA graph (with its backward pass by
+            torch.autograd.grad: `Tensor.backward` adds to a leaf on the stream on which the leaf
+            was first used, which the capture does not see).
         reduction (str, optional): "none" (default), "sum" or "mean", the latter over the nodes
             that there are.
     """
