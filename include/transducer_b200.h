@@ -369,8 +369,7 @@ int tb200_sample_words(const void* emissions, const void* predictions, int bf16,
  * softmax(z / temperature), whose words that are not listed are one outcome if rest is given.  0
  * where there is no node or the record has no weight; +inf where the student masks a word that the
  * teacher does not (the gradient is then its limit).
- * saved: what the backward call needs, tb200_distill_saved_bytes(), or NULL if none follows.  With
- * rest the alphabet is limited to 2^20 words.
+ * saved: what the backward call needs, tb200_distill_saved_bytes(), or NULL if none follows.
  * The backward call writes egrads [B, maxT, V] and pgrads [B, maxU, V] whole and contiguous (either
  * may be NULL): the gradients of sum weights[b,n] costs[b,n].  They are added up in the nodes' order,
  * in fp32, and rounded once: the bits are the same from run to run.  Fastest where the nodes of an

@@ -155,7 +155,7 @@ def test_c_abi_refusals():
         return lib.tb200_distill_forward(None, None, 0, *strides, None, None, None, None, rest, None, some,
                                          saved_bytes, B, 5, 3, V, 4, K, 1.0)
 
-    for bad in (dict(K=0), dict(K=257), dict(saved_bytes=saved - 1), dict(V=(1 << 20) + 1, rest=some)):
+    for bad in (dict(K=0), dict(K=257), dict(saved_bytes=saved - 1), dict(V=(1 << 28) + 1, rest=some)):
         assert forward(**bad) == 1, bad
     assert forward(B=0) == 0
 

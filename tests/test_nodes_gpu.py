@@ -201,6 +201,29 @@ def test_distillation_long_groups(V, B, T, U, N, kind, with_rest):
     check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.0, g, 5)
 
 
+@pytest.mark.parametrize("scale,offset", [(300.0, 0.0), (1.0, 3e5), (1.0, -2e6), (50.0, 4e8), (1e33, 0.0)])
+@pytest.mark.parametrize("V", [264, 1025, 3000])
+@pytest.mark.parametrize("kind", ["any", "path"])
+@pytest.mark.parametrize("with_rest", [False, True])
+def test_distillation_of_wide_scores(scale, offset, V, kind, with_rest):
+    """Scores of any size, rows that start masked and rows that rise from word to word."""
+    E, P, frames, positions, g = make(2, 9, 3, V, 14, seed=V, kind=kind, holes=False)
+    E = E * scale + offset
+    E[0] = E[0].sort(-1).values
+    E[1, :, :V // 2] = -math.inf
+    words = torch.randint(0, V, (2, 14, 5), generator=g).int().cuda()
+    words[1] = words[1] // 2 + V // 2
+    logits = torch.randn(2, 14, 5, generator=g).cuda()
+    rest = torch.randn(2, 14, generator=g).cuda()
+    check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.5, g, 5)
+
+
+def test_distillation_with_a_very_large_alphabet():
+    E, P, frames, positions, g = make(1, 2, 1, (1 << 20) + 5, 3, holes=False)
+    words, logits, rest = teacher(E, P, frames, positions, 7, g)
+    check_distill(E, P, frames, positions, words, logits, rest, 1.0, g, 7)
+
+
 @pytest.mark.parametrize("V", [30, 64, 1025])
 @pytest.mark.parametrize("gap", [10, 100])
 def test_distillation_paths_with_gaps(V, gap):

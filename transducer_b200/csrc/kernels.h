@@ -269,7 +269,6 @@ void launch_node_summary(const int* frames, const int* positions, i64 nodes, con
 
 constexpr int kMaxListedWords = 256;   // longest list of words per node
 // Largest vocabulary of a distillation with the rest's weight: a bit per word in shared memory.
-constexpr int kDistillMaxBits = 1 << 20;
 
 // Whether every row can be moved in 16-byte vectors.
 bool node_rows_aligned(const NodeArgs& a);
@@ -292,7 +291,7 @@ void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, f
 // would be a difference of large numbers for the listed words: theirs is -share alone, the others' -2^(x - A).  The
 // listed words' whole gradients are kept too.
 struct DistillSaved {
-  float4* node;     // [B*N] m, A, sign, unused
+  float4* node;     // [B*N] m, A, sign (where that is -2, m and A are the others' own), unused
   float2* listed;   // [B*N*K] share (kNoShare: the word is to be ignored), gradient
   // where the nodes lie, of each utterance's N
   int2* spans;      // of the B * T frames, then the B * U positions: (N - first node, last node + 1), or 0

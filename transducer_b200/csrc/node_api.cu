@@ -126,7 +126,6 @@ int tb200_distill_forward(const void* E, const void* P, int bf16, long long eStr
                                  maxU, V, N);
     check_listed(K);
     check_temperature(temperature);
-    check(!rest || V <= kDistillMaxBits, "the alphabet must not exceed 2^20 words where the rest's weight is given");
     if (saved) need(savedBytes, distill_saved_bytes(B, maxT, maxU, N, K), saved, "saved state");
     const DistillSaved state = distill_saved(B > 0 ? saved : nullptr, B, maxT, maxU, V, N, K);
     launch_distill_forward(a, words, logits, rest, costs, state, K, temperature, api_stream());

@@ -17,7 +17,7 @@
 namespace tb200 {
 namespace {
 
-constexpr int kForwardBytes = 150 * 1024;   // of shared memory: 2^20 bits, 256 words of a record and more
+constexpr int kForwardBytes = 64 * 1024;   // of shared memory, at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Running maximum of the scores and sum of 2^((score - maximum) scale2).  The maximum is subtracted
@@ -52,6 +52,49 @@ struct RunningSum {
   // log2 of the sum, relative to a maximum `ref` that is no smaller; -inf where there is no word
   __device__ __forceinline__ float log2sum(float ref, float scale2) const {
     return s == 0.0f ? neg_inf() : (m - ref) * scale2 + log2f(s);
+  }
+};
+
+// The same with two operations less per word: sum of 2^(z scale2 - r) for a whole number r, one fused operation for
+// the exponent, whatever the words' maximum: r follows when the sum gets large.  Scores whose multiples by scale2 lie
+// beyond +-2^20 are left to RunningSum, as are sums that are not finite.
+struct QuickSum {
+  static constexpr float kRange = 0x1p20f;
+  float r = -kRange, s = 0.0f;
+  template <int N>
+  __device__ __forceinline__ float weights(const float (&z)[N], float scale2) const {
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i % 2] += ex2(fmaf(z[i], scale2, -r));
+    return sum[0] + sum[1];
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&z)[N], float scale2) {
+    float sum = weights(z, scale2);
+    if (!(sum < 0x1p60f)) {
+      float top = z[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+      const float to = fminf(rintf(top * scale2), kRange);
+      s *= ex2(r - to);
+      r = to;
+      sum = weights(z, scale2);
+    }
+    s += sum;
+  }
+  // s in [1, 2) relative to a score; NaN where RunningSum has to do it
+  __device__ __forceinline__ RunningSum sum(float scale2) const {
+    RunningSum x;
+    if (s == 0.0f) return x;
+    if (!(s >= 0.5f && s < pos_inf())) {   // (below 0.5: no word has come near r)
+      x.s = __int_as_float(0x7fffffff);
+      return x;
+    }
+    const int exponent = (int)(__float_as_uint(s) >> 23) - 127;
+    const float whole = r + (float)exponent;
+    x.m = __fdividef(whole, scale2);
+    x.s = __uint_as_float(__float_as_uint(s) - ((unsigned)exponent << 23)) * ex2(-fmaf(x.m, scale2, -whole));
+    return x;
   }
 };
 
@@ -92,21 +135,27 @@ constexpr int kWarpNodes = 8;   // nodes per CTA where a warp has a node
 template <int G>
 constexpr int kCta = G == 32 ? 32 * kWarpNodes : G;
 
-// One group of G threads per node.  Dynamic shared memory, per node: its record, K Listed; with REST a bit per word
-// of the vocabulary, set for listed ones.
+// The row of E comes through a ring in shared memory, a turn of kTurn vectors of each lane at a time, and the listed words
+// are masked there by whoever has their places.
+template <int VEC>
+constexpr int kTurn = VEC == 1 ? 8 : 2;
+constexpr int kTurns = 4;   // in the ring
+template <typename TIn, int VEC>
+constexpr int kRingWords = kTurns * kTurn<VEC> * 32 * VEC;   // of a warp
+
+// One group of G threads per node.  Dynamic shared memory: the warps' rings, and per node its record, K Listed.
 template <typename TIn, int VEC, int G, bool REST>
-__global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCta<G>) distill_forward_kernel(
+__global__ void __launch_bounds__(kCta<G>, (VEC == 1 && sizeof(TIn) == 4 ? 768 : 1024) / kCta<G>) distill_forward_kernel(
     NodeArgs a, const int* __restrict__ words, const float* __restrict__ logits,
     const float* __restrict__ rest, float* __restrict__ costs, DistillSaved saved, int K, float scale2) {
-  constexpr int kNodes = kCta<G> / G, kTurn = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;   // vectors of a row at a time
+  constexpr int kNodes = kCta<G> / G;
   extern __shared__ __align__(16) unsigned char memory[];
   __shared__ double2 scratch[64];
   const int sub = threadIdx.x / G, tid = threadIdx.x % G;
   const i64 node = (i64)blockIdx.x * kNodes + sub;
   if (node >= (i64)a.B * a.N) return;
-  const int bitWords = (a.V + 31) / 32;
-  Listed* const record = reinterpret_cast<Listed*>(memory) + sub * K;
-  unsigned* const bits = reinterpret_cast<unsigned*>(memory + kNodes * K * sizeof(Listed)) + sub * bitWords;
+  TIn* const ring = reinterpret_cast<TIn*>(memory) + threadIdx.x / 32 * kRingWords<TIn, VEC>;
+  Listed* const record = reinterpret_cast<Listed*>(memory + kCta<G> / 32 * kRingWords<TIn, VEC> * sizeof(TIn)) + sub * K;
   float2* const savedListed = saved.listed ? saved.listed + node * K : nullptr;
   const NodeScores<TIn> s = node_scores<TIn>(a, node);
   if (!s.here) {
@@ -123,6 +172,78 @@ __global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCt
   int around = -1;
   if (savedListed && tid < 4 && (tid < 2 ? n > 0 : n + 1 < a.N)) around = (tid & 1 ? a.positions : a.frames)[beside];
   Group<G> g(tid, scratch);
+  // vectors c = 0, 1, ... of this thread, the words (c * G + tid) * VEC and on, are in turn c / kTurn; where c is in the ring
+  const int turns = div_up(a.V, G * VEC * kTurn<VEC>);
+  auto place = [&](int c) { return c % (kTurns * kTurn<VEC>) * 32 * VEC; };
+  auto fetch = [&](int turn) {
+    if (turn < turns) {
+#pragma unroll
+      for (int j = 0; j < kTurn<VEC>; ++j) {
+        const int c = turn * kTurn<VEC> + j, v = (c * G + tid) * VEC;
+        TIn* const slot = ring + place(c) + g.lane * VEC;
+        if (v >= a.V) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) from_f32(slot[i], neg_inf());
+        } else if constexpr (VEC * sizeof(TIn) >= 4) {
+          copy_async<VEC * sizeof(TIn)>(slot, s.e + v);
+        } else {
+          *slot = s.e[v];   // (too small for an asynchronous copy)
+        }
+      }
+    }
+    commit_copies();
+  };
+  // the student's sum over the words that are not listed (all words, without REST)
+  auto begin = [&] {
+#pragma unroll 1
+    for (int i = 0; i < kTurns - 1; ++i) fetch(i);
+  };
+  auto add_row = [&](auto& sum) {
+    // the listed words of this lane: the turn, and the place in the ring (-1: another warp's)
+    auto find = [&](int k, int& turn, int& at) {
+      const int v = k < K ? record[k].word : -1;
+      const int q = v / VEC, c = q / G, owner = q % G;
+      turn = v >= 0 && owner / 32 == g.warp ? c / kTurn<VEC> : -1;
+      at = place(c) + owner % 32 * VEC + v % VEC;
+    };
+    [[maybe_unused]] int hit = -1, at = 0;
+    if constexpr (REST) find(g.lane, hit, at);
+#pragma unroll 1
+    for (int turn = 0; turn < turns; ++turn) {
+      RawWords<TIn, VEC> p[kTurn<VEC>];
+#pragma unroll
+      for (int j = 0; j < kTurn<VEC>; ++j) {
+        const int v = ((turn * kTurn<VEC> + j) * G + tid) * VEC;
+        p[j].load(s.p + (v < a.V ? v : 0));
+      }
+      fetch(turn + kTurns - 1);
+      wait_copies<kTurns - 1>();
+      if constexpr (REST) {
+        __syncwarp();
+        if (turn == hit) from_f32(ring[at], neg_inf());
+        if (K > 32) {
+#pragma unroll 1
+          for (int k = g.lane + 32; k < K; k += 32) {
+            int turnOf, there;
+            find(k, turnOf, there);
+            if (turn == turnOf) from_f32(ring[there], neg_inf());
+          }
+        }
+        __syncwarp();
+      }
+      float z[VEC * kTurn<VEC>];
+#pragma unroll
+      for (int j = 0; j < kTurn<VEC>; ++j) {
+        RawWords<TIn, VEC> e;
+        e.load(ring + place(turn * kTurn<VEC> + j) + g.lane * VEC);
+        const Words<VEC> x = e.words(), y = p[j].words();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[j * VEC + i] = x.x[i] + y.x[i];
+      }
+      sum.add(z, scale2);
+    }
+  };
+  begin();
   // the teacher's shares
   const float lRest = REST ? rest[node] : neg_inf();
   float top = lRest;
@@ -133,8 +254,6 @@ __global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCt
     record[k] = x;
     top = fmaxf(top, x.share);
   }
-  if constexpr (REST)
-    for (int i = tid; i < bitWords; i += G) bits[i] = 0;
   top = g.max(top);
   float sum = 0.0f;
   for (int k = tid; k < K; k += G) {
@@ -148,7 +267,7 @@ __global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCt
   const bool empty = top == neg_inf();   // the record has no weight: cost and gradient are 0
   const float one = empty ? 0.0f : 1.0f / sum;
   r *= one;
-  // A word that is listed more than once: its first place has all its shares.  Then its bit.
+  // A word that is listed more than once: its first place has all its shares.
   bool twice = false;
   if (G == 32 && K <= 32) {
     const int v = tid < K ? record[tid].word : -1 - tid;
@@ -177,8 +296,6 @@ __global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCt
         }
       all[i] = first ? x * one : kNoShare;
     }
-    if constexpr (REST)
-      if (all[i] != kNoShare) atomicOr(&bits[v >> 5], 1u << (v & 31));
   }
   if (repeated) g.sync();   // (everybody has read the record)
 #pragma unroll
@@ -187,34 +304,16 @@ __global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCt
     if (k < K) record[k].share = all[i];
   }
   g.sync();
-  // the student's sums: of the words that are not listed (all words, without REST), and of all
-  RunningSum others;
-  for (int v0 = tid * VEC; v0 < a.V; v0 += G * VEC * kTurn) {
-    RawWords<TIn, VEC> e[kTurn], p[kTurn];
-#pragma unroll
-    for (int j = 0; j < kTurn; ++j) {
-      const int v = v0 + j * G * VEC;
-      if (v < a.V) e[j].load(s.e + v), p[j].load(s.p + v);
-    }
-    float z[VEC * kTurn];
-#pragma unroll
-    for (int j = 0; j < kTurn; ++j) {
-      const int v = v0 + j * G * VEC;
-      const Words<VEC> x = e[j].words(), y = p[j].words();
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) z[j * VEC + i] = v < a.V ? x.x[i] + y.x[i] : neg_inf();
-      if constexpr (REST) {
-        const unsigned listed = v < a.V ? bits[v >> 5] >> (v & 31) & ((1u << VEC) - 1) : 0u;
-        if (listed) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            if (listed >> i & 1) z[j * VEC + i] = neg_inf();
-        }
-      }
-    }
-    others.add(z, scale2);
-  }
+  QuickSum quick;
+  add_row(quick);
+  RunningSum others = quick.sum(scale2);
   others.join(g, scale2);
+  if (!(others.s > 0.0f && others.s < pos_inf())) {   // (the same for the whole group)
+    others = RunningSum();
+    begin();
+    add_row(others);
+    others.join(g, scale2);
+  }
   RunningSum full = others;
   if constexpr (REST) {
     RunningSum mine;
@@ -251,12 +350,16 @@ __global__ void __launch_bounds__(kCta<G>, (sizeof(TIn) == 2 ? 1024 : 768) / kCt
   if (!savedListed) return;
   // (an empty record has no gradient, and a student without any word left has p = 0)
   const float L = empty || all2 == neg_inf() ? pos_inf() : all2;
-  float A = L, sign = 1.0f;
-  if (logRatio != neg_inf()) {
-    sign = apart ? -2.0f : logRatio > 0.0f ? -1.0f : 1.0f;
+  float m = full.m, A = L, sign = 1.0f;
+  if (apart && !empty) {   // (r - rho times the others' own softmax, however far they are below the listed words)
+    sign = -2.0f;
+    m = others.m;
+    A = log2f(others.s) - log2f(r - ex2(other2 - all2));
+  } else if (logRatio != neg_inf()) {
+    sign = logRatio > 0.0f ? -1.0f : 1.0f;
     A = L - (fmaxf(logRatio, 0.0f) + log1pf(-expf(-fabsf(logRatio)))) * kLog2e;
   }
-  saved.node[node] = make_float4(full.m, A, sign, 0.0f);
+  saved.node[node] = make_float4(m, A, sign, 0.0f);
   mark_spans(a, saved, node, n, s.t, s.u, tBefore, uBefore, tAfter, uAfter);
 }
 
@@ -325,15 +428,15 @@ void launch_distill_forward(const NodeArgs& a, const int* words, const float* lo
       auto launch = [&](auto group) {
         constexpr int G = group, rows = kCta<G> / G;
         auto kernel = distill_forward_kernel<TIn, vec, G, has_rest>;
-        const int smem = rows * (K * (int)sizeof(Listed) + (has_rest ? div_up(a.V, 32) * 4 : 0));
+        const int smem = kCta<G> / 32 * kRingWords<TIn, vec> * (int)sizeof(TIn) + rows * K * (int)sizeof(Listed);
         if (smem > 40 * 1024) allow_dyn_smem(kernel, kForwardBytes);
         ScopedKernel prof("distill_forward", stream);
         kernel<<<(unsigned)div_up64(nodes, rows), kCta<G>, smem, stream>>>(a, words, logits, rest, costs, saved,
                                                                          K, scale2);
         TB200_CHECK_LAUNCH();
       };
-      // a warp per node where there are warps enough to fill the chip and their shared memory is small
-      if (a.V <= 1024 || (nodes >= 148 * 16 && a.V <= 65536)) launch(std::integral_constant<int, 32>{});
+      // a warp per node where there are warps enough to fill the chip
+      if (a.V <= 1024 || nodes >= 148 * 16) launch(std::integral_constant<int, 32>{});
       else launch(std::integral_constant<int, 256>{});
     });
   });

@@ -37,21 +37,6 @@ struct GradArgs {
   int tiles, eSplits, pSplits;
 };
 
-// (16 bytes: past the L1, most of which is shared memory here)
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from) {
-  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void wait_copies() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
-}
-
 // A warp's tile: 32 * COLS words, vector j of a lane being the words (j * 32 + lane) * VEC and on.
 template <typename TIn, int VEC, int COLS>
 struct Tile {
@@ -137,6 +122,58 @@ struct Terms {
   }
 };
 
+// The same for whole vectors with fewer operations: `weight` 2^(z scale2 - r), r next to m scale2 + A and the weight what
+// is left of it, or, where gradients are rounded to 8 bits anyway, the weight in r too and its sign in `weight`: r is
+// rounded by 2^-25 |r| then, by 2^-15 at most, and a gradient by as much of itself.  Not where r is larger.
+template <int VEC>
+struct QuickTerms {
+  static constexpr bool kFolded = VEC == 8;
+  float r, weight;
+  bool fits;
+  __device__ __forceinline__ static QuickTerms of(const Terms& x, float scale2) {
+    QuickTerms q;   // (apart: the listed words' gradients must not come by with the others')
+    if constexpr (kFolded) {
+      q.r = fmaf(x.m, scale2, x.A) - log2f(fabsf(x.ws));
+      q.weight = copysignf(1.0f, x.ws);
+      q.fits = !(fabsf(q.r) > 0x1p10f && fabsf(q.r) < pos_inf());
+    } else {
+      q.r = rintf(fmaf(x.m, scale2, x.A));
+      q.weight = x.ws * ex2(-(fmaf(x.m, scale2, -q.r) + x.A));
+      q.fits = fabsf(q.r) < 0x1p24f;
+    }
+    q.fits = q.fits && !x.apart;
+    return q;
+  }
+  // acc += gradients, and these in storage form to `row`
+  template <typename T>
+  __device__ __forceinline__ void vector(const Words<VEC>& e, const Words<VEC>& p, float scale2, float* acc, T* row) const {
+    float g[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float x = ex2(fmaf(e.x[i] + p.x[i], scale2, -r));
+      if constexpr (kFolded) {
+        g[i] = x;
+        acc[i] = fmaf(weight, x, acc[i]);
+      } else {
+        g[i] = weight * x;
+        acc[i] += g[i];
+      }
+    }
+    if (!row) return;
+    if constexpr (kFolded) {
+      unsigned u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(g[2 * i + 1]), "f"(g[2 * i]));
+        u[i] ^= weight < 0.0f ? 0x80008000u : 0u;
+      }
+      *reinterpret_cast<uint4*>(row) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+      store_words<VEC>(row, g);
+    }
+  }
+};
+
 // A node's number, and 32 words of its record, one in each lane.
 struct Record {
   i64 at;   // of the record's first word among all
@@ -179,11 +216,12 @@ __device__ __forceinline__ void add_record(const GradArgs& k, Record r, float w,
 }
 
 // A node as its CTA comes to it: all that can be known beforehand, made for 32 nodes at a time by a lane each.
-struct __align__(16) Step {
+template <int VEC>
+struct Step {
   Terms terms;
-  int flags, u;
-  i64 row, out, record;   // from the utterance's first: the frame's row of E and of dE; the node's record
-  i64 target;             // of a new position: its row of dP, or -1 less its place among the partial rows
+  QuickTerms<VEC> quick;
+  int flags, n, t, u;
+  i64 target;   // of a new position: its row of dP, or -1 less its place among the partial rows
 };
 constexpr int kNewFrame = 1, kMoreOfFrame = 2, kNewPosition = 4;   // another than the node's before; not the last node
 constexpr int kSteps = 64;    // in shared memory
@@ -192,13 +230,17 @@ template <typename TIn>
 constexpr int kAhead = sizeof(TIn) == 2 ? 3 : 2;   // rows of E that are on their way
 template <typename TIn>
 struct __align__(16) PathWarp {
+  static constexpr int kRecords = kAhead<TIn> + 1;
   TIn rows[kAhead<TIn> + 1][32 * kCols];
   TIn nextP[32 * kCols];   // the row of P of the next new position
   float subE[32 * kCols], subP[32 * kCols];
   unsigned marks[32];
+  int words[kRecords][32];   // of the records on their way, up to 32 words
+  float2 listed[kRecords][32];
 };
+template <int VEC>
 struct __align__(16) PathCta {
-  Step steps[kSteps];
+  Step<VEC> steps[kSteps];
   int appended, base, lastT, lastU;
 };
 
@@ -213,8 +255,8 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
   constexpr int COLS = kCols, NV = COLS / VEC, kA = kAhead<TIn>;
   extern __shared__ __align__(16) unsigned char memory[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  PathCta& cta = *reinterpret_cast<PathCta*>(memory);
-  PathWarp<TIn>& mem = reinterpret_cast<PathWarp<TIn>*>(memory + sizeof(PathCta))[warp];
+  PathCta<VEC>& cta = *reinterpret_cast<PathCta<VEC>*>(memory);
+  PathWarp<TIn>& mem = reinterpret_cast<PathWarp<TIn>*>(memory + sizeof(PathCta<VEC>))[warp];
   const int groups = (k.tiles + warps - 1) / warps;   // of tiles
   const i64 bs = blockIdx.x / groups;
   const int b = (int)(bs / k.saved.segs), seg = (int)(bs - (i64)b * k.saved.segs);
@@ -240,6 +282,7 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
   if (n1 == 0) return;   // (the same for all warps)
   for (int i = lane; i < 32 * COLS; i += 32) mem.subE[i] = mem.subP[i] = 0.0f;
   mem.marks[lane] = 0;
+  for (int i = 0; i <= kA; ++i) mem.words[i][lane] = -1;
   if (threadIdx.x == 0) cta.appended = 0, cta.base = n0, cta.lastT = cta.lastU = -1;
   auto append = [&] {   // the next 32 places with a node, by one warp
     int base = cta.base;
@@ -247,26 +290,23 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
     __syncwarp();
     unsigned all = 0;
     for (; !all && base < n1; base += 32) {
-      Step x;
-      int t = -1;
-      x.u = -1;
-      const int n = base + lane;
-      if (n < n1) {
-        const i64 node = (i64)b * a.N + n;
-        t = a.frames[node], x.u = a.positions[node];
+      Step<VEC> x;
+      x.t = x.u = -1;
+      x.n = base + lane;
+      if (x.n < n1) {
+        const i64 node = (i64)b * a.N + x.n;
+        x.t = a.frames[node], x.u = a.positions[node];
         x.terms = Terms::of(k.saved.node[node], k.weights[node] * k.scale);
-        x.row = t * a.eStrideT;
-        x.out = (i64)t * a.V;
-        x.record = node * k.K;
+        x.quick = QuickTerms<VEC>::of(x.terms, k.scale2);
       }
-      const bool here = (unsigned)t < (unsigned)a.T && (unsigned)x.u < (unsigned)a.U;
+      const bool here = (unsigned)x.t < (unsigned)a.T && (unsigned)x.u < (unsigned)a.U;
       all = __ballot_sync(0xffffffffu, here);
       const unsigned before = all & ((1u << lane) - 1), after = all & ~before & ~(1u << lane);
-      const int tBefore = __shfl_sync(0xffffffffu, t, before ? 31 - __clz(before) : 0);
+      const int tBefore = __shfl_sync(0xffffffffu, x.t, before ? 31 - __clz(before) : 0);
       const int uBefore = __shfl_sync(0xffffffffu, x.u, before ? 31 - __clz(before) : 0);
-      const int tAfter = __shfl_sync(0xffffffffu, t, after ? __ffs(after) - 1 : 0);
-      x.flags = (t != (before ? tBefore : lastT) ? kNewFrame : 0) |
-                (x.u != (before ? uBefore : lastU) ? kNewPosition : 0) | (after && t == tAfter ? kMoreOfFrame : 0);
+      const int tAfter = __shfl_sync(0xffffffffu, x.t, after ? __ffs(after) - 1 : 0);
+      x.flags = (x.t != (before ? tBefore : lastT) ? kNewFrame : 0) |
+                (x.u != (before ? uBefore : lastU) ? kNewPosition : 0) | (after && x.t == tAfter ? kMoreOfFrame : 0);
       if (here && (x.flags & kNewPosition) && k.pgrads) {
         const int2 s = k.saved.spans[(i64)a.B * a.T + (i64)b * a.U + x.u];
         const int* frames = a.frames + (i64)b * a.N;
@@ -275,8 +315,8 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
       }
       if (here) {
         cta.steps[(appended + __popc(before)) % kSteps] = x;
-        if (!before && appended > 0 && t == lastT) cta.steps[(appended - 1) % kSteps].flags |= kMoreOfFrame;
-        if (!after) cta.lastT = t, cta.lastU = x.u;
+        if (!before && appended > 0 && x.t == lastT) cta.steps[(appended - 1) % kSteps].flags |= kMoreOfFrame;
+        if (!after) cta.lastT = x.t, cta.lastU = x.u;
       }
     }
     if (lane == 0) cta.appended = appended + __popc(all), cta.base = base;
@@ -308,14 +348,21 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
 #pragma unroll
     for (int i = 0; i < COLS; ++i) accP[i] = 0.0f;
   };
-  int ringTo = 0;
+  int ringTo = 0, recordTo = 0;
+  const i64 firstNode = (i64)b * a.N;
   const TIn* P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
   int stepP = -1;   // whose row of P is in nextP, or on its way there
-  auto fetch_row = [&](int i) {   // of step i, if it is another than the one before; a group of copies per step
+  auto fetch_row = [&](int i) {   // of step i, if it is another than the one before, and the record; a group of copies per step
     if (i < appended) {
-      const Step& x = cta.steps[i % kSteps];
+      const Step<VEC>& x = cta.steps[i % kSteps];
+      if (lane < k.K) {
+        const i64 at = (firstNode + x.n) * k.K + lane;
+        copy_async<4>(&mem.words[recordTo][lane], k.words + at);
+        copy_async<8>(&mem.listed[recordTo][lane], k.saved.listed + at);
+      }
+      recordTo = recordTo == kA ? 0 : recordTo + 1;
       if (x.flags & kNewFrame) {
-        tile.fetch(E + x.row, mem.rows[ringTo]);
+        tile.fetch(E + x.t * a.eStrideT, mem.rows[ringTo]);
         ringTo = ringTo == kA ? 0 : ringTo + 1;
       }
       if ((x.flags & kNewPosition) && stepP < 0) {
@@ -325,8 +372,7 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
     }
     commit_copies();
   };
-  Record next;
-  int slot = kA;
+  int slot = kA, recordAt = 0;
   for (int i = 0; i < appended; ++i) {
     while (more && appended < i + kA + 2) {
       __syncthreads();   // (everybody is here: the steps before are free)
@@ -335,21 +381,18 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
       appended = cta.appended;
       more = cta.base < n1;
     }
-    if (i == 0) {
+    if (i == 0)
       for (int j = 0; j < kA; ++j) fetch_row(j);
-      next.load(k, cta.steps[0].record, 0, lane);
-    }
     fetch_row(i + kA);
-    const Record record = next;
-    if (i + 1 < appended) next.load(k, cta.steps[(i + 1) % kSteps].record, 0, lane);
-    const Step& step = cta.steps[i % kSteps];
-    const Terms terms = step.terms;
+    wait_copies<kA>();
+    const Step<VEC>& step = cta.steps[i % kSteps];
     const int flags = step.flags;
+    const Record record{(firstNode + step.n) * k.K, mem.words[recordAt][lane], mem.listed[recordAt][lane]};
+    recordAt = recordAt == kA ? 0 : recordAt + 1;
     if (flags & kNewPosition) {
       if (i > 0) finish_position();
       target = step.target;
       if (stepP == i) {
-        wait_copies<kA>();
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           p[j].clear();
@@ -362,20 +405,18 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
     }
     if (flags & kNewFrame) slot = slot == kA ? 0 : slot + 1;
     const TIn* row = mem.rows[slot];
-    TIn* out = dE + step.out;
+    TIn* out = dE + (i64)step.t * a.V;
     const bool whole = (flags & (kNewFrame | kMoreOfFrame)) == kNewFrame;   // the frame's only node
-    if (whole && !terms.apart) {
-      wait_copies<kA>();
+    if (whole && step.quick.fits) {
+      const QuickTerms<VEC> quick = step.quick;
+      const float weight = step.terms.w;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         RawWords<TIn, VEC> e;
         e.clear();
         if (tile.in(j)) e.load(row + tile.place(j));
-        float g[VEC];
-        terms.vector(e.words(), p[j].words(), 0u, k.scale2, g);
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) accP[j * VEC + c] += g[c];
-        if (dE) tile.store(out, j, g);
+        quick.vector(e.words(), p[j].words(), k.scale2, accP + j * VEC,
+                     dE && tile.in(j) ? out + tile.first + tile.place(j) : nullptr);
       }
       __syncwarp();
       // the listed words' gradients take the place of what has been stored for them
@@ -383,8 +424,8 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
       for (int k0 = 0;;) {
         int at;
         if (r.template hits<32 * COLS>(tile.first, at)) {
-          if (dE) from_f32(out[tile.first + at], terms.w * r.listed.y);
-          mem.subP[at] -= terms.w * r.listed.x;
+          if (dE) from_f32(out[tile.first + at], weight * r.listed.y);
+          mem.subP[at] -= weight * r.listed.x;
         }
         k0 += 32;
         if (k0 >= k.K) break;
@@ -393,11 +434,11 @@ __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
       __syncwarp();
       continue;
     }
+    const Terms terms = step.terms;
     add_record<VEC, COLS>(k, record, terms.w, tile.first, mem.subE, mem.subP, mem.marks, lane);
     __syncwarp();
     const unsigned listed = mem.marks[lane];
     if (listed) mem.marks[lane] = 0;
-    wait_copies<kA>();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!tile.in(j)) break;
@@ -719,8 +760,8 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
       int warps = kPathWarps;   // with the fewest that have no tile
       for (int w = kPathWarps - 1; w > 0; --w)
         if (div_up(p.tiles, w) * w < div_up(p.tiles, warps) * warps) warps = w;
-      const int smem = (int)sizeof(PathCta) + warps * (int)sizeof(PathWarp<TIn>);
-      allow_dyn_smem(distill_path_kernel<TIn, VEC>, (int)sizeof(PathCta) + kPathWarps * (int)sizeof(PathWarp<TIn>));
+      const int smem = (int)sizeof(PathCta<VEC>) + warps * (int)sizeof(PathWarp<TIn>);
+      allow_dyn_smem(distill_path_kernel<TIn, VEC>, (int)sizeof(PathCta<VEC>) + kPathWarps * (int)sizeof(PathWarp<TIn>));
       distill_path_kernel<TIn, VEC><<<(unsigned)((i64)a.B * p.segs * div_up(p.tiles, warps)), warps * 32, smem, stream>>>(
           a, k);
       TB200_CHECK_LAUNCH();

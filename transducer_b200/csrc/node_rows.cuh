@@ -71,6 +71,22 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Asynchronous copies to shared memory.
+// (16 bytes: past the L1)
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
 // The scores of one node.
 template <typename TIn>
 struct NodeScores {
