@@ -169,8 +169,8 @@ __device__ __forceinline__ void bring_row(const Place<TIn, VEC>& at, float* w, i
 
 // ---- launches ---------------------------------------------------------------------------------
 
-// launch(group, resident): group sizes for rows of V words.  A warp has up to 1024, a CTA of 128 or 256 threads 32 to 64
-// words a thread; rows beyond shared memory are read again for every pass.
+// launch(group, resident): group sizes for rows of V words.  A warp has up to 1024, a CTA of 128 or 256 threads 32 to
+// 64 words a thread; rows beyond shared memory are read again for every pass.
 template <typename F>
 void with_group(int V, bool warps, F launch) {
   using std::integral_constant;
