@@ -78,6 +78,8 @@ def distill(z, here, words, logits, rest=None, temperature=1.0):
     if rest is not None:
         l = torch.cat((l, rest.cpu().double()[..., None]), -1)
     full = (l > -torch.inf).any(-1) & here
+    # (the teacher's too relative to its greatest: shares that add up to 1, at -3e38 as elsewhere)
+    l = l - torch.where(l.amax(-1, keepdim=True) > -torch.inf, l.amax(-1, keepdim=True), 0.0)
     q_bins = torch.where(full[..., None], (l - lse(l)[..., None]).exp(), 0.0)
     at = words.clamp(0, V - 1).long()
     q = torch.zeros_like(x).scatter_add_(-1, at, torch.where(there, q_bins[..., :K], 0.0))

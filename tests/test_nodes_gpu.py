@@ -218,6 +218,22 @@ def test_distillation_of_wide_scores(scale, offset, V, kind, with_rest):
     check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.5, g, 5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 1e-30, 1e20])
+@pytest.mark.parametrize("V", [264, 1025])
+@pytest.mark.parametrize("with_rest", [False, True])
+def test_distillation_at_the_ends_of_the_range(dtype, temperature, V, with_rest):
+    """Rows of the type's lowest number along a path, temperatures that leave one word or make all alike."""
+    E, P, frames, positions, g = make(2, 9, 3, V, 14, dtype, seed=V, kind="path", holes=False)
+    lowest = torch.finfo(dtype).min
+    E[0, 1] = lowest
+    E[0, 2, 5:] = lowest
+    E[1, 3, :V // 2] = lowest
+    words, logits, _ = top_words(E, P, frames, positions, 4)
+    rest = torch.randn(2, 14, generator=g).cuda()
+    check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, temperature, g, 4)
+
+
 def test_distillation_with_a_very_large_alphabet():
     E, P, frames, positions, g = make(1, 2, 1, (1 << 20) + 5, 3, holes=False)
     words, logits, rest = teacher(E, P, frames, positions, 7, g)

@@ -135,7 +135,8 @@ struct QuickTerms {
     if constexpr (kFolded) {
       q.r = fmaf(x.m, scale2, x.A) - log2f(fabsf(x.ws));
       q.weight = copysignf(1.0f, x.ws);
-      q.fits = !(fabsf(q.r) > 0x1p10f && fabsf(q.r) < pos_inf());
+      // (r = +inf: A says that there is no gradient, or the weight is 0)
+      q.fits = fabsf(x.m * scale2) < 0x1p10f && (fabsf(q.r) < 0x1p10f || q.r == pos_inf());
     } else {
       q.r = rintf(fmaf(x.m, scale2, x.A));
       q.weight = x.ws * ex2(-(fmaf(x.m, scale2, -q.r) + x.A));

@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         // by one warp: lane i has entries 2 i and 2 i + 1.  In 32 bits, or, where the sum up to a word is too close
         // to the target to tell, in 64 bits from memory.
         const int i0 = 2 * g.lane, i1 = i0 + 1;
-        auto judge = [&](double above, double share, double w0, double w1, double margin) {
+        auto settle = [&](double above, double share, double w0, double w1, double margin) {
           double upto = w0 + w1;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -506,13 +506,13 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
           if (g.lane == 0) *filled = 4 * (__popc(b0) + __popc(b1)) + (end >= 0.0 ? 2 : 0) + (any ? 1 : 0);
         };
         auto score = [&](int i) { return i < c ? key_score(entry_key(sorted[i])) : neg_inf(); };
-        if (g.warp == 0) judge((double)vHi, target, (double)weight(score(i0)), (double)weight(score(i1)), unsure);
+        if (g.warp == 0) settle((double)vHi, target, (double)weight(score(i0)), (double)weight(score(i1)), unsure);
         g.sync();
         if (*filled & 1) {
           const ExactSums sums = exact_sums<TIn, VEC, G>(s, a.V, g, keep, weight, hi);
           target = rule.topP * sums.all;
           g.sync();
-          if (g.warp == 0) judge(sums.above, target, keep.exact(score(i0)), keep.exact(score(i1)), -1.0);
+          if (g.warp == 0) settle(sums.above, target, keep.exact(score(i0)), keep.exact(score(i1)), -1.0);
           g.sync();
         }
         kept = *filled >> 2;
