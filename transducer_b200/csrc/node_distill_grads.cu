@@ -54,12 +54,17 @@ struct Tile {
   }
   // to shared memory: each lane its own words
   __device__ __forceinline__ void fetch(const TIn* row, TIn* slot) const {
+    if constexpr (VEC * sizeof(TIn) >= 4) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (in(j)) {
-        if constexpr (VEC * sizeof(TIn) >= 4) copy_async<VEC * sizeof(TIn)>(slot + place(j), row + first + place(j));
-        else slot[place(j)] = row[first + place(j)];   // (too small for an asynchronous copy)
-      }
+      for (int j = 0; j < NV; ++j)
+        if (in(j)) copy_async<VEC * sizeof(TIn)>(slot + place(j), row + first + place(j));
+    } else {   // (too small for an asynchronous copy: all on their way before the first is stored)
+      Row x;
+      load(row, x);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (in(j)) slot[place(j)] = x[j].bits;
+    }
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, int j, const float* x) const {   // vector j
