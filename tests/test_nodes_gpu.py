@@ -240,6 +240,14 @@ def test_distillation_with_a_very_large_alphabet():
     check_distill(E, P, frames, positions, words, logits, rest, 1.0, g, 7)
 
 
+@pytest.mark.parametrize("off", [(0,), (31, 32), (69,), (5, 40, 64, 65), tuple(range(70))])
+def test_distillation_of_many_utterances_some_off_path(off):
+    E, P, frames, positions, g = make(70, 6, 3, 40, 10, seed=len(off), kind="path")
+    frames[list(off)] = frames[list(off)].flip(1)
+    words, logits, rest = teacher(E, P, frames, positions, 4, g)
+    check_distill(E, P, frames, positions, words, logits, rest, 1.0, g, 4)
+
+
 @pytest.mark.parametrize("V", [30, 64, 1025])
 @pytest.mark.parametrize("gap", [10, 100])
 def test_distillation_paths_with_gaps(V, gap):

@@ -517,8 +517,19 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
   __syncwarp();
   const i64 ePer = (i64)a.T * k.eSplits * k.tiles, pPer = (i64)a.U * k.pSplits * k.tiles;   // tasks of an utterance
   const i64 step = (i64)gridDim.x * kWarps;
-  for (int b = 0; b < a.B; ++b) {
-    if (!k.saved.offPath[b]) continue;
+  int b = -1;
+  unsigned off = 0;   // of the 32 utterances that b is one of, those that are left
+  auto next_off_path = [&] {
+    for (int from = off ? b : (b + 32) / 32 * 32; !off; from += 32) {
+      if (from >= a.B) return false;
+      off = __ballot_sync(0xffffffffu, from + lane < a.B && k.saved.offPath[from + lane]);
+      b = from;
+    }
+    b = b / 32 * 32 + __ffs(off) - 1;
+    off &= off - 1;
+    return true;
+  };
+  while (next_off_path()) {
     for (i64 task = (i64)blockIdx.x * kWarps + warp; task < ePer + pPer; task += step) {
       const bool ofFrames = task < ePer;
       if ((ofFrames ? k.egrads : k.pgrads) == nullptr) continue;
