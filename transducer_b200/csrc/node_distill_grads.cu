@@ -251,13 +251,13 @@ struct __align__(16) PathCta {
   int appended, base, lastT, lastU;
 };
 
-// A warp's tile: rows of E and the nodes' records come through rings in shared memory, the row of P in use and the
-// sums for it are in registers, a frame's gradients are written when its last node comes by and wait in `subE` until
-// then.  The warps of a CTA go along the same nodes.  Bound by latencies: 16 warps an SM, whose issue slots are half
-// used, about 150 instructions for a node and tile besides 8 for each of a lane's 16 words.  More warps spill
-// registers, and next to this much shared memory the L1 does not hold them.  Records loaded one node ahead, into
-// registers, were waited for at every node: 774 us against 571 for 58800 nodes of 10000 bf16 words (4.3 TB/s of E and
-// its gradients; the copy rate would be 388); 8 utterances in fp32 224 us (5.2 TB/s).
+// A warp's tile: rows of E and the nodes' records come through rings in shared memory, the row of P in use and the sums
+// for it are in registers, a frame's gradients are written when its last node comes by and wait in `subE` until then.
+// The warps of a CTA go along the same nodes.  Bound by latencies and issue: 16 warps an SM, 63 % of the issue slots, 360
+// instructions for a node and tile, of which 8 for each of a lane's 16 words.  More warps spill registers, and next to
+// this much shared memory the L1 does not hold them.  Records loaded one node ahead, into registers, were waited for at
+// every node: 774 us against 571 for 58800 nodes of 10000 bf16 words (4.2 TB/s of E and its gradients; at the copy rate
+// 365); 8 utterances in fp32 224 us (5.2 TB/s).
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
     distill_path_kernel(NodeArgs a, GradArgs k) {
