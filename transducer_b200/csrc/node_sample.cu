@@ -18,10 +18,10 @@ namespace tb200 {
 namespace {
 
 // exp(x) for x <= 0 in 64 bits: 2^n times the Taylor series of exp(f) for |f| <= log(2) / 2, whose twelfth power
-// is below 2^-46 of it and whose 13th of 1e-15; 0 below exp(-700).  The library's own takes about twice the
-// instructions, and a row's 64-bit sums are nothing but these.
+// is below 2^-46 of it and whose 13th of 1e-15; down to the least of the 64-bit numbers, by way of 2^(n + 100).  The
+// library's own takes about twice the instructions, and a row's 64-bit sums are nothing but these.
 __device__ __forceinline__ double exp64(double x) {
-  if (!(x > -700.0)) return x != x ? x : 0.0;
+  if (!(x > -746.0)) return x != x ? x : 0.0;
   const double n = rint(x * 1.4426950408889634074);
   // log(2) as its 32-bit rounding, n times which is exact, and the rest
   const double f = fma(-n, -1.904654299957767878541823e-9, fma(-n, (double)0.69314718246459960937f, x));
@@ -30,14 +30,17 @@ __device__ __forceinline__ double exp64(double x) {
   double y = inverse[12];
 #pragma unroll
   for (int i = 11; i >= 0; --i) y = fma(y, f, inverse[i]);
-  return __hiloint2double(__double2hiint(y) + ((int)n << 20), __double2loint(y));
+  const bool low = x < -700.0;
+  y = __hiloint2double(__double2hiint(y) + (((int)n + (low ? 100 : 0)) << 20), __double2loint(y));
+  return low ? y * 0x1p-100 : y;
 }
 
 // exp((z - m) scale) in 64 bits.
 struct ExactWeight {
   float m;
   double scale;
-  __device__ __forceinline__ double operator()(float z) const { return exp64(((double)z - (double)m) * scale); }
+  __device__ __forceinline__ double exponent(float z) const { return ((double)z - (double)m) * scale; }
+  __device__ __forceinline__ double operator()(float z) const { return exp64(exponent(z)); }
 };
 
 __device__ __forceinline__ float lg2(float x) {
@@ -86,7 +89,9 @@ struct Weight {
 };
 
 // Which words stay: those of weight hi and above, and of those between lo and hi the ones before the cut;
-// in any case those of minP and above (`exact` decides where that is close).
+// in any case those of minP and above (`exact` decides where that is close).  In 32 bits weights below FLT_MIN are 0:
+// a row's words with such add up to less than 2^-98 of its weight, which is below what is unsure of any sum, so that
+// it is for the 64-bit draw to have them.
 struct Keep {
   float lo = FLT_MIN, hi = FLT_MIN;
   Cut cut{0u, 0x7fffffff};
@@ -96,6 +101,12 @@ struct Keep {
     if (w < lo || (w < hi && !cut.keeps(z, v))) return false;
     if (w >= sure()) return true;
     return w >= (float)minP * 0.9999f && exact(z) >= minP;
+  }
+  // The 64-bit weight of a word that stays, however small, or 0.  (lo = FLT_MIN: no word is out for its weight.)
+  __device__ __forceinline__ double exactly(float w, float z, int v) const {
+    if ((w < lo && lo > FLT_MIN) || (w < hi && !cut.keeps(z, v))) return 0.0;
+    const double x = exact(z);
+    return x >= minP ? x : 0.0;
   }
   __device__ __forceinline__ float sure() const { return (float)minP * 1.0001f; }   // of minP, whatever the rounding
 };
@@ -123,7 +134,7 @@ template <typename TIn, int VEC, int G>
 __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group<G> g, Keep keep,
                                         Weight weight, float u, int* word, float* logProb) {
   const Place<TIn, VEC> at(s, V, seg, g.warp, g.lane);
-  auto kept = [&](float z, int v) { return keep(weight(z), z, v) ? keep.exact(z) : 0.0; };
+  auto kept = [&](float z, int v) { return keep.exactly(weight(z), z, v); };
   double part = 0.0;
 #pragma unroll 1
   for (int v = at.first + g.lane * VEC; v < at.end; v += 32 * VEC) {
@@ -148,7 +159,7 @@ __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group
   const unsigned some = __ballot_sync(0xffffffffu, part > 0.0 && g.lane < Group<G>::kWarps);
   const int pick = past ? __ffs(past) - 1 : 31 - __clz(some);
   if (g.warp != pick) return;
-  double before = __shfl_sync(0xffffffffu, upto - part, pick), weightOf = 0.0;
+  double before = __shfl_sync(0xffffffffu, upto - part, pick);
   int found = -1;   // the first word past the target, or (rounding) the last one that stays
 #pragma unroll 1
   for (int j = 0; at.first + j * 32 * VEC < at.end; ++j) {
@@ -171,21 +182,20 @@ __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group
     const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
     if (any) {
       int word = -1;
-      double weightHere = 0.0, c = before + (scan - sum);
+      double c = before + (scan - sum);
       bool over = false;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         c += w[i];
-        if (w[i] > 0.0 && !over) word = v + i, weightHere = w[i], over = c > target;
+        if (w[i] > 0.0 && !over) word = v + i, over = c > target;
       }
       const int owner = hit ? __ffs(hit) - 1 : 31 - __clz(any);
       found = __shfl_sync(0xffffffffu, word, owner);
-      weightOf = __shfl_sync(0xffffffffu, weightHere, owner);
     }
     if (hit) break;
     before += __shfl_sync(0xffffffffu, scan, 31);
   }
-  if (g.lane == 0) *word = found, *logProb = (float)log(weightOf / total);
+  if (g.lane == 0) *word = found, *logProb = (float)(keep.exact.exponent(at.score(found)) - log(total));
 }
 
 // One group of threads per node; the row's weights take the scores' place in shared memory.  Each threshold tried is a
@@ -528,6 +538,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
       }
       if (hi < kAbove && (kept == 0 || y * 1.000004f >= hi)) t = hi * 1.00003f, x = xHi;
       else if (lo > FLT_MIN && (!enough || y * 0.999996f < lo)) t = fmaxf(lo * 0.99997f, FLT_MIN), x = xLo;
+      else if (!kByWeight && y * 0.999996f < lo) break;   // (beside weights that are 0 here)
       else if (kept > 0 && enough) done = true;
       else break;
       if constexpr (RESIDENT)   // what lies between and does not stay
@@ -553,8 +564,10 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     return true;
   };
   bool cutAny = false;   // `keep` says something that has not been applied
+  bool open = false;     // the cut lies among weights that are 0 in 32 bits
   if (rule.topK > 0 && rule.topK < a.V) {
     cutAny = find_cut(std::false_type{}, rule.topK, 0x1p-8f);
+    open = !cutAny && rule.topP == 1.0;
     if (cutAny && rule.topP < 1.0) total = g.sum(apply());
   }
   if (rule.topP < 1.0) {
@@ -673,6 +686,11 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   }
   g.sync();
   if (*sure) return;
+  if (open) {
+    keep.cut = general_first_k<TIn, VEC, G>(s, a.V, g, rule.topK);
+    keep.hi = kAbove;
+    g.sync();
+  }
   exact_draw<TIn, VEC, G>(s, a.V, seg, g, keep, weight, u, words + node, logProbs + node);
 }
 
