@@ -36,3 +36,22 @@ def test_draws_with_the_smallest_numbers(V, dtype):
     for temperature in (0.3, 0.1, 0.04):
         for rule in SMALL_RULES:
             check_sample(E, P, frames, positions, uniforms, temperature=temperature, **rule)
+
+
+# ---- alphabets beyond the whole numbers of 32-bit floats ----------------------------------------
+
+def test_top_k_beyond_the_whole_numbers_of_32_bit_floats():
+    """2^24 words of weight 1 and, after them, others that fall: the k first are the k best."""
+    ones, falling = 2 ** 24, 40000
+    E = torch.zeros(1, 1, ones + falling)
+    E[0, 0, ones:] = -0.01 - 1e-5 * torch.arange(falling)
+    upto = ones + torch.cumsum(E[0, 0, ones:].double().exp(), 0)
+    P, zero = torch.zeros_like(E).cuda(), torch.zeros(1, 1, dtype=torch.int32).cuda()
+    E = E.cuda()
+    u = 1.0 - 2.0 ** -24
+    for more in (12344, 12345, 12346, 12347, 20001, 20003, 30007, 39999):
+        total = upto[more - 1].item()
+        want = int((upto[:more] <= u * total).sum())
+        assert (upto[:more] - u * total).abs().min() > 1e-3   # (64-bit sums are good to 1e-5 here)
+        word, _ = sample_words(E, P, zero, zero, torch.full((1, 1), u).cuda(), top_k=ones + more)
+        assert word.item() == ones + want, more

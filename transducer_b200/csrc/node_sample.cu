@@ -379,6 +379,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
   auto find_cut = [&](auto by_weight, int k, float guess) {
     constexpr bool kByWeight = decltype(by_weight)::value;
     double target = kByWeight ? rule.topP * total : (double)k;
+    // (counts decide as whole numbers: 32-bit floats have all of them up to 2^24 only)
+    int count = 0, countHi = 0;   // measured last, and at `hi`
     auto measure = [&](float t) -> float {
       if constexpr (!kByWeight) {
         int c = 0;
@@ -386,7 +388,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
 #pragma unroll
           for (int i = 0; i < kPass; ++i) c += y[i] >= t ? 1 : 0;
         });
-        return (float)g.sum(c);
+        count = g.sum(c);
+        return (float)count;
       } else if constexpr (RESIDENT) {
         float sum[8] = {};
         const float4* q = reinterpret_cast<const float4*>(w + own);
@@ -434,8 +437,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
 #pragma unroll 1
     for (int round = 0; round < 64 && !done; ++round) {
       const float v = measure(t), l = level(v);
-      if (v >= want) lo = t, vLo = v, xLo = x, lLo = l;
-      else hi = t, vHi = v, xHi = x, lHi = l;
+      if (kByWeight ? v >= want : count >= k) lo = t, vLo = v, xLo = x, lLo = l;
+      else hi = t, vHi = v, xHi = x, lHi = l, countHi = count;
       if (vLo == 0.0f) {   // nothing is known from below yet
         if (t == FLT_MIN) return false;   // there are no more words than that
         t = round == 0 && t > 1e-9f ? t * 1e-3f : FLT_MIN;
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         }
       }
       g.sync();
-      int kept = k - (int)vHi;
+      int kept = k - countHi;
       bool enough = true;
       if (kByWeight) {
         // by one warp: lane i has entries 2 i and 2 i + 1.  In 32 bits, or, where the sum up to a word is too close
