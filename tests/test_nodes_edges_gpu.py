@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from test_nodes_gpu import UNIT, check_sample, make
-from transducer_b200 import sample_words
+from test_nodes_gpu import UNIT, check_distill, check_sample, make, teacher
+from transducer_b200 import sample_words, top_words
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,23 @@ def test_top_k_beyond_the_whole_numbers_of_32_bit_floats():
         assert (upto[:more] - u * total).abs().min() > 1e-3   # (64-bit sums are good to 1e-5 here)
         word, _ = sample_words(E, P, zero, zero, torch.full((1, 1), u).cuda(), top_k=ones + more)
         assert word.item() == ones + want, more
+
+
+# ---- bf16 gradients along a path whose scores are far from 0 -------------------------------------
+
+@pytest.mark.parametrize("offset", [0.0, 120.0, 496.0, -496.0, 30000.0])
+@pytest.mark.parametrize("temperature", [0.75, 1.0, 8.0])
+@pytest.mark.parametrize("own_record", [True, False])
+def test_bf16_paths_with_scores_far_from_0(offset, temperature, own_record):
+    """Where the record is the student's own distribution the gradients are small differences, however far the scores
+    are from 0: one node for each frame and position, so that nothing averages."""
+    B, N, V, K = 4, 40, 16, 16 if own_record else 5
+    g = torch.Generator().manual_seed(int(abs(offset)) + own_record)
+    E = (offset + 2.0 * torch.randint(-2, 3, (B, N, V), generator=g)).bfloat16().cuda()
+    P = torch.randn(B, N, V, generator=g).bfloat16().cuda()
+    nodes = torch.arange(N).expand(B, N).contiguous().int().cuda()
+    if own_record:
+        words, logits, _ = top_words(E, P, nodes, nodes, K, temperature)
+    else:
+        words, logits, _ = teacher(E, P, nodes, nodes, K, g, temperature)
+    check_distill(E, P, nodes, nodes, words, logits, None, temperature, g, K)

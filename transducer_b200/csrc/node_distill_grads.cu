@@ -128,8 +128,10 @@ struct Terms {
 };
 
 // The same for whole vectors with fewer operations: `weight` 2^(z scale2 - r), r next to m scale2 + A and the weight
-// what is left of it, or, where gradients are rounded to 8 bits anyway, the weight in r too and its sign in `weight`:
-// r is rounded by 2^-25 |r| then, by 2^-15 at most, and a gradient by as much of itself.  Not where r is larger.
+// what is left of it, or, where gradients are rounded to 8 bits anyway, the weight in r too, and in `weight` its sign
+// and what the rounding of r has left, 2^-15 at most (not where r is larger).  The sums take that with them: beside
+// listed words they are differences, p - q, whose terms have to be good to 32 bits.  A gradient that is stored for
+// itself goes without, its own rounding being 2^-9 to 2^-8 (where it belongs to a listed word it is replaced).
 template <int VEC>
 struct QuickTerms {
   static constexpr bool kFolded = VEC == 8;
@@ -138,8 +140,9 @@ struct QuickTerms {
   __device__ __forceinline__ static QuickTerms of(const Terms& x, float scale2) {
     QuickTerms q;   // (apart: the listed words' gradients must not come by with the others')
     if constexpr (kFolded) {
-      q.r = fmaf(x.m, scale2, x.A) - log2f(fabsf(x.ws));
-      q.weight = copysignf(1.0f, x.ws);
+      const double r = fma((double)x.m, (double)scale2, (double)x.A) - (double)log2f(fabsf(x.ws));
+      q.r = (float)r;
+      q.weight = copysignf(fabsf(q.r) < pos_inf() ? ex2((float)((double)q.r - r)) : 1.0f, x.ws);
       // (r = +inf: A says that there is no gradient, or the weight is 0)
       q.fits = fabsf(x.m * scale2) < 0x1p10f && (fabsf(q.r) < 0x1p10f || q.r == pos_inf());
     } else {
