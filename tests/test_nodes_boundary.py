@@ -117,6 +117,20 @@ def test_bad_records():
         NodeDistillationLoss(reduction="average")
 
 
+@pytest.mark.parametrize("student", [False, True])
+@pytest.mark.parametrize("which", [0, 1])
+def test_records_that_want_gradients(which, student):
+    words, logits = record()
+    rest = torch.zeros(2, 4)
+    (logits, rest)[which].requires_grad_(True)
+    a = nodes()
+    a[0].requires_grad_(student)
+    with pytest.raises(ValueError, match="not differentiable w.r.t. the teacher's record"):
+        NodeDistillationLoss()(*a, words, logits, rest)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA tensors only"):
+        NodeDistillationLoss()(*a, words, logits, rest)
+
+
 # ---- the C ABI: every refusal comes before the first CUDA call ------------------------------
 
 def test_c_abi_refusals():

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_nodes_gpu import UNIT, check_distill, check_sample, make, teacher
-from transducer_b200 import sample_words, top_words
+from transducer_b200 import NodeDistillationLoss, sample_words, top_words
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +75,20 @@ def test_bf16_paths_with_scores_far_from_0(offset, temperature, own_record):
     else:
         words, logits, _ = teacher(E, P, nodes, nodes, K, g, temperature)
     check_distill(E, P, nodes, nodes, words, logits, None, temperature, g, K)
+
+
+# ---- records that want gradients ---------------------------------------------------------
+
+@pytest.mark.parametrize("student", [False, True])
+@pytest.mark.parametrize("which", ["logits", "rest"])
+def test_records_that_want_gradients_are_refused(student, which):
+    E, P, frames, positions, g = make(2, 5, 3, 20, 7, holes=False)
+    words, logits, rest = teacher(E, P, frames, positions, 4, g)
+    E.requires_grad_(student)
+    (logits if which == "logits" else rest).requires_grad_(True)
+    criterion = NodeDistillationLoss()
+    with pytest.raises(ValueError, match="not differentiable w.r.t. the teacher's record"):
+        criterion(E, P, frames, positions, words, logits, rest)
+    with torch.no_grad():
+        costs = criterion(E, P, frames, positions, words, logits, rest)
+    assert torch.equal(costs, criterion(E, P, frames, positions, words, logits.detach(), rest.detach()).detach())

@@ -279,7 +279,7 @@ class NodeDistillationLoss(torch.nn.Module):
         emissions, predictions, frames, positions  the student's nodes (see the module's docstring)
         words   int32 [B, N, K]    the teacher's listed words, K <= 256; a negative one is ignored,
                                    equal ones of a node add up
-        logits  float32 [B, N, K]  the teacher's logits for them
+        logits  float32 [B, N, K]  the teacher's logits for them (gradients w.r.t. them and rest: refused)
         rest    float32 [B, N], optional  log-sum-exp of the teacher's logits over all other words
                                    (without it the teacher's distribution is the listed words' alone)
         Returns costs float32 [B, N] (0 where there is no node or nothing is listed, +inf where the
@@ -308,6 +308,8 @@ class NodeDistillationLoss(torch.nn.Module):
             if rest.shape != frames.shape:
                 raise ValueError("must have a rest per node.")
             check_device(emissions, rest)
+        if torch.is_grad_enabled() and (logits.requires_grad or (rest is not None and rest.requires_grad)):
+            raise ValueError("the costs are not differentiable w.r.t. the teacher's record: detach logits and rest")
         save = torch.is_grad_enabled() and (emissions.requires_grad or predictions.requires_grad)
         costs = NodeDistillation.apply(emissions, predictions, frames, positions, words, logits,
                                        rest, self.temperature, save, self.validate_nodes)
