@@ -131,6 +131,22 @@ def test_records_that_want_gradients(which, student):
         NodeDistillationLoss()(*a, words, logits, rest)
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_tangents(which):
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        a = nodes()
+        for call in (lambda: top_words(*a, 2), lambda: sample_words(*a, torch.zeros(2, 4))):
+            with pytest.raises(ValueError, match="CUDA tensors only"):
+                call()
+        a[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+        for call in (lambda: top_words(*a, 2), lambda: sample_words(*a, torch.zeros(2, 4))):
+            with pytest.raises(RuntimeError, match="no tangents"):
+                call()
+        with pytest.raises((RuntimeError, ValueError)):
+            NodeDistillationLoss()(*a, *record())
+
+
 # ---- the C ABI: every refusal comes before the first CUDA call ------------------------------
 
 def test_c_abi_refusals():

@@ -92,3 +92,28 @@ def test_records_that_want_gradients_are_refused(student, which):
     with torch.no_grad():
         costs = criterion(E, P, frames, positions, words, logits, rest)
     assert torch.equal(costs, criterion(E, P, frames, positions, words, logits.detach(), rest.detach()).detach())
+
+
+# ---- what is not differentiable --------------------------------------------------------------------
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    E, P, frames, positions, g = make(2, 5, 3, 20, 7, holes=False)
+    words, logits, rest = teacher(E, P, frames, positions, 4, g)
+    uniforms = torch.rand(2, 7, generator=g).cuda()
+    with forward_ad.dual_level():
+        top_words(E, P, frames, positions, 4)    # (no tangent)
+        for e, p in ((forward_ad.make_dual(E, torch.ones_like(E)), P), (E, forward_ad.make_dual(P, torch.ones_like(P)))):
+            with pytest.raises(RuntimeError, match="no tangents"):
+                top_words(e, p, frames, positions, 4)
+            with pytest.raises(RuntimeError, match="no tangents"):
+                sample_words(e, p, frames, positions, uniforms)
+            with pytest.raises(RuntimeError):
+                NodeDistillationLoss()(e, p, frames, positions, words, logits, rest)
+
+
+def test_best_words_and_draws_are_detached():
+    E, P, frames, positions, g = make(2, 5, 3, 20, 7, holes=False)
+    E.requires_grad_(True)
+    assert not any(x.requires_grad for x in top_words(E, P, frames, positions, 4))
+    assert not any(x.requires_grad for x in sample_words(E, P, frames, positions, torch.rand(2, 7, generator=g).cuda()))

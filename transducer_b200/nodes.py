@@ -15,6 +15,7 @@ utterance passes its frames [B, 1], positions of 0 and predictions [B, 1, V].
 
 CUDA tensors only, like `TransducerLoss`; the work is enqueued on torch's current stream."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _transducer
 from .torch_binding import _workspace, check_contiguous, check_dim, check_type
@@ -96,6 +97,15 @@ def check_device(first, *others):
             raise ValueError("all inputs must be on the same device.")
 
 
+def check_no_tangents(*scores):
+    """For results that are not differentiable: a tangent (forward-mode differentiation) would be lost."""
+    if forward_ad._current_level < 0:
+        return
+    for x in scores:
+        if forward_ad.unpack_dual(x).tangent is not None:
+            raise RuntimeError("this call has no derivatives and takes no tangents")
+
+
 def check_temperature(temperature):
     if not 1e-38 <= temperature <= 1e30:
         raise ValueError("temperature must be positive, at least 1e-38 and at most 1e30")
@@ -121,9 +131,12 @@ def top_words(emissions, predictions, frames, positions, k, temperature=1.0, val
     Returns words int32 [B, N, k] (the greater score first, of equal ones the lower word), their
     logits float32 [B, N, k] = scores / temperature, and rest float32 [B, N], the log-sum-exp of
     scores / temperature over all other words (-inf where there are none).  Where there is no node:
-    -1, -inf, -inf.  ``validate_nodes=False`` skips the check of the indices, which waits for the
+    -1, -inf, -inf.  They are detached from the inputs' graph: nothing here is differentiable (the
+    log-probability of a word with gradients is minus the cost of `NodeDistillationLoss` with that
+    word listed alone).  ``validate_nodes=False`` skips the check of the indices, which waits for the
     kernels, so that the call only enqueues work."""
     certify_nodes(emissions, predictions, frames, positions)
+    check_no_tangents(emissions, predictions)
     check_temperature(temperature)
     if not 1 <= k <= min(MAX_LISTED_WORDS, emissions.shape[2]):
         raise ValueError("k must be between 1 and min(%d, vocabulary)" % MAX_LISTED_WORDS)
@@ -155,8 +168,9 @@ def sample_words(emissions, predictions, frames, positions, uniforms, temperatur
     Returns words int32 [B, N] and log_probs float32 [B, N], the logarithm of the word's
     probability among those that stay.  Where there is no node: -1 and 0; where every word is
     masked: -1 and -inf; where a score is NaN or +inf: -1 and NaN.  Draws on the same inputs give
-    the same words.  ``validate_nodes``: see `top_words`."""
+    the same words.  Both results are detached; ``validate_nodes``: see `top_words`."""
     certify_nodes(emissions, predictions, frames, positions)
+    check_no_tangents(emissions, predictions)
     check_dim(uniforms, 2, "uniforms")
     check_type(uniforms, torch.float32, "uniforms")
     check_contiguous(uniforms, "uniforms")
