@@ -1,8 +1,10 @@
 """Node operators (transducer_b200.nodes) at the edges of what their documentation allows."""
+import math
 
 import pytest
 import torch
 
+import node_reference as ref
 from test_nodes_gpu import UNIT, check_distill, check_sample, make, teacher
 from transducer_b200 import NodeDistillationLoss, sample_words, top_words
 
@@ -55,6 +57,60 @@ def test_top_k_beyond_the_whole_numbers_of_32_bit_floats():
         assert (upto[:more] - u * total).abs().min() > 1e-3   # (64-bit sums are good to 1e-5 here)
         word, _ = sample_words(E, P, zero, zero, torch.full((1, 1), u).cuda(), top_k=ones + more)
         assert word.item() == ones + want, more
+
+
+# ---- long lists over short rows ------------------------------------------------------------------
+
+@pytest.mark.parametrize("V", [513, 514, 520, 600, 640, 768, 776, 1000, 1025, 1032])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [65, 190, 196, 197, 256])
+@pytest.mark.parametrize("kind", ["spread", "equal", "masked", "broken"])
+def test_long_lists_over_short_rows(V, dtype, k, kind):
+    E, P, frames, positions, g = make(2, 5, 3, V, 9, dtype, seed=V + k, holes=False)
+    if kind == "equal":
+        E, P = E.round(), P.round()
+        E[0], P[0] = 0.0, 0.0
+    elif kind == "masked":
+        E[0, :, torch.randperm(V, generator=g)[k - 10:]] = -math.inf
+        E[1, :, torch.randperm(V, generator=g)[:V - k]] = torch.finfo(dtype).min
+    elif kind == "broken":
+        E[0, 1, V // 3], E[0, 2, 5] = math.nan, math.inf
+        E[1, 3, :k + 3] = math.nan
+    words, logits, rest = top_words(E, P, frames, positions, k)
+    z, here = ref.scores(E, P, frames, positions)
+    w, l, r = ref.top_words(z, here, k)
+    if kind == "broken":   # (NaN stands first: among NaN, and beside them, the order is the reference's)
+        whole = z.isfinite().all(-1)
+        assert whole.any() and not whole.all()
+        assert torch.equal(words.cpu()[whole], w[whole])
+        torch.testing.assert_close(rest.cpu().double()[whole], r[whole], rtol=64 * UNIT, atol=128 * UNIT)
+        assert torch.equal(words.cpu(), w)
+        torch.testing.assert_close(logits.cpu().double(), l, rtol=0, atol=0, equal_nan=True)
+        return
+    assert torch.equal(words.cpu(), w)
+    assert torch.equal(logits.cpu().double(), l)
+    torch.testing.assert_close(rest.cpu().double(), r, rtol=64 * UNIT, atol=128 * UNIT)
+
+
+def microseconds(call, runs=15):
+    times = []
+    for _ in range(runs):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        times.append(1e3 * a.elapsed_time(b))
+    return sorted(times[3:])[len(times[3:]) // 2]
+
+
+def test_long_lists_over_short_rows_take_no_longer_than_over_longer_ones():
+    """196 words of rows of 520 were found by going through the row from memory for every bit of a score, in 2.3 times
+    the time of rows of twice the words (now 1.1)."""
+    def time(V):
+        E, P, frames, positions, _ = make(8, 60, 30, V, 1000, torch.bfloat16, seed=V, holes=False)
+        return microseconds(lambda: top_words(E, P, frames, positions, 196, validate_nodes=False))
+    assert time(520) <= 1.6 * time(1040)
 
 
 # ---- bf16 gradients along a path whose scores are far from 0 -------------------------------------

@@ -80,16 +80,17 @@ __device__ __forceinline__ int smallest_index(int V, F reaches) {
   return lo;
 }
 
-// The k first words of the order (0 < k <= V).
+// The k first words of the order (0 < k <= V).  `key`: of the k-th, if it is known.
 template <typename TIn, int VEC, int G>
-__device__ __noinline__ Cut general_first_k(NodeScores<TIn> s, int V, Group<G> g, int k) {
+__device__ __noinline__ Cut general_first_k(NodeScores<TIn> s, int V, Group<G> g, int k, unsigned key = 0) {
   auto count = [&](auto pick) {
     int c = 0;
     each_score<TIn, VEC, G>(s, V, g.tid, [&](float z, int v) { c += pick(score_key(z), v) ? 1 : 0; });
     return g.sum(c);
   };
   Cut cut;
-  cut.key = largest_key([&](unsigned x) { return count([&](unsigned u, int) { return u >= x; }) >= k; });
+  cut.key = key ? key
+                : largest_key([&](unsigned x) { return count([&](unsigned u, int) { return u >= x; }) >= k; });
   const int above = count([&](unsigned u, int) { return u > cut.key; });
   cut.last = smallest_index(V, [&](int y) {
     return count([&](unsigned u, int v) { return u == cut.key && v <= y; }) >= k - above;

@@ -7,8 +7,9 @@ namespace {
 
 template <typename TIn, int VEC, int G>
 __device__ __noinline__ void general_top_words(NodeScores<TIn> s, int V, Group<G> g, Entry* list, int* filled,
-                                               int* words, float* logits, float* rest, int k, float scale) {
-  const Cut cut = general_first_k<TIn, VEC, G>(s, V, g, k);
+                                               int* words, float* logits, float* rest, int k, float scale,
+                                               unsigned key) {
+  const Cut cut = general_first_k<TIn, VEC, G>(s, V, g, k, key);
   g.sync();
   if (g.tid == 0) *filled = 0;
   g.sync();
@@ -168,28 +169,51 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) top_words_kernel(Node
                                    : min(min(least(key[0]), least(key[1])), min(least(key[2]), least(key[3])))),
                      most, n, reach);
   }
-  if (tid == 0) *filled = 0, edge[0] = edge[1] = 0;
-  g.sync();
   const unsigned lowest = score_key(neg_inf());
-  const float bound = key_score(max(lo, lowest));
-  auto append = [&](float x, int v) {
-    const int i = atomicAdd(filled, 1);
-    if (i < kListed) list[i] = entry_of(x, v);
-  };
-  each([&](const float (&z)[kPass], int v) {
-    unsigned in = 0;
+  // The words that reach the threshold: how many there are, and the first kListed to come in the list.
+  auto list_words = [&] {
+    if (tid == 0) *filled = 0, edge[0] = edge[1] = 0;
+    g.sync();
+    const float bound = key_score(max(lo, lowest));
+    auto append = [&](float x, int v) {
+      const int i = atomicAdd(filled, 1);
+      if (i < kListed) list[i] = entry_of(x, v);
+    };
+    each([&](const float (&z)[kPass], int v) {
+      unsigned in = 0;
 #pragma unroll
-    for (int i = 0; i < kPass; ++i) in |= z[i] >= bound ? 1u << i : 0u;
+      for (int i = 0; i < kPass; ++i) in |= z[i] >= bound ? 1u << i : 0u;
 #pragma unroll 1
-    for (; in; in &= in - 1) {
-      const int i = __ffs(in) - 1;
-      if (v + i < a.V) append(RESIDENT ? w[v + i - at.first] : at.score(v + i), v + i);
+      for (; in; in &= in - 1) {
+        const int i = __ffs(in) - 1;
+        if (v + i < a.V) append(RESIDENT ? w[v + i - at.first] : at.score(v + i), v + i);
+      }
+    });
+    g.sync();
+    return *filled;
+  };
+  auto general = [&](unsigned key) {
+    general_top_words<TIn, VEC, G>(s, a.V, g, list, filled, words, logits, rest, k, scale, key);
+  };
+  int c = list_words();
+  if (RESIDENT && c > min(kListed, k + k / 2 + 64)) {
+    auto reach = [&](unsigned t) {   // (NaN counts as the greatest, as the order has it, and is not listed)
+      int n = 0;
+      each([&](const float (&z)[kPass], int v) {
+#pragma unroll
+        for (int i = 0; i < kPass; ++i) n += v + i < a.V && score_key(z[i]) >= t ? 1 : 0;
+      });
+      return g.sum(n);
+    };
+    lo = max(lo, lowest);
+    const int n = reach(lo + 1);
+    if (n >= k) {
+      lo = threshold(lo + 1, 0xfffffffeu, n, reach);
+      c = list_words();
     }
-  });
-  g.sync();
-  const int c = *filled;
-  auto general = [&] { general_top_words<TIn, VEC, G>(s, a.V, g, list, filled, words, logits, rest, k, scale); };
-  if (c > kListed || c < k) return general();   // (fewer than k: some are NaN)
+    if (c > kListed) return general(lo);   // (equal scores: lo is the greatest key that k words reach)
+  }
+  if (c > kListed || c < k) return general(0);   // (fewer than k: some are NaN)
   constexpr int kShare = G >= 128 ? 4 : 1;   // threads per entry, each looking at its part of the others
 #pragma unroll 1
   for (int i0 = 0; i0 < c; i0 += G / kShare) {
@@ -225,7 +249,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) top_words_kernel(Node
       sum[i % 4] += z[i] >= last ? 0.0f : ex2((z[i] - last) * scale2);
   });
   float all = g.sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-  if (all != all) return general();
+  if (all != all) return general(0);
   if (!rest) return;
   all += (float)ties;
   float ref = last;
