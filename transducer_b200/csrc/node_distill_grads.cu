@@ -501,10 +501,11 @@ struct Batch {
   }
 };
 
-// Rows of either gradient of utterances whose nodes are not a path.  Tasks: (row, split, tile) of E, then of P.
+// Rows of either gradient of utterances whose nodes are not a path.  Tasks of an utterance: (row, split, tile) of E, then
+// of P.
 // Bound by the latency of a node's record and row, one node ahead, and by instructions: the whole lattices of 4
-// utterances, 5700 nodes of 512 words, take 36 us, of which reading both sides' rows for every node is 4 at the L2's
-// rate.
+// utterances, 5700 nodes of 512 words, take 19 us, of which reading both sides' rows for every node is 4 at the L2's
+// rate.  Utterances lie side by side in the grid (one after another in every warp they took 37).
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a, GradArgs k) {
   constexpr int COLS = kCols, NV = COLS / VEC;
@@ -520,16 +521,20 @@ __global__ void __launch_bounds__(kWarps * 32, 4) distill_rows_kernel(NodeArgs a
   __syncwarp();
   const i64 ePer = (i64)a.T * k.eSplits * k.tiles, pPer = (i64)a.U * k.pSplits * k.tiles;   // tasks of an utterance
   const i64 step = (i64)gridDim.x * kWarps;
-  int b = -1;
-  unsigned off = 0;   // of the 32 utterances that b is one of, those that are left
+  // the utterances of this row of the grid: blockIdx.y, blockIdx.y + gridDim.y and so on
+  const int utterances = (a.B - 1 - (int)blockIdx.y) / (int)gridDim.y + 1;
+  int b = 0, at = -1;   // and which of them b is
+  unsigned off = 0;     // of the 32 that it is one of, those off a path that are left
   auto next_off_path = [&] {
-    for (int from = off ? b : (b + 32) / 32 * 32; !off; from += 32) {
-      if (from >= a.B) return false;
-      off = __ballot_sync(0xffffffffu, from + lane < a.B && k.saved.offPath[from + lane]);
-      b = from;
+    auto numbered = [&](int i) { return i * (int)gridDim.y + (int)blockIdx.y; };
+    for (int from = off ? at : (at + 32) / 32 * 32; !off; from += 32) {
+      if (from >= utterances) return false;
+      off = __ballot_sync(0xffffffffu, from + lane < utterances && k.saved.offPath[numbered(from + lane)]);
+      at = from;
     }
-    b = b / 32 * 32 + __ffs(off) - 1;
+    at = at / 32 * 32 + __ffs(off) - 1;
     off &= off - 1;
+    b = numbered(at);
     return true;
   };
   while (next_off_path()) {
@@ -796,8 +801,10 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
     if (nodes > 1) {   // (a single node is a path)
       ScopedKernel prof("distill_rows", stream);
       const i64 tasks = ((i64)a.T * p.eSplits + (i64)a.U * p.pSplits) * p.tiles;
-      const i64 ctas = std::min<i64>(div_up64(tasks, kWarps), 148 * 6);
-      distill_rows_kernel<TIn, VEC><<<(unsigned)ctas, kWarps * 32, 0, stream>>>(a, k);
+      // an utterance's tasks along x, and as many utterances side by side as fill the chip
+      const i64 most = 148 * 6, x = std::min<i64>(div_up64(tasks, kWarps), most);
+      const dim3 grid((unsigned)x, (unsigned)std::min<i64>(a.B, div_up64(most, x)));
+      distill_rows_kernel<TIn, VEC><<<grid, kWarps * 32, 0, stream>>>(a, k);
       TB200_CHECK_LAUNCH();
     }
     const i64 eRows = p.eSplits > 1 ? frameRows : 0;
