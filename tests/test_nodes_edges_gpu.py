@@ -216,3 +216,30 @@ def test_small_lattices_share_the_chip():
                         saved.numel(), weights.data_ptr(), dE.data_ptr(), dP.data_ptr(), sizes, 4, 1.0, ws.data_ptr(), n)
             return microseconds(backward)
     assert time(32) <= 4.0 * time(1)
+
+
+# ---- two-byte rows along paths of many segments ----------------------------------------------------
+
+@pytest.mark.parametrize("V", [1032, 2051, 2568])
+@pytest.mark.parametrize("gap", [10, 100])
+@pytest.mark.parametrize("with_rest", [False, True])
+def test_bf16_paths_of_many_segments(V, gap, with_rest):
+    """As test_distillation_paths_with_gaps, in bf16, with rows of several tiles and turns of the ring, and nodes enough
+    for a warp each."""
+    E, P, frames, positions, g = make(4, 500, 6, V, 620, torch.bfloat16, seed=V + gap, kind="path", holes=False)
+    frames[0, 60:] = -1
+    frames[2, 200:200 + gap] = -1
+    frames[3, :400] = -1
+    words, logits, rest = teacher(E, P, frames, positions, 5, g)
+    check_distill(E, P, frames, positions, words, logits, rest if with_rest else None, 1.0, g, 5)
+
+
+@pytest.mark.parametrize("V,B,T,U,N", [(64, 3, 300, 2, 302), (96, 2, 400, 90, 520), (56, 2, 3, 200, 230),
+                                       (1032, 1, 200, 1, 260), (520, 2, 90, 60, 150)])
+@pytest.mark.parametrize("kind", ["any", "path"])
+@pytest.mark.parametrize("K", [5, 40])
+def test_bf16_long_groups(V, B, T, U, N, kind, K):
+    """One position with many frames, many positions on few frames, in bf16."""
+    E, P, frames, positions, g = make(B, T, U, V, N, torch.bfloat16, seed=N, kind=kind)
+    words, logits, rest = teacher(E, P, frames, positions, K, g)
+    check_distill(E, P, frames, positions, words, logits, rest, 1.0, g, K)
