@@ -268,7 +268,6 @@ void launch_node_summary(const int* frames, const int* positions, i64 nodes, con
                          int* most, cudaStream_t stream);
 
 constexpr int kMaxListedWords = 256;   // longest list of words per node
-// Largest vocabulary of a distillation with the rest's weight: a bit per word in shared memory.
 
 // Whether every row can be moved in 16-byte vectors.
 bool node_rows_aligned(const NodeArgs& a);

@@ -1,4 +1,5 @@
 // C ABI of the operators on single lattice nodes (include/transducer_b200.h, last part).
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -59,6 +60,15 @@ void need(size_t have, size_t want, const void* p, const char* what) {
 }
 
 }  // namespace
+
+bool node_rows_aligned(const NodeArgs& a) {
+  const int size = a.dtype == kDtypeBf16 ? 2 : 4;
+  const i64 bytes[] = {(i64)reinterpret_cast<uintptr_t>(a.E), (i64)reinterpret_cast<uintptr_t>(a.P),
+                       a.eStrideB * size, a.eStrideT * size, a.pStrideB * size, a.pStrideU * size,
+                       (i64)a.V * size};
+  return std::all_of(std::begin(bytes), std::end(bytes), [](i64 x) { return x % 16 == 0; });
+}
+
 }  // namespace tb200
 
 using namespace tb200;

@@ -393,16 +393,6 @@ __global__ void __launch_bounds__(512) node_summary_kernel(const int* __restrict
 }
 
 template <typename F>
-void with_type(int dtype, bool wide, F launch) {
-  if (dtype == kDtypeBf16) {
-    if (wide) launch(bf16{}, std::integral_constant<int, 8>{});
-    else launch(bf16{}, std::integral_constant<int, 1>{});
-  } else {
-    if (wide) launch(float{}, std::integral_constant<int, 4>{});
-    else launch(float{}, std::integral_constant<int, 1>{});
-  }
-}
-template <typename F>
 void with_flag(bool on, F launch) {
   if (on) launch(std::true_type{});
   else launch(std::false_type{});

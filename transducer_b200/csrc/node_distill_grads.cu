@@ -817,14 +817,7 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
       TB200_CHECK_LAUNCH();
     }
   };
-  using std::integral_constant;
-  if (a.dtype == kDtypeBf16) {
-    if (wide) run(bf16{}, integral_constant<int, 8>{});
-    else run(bf16{}, integral_constant<int, 1>{});
-  } else {
-    if (wide) run(float{}, integral_constant<int, 4>{});
-    else run(float{}, integral_constant<int, 1>{});
-  }
+  with_type(a.dtype, wide, run);
 }
 
 }  // namespace tb200

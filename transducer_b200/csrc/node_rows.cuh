@@ -184,6 +184,19 @@ struct Group {
   }
 };
 
+// launch(storage type, words moved at a time), `wide`: 16 bytes.
+template <typename F>
+void with_type(int dtype, bool wide, F launch) {
+  using std::integral_constant;
+  if (dtype == kDtypeBf16) {
+    if (wide) launch(bf16{}, integral_constant<int, 8>{});
+    else launch(bf16{}, integral_constant<int, 1>{});
+  } else {
+    if (wide) launch(float{}, integral_constant<int, 4>{});
+    else launch(float{}, integral_constant<int, 1>{});
+  }
+}
+
 // Order-preserving integer of a score: NaN above everything, -0 as +0; 0 is below every score.
 __device__ __forceinline__ unsigned score_key(float z) {
   if (z != z) return 0xffffffffu;

@@ -8,7 +8,6 @@
 // of the sum itself (a thread has eight sums of up to nine weights, then come eleven steps; the row's whole and the
 // draw's sums are of fours in 32 bits and 64 bits from there) that is `unsure` below.  Where a comparison is closer
 // than that the sums are formed anew from memory with exponentials in 64 bits.
-#include <algorithm>
 #include <cfloat>
 
 #include "node_select.cuh"
@@ -699,21 +698,11 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
 
 }  // namespace
 
-// Whether words can be moved 16 bytes at a time: every row starts on a 16-byte boundary and has whole
-// vectors.
-bool node_rows_aligned(const NodeArgs& a) {
-  const int size = a.dtype == kDtypeBf16 ? 2 : 4;
-  const i64 bytes[] = {(i64)reinterpret_cast<uintptr_t>(a.E), (i64)reinterpret_cast<uintptr_t>(a.P),
-                       a.eStrideB * size, a.eStrideT * size, a.pStrideB * size, a.pStrideU * size,
-                       (i64)a.V * size};
-  return std::all_of(std::begin(bytes), std::end(bytes), [](i64 x) { return x % 16 == 0; });
-}
-
 void launch_sample_words(const NodeArgs& a, const float* uniforms, int* words, float* logProbs,
                          SampleRule rule, cudaStream_t stream) {
   const i64 nodes = (i64)a.B * a.N;
   if (nodes == 0) return;
-  with_type(a, [&](auto type, auto vec) {
+  with_type(a.dtype, node_rows_aligned(a), [&](auto type, auto vec) {
     using TIn = decltype(type);
     with_group(a.V, true, [&](auto group, auto resident) {
       constexpr int G = decltype(group)::value, rows = kCta<G> / G;

@@ -182,16 +182,4 @@ void with_group(int V, bool warps, F launch) {
   else launch(integral_constant<int, 1024>{}, std::false_type{});
 }
 
-template <typename F>
-void with_type(const NodeArgs& a, F launch) {
-  const bool wide = node_rows_aligned(a);
-  if (a.dtype == kDtypeBf16) {
-    if (wide) launch(bf16{}, std::integral_constant<int, 8>{});
-    else launch(bf16{}, std::integral_constant<int, 1>{});
-  } else {
-    if (wide) launch(float{}, std::integral_constant<int, 4>{});
-    else launch(float{}, std::integral_constant<int, 1>{});
-  }
-}
-
 }  // namespace tb200

@@ -277,7 +277,7 @@ void launch_top_words(const NodeArgs& a, int* words, float* logits, float* rest,
                       cudaStream_t stream) {
   const i64 nodes = (i64)a.B * a.N;
   if (nodes == 0) return;
-  with_type(a, [&](auto type, auto vec) {
+  with_type(a.dtype, node_rows_aligned(a), [&](auto type, auto vec) {
     using TIn = decltype(type);
     // (a warp's list holds 256 entries, and its 128 maxima tell the best 64 at most)
     with_group(a.V, k <= 64, [&](auto group, auto resident) {
