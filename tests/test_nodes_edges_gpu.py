@@ -113,6 +113,39 @@ def test_long_lists_over_short_rows_take_no_longer_than_over_longer_ones():
     assert time(520) <= 1.6 * time(1040)
 
 
+# ---- shares that end at a gap ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [520, 1025, 10000, 20000, 60000])
+@pytest.mark.parametrize("off", [-1e-7, -1e-9, -1e-12, 1e-12, 1e-9, 1e-7])   # (0: sums in 64 bits round)
+def test_shares_next_to_the_sum_of_the_words_above_a_gap(V, dtype, off):
+    """Twenty words have nearly all of the weight: the share is theirs, or a little less or more than 32 bits can tell."""
+    E, top_p, frames, zero, uniforms = gap(V, dtype, 6, 1.0 + off)
+    check_sample(E, torch.zeros_like(E), frames, zero, uniforms, top_p=top_p)
+
+
+def gap(V, dtype, N, factor):
+    g = torch.Generator().manual_seed(V)
+    E = -9.0 - torch.rand(1, N, V, generator=g)
+    for n in range(N):
+        E[0, n, torch.randperm(V, generator=g)[:20]] = -torch.rand(20, generator=g)
+    E[0, :] = E[0, :1]
+    E = E.to(dtype)
+    w = (E[0, 0].double() - E[0, 0].double().max()).exp().sort(descending=True).values
+    frames = torch.arange(N)[None].int().cuda()
+    top_p = (w[:20].sum() / w.sum()).item() * factor
+    return E.cuda(), top_p, frames, torch.zeros_like(frames), torch.rand(1, N, generator=g).cuda()
+
+
+def test_a_share_next_to_a_gap_is_found_as_fast_as_another():
+    """64 rounds and 48 passes in 64 bits were made: 27 times as long as for another share (now 4)."""
+    def time(factor):
+        E, top_p, frames, zero, uniforms = gap(10000, torch.float32, 64, factor)
+        P = torch.zeros_like(E)
+        return microseconds(lambda: sample_words(E, P, frames, zero, uniforms, top_p=top_p, validate_nodes=False))
+    assert max(time(1.0 - 1e-9), time(1.0 + 1e-9)) <= 10.0 * time(0.99)
+
+
 # ---- bf16 gradients along a path whose scores are far from 0 -------------------------------------
 
 @pytest.mark.parametrize("offset", [0.0, 120.0, 496.0, -496.0, 30000.0])

@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         return (float)g.sum(sum);
       }
     };
-    const float floor = (float)(1e-5 * total), all = (float)total, want = (float)target;
+    const float floor = (float)(1e-5 * total), all = (float)total;
+    float want = (float)target;
     auto level = [&](float v) {
       return kByWeight ? lg2(fmaxf(v, 0.25f)) - lg2(fmaxf(all - v, floor)) : -lg2(fmaxf(v, 0.5f));
     };
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     }
     float t = guess, x = lg2(guess), had = 3e38f;
     const float lWant = level(want);
-    int stuck = 0;
+    int stuck = 0, wrong = 0;
     bool done = false;
     Cut cut;
 #pragma unroll 1
@@ -530,19 +531,25 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
         kept = *filled >> 2;
         enough = *filled & 2;
       }
+      // A threshold whose side 32 bits have taken wrongly, the target being closer to the sum there than they can tell:
+      // the next one is beyond it, farther and farther off until a word has been passed (in steps of a rounding that
+      // took up to 54 rounds), and what is wanted is moved past the sum so that none on the way is taken wrongly again.
+      if (kByWeight && (!enough || kept == 0)) {
+        const float step = ex2((float)(4 * wrong++ - 14));
+        want = enough ? vHi : __uint_as_float(__float_as_uint(vLo) + 1);
+        x = enough ? xHi + step : xLo - step;
+        t = fminf(fmaxf(ex2(x), FLT_MIN), kAbove);
+        continue;
+      }
       // (32-bit weights of different scores may come out in the wrong order by a rounding: not so the
       // cut's and those beyond the thresholds)
-      float y = 0.0f;
-      if (kept > 0) {
-        const Entry last = sorted[kept - 1];
-        cut = Cut{entry_key(last), entry_word(last)};
-        y = weight(key_score(cut.key));
-      }
-      if (hi < kAbove && (kept == 0 || y * 1.000004f >= hi)) t = hi * 1.00003f, x = xHi;
-      else if (lo > FLT_MIN && (!enough || y * 0.999996f < lo)) t = fmaxf(lo * 0.99997f, FLT_MIN), x = xLo;
-      else if (!kByWeight && y * 0.999996f < lo) break;   // (beside weights that are 0 here)
-      else if (kept > 0 && enough) done = true;
-      else break;
+      const Entry last = sorted[kept - 1];
+      cut = Cut{entry_key(last), entry_word(last)};
+      const float y = weight(key_score(cut.key));
+      if (hi < kAbove && y * 1.000004f >= hi) t = hi * 1.00003f, x = xHi;
+      else if (!(y * 0.999996f < lo)) done = true;
+      else if (lo > FLT_MIN) t = fmaxf(lo * 0.99997f, FLT_MIN), x = xLo;
+      else break;   // (beside weights that are 0 here)
       if constexpr (RESIDENT)   // what lies between and does not stay
         if (done)
           for (int i = kept + tid; i < c; i += G) row[entry_word(sorted[i])] = 0.0f;
