@@ -373,7 +373,8 @@ int tb200_sample_words(const void* emissions, const void* predictions, int bf16,
  * The backward call writes egrads [B, maxT, V] and pgrads [B, maxU, V] whole and contiguous (either
  * may be NULL): the gradients of sum weights[b,n] costs[b,n].  They are added up in the nodes' order,
  * in fp32, and rounded once: the bits are the same from run to run.  Fastest where the nodes of an
- * utterance are a path, neither frames nor positions going back from one to the next. */
+ * utterance are a path, neither frames nor positions going back from one to the next (and no more
+ * than 64 places without a node before one: beyond that the same sums are formed row by row). */
 size_t tb200_distill_saved_bytes(int batchSize, int maxInputLength, int maxLabelLength, int nodes,
                                  int K);
 int tb200_distill_forward(const void* emissions, const void* predictions, int bf16,

@@ -6,7 +6,7 @@ import torch
 
 import node_reference as ref
 from test_nodes_gpu import UNIT, check_distill, check_sample, make, teacher
-from transducer_b200 import NodeDistillationLoss, sample_words, top_words
+from transducer_b200 import NodeDistillationLoss, TransducerLoss, sample_words, top_words
 
 pytestmark = pytest.mark.gpu
 
@@ -276,3 +276,29 @@ def test_bf16_long_groups(V, B, T, U, N, kind, K):
     E, P, frames, positions, g = make(B, T, U, V, N, torch.bfloat16, seed=N, kind=kind)
     words, logits, rest = teacher(E, P, frames, positions, K, g)
     check_distill(E, P, frames, positions, words, logits, rest, 1.0, g, K)
+
+
+# ---- the nodes of an alignment -------------------------------------------------------------------
+
+def test_nodes_of_an_alignment():
+    """On one frame there is one alignment: its nodes' costs add up to the lattice's."""
+    B, U, V = 3, 5, 40
+    g = torch.Generator().manual_seed(8)
+    E, P = torch.randn(B, 1, V, generator=g).cuda(), torch.randn(B, U + 1, V, generator=g).cuda()
+    labels = torch.randint(1, V, (B, U), generator=g).int().cuda()
+    lengths = torch.tensor([5, 0, 3]).cuda()
+    moves = (torch.arange(U + 1, device="cuda") < lengths[:, None]).long()
+    n_moves = lengths + 1
+    n = torch.arange(moves.shape[1], device=moves.device)
+    positions = moves.cumsum(1) - moves
+    frames = n - positions
+    gone = n >= n_moves[:, None]
+    frames, positions = (x.masked_fill(gone, -1).int() for x in (frames, positions))
+    words = torch.where(moves.bool(), torch.nn.functional.pad(labels, (0, 1)), 0).int()[..., None].contiguous()
+    E.requires_grad_(True), P.requires_grad_(True)
+    costs = NodeDistillationLoss()(E, P, frames, positions, words, torch.zeros(B, U + 1, 1).cuda())
+    grads = torch.autograd.grad(costs.sum(), (E, P))
+    whole = TransducerLoss()(E, P, labels, torch.ones(B, dtype=torch.int32).cuda(), lengths.int())
+    torch.testing.assert_close(costs.sum(1), whole, rtol=1e-5, atol=1e-4)
+    for a, b in zip(grads, torch.autograd.grad(whole.sum(), (E, P))):
+        torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-4)

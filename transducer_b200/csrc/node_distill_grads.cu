@@ -259,8 +259,8 @@ struct __align__(16) PathCta {
 // The warps of a CTA go along the same nodes.  Bound by latencies and issue: 16 warps an SM, 63 % of the issue slots, 360
 // instructions for a node and tile, of which 8 for each of a lane's 16 words.  More warps spill registers, and next to
 // this much shared memory the L1 does not hold them.  Records loaded one node ahead, into registers, were waited for at
-// every node: 774 us against 571 for 58800 nodes of 10000 bf16 words (4.2 TB/s of E and its gradients; at the copy rate
-// 365); 8 utterances in fp32 224 us (5.2 TB/s).
+// every node: 774 us against 571 for 58800 nodes of 10000 bf16 words (now 576, 4.2 TB/s of E and its gradients; at the copy
+// rate 365); 8 utterances in fp32 224 us (5.2 TB/s).
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(kPathWarps * 32, 16 / kPathWarps)
     distill_path_kernel(NodeArgs a, GradArgs k) {

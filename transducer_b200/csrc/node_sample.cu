@@ -198,9 +198,10 @@ __device__ __noinline__ void exact_draw(NodeScores<TIn> s, int V, int seg, Group
 }
 
 // One group of threads per node; the row's weights take the scores' place in shared memory.  Each threshold tried is a
-// pass over them, and there the time goes (issue and barriers): 14900 nodes of 10000 fp32 words take 252 us without a
+// pass over them, and there the time goes (issue and barriers): 14900 nodes of 10000 fp32 words take 250 us without a
 // rule (2.3 TB/s of new rows) and 587 with topP = 0.9, four to five thresholds and the list; one row of 32000 words 27,
-// latency.  Sums of the weights in 32 bits throughout left more draws to the 64-bit pass and were slower.
+// latency.  Sums of the weights in 32 bits throughout left more draws to the 64-bit pass and were slower.  The 64
+// registers that 1024 threads an SM leave are not enough: 8 to 104 bytes a thread are spilled, most by a warp per row.
 template <typename TIn, int VEC, int G, bool RESIDENT>
 __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) sample_words_kernel(
     NodeArgs a, const float* __restrict__ uniforms, int* __restrict__ words, float* __restrict__ logProbs,

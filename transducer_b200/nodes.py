@@ -10,8 +10,11 @@ no node.  Its scores are ``emissions[b, frame, :] + predictions[b, position, :]`
     emissions    float32 [B, T, V], or both bfloat16; any strides (the words of a row are made
     predictions  float32 [B, U, V]  adjacent if they are not)
 
-The nodes of an alignment are one per blank and label; a decoder that extends one hypothesis per
-utterance passes its frames [B, 1], positions of 0 and predictions [B, 1, V].
+The nodes of an alignment are one per blank and label: with its moves, labels being 1, the nodes
+that they leave from have positions ``moves.cumsum(1) - moves`` and frames ``arange(N) - positions``.
+They are a path (neither frames nor positions go back), which is what the gradients are fastest for;
+more than 64 places without a node before another one of the utterance make it none.  A decoder that
+extends one hypothesis per utterance passes its frames [B, 1], positions of 0 and predictions [B, 1, V].
 
 CUDA tensors only, like `TransducerLoss`; the work is enqueued on torch's current stream."""
 import torch
@@ -322,9 +325,11 @@ class NodeDistillationLoss(torch.nn.Module):
             if rest.shape != frames.shape:
                 raise ValueError("must have a rest per node.")
             check_device(emissions, rest)
-        if torch.is_grad_enabled() and (logits.requires_grad or (rest is not None and rest.requires_grad)):
-            raise ValueError("the costs are not differentiable w.r.t. the teacher's record: detach logits and rest")
-        save = torch.is_grad_enabled() and (emissions.requires_grad or predictions.requires_grad)
+        save = torch.is_grad_enabled()
+        if save:
+            if logits.requires_grad or (rest is not None and rest.requires_grad):
+                raise ValueError("the costs are not differentiable w.r.t. the teacher's record: detach logits and rest")
+            save = emissions.requires_grad or predictions.requires_grad
         costs = NodeDistillation.apply(emissions, predictions, frames, positions, words, logits,
                                        rest, self.temperature, save, self.validate_nodes)
         if self.reduction == "sum":
