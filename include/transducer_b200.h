@@ -395,6 +395,59 @@ int tb200_distill_backward(const void* emissions, const void* predictions, int b
                            int K, double temperature, void* workspace,
                            size_t workspaceBytes);
 
+/* ---- a beam search's step, and the words' embeddings that it goes on with ----
+ * No counterpart in the reference, which decodes given transcripts only. */
+
+/* The best extensions of every utterance's hypotheses.  Hypothesis n < N of utterance b has the score
+ * scores[b,n] (a log-probability) and is at the node frames[b,n], positions[b,n]; word v, the blank like
+ * any other, extends it to
+ *   d(n, v) = scores[b,n] + (z[v] - log sum exp(z)),   z[v] = E[b, frame, v] + P[b, position, v].
+ * A hypothesis without a node is finished: it stays as it is, d(n, -1) = scores[b,n].  One with a score of
+ * -inf is not there, and nothing is read for it; words whose z is -inf are no extensions.  The `width`
+ * (1 to 256) greatest are returned in order, of equal ones the lower parent, then the lower word
+ * first: outScores, parents, words [B, width]; where there are fewer: -inf, -1, -1.  The order is
+ * that of 64-bit arithmetic on z.  An utterance one of whose hypotheses has a score of NaN or +inf, or
+ * such a z, gets NaN, -1, -1 throughout.  workspace: 16-byte aligned. */
+size_t tb200_extend_beams_workspace_bytes(int batchSize, int alphabetSize, int nodes);
+int tb200_extend_beams(const void* emissions, const void* predictions, int bf16, long long eStrideB,
+                       long long eStrideT, long long pStrideB, long long pStrideU, const int* frames,
+                       const int* positions, const float* scores, float* outScores, int* parents,
+                       int* words, int batchSize, int maxInputLength, int maxLabelLength,
+                       int alphabetSize, int nodes, int width, void* workspace,
+                       size_t workspaceBytes);
+
+/* States that follow their hypotheses.  In each of `count` tensors (host array) the rowBytes bytes at
+ * to + b * toStrideB + w * toStrideN become those at from + b * fromStrideB + n * fromStrideN with
+ * n = parents[b,w] (strides in bytes, rows of any alignment).  Where n is not in [0, hypotheses) the row
+ * is set to zeros, or left as it is if `kept`.  from == to with equal strides: in place (rows without a
+ * parent are left as they are, at most 8192 of them per utterance); else the two must not overlap, nor
+ * may the rows that are written. */
+typedef struct {
+  const void* from;
+  void* to;
+  long long fromStrideB, fromStrideN, toStrideB, toStrideN, rowBytes;
+} tb200_states;
+int tb200_reorder_states(const tb200_states* states, int count, const int* parents, int batchSize,
+                         int hypotheses, int width, int kept);
+
+/* Rows of a table [R, H] (`stride` elements from one row to the next) for words [count]:
+ *   rows[n,h] = factor * table[words[n], h] where number (n, h) stays, else 0,
+ * in fp32, rounded once (bf16 = 1: table, rows, deltas and grad are bfloat16); a row of zeros where the
+ * word is not in [0, R).  Of 65536 numbers k = round(65536 * dropout), 65535 at most, are dropped, and
+ * factor = scale * 65536 / (65536 - k).  Number (n, h) is dropped if 16 bits of Philox4x32-10 are below
+ * k: counter (n mod 2^32, n / 2^32, h / 8, 0), key (seed mod 2^32, seed / 2^32), of its four numbers x the low
+ * (h even) or high half of x[h % 8 / 2].  seedAt (device memory): the seed is there instead, if not NULL.
+ * The backward call writes grad [R, H] whole: the sums of factor * deltas[n,h] over the numbers that stay
+ * of the rows that are a word's, in fp32, rounded once; the same bits from run to run.
+ * count is below 2^31 - 1, R 2^28 and H 2^23 at most. */
+int tb200_embed_words(const void* table, int bf16, long long stride, const int* words, long long count,
+                      void* rows, int R, int H, double scale, double dropout, long long seed,
+                      const long long* seedAt);
+size_t tb200_embed_backward_workspace_bytes(long long count, int R, int H);
+int tb200_embed_backward(const void* deltas, int bf16, const int* words, long long count, void* grad, int R,
+                         int H, double scale, double dropout, long long seed, const long long* seedAt,
+                         void* workspace, size_t workspaceBytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,7 +6,7 @@ used, so helper modules that need no GPU (``transducer_b200.workloads``,
 ``transducer_b200.distributed``) can be imported by processes that must not load it."""
 
 __all__ = ["TransducerLoss", "HostLossPipeline", "DeviceStatusError", "NodeDistillationLoss",
-           "top_words", "sample_words"]
+           "top_words", "sample_words", "extend_beams", "reorder_states", "embed_words"]
 
 
 def __getattr__(name):
@@ -16,6 +16,14 @@ def __getattr__(name):
     if name in ("NodeDistillationLoss", "top_words", "sample_words"):
         from . import nodes
         value = globals()[name] = getattr(nodes, name)
+        return value
+    if name in ("extend_beams", "reorder_states"):
+        from . import beams
+        value = globals()[name] = getattr(beams, name)
+        return value
+    if name == "embed_words":
+        from . import embeddings
+        value = globals()[name] = embeddings.embed_words
         return value
     if name == "HostLossPipeline":
         from .host_pipeline import HostLossPipeline

@@ -13,6 +13,7 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/transducer.h"
 #include "../../include/transducer_b200.h"
@@ -247,6 +248,49 @@ PYBIND11_MODULE(_transducer, m) {
         },
         "scores"_a, "frames"_a, "positions"_a, "words"_a, "saved"_a, "saved_bytes"_a, "weights"_a, "egrads"_a,
         "pgrads"_a, "sizes"_a, "k"_a, "temperature"_a, "workspace"_a, "workspace_bytes"_a);
+
+  // ---- a beam search's step, words' embeddings -----------------------------------------
+  m.def("extend_beams_workspace_bytes", &tb200_extend_beams_workspace_bytes);
+  m.def("extend_beams",
+        [](const Scores& s, addr frames, addr positions, addr scores, addr out_scores, addr parents, addr words,
+           const Sizes& n, int width, addr ws, size_t ws_bytes) {
+          check(tb200_extend_beams(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)), std::get<2>(s),
+                                   std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s),
+                                   at<const int>(frames), at<const int>(positions), at<const float>(scores),
+                                   at<float>(out_scores), at<int>(parents), at<int>(words), std::get<0>(n),
+                                   std::get<1>(n), std::get<2>(n), std::get<3>(n), std::get<4>(n), width,
+                                   at<void>(ws), ws_bytes));
+        },
+        "scores"_a, "frames"_a, "positions"_a, "beam_scores"_a, "out_scores"_a, "parents"_a, "words"_a, "sizes"_a,
+        "width"_a, "workspace"_a, "workspace_bytes"_a);
+  // `states`: of each tensor (from, to, their strides in bytes by utterance and by hypothesis, bytes of a row)
+  using Moved = std::tuple<addr, addr, long long, long long, long long, long long, long long>;
+  m.def("reorder_states",
+        [](const std::vector<Moved>& states, addr parents, int B, int N, int W, bool kept) {
+          std::vector<tb200_states> all;
+          for (const Moved& s : states)
+            all.push_back(tb200_states{at<const void>(std::get<0>(s)), at<void>(std::get<1>(s)), std::get<2>(s),
+                                       std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s)});
+          check(tb200_reorder_states(all.data(), (int)all.size(), at<const int>(parents), B, N, W, kept));
+        },
+        "states"_a, "parents"_a, "batch_size"_a, "hypotheses"_a, "width"_a, "kept"_a);
+  m.def("embed_words",
+        [](addr table, bool bf16, long long stride, addr words, long long count, addr rows, int R, int H, double scale,
+           double dropout, long long seed, addr seed_at) {
+          check(tb200_embed_words(at<const void>(table), bf16, stride, at<const int>(words), count, at<void>(rows), R, H,
+                                  scale, dropout, seed, at<const long long>(seed_at)));
+        },
+        "table"_a, "bf16"_a, "stride"_a, "words"_a, "count"_a, "rows"_a, "R"_a, "H"_a, "scale"_a, "dropout"_a, "seed"_a,
+        "seed_at"_a);
+  m.def("embed_backward_workspace_bytes", &tb200_embed_backward_workspace_bytes);
+  m.def("embed_backward",
+        [](addr deltas, bool bf16, addr words, long long count, addr grad, int R, int H, double scale, double dropout,
+           long long seed, addr seed_at, addr ws, size_t ws_bytes) {
+          check(tb200_embed_backward(at<const void>(deltas), bf16, at<const int>(words), count, at<void>(grad), R, H,
+                                     scale, dropout, seed, at<const long long>(seed_at), at<void>(ws), ws_bytes));
+        },
+        "deltas"_a, "bf16"_a, "words"_a, "count"_a, "grad"_a, "R"_a, "H"_a, "scale"_a, "dropout"_a, "seed"_a,
+        "seed_at"_a, "workspace"_a, "workspace_bytes"_a);
 
   // ---- device status (bounded waits that ran out) -----------------------------------
   // Returns the code of tb200_check_status (0, or 5 = a kernel gave up) without throwing, so the

@@ -1,32 +1,12 @@
 // C ABI of the operators on single lattice nodes (include/transducer_b200.h, last part).
 #include <algorithm>
 #include <cmath>
-#include <string>
 
-#include "../../include/transducer_b200.h"
-#include "api_internal.h"
+#include "api_guard.h"
 #include "kernels.h"
 
 namespace tb200 {
 namespace {
-
-template <typename F>
-int guarded(F&& body) {
-  try {
-    body();
-    return kOk;
-  } catch (const CudaError& e) {
-    return api_fail(kErrCuda, e.what());
-  } catch (const std::invalid_argument& e) {
-    return api_fail(kErrInvalidArgument, e.what());
-  } catch (const std::exception& e) {
-    return api_fail(kErrCuda, e.what());
-  }
-}
-
-void check(bool ok, const char* what) {
-  if (!ok) throw std::invalid_argument(what);
-}
 
 NodeArgs node_args(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
                    long long pStrideB, long long pStrideU, const int* frames, const int* positions, int B,
@@ -49,14 +29,6 @@ void check_temperature(double t) {
   // (it and its reciprocal are used in 32 bits)
   check(t > 0.0 && t <= 1e30 && std::isfinite((float)(1.4426950408889634 / t)),
         "temperature must be positive, at least 1e-38 and at most 1e30");
-}
-
-void need(size_t have, size_t want, const void* p, const char* what) {
-  if (want > 0 && (p == nullptr || have < want))
-    throw std::invalid_argument(std::string(what) + " too small: need " + std::to_string(want) + " bytes, got " +
-                                std::to_string(have));
-  if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
-    throw std::invalid_argument(std::string(what) + " must be 16-byte aligned");
 }
 
 }  // namespace
@@ -119,6 +91,21 @@ int tb200_sample_words(const void* E, const void* P, int bf16, long long eStride
     check(topP > 0.0 && topP <= 1.0, "top_p must be above 0 and at most 1");
     check(minP >= 0.0 && minP <= 1.0, "min_p must be between 0 and 1");
     launch_sample_words(a, uniforms, words, logProbs, SampleRule{temperature, topK, topP, minP}, api_stream());
+  });
+}
+
+size_t tb200_extend_beams_workspace_bytes(int B, int V, int N) { return extend_workspace_bytes(B, V, N); }
+
+int tb200_extend_beams(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
+                       long long pStrideB, long long pStrideU, const int* frames, const int* positions,
+                       const float* scores, float* outScores, int* parents, int* words, int B, int maxT, int maxU,
+                       int V, int N, int width, void* workspace, size_t workspaceBytes) {
+  return guarded([&] {
+    const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
+                                 maxU, V, N);
+    check(width >= 1 && width <= kMaxListedWords, "the number of extensions must be between 1 and 256");
+    need(workspaceBytes, extend_workspace_bytes(B, V, N), workspace, "workspace");
+    launch_extend_beams(a, scores, outScores, parents, words, width, workspace, api_stream());
   });
 }
 

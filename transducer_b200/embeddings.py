@@ -1,0 +1,123 @@
+"""Rows of a table for words (`embed_words`): a prediction network's inputs, or the predictions themselves where
+they depend on the word before alone.  The reference starts from given predictions and has no counterpart.
+
+CUDA tensors only, like `TransducerLoss`; the work is enqueued on torch's current stream."""
+import math
+
+import torch
+
+from . import _transducer
+from .nodes import OnDevice, check_device, check_no_tangents
+from .torch_binding import _workspace, check_contiguous, check_dim, check_type
+
+
+class WordEmbedding(torch.autograd.Function):
+    """Autograd node for the rows."""
+
+    @staticmethod
+    def forward(ctx, table, words, scale, dropout, seed, validate_words):
+        if table.stride(1) != 1 and table.shape[1] != 1:
+            table = table.contiguous()
+        R, H = table.shape
+        device = table.device
+        bf16 = table.dtype is torch.bfloat16
+        numbers, place = _seed(seed)
+        with OnDevice(device):
+            rows = torch.empty(tuple(words.shape) + (H,), device=device, dtype=table.dtype)
+            _transducer.embed_words(table.data_ptr(), bf16, table.stride(0), words.data_ptr(), words.numel(),
+                                    rows.data_ptr(), R, H, scale, dropout, numbers, place)
+            if validate_words:
+                certify_words(words, R)
+        ctx.save_for_backward(words, seed if place else None)
+        ctx.rest = (R, H, bf16, scale, dropout, numbers)
+        return rows
+
+    @staticmethod
+    def backward(ctx, deltas):
+        words, seed = ctx.saved_tensors
+        R, H, bf16, scale, dropout, numbers = ctx.rest
+        deltas = deltas.contiguous()
+        device = deltas.device
+        with OnDevice(device):
+            grad = torch.empty((R, H), device=device, dtype=deltas.dtype)
+            nbytes = _transducer.embed_backward_workspace_bytes(words.numel(), R, H)
+            ws = _workspace(nbytes, device)
+            _transducer.embed_backward(deltas.data_ptr(), bf16, words.data_ptr(), words.numel(), grad.data_ptr(),
+                                       R, H, scale, dropout, numbers, 0 if seed is None else seed.data_ptr(),
+                                       ws.data_ptr(), nbytes)
+        if torch.is_grad_enabled():   # (somebody wants to differentiate it)
+            grad = Once.apply(grad, deltas)
+        return (grad,) + (None,) * 5
+
+
+class Once(torch.autograd.Function):
+    """A gradient that is not differentiable again: asking for it is an error, not 0."""
+
+    @staticmethod
+    def forward(ctx, grad, deltas):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *deltas):
+        raise RuntimeError("embedded words are differentiable once only")
+
+
+def _seed(seed):
+    """The seed as a number, and the address of one on the device (0: none)."""
+    if isinstance(seed, torch.Tensor):
+        return 0, seed.data_ptr()
+    return 0 if seed is None else seed, 0
+
+
+def certify_words(words, R):
+    """That no word lies beyond the table; see nodes.certify_indices."""
+    if words.numel() == 0:
+        return
+    scratch = torch.empty(_transducer.node_summary_scratch_bytes, dtype=torch.uint8, device=words.device)
+    most = _transducer.node_summary(0, 0, 0, words.data_ptr(), words.numel(), scratch.data_ptr())[2]
+    if most >= R:
+        raise ValueError("Word index mismatch")
+
+
+def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=True):
+    """The rows of ``table`` (float32 or bfloat16 [R, H]) for ``words`` (int32, any shape), times ``scale``:
+    a tensor [*words.shape, H] of the table's type.  A negative word has a row of zeros.
+
+    With ``dropout`` above 0 that share of the numbers, to the nearest 65536th, is dropped and the others
+    are divided by what is left of 1.  Which ones follows from ``seed`` and a number's place alone (Philox4x32-10; the C
+    ABI's header says how), so that no mask is stored, and the same seed drops the same places: take
+    another one for every call.  It is a whole number, or one int64 on the device, which is read when the kernels run: a
+    captured call whose seed is written between its replays drops other numbers each time.
+
+    Differentiable once w.r.t. the table: the gradient is dense, its sums are made in fp32 in the words'
+    order and are the same bits from run to run.  ``validate_words=False`` skips the check that no word is R or
+    more (such ones have rows of zeros), which waits for the kernels, so that the call only enqueues work and
+    can be captured in a CUDA graph (its backward pass by torch.autograd.grad).
+
+    Previous words of transcripts, as a prediction network takes them (0: the start symbol)::
+
+        n = torch.arange(U + 1, device=labels.device)
+        words = torch.nn.functional.pad(labels, (1, 0))
+        words = words.masked_fill(n > label_lengths[:, None], -1)
+    """
+    check_dim(table, 2, "table")
+    if table.dtype is not torch.bfloat16:
+        check_type(table, torch.float32, "table")
+    check_type(words, torch.int32, "words")
+    check_contiguous(words, "words")
+    check_device(table, words)
+    check_no_tangents(table)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not 0.0 <= dropout < 1.0:
+        raise ValueError("dropout must be at least 0 and below 1")
+    if dropout > 0.0 and seed is None:
+        raise ValueError("dropout needs a seed")
+    if isinstance(seed, torch.Tensor):
+        check_type(seed, torch.int64, "seed")
+        if seed.numel() != 1:
+            raise ValueError("seed must be one number")
+        check_device(table, seed)
+    elif seed is not None and not -2 ** 63 <= seed < 2 ** 63:
+        raise ValueError("seed must fit 64 bits")
+    return WordEmbedding.apply(table, words, scale, dropout, seed, validate_words)
