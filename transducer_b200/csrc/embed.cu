@@ -16,17 +16,6 @@ namespace {
 
 constexpr int kWarps = 8, kGroup = 8;   // numbers of one counter, all in one lane
 
-// Philox4x32-10 (Salmon, Moraes, Dror and Shaw: Parallel random numbers: as easy as 1, 2, 3; SC 2011).
-__device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const unsigned long long a = 0xd2511f53ull * c.x, b = 0xcd9e8d57ull * c.z;
-    c = make_uint4((unsigned)(b >> 32) ^ c.y ^ k0, (unsigned)b, (unsigned)(a >> 32) ^ c.w ^ k1, (unsigned)a);
-    k0 += 0x9e3779b9u, k1 += 0xbb67ae85u;
-  }
-  return c;
-}
-
 struct Seed {
   unsigned low, high;
   __device__ __forceinline__ explicit Seed(const EmbedArgs& a) {
@@ -35,17 +24,20 @@ struct Seed {
   }
 };
 
-// Bit i: number i of the group stays.
-__device__ __forceinline__ unsigned kept(i64 n, int group, Seed seed, unsigned dropped) {
-  const uint4 x = philox(make_uint4((unsigned)n, (unsigned)((unsigned long long)n >> 32), group, 0), seed.low, seed.high);
-  const unsigned u[4] = {x.x, x.y, x.z, x.w};
-  unsigned bits = 0;
+// Philox4x32-10 (Salmon, Moraes, Dror and Shaw: Parallel random numbers: as easy as 1, 2, 3; SC 2011) of several counters
+// at once, which share the rounds' keys.
+template <int K>
+__device__ __forceinline__ void philox(uint4 (&c)[K], Seed key) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    bits |= (u[i] & 0xffffu) >= dropped ? 1u << 2 * i : 0u;
-    bits |= u[i] >> 16 >= dropped ? 2u << 2 * i : 0u;
+  for (int i = 0; i < 10; ++i) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const unsigned long long a = (unsigned long long)c[k].x * 0xd2511f53u, b = (unsigned long long)c[k].z * 0xcd9e8d57u;
+      c[k] = make_uint4((unsigned)(b >> 32) ^ c[k].y ^ key.low, (unsigned)b,
+                        (unsigned)(a >> 32) ^ c[k].w ^ key.high, (unsigned)a);
+    }
+    key.low += 0x9e3779b9u, key.high += 0xbb67ae85u;
   }
-  return bits;
 }
 
 // The numbers of a row that a lane of a warp has, of 256 that begin at `first`: eight that follow each other where rows
@@ -82,16 +74,41 @@ struct Numbers {
   }
 };
 
-// Bit i: number i that a lane has of row n stays.  All lanes: each makes the bits of a whole counter.
+// Which of its numbers of a row a lane keeps: bits of the generator to be compared with 2^16 `dropped`, the
+// number of row n and 256 that begin at `first`.  All lanes: each makes the bits of a whole counter.
 template <int VEC>
-__device__ __forceinline__ unsigned stays(i64 n, int first, int lane, Seed seed, unsigned dropped) {
-  const unsigned mine = kept(n, first / kGroup + lane, seed, dropped);
-  if constexpr (VEC > 1) return mine;
-  unsigned bits = 0;
+struct Stays {
+  uint4 bits;   // VEC == 1: bit i of x for number i
+  __device__ __forceinline__ bool operator()(int i, unsigned dropped) const {
+    if constexpr (VEC == 1) return bits.x >> i & 1;
+    const unsigned u = i / 2 == 0 ? bits.x : i / 2 == 1 ? bits.y : i / 2 == 2 ? bits.z : bits.w;
+    return (i % 2 == 0 ? u << 16 : u) >= dropped << 16;   // (what is below the upper half's last bit tells equals apart: >=)
+  }
+};
+template <int VEC, int K, typename N>
+__device__ __forceinline__ void stays(Stays<VEC> (&out)[K], N place, int first, int lane, Seed seed, unsigned dropped) {
+  uint4 c[K];
 #pragma unroll
-  for (int i = 0; i < kGroup; ++i)
-    bits |= (__shfl_sync(0xffffffffu, mine, 4 * i + lane / kGroup) >> lane % kGroup & 1) << i;
-  return bits;
+  for (int k = 0; k < K; ++k) {
+    const unsigned long long n = place(k);
+    c[k] = make_uint4((unsigned)n, (unsigned)(n >> 32), first / kGroup + lane, 0);
+  }
+  philox(c, seed);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if constexpr (VEC == 1) {
+      const Stays<2> whole{c[k]};
+      unsigned mine = 0, bits = 0;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) mine |= whole(i, dropped) ? 1u << i : 0u;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i)
+        bits |= (__shfl_sync(0xffffffffu, mine, 4 * i + lane / kGroup) >> lane % kGroup & 1) << i;
+      out[k].bits.x = bits;
+    } else {
+      out[k].bits = c[k];
+    }
+  }
 }
 
 // A warp writes 256 numbers of each of ROWS rows that follow each other.
@@ -109,16 +126,16 @@ __global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __re
   for (int k = 0; k < ROWS; ++k)
     if ((unsigned)r[k] < (unsigned)a.R) x[k].load(static_cast<const T*>(a.table) + r[k] * a.stride, first, lane, a.H);
     else x[k].clear();
+  Stays<VEC> stay[ROWS];
+  if constexpr (DROP)
+    stays<VEC, ROWS>(stay, [&](int k) { return n0 + k; }, first, lane, Seed(a), a.dropped);
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
     if (n0 + k >= a.N) break;
     float y[kGroup];
     x[k].get(y);
-    unsigned stay = (unsigned)r[k] < (unsigned)a.R ? 0xff : 0;
-    if constexpr (DROP)
-      if (stay) stay = stays<VEC>(n0 + k, first, lane, Seed(a), a.dropped);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) y[i] = stay >> i & 1 ? y[i] * a.factor : 0.0f;
+    for (int i = 0; i < kGroup; ++i) y[i] = !DROP || stay[k](i, a.dropped) ? y[i] * a.factor : 0.0f;
     Numbers<T, VEC>::store(rows + (n0 + k) * a.H, first, lane, a.H, y);
   }
 }
@@ -127,56 +144,66 @@ __global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __re
 
 constexpr int kSortWarps = 32, kSortRows = 256;   // rows per CTA
 
-// A word and its place; places [start[r], start[r + 1]) of the order are row r's.
+// Words and their places, all of a word next to each other and in order.  Which word comes first does not matter.
 struct Sorted {
   int2* order;   // (place, word), [N]
-  int* start;    // [R + 1]
+  int2* range;   // [R] where a row's begin and end; behind them how many there are in all
+  int R;
+  __device__ __forceinline__ int all() const { return range[R].x; }
 };
 
-// CTA c has the rows from c * rows on.  Every CTA goes through all words: it counts those of lower rows, which tells where
-// its own begin, and per warp those of each of its rows; then every warp puts the places of its words where they belong.
-__global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* __restrict__ words, i64 N, int R, int rows,
+// CTA c of 2^bits has the rows r with r mod 2^bits = c, so that frequent words that follow each other in the table are not
+// all its own.  Every CTA goes through all words: it counts those of the CTAs before it, which tells where its own begin, and
+// per warp those of each of its rows; then every warp puts the places of its words where they belong.
+__global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* __restrict__ words, int N, int bits,
                                                                      Sorted out) {
   constexpr int kBatch = 16;   // words on their way at a time, per lane
   __shared__ int count[kSortWarps][kSortRows];
   __shared__ int total[kSortRows];
   __shared__ int below;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int lo = blockIdx.x * rows, mine = min(rows, R - lo);
+  const int cta = blockIdx.x, low = (1 << bits) - 1;
   cudaTriggerProgrammaticLaunchCompletion();
   for (int i = tid; i < kSortWarps * kSortRows; i += 32 * kSortWarps) (&count[0][0])[i] = 0;
   if (tid == 0) below = 0;
   __syncthreads();
-  const i64 seg = round_up64(div_up64(N, kSortWarps), 32);
-  const i64 first = warp * seg, end = min(N, first + seg);
-  // f(words, places of the first) for the warp's words, 32 that follow each other at a time, in order
+  const int seg = (int)round_up64(div_up(N, kSortWarps), 32);
+  const int first = (int)min((i64)N, (i64)warp * seg), end = (int)min((i64)N, (i64)first + seg);
+  // f(word or -1, place of the first) for the warp's words, 32 that follow each other at a time, in order
   auto each = [&](auto f) {
+    int n = first;
 #pragma unroll 1
-    for (i64 n = first; n < end; n += 32 * kBatch) {
+    for (; end - n >= 32 * kBatch; n += 32 * kBatch) {
       int r[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) r[j] = n + 32 * j + lane < end ? words[n + 32 * j + lane] : -1;
+      for (int j = 0; j < kBatch; ++j) r[j] = words[n + 32 * j + lane];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) f(r[j], n + 32 * j);
     }
+#pragma unroll 4
+    for (; n < end; n += 32) f(lane < end - n ? words[n + lane] : -1, n);
   };
+  auto counts = [&](int r) { return (unsigned)r < (unsigned)out.R; };
   int lower = 0;
-  each([&](int r, i64) {
-    lower += (unsigned)r < (unsigned)lo ? 1 : 0;
-    if ((unsigned)r - (unsigned)lo < (unsigned)mine) atomicAdd(&count[warp][r - lo], 1);
+  each([&](int r, int) {
+    const int c = r & low;
+    if (counts(r) && c <= cta) {
+      if (c < cta) ++lower;
+      else atomicAdd(&count[warp][r >> bits], 1);
+    }
   });
   lower = __reduce_add_sync(0xffffffffu, lower);
   if (lane == 0) atomicAdd(&below, lower);
   __syncthreads();
+  int mine = 0;   // of row tid
   if (tid < kSortRows) {
-    int sum = 0;
 #pragma unroll 8
     for (int w = 0; w < kSortWarps; ++w) {
       const int c = count[w][tid];
-      count[w][tid] = sum;
-      sum += c;
+      count[w][tid] = mine;
+      mine += c;
     }
-    total[tid] = sum;
+    total[tid] = mine;
   }
   __syncthreads();
   if (warp == 0) {   // (the rows' sums to where each begins)
@@ -192,23 +219,25 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* 
     before += below - all;
 #pragma unroll
     for (int i = 0; i < kSortRows / 32; ++i) total[lane * (kSortRows / 32) + i] = before + sum[i];
-    if (lane == 31 && lo + mine == R) out.start[R] = before + all;
+    if (lane == 31 && cta == low) out.range[out.R] = make_int2(before + all, 0);
   }
   __syncthreads();
-  if (tid < mine) out.start[lo + tid] = total[tid];
+  if (tid < kSortRows && ((i64)tid << bits) + cta < out.R)
+    out.range[(tid << bits) + cta] = make_int2(total[tid], total[tid] + mine);
   int* const at = count[warp];
-  for (int i = lane; i < mine; i += 32) at[i] += total[i];
+#pragma unroll
+  for (int i = lane; i < kSortRows; i += 32) at[i] += total[i];
   __syncwarp();
-  each([&](int r, i64 n) {
-    const bool in = (unsigned)r - (unsigned)lo < (unsigned)mine;
+  each([&](int r, int n) {
+    const bool in = counts(r) && (r & low) == cta;
     const unsigned any = __ballot_sync(0xffffffffu, in);
     if (!in) return;
     const unsigned same = __match_any_sync(any, r);
     const int rank = __popc(same & ((1u << lane) - 1));
-    const int base = at[r - lo];
+    const int base = at[r >> bits];
     __syncwarp(any);
-    out.order[base + rank] = make_int2((int)n + lane, r);
-    if (rank == 0) at[r - lo] = base + __popc(same);
+    out.order[base + rank] = make_int2(n + lane, r);
+    if (rank == 0) at[r >> bits] = base + __popc(same);
     __syncwarp(any);
   });
 }
@@ -232,14 +261,16 @@ constexpr int kMostPart = 32;
 template <typename T, int VEC, bool DROP>
 __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
                                                                  Parts parts, T* __restrict__ grad) {
-  constexpr int kBatch = 8;   // rows on their way at a time
+  constexpr int kBatch = 8, kAtOnce = 4;   // rows on their way at a time, and counters
   const i64 id = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const i64 fill = id - parts.items * parts.pieces;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   if (fill >= 0) {
-    if (fill >= a.R || s.start[fill] != s.start[fill + 1]) return;
+    if (fill >= a.R) return;
+    const int2 range = s.range[fill];
+    if (range.x != range.y) return;
     const float zero[kGroup] = {};
     for (int first = 0; first < a.H; first += 32 * kGroup)
       Numbers<T, VEC>::store(grad + fill * a.H, first, lane, a.H, zero);
@@ -247,7 +278,7 @@ __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, co
   }
   const i64 item = id / parts.pieces;
   const int piece = (int)(id % parts.pieces), first = piece * 32 * kGroup;
-  const int from = (int)(item * parts.part), all = s.start[a.R];
+  const int from = (int)(item * parts.part), all = s.all();
   if (from >= all) return;
   const int to = (int)min((i64)from + parts.part, (i64)all);
   // lane i: the item's place i; the rows before it and behind it
@@ -272,6 +303,7 @@ __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, co
 #pragma unroll 1
   for (int i = 0; i < to - from; i += kBatch) {
     Numbers<T, VEC> x[kBatch];
+    Stays<VEC> stay[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int n = __shfl_sync(0xffffffffu, mine.x, i + j);
@@ -280,7 +312,11 @@ __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, co
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (i + j >= to - from) break;
-      const int n = __shfl_sync(0xffffffffu, mine.x, i + j), r = __shfl_sync(0xffffffffu, mine.y, i + j);
+      if constexpr (DROP)
+        if (j % kAtOnce == 0)
+          stays<VEC, kAtOnce>(stay, [&](int k) { return __shfl_sync(0xffffffffu, mine.x, (i + j + k) & 31); }, first, lane,
+                              seed, a.dropped);
+      const int r = __shfl_sync(0xffffffffu, mine.y, i + j);
       if (r != row) {
         finish(false);
 #pragma unroll
@@ -289,10 +325,9 @@ __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, co
       }
       float y[kGroup];
       x[j].get(y);
-      unsigned stay = 0xff;
-      if constexpr (DROP) stay = stays<VEC>(n, first, lane, seed, a.dropped);
 #pragma unroll
-      for (int k = 0; k < kGroup; ++k) sum[k] += stay >> k & 1 ? y[k] : 0.0f;
+      for (int k = 0; k < kGroup; ++k)
+        if (!DROP || stay[j % kAtOnce](k, a.dropped)) sum[k] += y[k];
     }
   }
   finish(true);
@@ -308,24 +343,40 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const i64 base = (i64)blockIdx.x * kWarps;
   cudaGridDependencySynchronize();
-  // the row that warp w begins, or -1
-  auto row_of = [&](int w, int& slot, i64& items) {
-    const i64 item = (base + w) / parts.pieces;
-    const i64 last = item * parts.part + parts.part - 1;
-    if (item >= parts.items || last >= s.start[a.R]) return -1;
-    const int r = s.order[last].y, from = s.start[r];
-    items = (s.start[r + 1] - 1) / parts.part - item + 1;
-    slot = from % parts.part == 0 ? 0 : 1;
-    return from / parts.part == item && items > 1 ? r : -1;
+  // (items that follow each other, of one piece: rows of many items are in different CTAs)
+  struct Row {
+    int row, slot, piece;   // -1: none begins in the item
+    i64 item, items;
   };
-  // items [from, to) of the row, the first of them at `slot`
-  auto add = [&](i64 item, int piece, int slot, i64 from, i64 to, float (&sum)[kGroup]) {
-#pragma unroll 8
-    for (i64 i = from; i < to; ++i) {
-      const float4* p = parts.at(item + i, i == 0 ? slot : 0, piece, lane);
-      const float4 x = p[0], y = p[1];
-      sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
-      sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
+  auto row_of = [&](int w) {
+    Row x{-1, 0, (int)((base + w) / parts.items), (base + w) % parts.items, 0};
+    const i64 last = x.item * parts.part + parts.part - 1;
+    if (x.piece >= parts.pieces || last >= s.all()) return x;
+    const int r = s.order[last].y;
+    const int2 range = s.range[r];
+    x.items = (range.y - 1) / parts.part - x.item + 1;
+    x.slot = range.x % parts.part == 0 ? 0 : 1;
+    if (range.x / parts.part == x.item && x.items > 1) x.row = r;
+    return x;
+  };
+  // the row's shares of its items [from, to)
+  auto add = [&](const Row& row, i64 from, i64 to, float (&sum)[kGroup]) {
+    constexpr int kBatch = 8;
+#pragma unroll 1
+    for (i64 i = from; i < to; i += kBatch) {
+      float4 x[kBatch][2];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i + j < to) {
+          const float4* p = parts.at(row.item + i + j, i + j == 0 ? row.slot : 0, row.piece, lane);
+          x[j][0] = p[0], x[j][1] = p[1];
+        }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i + j < to) {
+          sum[0] += x[j][0].x, sum[1] += x[j][0].y, sum[2] += x[j][0].z, sum[3] += x[j][0].w;
+          sum[4] += x[j][1].x, sum[5] += x[j][1].y, sum[6] += x[j][1].z, sum[7] += x[j][1].w;
+        }
     }
   };
   auto write = [&](int r, int piece, float (&sum)[kGroup]) {
@@ -333,25 +384,21 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
     for (int k = 0; k < kGroup; ++k) sum[k] *= a.factor;
     Numbers<T, VEC>::store(grad + (i64)r * a.H, piece * 32 * kGroup, lane, a.H, sum);
   };
-  int slot = 0;
-  i64 items = 0;
-  const int r = row_of(warp, slot, items);
-  if (lane == 0) many[warp] = r >= 0 && items >= kMany;
-  if (r >= 0 && items < kMany) {
+  const Row own = row_of(warp);
+  if (lane == 0) many[warp] = own.row >= 0 && own.items >= kMany;
+  if (own.row >= 0 && own.items < kMany) {
     float sum[kGroup] = {};
-    add((base + warp) / parts.pieces, (int)((base + warp) % parts.pieces), slot, 0, items, sum);
-    write(r, (int)((base + warp) % parts.pieces), sum);
+    add(own, 0, own.items, sum);
+    write(own.row, own.piece, sum);
   }
   __syncthreads();
 #pragma unroll 1
   for (int w = 0; w < kWarps; ++w) {
     if (!many[w]) continue;
-    const int row = row_of(w, slot, items);
-    const i64 item = (base + w) / parts.pieces;
-    const int piece = (int)((base + w) % parts.pieces);
-    const i64 share = div_up64(items, kWarps);
+    const Row row = row_of(w);
+    const i64 share = div_up64(row.items, kWarps);
     float sum[kGroup] = {};
-    add(item, piece, slot, warp * share, min(items, (warp + 1) * share), sum);
+    add(row, warp * share, min(row.items, (warp + 1) * share), sum);
     shares[warp][lane][0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
     shares[warp][lane][1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
     __syncthreads();
@@ -364,7 +411,7 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
         sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
         sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
       }
-      write(row, piece, sum);
+      write(row.row, row.piece, sum);
     }
     __syncthreads();
   }
@@ -428,7 +475,7 @@ void launch_embed_words(const EmbedArgs& a, void* rows, cudaStream_t stream) {
 size_t embed_backward_workspace_bytes(i64 N, int R, int H) {
   if (N <= 0 || R <= 0 || H <= 0) return 0;
   const int pieces = div_up(H, 32 * kGroup);
-  return (size_t)(round_up64(N * 8, 16) + round_up64((R + 1ll) * 4, 16) +
+  return (size_t)(round_up64(N * 8, 16) + round_up64((R + 1ll) * 8, 16) +
                   div_up64(N, places_per_item(N, pieces)) * 2 * pieces * 32 * kGroup * 4);
 }
 
@@ -443,12 +490,14 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
   char* at = static_cast<char*>(workspace);
   Sorted s;
   s.order = reinterpret_cast<int2*>(at), at += round_up64(a.N * 8, 16);
-  s.start = reinterpret_cast<int*>(at), at += round_up64((a.R + 1ll) * 4, 16);
+  s.range = reinterpret_cast<int2*>(at), at += round_up64((a.R + 1ll) * 8, 16);
+  s.R = a.R;
   const Parts parts{reinterpret_cast<float*>(at), part, pieces, div_up64(a.N, part)};
   {
-    const int rows = std::max(1, std::min(kSortRows, div_up(a.R, 148)));
+    int bits = 0;   // CTAs: up to 128, and no more than 256 rows each
+    while ((bits < 7 && 2 << bits <= a.R) || (i64)kSortRows << bits < a.R) ++bits;
     ScopedKernel prof("embed_sort", stream);
-    sort_words_kernel<<<div_up(a.R, rows), 32 * kSortWarps, 0, stream>>>(a.words, a.N, a.R, rows, s);
+    sort_words_kernel<<<1u << bits, 32 * kSortWarps, 0, stream>>>(a.words, (int)a.N, bits, s);
     TB200_CHECK_LAUNCH();
   }
   EmbedArgs d = a;
