@@ -79,10 +79,15 @@ struct Numbers {
 template <int VEC>
 struct Stays {
   uint4 bits;   // VEC == 1: bit i of x for number i
-  __device__ __forceinline__ bool operator()(int i, unsigned dropped) const {
-    if constexpr (VEC == 1) return bits.x >> i & 1;
-    const unsigned u = i / 2 == 0 ? bits.x : i / 2 == 1 ? bits.y : i / 2 == 2 ? bits.z : bits.w;
-    return (i % 2 == 0 ? u << 16 : u) >= dropped << 16;   // (what is below the upper half's last bit tells equals apart: >=)
+  __device__ __forceinline__ void get(bool (&stay)[kGroup], unsigned dropped) const {
+    if constexpr (VEC == 1) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) stay[i] = bits.x >> i & 1;
+    } else {
+      const unsigned u[4] = {bits.x, bits.y, bits.z, bits.w}, least = dropped * 0x10001u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) __vibmax_u16x2(u[i], least, &stay[2 * i + 1], &stay[2 * i]);
+    }
   }
 };
 template <int VEC, int K, typename N>
@@ -98,9 +103,11 @@ __device__ __forceinline__ void stays(Stays<VEC> (&out)[K], N place, int first, 
   for (int k = 0; k < K; ++k) {
     if constexpr (VEC == 1) {
       const Stays<2> whole{c[k]};
+      bool stay[kGroup];
+      whole.get(stay, dropped);
       unsigned mine = 0, bits = 0;
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) mine |= whole(i, dropped) ? 1u << i : 0u;
+      for (int i = 0; i < kGroup; ++i) mine |= stay[i] ? 1u << i : 0u;
 #pragma unroll
       for (int i = 0; i < kGroup; ++i)
         bits |= (__shfl_sync(0xffffffffu, mine, 4 * i + lane / kGroup) >> lane % kGroup & 1) << i;
@@ -133,16 +140,27 @@ __global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __re
   for (int k = 0; k < ROWS; ++k) {
     if (n0 + k >= a.N) break;
     float y[kGroup];
+    bool keep[kGroup] = {true, true, true, true, true, true, true, true};
     x[k].get(y);
+    if constexpr (DROP) stay[k].get(keep, a.dropped);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) y[i] = !DROP || stay[k](i, a.dropped) ? y[i] * a.factor : 0.0f;
+    for (int i = 0; i < kGroup; ++i) y[i] = keep[i] ? y[i] * a.factor : 0.0f;
     Numbers<T, VEC>::store(rows + (n0 + k) * a.H, first, lane, a.H, y);
   }
 }
 
 // ---- the words' places in the order of the words ------------------------------------------------
 
-constexpr int kSortWarps = 32, kSortRows = 256;   // rows per CTA
+constexpr int kSortRows = 256;   // of a CTA
+// Words of a warp's that are its CTA's are listed; where there are more it looks again.
+constexpr int kSortListed = 1024;
+template <int WARPS>
+struct SortRoom {
+  int count[WARPS][kSortRows];
+  int total[kSortRows];
+  int below;
+  unsigned listed[WARPS][kSortListed];   // (place behind the warp's first, row of the CTA's)
+};
 
 // Words and their places, all of a word next to each other and in order.  Which word comes first does not matter.
 struct Sorted {
@@ -154,20 +172,23 @@ struct Sorted {
 
 // CTA c of 2^bits has the rows r with r mod 2^bits = c, so that frequent words that follow each other in the table are not
 // all its own.  Every CTA goes through all words: it counts those of the CTAs before it, which tells where its own begin, and
-// per warp those of each of its rows; then every warp puts the places of its words where they belong.
-__global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* __restrict__ words, int N, int bits,
-                                                                     Sorted out) {
+// per warp those of each of its rows, which it lists; then every warp puts the places of its words where they belong.
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __restrict__ words, int N, int bits, Sorted out) {
   constexpr int kBatch = 16;   // words on their way at a time, per lane
-  __shared__ int count[kSortWarps][kSortRows];
-  __shared__ int total[kSortRows];
-  __shared__ int below;
+  extern __shared__ __align__(16) char shared[];
+  SortRoom<WARPS>& room = *reinterpret_cast<SortRoom<WARPS>*>(shared);
+  auto& count = room.count;
+  auto& total = room.total;
+  auto& listed = room.listed;
+  int& below = room.below;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cta = blockIdx.x, low = (1 << bits) - 1;
   cudaTriggerProgrammaticLaunchCompletion();
-  for (int i = tid; i < kSortWarps * kSortRows; i += 32 * kSortWarps) (&count[0][0])[i] = 0;
+  for (int i = tid; i < WARPS * kSortRows; i += 32 * WARPS) (&count[0][0])[i] = 0;
   if (tid == 0) below = 0;
   __syncthreads();
-  const int seg = (int)round_up64(div_up(N, kSortWarps), 32);
+  const int seg = (int)round_up64(div_up(N, WARPS), 32);
   const int first = (int)min((i64)N, (i64)warp * seg), end = (int)min((i64)N, (i64)first + seg);
   // f(word or -1, place of the first) for the warp's words, 32 that follow each other at a time, in order
   auto each = [&](auto f) {
@@ -183,14 +204,20 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* 
 #pragma unroll 4
     for (; n < end; n += 32) f(lane < end - n ? words[n + lane] : -1, n);
   };
-  auto counts = [&](int r) { return (unsigned)r < (unsigned)out.R; };
-  int lower = 0;
-  each([&](int r, int) {
-    const int c = r & low;
-    if (counts(r) && c <= cta) {
-      if (c < cta) ++lower;
-      else atomicAdd(&count[warp][r >> bits], 1);
+  const unsigned before = (1u << lane) - 1;
+  int lower = 0, found = 0;
+  each([&](int r, int n) {
+    const bool is = (unsigned)r < (unsigned)out.R;
+    lower += is && (r & low) < cta ? 1 : 0;
+    const bool in = is && (r & low) == cta;
+    const unsigned any = __ballot_sync(0xffffffffu, in);
+    if (any == 0) return;
+    if (in) {
+      atomicAdd(&count[warp][r >> bits], 1);
+      const int i = found + __popc(any & before);
+      if (i < kSortListed) listed[warp][i] = (unsigned)(n + lane - first) << 8 | (unsigned)(r >> bits);
     }
+    found += __popc(any);
   });
   lower = __reduce_add_sync(0xffffffffu, lower);
   if (lane == 0) atomicAdd(&below, lower);
@@ -198,7 +225,7 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* 
   int mine = 0;   // of row tid
   if (tid < kSortRows) {
 #pragma unroll 8
-    for (int w = 0; w < kSortWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const int c = count[w][tid];
       count[w][tid] = mine;
       mine += c;
@@ -210,16 +237,16 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* 
     int sum[kSortRows / 32], all = 0;
 #pragma unroll
     for (int i = 0; i < kSortRows / 32; ++i) sum[i] = all, all += total[lane * (kSortRows / 32) + i];
-    int before = all;
+    int upto = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += x;
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
-    before += below - all;
+    upto += below - all;
 #pragma unroll
-    for (int i = 0; i < kSortRows / 32; ++i) total[lane * (kSortRows / 32) + i] = before + sum[i];
-    if (lane == 31 && cta == low) out.range[out.R] = make_int2(before + all, 0);
+    for (int i = 0; i < kSortRows / 32; ++i) total[lane * (kSortRows / 32) + i] = upto + sum[i];
+    if (lane == 31 && cta == low) out.range[out.R] = make_int2(upto + all, 0);
   }
   __syncthreads();
   if (tid < kSortRows && ((i64)tid << bits) + cta < out.R)
@@ -228,18 +255,26 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_words_kernel(const int* 
 #pragma unroll
   for (int i = lane; i < kSortRows; i += 32) at[i] += total[i];
   __syncwarp();
-  each([&](int r, int n) {
-    const bool in = counts(r) && (r & low) == cta;
+  auto put = [&](int r, int n, bool in) {
     const unsigned any = __ballot_sync(0xffffffffu, in);
     if (!in) return;
     const unsigned same = __match_any_sync(any, r);
-    const int rank = __popc(same & ((1u << lane) - 1));
+    const int rank = __popc(same & before);
     const int base = at[r >> bits];
     __syncwarp(any);
-    out.order[base + rank] = make_int2(n + lane, r);
+    out.order[base + rank] = make_int2(n, r);
     if (rank == 0) at[r >> bits] = base + __popc(same);
     __syncwarp(any);
-  });
+  };
+  if (found <= kSortListed && seg <= 1 << 24) {
+#pragma unroll 1
+    for (int i = 0; i < found; i += 32) {
+      const unsigned x = i + lane < found ? listed[warp][i + lane] : 0;
+      put((int)(x & 255) << bits | cta, first + (int)(x >> 8), i + lane < found);
+    }
+  } else {
+    each([&](int r, int n) { put(r, n + lane, (unsigned)r < (unsigned)out.R && (r & low) == cta); });
+  }
 }
 
 // ---- the gradient -------------------------------------------------------------------------------
@@ -255,25 +290,27 @@ struct Parts {
   }
 };
 
-constexpr int kMostPart = 32;
+constexpr int kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
 
-// The first items * pieces warps add up 256 numbers of an item's rows each; the others fill a row that no word has.
+// The first items * pieces warps add up 256 numbers of an item's rows each; the others fill rows that no word has.
 template <typename T, int VEC, bool DROP>
-__global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
+__global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
                                                                  Parts parts, T* __restrict__ grad) {
-  constexpr int kBatch = 8, kAtOnce = 4;   // rows on their way at a time, and counters
+  constexpr int kBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows on their way while as many are added (more: registers)
   const i64 id = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const i64 fill = id - parts.items * parts.pieces;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   if (fill >= 0) {
-    if (fill >= a.R) return;
-    const int2 range = s.range[fill];
-    if (range.x != range.y) return;
+    const i64 mine = fill * kFilled + lane;
+    int2 range = make_int2(0, 1);
+    if (lane < kFilled && mine < a.R) range = s.range[mine];
+    unsigned empty = __ballot_sync(0xffffffffu, range.x == range.y);
     const float zero[kGroup] = {};
-    for (int first = 0; first < a.H; first += 32 * kGroup)
-      Numbers<T, VEC>::store(grad + fill * a.H, first, lane, a.H, zero);
+    for (; empty; empty &= empty - 1)
+      for (int first = 0; first < a.H; first += 32 * kGroup)
+        Numbers<T, VEC>::store(grad + (fill * kFilled + __ffs(empty) - 1) * a.H, first, lane, a.H, zero);
     return;
   }
   const i64 item = id / parts.pieces;
@@ -300,22 +337,28 @@ __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, co
       p[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
     }
   };
-#pragma unroll 1
-  for (int i = 0; i < to - from; i += kBatch) {
-    Numbers<T, VEC> x[kBatch];
-    Stays<VEC> stay[kAtOnce];
+  Numbers<T, VEC> next[kBatch];
+  auto bring = [&](int i) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int n = __shfl_sync(0xffffffffu, mine.x, i + j);
-      if (i + j < to - from) x[j].load(deltas + (i64)n * a.H, first, lane, a.H);
+      const int n = __shfl_sync(0xffffffffu, mine.x, (i + j) & 31);
+      if (i + j < to - from) next[j].load(deltas + (i64)n * a.H, first, lane, a.H);
     }
+  };
+  bring(0);
+#pragma unroll 2
+  for (int i = 0; i < to - from; i += kBatch) {
+    Numbers<T, VEC> x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = next[j];
+    bring(i + kBatch);
+    Stays<VEC> stay[kBatch];
+    if constexpr (DROP)
+      stays<VEC, kBatch>(stay, [&](int k) { return __shfl_sync(0xffffffffu, mine.x, i + k); }, first, lane, seed,
+                         a.dropped);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (i + j >= to - from) break;
-      if constexpr (DROP)
-        if (j % kAtOnce == 0)
-          stays<VEC, kAtOnce>(stay, [&](int k) { return __shfl_sync(0xffffffffu, mine.x, (i + j + k) & 31); }, first, lane,
-                              seed, a.dropped);
       const int r = __shfl_sync(0xffffffffu, mine.y, i + j);
       if (r != row) {
         finish(false);
@@ -324,30 +367,34 @@ __global__ void __launch_bounds__(32 * kWarps) embed_sums_kernel(EmbedArgs a, co
         row = r, begins = false;
       }
       float y[kGroup];
+      bool keep[kGroup] = {true, true, true, true, true, true, true, true};
       x[j].get(y);
+      if constexpr (DROP) stay[j].get(keep, a.dropped);
 #pragma unroll
       for (int k = 0; k < kGroup; ++k)
-        if (!DROP || stay[j % kAtOnce](k, a.dropped)) sum[k] += y[k];
+        if (keep[k]) sum[k] += y[k];
     }
   }
   finish(true);
 }
 
+constexpr int kJoinWarps = 16;
+
 // Rows that lie in several items, each by the warp (or, of many items, the CTA) that has the first of them.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, Sorted s, Parts parts,
+__global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArgs a, Sorted s, Parts parts,
                                                                  T* __restrict__ grad) {
   constexpr int kMany = 32;   // items from which on the CTA adds them up together
-  __shared__ float4 shares[kWarps][32][2];
-  __shared__ int many[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const i64 base = (i64)blockIdx.x * kWarps;
-  cudaGridDependencySynchronize();
-  // (items that follow each other, of one piece: rows of many items are in different CTAs)
+  __shared__ float4 shares[kJoinWarps][32][2];
   struct Row {
     int row, slot, piece;   // -1: none begins in the item
     i64 item, items;
   };
+  __shared__ Row many[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const i64 base = (i64)blockIdx.x * kJoinWarps;
+  cudaGridDependencySynchronize();
+  // (items that follow each other, of one piece: rows of many items are in different CTAs)
   auto row_of = [&](int w) {
     Row x{-1, 0, (int)((base + w) / parts.items), (base + w) % parts.items, 0};
     const i64 last = x.item * parts.part + parts.part - 1;
@@ -361,7 +408,7 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
   };
   // the row's shares of its items [from, to)
   auto add = [&](const Row& row, i64 from, i64 to, float (&sum)[kGroup]) {
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 4;
 #pragma unroll 1
     for (i64 i = from; i < to; i += kBatch) {
       float4 x[kBatch][2];
@@ -385,7 +432,7 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
     Numbers<T, VEC>::store(grad + (i64)r * a.H, piece * 32 * kGroup, lane, a.H, sum);
   };
   const Row own = row_of(warp);
-  if (lane == 0) many[warp] = own.row >= 0 && own.items >= kMany;
+  if (lane == 0) many[warp] = own;
   if (own.row >= 0 && own.items < kMany) {
     float sum[kGroup] = {};
     add(own, 0, own.items, sum);
@@ -393,10 +440,10 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
   }
   __syncthreads();
 #pragma unroll 1
-  for (int w = 0; w < kWarps; ++w) {
-    if (!many[w]) continue;
-    const Row row = row_of(w);
-    const i64 share = div_up64(row.items, kWarps);
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const Row row = many[w];
+    if (row.row < 0 || row.items < kMany) continue;
+    const i64 share = div_up64(row.items, kJoinWarps);
     float sum[kGroup] = {};
     add(row, warp * share, min(row.items, (warp + 1) * share), sum);
     shares[warp][lane][0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
@@ -406,7 +453,7 @@ __global__ void __launch_bounds__(32 * kWarps) embed_join_kernel(EmbedArgs a, So
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) sum[k] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
+      for (int i = 0; i < kJoinWarps; ++i) {
         const float4 x = shares[i][lane][0], y = shares[i][lane][1];
         sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
         sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
@@ -435,8 +482,8 @@ void with_variant(const EmbedArgs& a, bool wide, F launch) {
   });
 }
 
-unsigned ctas(i64 rows, int pieces) {
-  const i64 n = div_up64(rows * pieces, kWarps);
+unsigned ctas(i64 rows, int pieces, int warps = kWarps) {
+  const i64 n = div_up64(rows * pieces, warps);
   if (n > 0x7fffffffLL) throw std::invalid_argument("too many rows");
   return (unsigned)n;
 }
@@ -497,8 +544,14 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     int bits = 0;   // CTAs: up to 128, and no more than 256 rows each
     while ((bits < 7 && 2 << bits <= a.R) || (i64)kSortRows << bits < a.R) ++bits;
     ScopedKernel prof("embed_sort", stream);
-    sort_words_kernel<<<1u << bits, 32 * kSortWarps, 0, stream>>>(a.words, (int)a.N, bits, s);
-    TB200_CHECK_LAUNCH();
+    auto sort = [&](auto warps) {
+      constexpr int WARPS = decltype(warps)::value;
+      allow_dyn_smem(sort_words_kernel<WARPS>, sizeof(SortRoom<WARPS>));
+      sort_words_kernel<WARPS><<<1u << bits, 32 * WARPS, sizeof(SortRoom<WARPS>), stream>>>(a.words, (int)a.N, bits, s);
+      TB200_CHECK_LAUNCH();
+    };
+    if (a.N <= 4096) sort(std::integral_constant<int, 8>{});
+    else sort(std::integral_constant<int, 32>{});
   }
   EmbedArgs d = a;
   d.table = deltas, d.stride = a.H;
@@ -508,12 +561,12 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     constexpr bool DROP = decltype(drop)::value;
     {
       ScopedKernel prof("embed_sums", stream);
-      launch_early(embed_sums_kernel<T, VEC, DROP>, ctas(parts.items * pieces + a.R, 1), 32 * kWarps, stream, a,
+      launch_early(embed_sums_kernel<T, VEC, DROP>, ctas(parts.items * pieces + div_up(a.R, kFilled), 1), 32 * kWarps, stream, a,
                    static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad));
     }
     if (parts.items > 1) {
       ScopedKernel prof("embed_join", stream);
-      launch_early(embed_join_kernel<T, VEC>, ctas(parts.items, pieces), 32 * kWarps, stream, a, s, parts,
+      launch_early(embed_join_kernel<T, VEC>, ctas(parts.items, pieces, kJoinWarps), 32 * kJoinWarps, stream, a, s, parts,
                    static_cast<T*>(grad));
     }
   });
