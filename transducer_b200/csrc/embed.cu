@@ -120,10 +120,9 @@ __device__ __forceinline__ void stays(Stays<VEC> (&out)[K], N place, int first, 
 
 // A warp writes 256 numbers of each of ROWS rows that follow each other.
 template <typename T, int VEC, bool DROP, int ROWS>
-__global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __restrict__ rows, int pieces) {
-  const i64 id = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, first = (int)(id % pieces) * 32 * kGroup;
-  const i64 n0 = id / pieces * ROWS;
+__global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __restrict__ rows) {
+  const int lane = threadIdx.x & 31, first = blockIdx.y * 32 * kGroup;
+  const i64 n0 = ((i64)blockIdx.x * kWarps + (threadIdx.x >> 5)) * ROWS;
   if (n0 >= a.N) return;
   int r[ROWS];
 #pragma unroll
@@ -284,25 +283,25 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
 struct Parts {
   float* sums;   // [items, 2, pieces, 32 lanes, 8]
   int part, pieces;
-  i64 items;
-  __device__ __forceinline__ float4* at(i64 item, int slot, int piece, int lane) const {
-    return reinterpret_cast<float4*>(sums + ((((item * 2 + slot) * pieces + piece) * 32 + lane) * kGroup));
+  int items;
+  __device__ __forceinline__ float4* at(int item, int slot, int piece, int lane) const {
+    return reinterpret_cast<float4*>(sums + (((((i64)item * 2 + slot) * pieces + piece) * 32 + lane) * kGroup));
   }
 };
 
 constexpr int kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
 
-// The first items * pieces warps add up 256 numbers of an item's rows each; the others fill rows that no word has.
+// CTAs (x, piece): the warps of the first sumCtas add up 256 numbers of an item's rows each; the others fill rows that
+// no word has.
 template <typename T, int VEC, bool DROP>
 __global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
-                                                                 Parts parts, T* __restrict__ grad) {
+                                                                 Parts parts, T* __restrict__ grad, int sumCtas) {
   constexpr int kBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows on their way while as many are added (more: registers)
-  const i64 id = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const i64 fill = id - parts.items * parts.pieces;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
-  if (fill >= 0) {
+  if (blockIdx.x >= sumCtas) {
+    const i64 fill = ((i64)(blockIdx.x - sumCtas) * parts.pieces + blockIdx.y) * kWarps + warp;
     const i64 mine = fill * kFilled + lane;
     int2 range = make_int2(0, 1);
     if (lane < kFilled && mine < a.R) range = s.range[mine];
@@ -313,10 +312,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a,
         Numbers<T, VEC>::store(grad + (fill * kFilled + __ffs(empty) - 1) * a.H, first, lane, a.H, zero);
     return;
   }
-  const i64 item = id / parts.pieces;
-  const int piece = (int)(id % parts.pieces), first = piece * 32 * kGroup;
-  const int from = (int)(item * parts.part), all = s.all();
-  if (from >= all) return;
+  const int item = blockIdx.x * kWarps + warp, piece = blockIdx.y, first = piece * 32 * kGroup;
+  const int all = s.all();
+  if (item >= parts.items || item * (i64)parts.part >= all) return;
+  const int from = item * parts.part;
   const int to = (int)min((i64)from + parts.part, (i64)all);
   // lane i: the item's place i; the rows before it and behind it
   const int2 mine = lane < to - from ? s.order[from + lane] : make_int2(0, -1);
@@ -387,35 +386,33 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArg
   constexpr int kMany = 32;   // items from which on the CTA adds them up together
   __shared__ float4 shares[kJoinWarps][32][2];
   struct Row {
-    int row, slot, piece;   // -1: none begins in the item
-    i64 item, items;
+    int row, slot;   // -1: none begins in the item
+    int item, items;
   };
   __shared__ Row many[kJoinWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const i64 base = (i64)blockIdx.x * kJoinWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, piece = blockIdx.y;
   cudaGridDependencySynchronize();
-  // (items that follow each other, of one piece: rows of many items are in different CTAs)
-  auto row_of = [&](int w) {
-    Row x{-1, 0, (int)((base + w) / parts.items), (base + w) % parts.items, 0};
-    const i64 last = x.item * parts.part + parts.part - 1;
-    if (x.piece >= parts.pieces || last >= s.all()) return x;
+  auto row_of = [&](int item) {
+    Row x{-1, 0, item, 0};
+    const i64 last = (i64)item * parts.part + parts.part - 1;
+    if (last >= s.all()) return x;
     const int r = s.order[last].y;
     const int2 range = s.range[r];
-    x.items = (range.y - 1) / parts.part - x.item + 1;
+    x.items = (range.y - 1) / parts.part - item + 1;
     x.slot = range.x % parts.part == 0 ? 0 : 1;
-    if (range.x / parts.part == x.item && x.items > 1) x.row = r;
+    if (range.x / parts.part == item && x.items > 1) x.row = r;
     return x;
   };
   // the row's shares of its items [from, to)
-  auto add = [&](const Row& row, i64 from, i64 to, float (&sum)[kGroup]) {
+  auto add = [&](const Row& row, int from, int to, float (&sum)[kGroup]) {
     constexpr int kBatch = 4;
 #pragma unroll 1
-    for (i64 i = from; i < to; i += kBatch) {
+    for (int i = from; i < to; i += kBatch) {
       float4 x[kBatch][2];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         if (i + j < to) {
-          const float4* p = parts.at(row.item + i + j, i + j == 0 ? row.slot : 0, row.piece, lane);
+          const float4* p = parts.at(row.item + i + j, i + j == 0 ? row.slot : 0, piece, lane);
           x[j][0] = p[0], x[j][1] = p[1];
         }
 #pragma unroll
@@ -426,26 +423,26 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArg
         }
     }
   };
-  auto write = [&](int r, int piece, float (&sum)[kGroup]) {
+  auto write = [&](int r, float (&sum)[kGroup]) {
 #pragma unroll
     for (int k = 0; k < kGroup; ++k) sum[k] *= a.factor;
     Numbers<T, VEC>::store(grad + (i64)r * a.H, piece * 32 * kGroup, lane, a.H, sum);
   };
-  const Row own = row_of(warp);
+  const Row own = row_of(blockIdx.x * kJoinWarps + warp);
   if (lane == 0) many[warp] = own;
   if (own.row >= 0 && own.items < kMany) {
     float sum[kGroup] = {};
     add(own, 0, own.items, sum);
-    write(own.row, own.piece, sum);
+    write(own.row, sum);
   }
   __syncthreads();
 #pragma unroll 1
   for (int w = 0; w < kJoinWarps; ++w) {
     const Row row = many[w];
     if (row.row < 0 || row.items < kMany) continue;
-    const i64 share = div_up64(row.items, kJoinWarps);
+    const int share = div_up(row.items, kJoinWarps);
     float sum[kGroup] = {};
-    add(row, warp * share, min(row.items, (warp + 1) * share), sum);
+    add(row, min(row.items, warp * share), min(row.items, (warp + 1) * share), sum);
     shares[warp][lane][0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
     shares[warp][lane][1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
     __syncthreads();
@@ -458,7 +455,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArg
         sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
         sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
       }
-      write(row.row, row.piece, sum);
+      write(row.row, sum);
     }
     __syncthreads();
   }
@@ -482,17 +479,17 @@ void with_variant(const EmbedArgs& a, bool wide, F launch) {
   });
 }
 
-unsigned ctas(i64 rows, int pieces, int warps = kWarps) {
-  const i64 n = div_up64(rows * pieces, warps);
+unsigned ctas(i64 warps, int ofCta = kWarps) {
+  const i64 n = div_up64(warps, ofCta);
   if (n > 0x7fffffffLL) throw std::invalid_argument("too many rows");
   return (unsigned)n;
 }
 
 // The launches of one call: each begins while the one before it ends, and waits for its results.
 template <typename... P, typename... A>
-void launch_early(void (*kernel)(P...), unsigned ctas, int threads, cudaStream_t stream, A... args) {
+void launch_early(void (*kernel)(P...), dim3 ctas, int threads, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(ctas), config.blockDim = dim3(threads), config.stream = stream;
+  config.gridDim = ctas, config.blockDim = dim3(threads), config.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
@@ -511,10 +508,10 @@ void launch_embed_words(const EmbedArgs& a, void* rows, cudaStream_t stream) {
     constexpr bool DROP = decltype(drop)::value;
     ScopedKernel prof("embed_words", stream);
     if (a.N * pieces <= 148 * 64)   // (a row per warp fits the chip at once)
-      embed_kernel<T, VEC, DROP, 1><<<ctas(a.N, pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows), pieces);
+      embed_kernel<T, VEC, DROP, 1><<<dim3(ctas(a.N), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows));
     else
       embed_kernel<T, VEC, DROP, 4>
-          <<<ctas(div_up64(a.N, 4), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows), pieces);
+          <<<dim3(ctas(div_up64(a.N, 4)), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows));
     TB200_CHECK_LAUNCH();
   });
 }
@@ -539,7 +536,7 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
   s.order = reinterpret_cast<int2*>(at), at += round_up64(a.N * 8, 16);
   s.range = reinterpret_cast<int2*>(at), at += round_up64((a.R + 1ll) * 8, 16);
   s.R = a.R;
-  const Parts parts{reinterpret_cast<float*>(at), part, pieces, div_up64(a.N, part)};
+  const Parts parts{reinterpret_cast<float*>(at), part, pieces, (int)div_up64(a.N, part)};
   {
     int bits = 0;   // CTAs: up to 128, and no more than 256 rows each
     while ((bits < 7 && 2 << bits <= a.R) || (i64)kSortRows << bits < a.R) ++bits;
@@ -561,12 +558,13 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     constexpr bool DROP = decltype(drop)::value;
     {
       ScopedKernel prof("embed_sums", stream);
-      launch_early(embed_sums_kernel<T, VEC, DROP>, ctas(parts.items * pieces + div_up(a.R, kFilled), 1), 32 * kWarps, stream, a,
-                   static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad));
+      const int sumCtas = div_up(parts.items, kWarps), filled = kFilled * kWarps * pieces;
+      launch_early(embed_sums_kernel<T, VEC, DROP>, dim3(sumCtas + div_up(a.R, filled), pieces), 32 * kWarps, stream, a,
+                   static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad), sumCtas);
     }
     if (parts.items > 1) {
       ScopedKernel prof("embed_join", stream);
-      launch_early(embed_join_kernel<T, VEC>, ctas(parts.items, pieces, kJoinWarps), 32 * kJoinWarps, stream, a, s, parts,
+      launch_early(embed_join_kernel<T, VEC>, dim3(ctas(parts.items, kJoinWarps), pieces), 32 * kJoinWarps, stream, a, s, parts,
                    static_cast<T*>(grad));
     }
   });
