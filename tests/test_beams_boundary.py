@@ -9,7 +9,7 @@ import torch
 import beam_reference as ref
 from test_nodes_boundary import BAD_NODES, nodes
 from transducer_b200 import _lib, embed_words, extend_beams, reorder_states
-from transducer_b200.beams import _check_apart, _together
+from transducer_b200.beams import _check_apart, _row
 
 lib = _lib.lib
 P = ctypes.c_void_p(64)   # (never followed: no kernel is launched)
@@ -91,16 +91,19 @@ def test_bad_parents_and_states():
 
 
 def test_outputs_that_overlap():
+    def accept(states, out, W):
+        _check_apart([_row(s) for s in states], out, states[0].shape[0], states[0].shape[1], W)
+
     def refuse(states, out, message):
         with pytest.raises(ValueError, match=message):
-            _check_apart(states, out, out[0].shape[1])
+            accept(states, out, out[0].shape[1])
     room = torch.zeros(2, 9, 5)
     s = room[:, :4]
-    _check_apart([s], [s], 4)                       # in place
-    _check_apart([s], [room[:, :7]], 7)             # in place, more of them
-    _check_apart([s], [s[:, :3]], 3)
-    _check_apart([s[:1]], [room[:1, 4:9]], 5)       # side by side
-    _check_apart([s], [torch.zeros(2, 3, 5)], 3)
+    accept([s], [s], 4)                       # in place
+    accept([s], [room[:, :7]], 7)             # in place, more of them
+    accept([s], [s[:, :3]], 3)
+    accept([s[:1]], [room[:1, 4:9]], 5)       # side by side
+    accept([s], [torch.zeros(2, 3, 5)], 3)
     refuse([s], [room[:, 1:5]], "a state itself or not overlap")
     refuse([s], [room[:, 4:8]], "a state itself or not overlap")   # (between the utterances' rows)
     refuse([s, torch.zeros(2, 4, 5)], [torch.zeros(2, 4, 5), s], "a state itself or not overlap")
@@ -116,9 +119,10 @@ def test_outputs_that_overlap():
 
 def test_numbers_together():
     x = torch.zeros(2, 3, 4, 5)
-    assert _together(x) and _together(x[:, ::2]) and _together(x.transpose(0, 1)) and _together(x[..., :1, :])
-    assert not _together(x[..., ::2]) and not _together(x.transpose(2, 3)) and not _together(x[:, :, ::2])
-    assert _together(x[:, :, :0]) and _together(x[..., 0, 0])
+    assert _row(x)[1:] == (240, 80, 80) and _row(x[:, ::2])[1:] == (240, 160, 80)
+    assert _row(x.transpose(0, 1))[1:] == (80, 240, 80) and _row(x[..., :1, :])[1:] == (240, 80, 20)
+    assert _row(x[..., 0, 0])[1:] == (240, 80, 4) and _row(x[:, :, :0])[3] == 0
+    assert _row(x[..., ::2]) is None and _row(x.transpose(2, 3)) is None and _row(x[:, :, ::2]) is None
 
 
 @pytest.mark.parametrize("change,kind,message", [

@@ -46,12 +46,12 @@ def extend_beams(emissions, predictions, frames, positions, scores, width, valid
     B, N = frames.shape
     device = emissions.device
     with OnDevice(device):
-        best = torch.empty((B, width), device=device, dtype=torch.float32)
-        parents = torch.empty((B, width), device=device, dtype=torch.int32)
-        words = torch.empty((B, width), device=device, dtype=torch.int32)
+        best = scores.new_empty((B, width))
+        parents = frames.new_empty((B, width))
+        words = torch.empty_like(parents)
         described, sizes = _describe(emissions, predictions, frames)
         nbytes = _transducer.extend_beams_workspace_bytes(B, sizes[3], N)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = frames.new_empty((nbytes + 3) // 4)
         _transducer.extend_beams(described, frames.data_ptr(), positions.data_ptr(), scores.data_ptr(),
                                  best.data_ptr(), parents.data_ptr(), words.data_ptr(), sizes, width,
                                  ws.data_ptr(), nbytes)
@@ -83,44 +83,65 @@ def reorder_states(states, parents, out=None, validate_parents=True):
     if not len(states):
         raise ValueError("there must be a state to reorder.")
     B, W = parents.shape
-    N = states[0].shape[1] if states[0].dim() >= 2 else 0
+    device = parents.device
+    N = -1
     for s in states:
-        if s.dim() < 2:
+        shape = s.shape
+        if len(shape) < 2:
             raise ValueError("states must have a dimension of utterances and one of hypotheses.")
-        if s.shape[0] != B:
+        if shape[0] != B:
             raise ValueError("must have states per example.")
-        if s.shape[1] != N:
+        if N >= 0 and shape[1] != N:
             raise ValueError("states must have the same number of hypotheses.")
-    check_device(parents, *states)
+        N = shape[1]
+        if s.device != device:
+            raise ValueError("all inputs must be on the same device.")
     check_no_tangents(*states)
     if out is not None:
-        if len(out) != len(states):
-            raise ValueError("must have an output per state.")
-        for s, o in zip(states, out):
-            if o.dtype != s.dtype:
-                raise TypeError("out must have the states' types")
-            if tuple(o.shape) != (B, W) + tuple(s.shape[2:]):
-                raise ValueError("out must have the shape of the reordered states.")
-            if not _together(o):
-                raise ValueError("out must be contiguous behind its second dimension")
-            if o.requires_grad:
-                raise ValueError("out must not require gradients")
-        check_device(parents, *out)
-    with OnDevice(parents.device):
-        kept = out is not None
-        states = [s if _together(s) else s.detach().contiguous() for s in states]
-        if kept:
-            _check_apart(states, out, W)
-        else:
-            out = [s.new_empty((B, W) + tuple(s.shape[2:])) for s in states]
+        _check_outputs(states, out, parents)
+    with OnDevice(device):
+        made = out is None
+        if made:
+            out = []
+        rows, moved = [], []
+        for i, s in enumerate(states):
+            row = _row(s)
+            if row is None:
+                s = s.detach().contiguous()
+                row = _row(s)
+            at, from_b, from_n, size = row
+            if made:
+                o = torch.empty_like(s) if W == N and s.is_contiguous() else s.new_empty((B, W) + s.shape[2:])
+                out.append(o)
+                moved += at, o.data_ptr(), from_b, from_n, W * size, size, size
+            else:
+                to, to_b, to_n, _ = _row(out[i])
+                rows.append(row)
+                moved += at, to, from_b, from_n, to_b, to_n, size
+        if not made:
+            _check_apart(rows, out, B, N, W)
         if B * W:
-            _transducer.reorder_states([_moved(s, o) for s, o in zip(states, out)], parents.data_ptr(), B, N, W,
-                                       kept)
-            if kept:   # (written behind autograd's back)
+            _transducer.reorder_states(moved, parents.data_ptr(), B, N, W, not made)
+            if not made:   # (written behind autograd's back)
                 torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
             if validate_parents:
                 certify_parents(parents, N)
     return out[0] if single else list(out)
+
+
+def _check_outputs(states, out, parents):
+    if len(out) != len(states):
+        raise ValueError("must have an output per state.")
+    for s, o in zip(states, out):
+        if o.dtype != s.dtype:
+            raise TypeError("out must have the states' types")
+        if o.shape[:2] != parents.shape or o.shape[2:] != s.shape[2:]:
+            raise ValueError("out must have the shape of the reordered states.")
+        if _row(o) is None:
+            raise ValueError("out must be contiguous behind its second dimension")
+        if o.requires_grad:
+            raise ValueError("out must not require gradients")
+    check_device(parents, *out)
 
 
 def certify_parents(parents, N):
@@ -131,68 +152,50 @@ def certify_parents(parents, N):
         raise ValueError("Parent index mismatch")
 
 
-def _row_numbers(s):
-    n = 1
-    for size in s.shape[2:]:
-        n *= size
-    return n
+def _row(s):
+    """Where a tensor begins, its bytes from one utterance and from one hypothesis to the next, and bytes of a row; None
+    where a hypothesis' numbers are not next to each other."""
+    shape = s.shape
+    if s.is_contiguous() and shape[0] * shape[1]:
+        size = s.nbytes // (shape[0] * shape[1])
+        return s.data_ptr(), shape[1] * size, size, size
+    stride, size = s.stride(), s.element_size()
+    numbers = 1
+    for i in range(len(shape) - 1, 1, -1):
+        n = shape[i]
+        if n != 1 and stride[i] != numbers and s.numel():
+            return None
+        numbers *= n
+    return s.data_ptr(), stride[0] * size, stride[1] * size, numbers * size
 
 
-def _together(s):
-    """Whether a hypothesis' numbers are next to each other."""
-    want = 1
-    for size, stride in zip(reversed(s.shape[2:]), reversed(s.stride()[2:])):
-        if size != 1 and stride != want:
-            return _row_numbers(s) == 0
-        want *= size
-    return True
+def _end(row, B, N):
+    """The address behind a tensor of B utterances and N hypotheses; its beginning if it is empty."""
+    return row[0] + ((B - 1) * row[1] + (N - 1) * row[2] + row[3] if B * N * row[3] else 0)
 
 
-def _moved(s, o):
-    size = s.element_size()
-    (sb, sn), (ob, on) = s.stride()[:2], o.stride()[:2]
-    return s.data_ptr(), o.data_ptr(), sb * size, sn * size, ob * size, on * size, _row_numbers(s) * size
-
-
-def _extent(s):
-    """Addresses from the first byte to behind the last one; None if there are none."""
-    if s.numel() == 0:
-        return None
-    last = sum((n - 1) * k for n, k in zip(s.shape, s.stride()))
-    return s.data_ptr(), s.data_ptr() + (last + 1) * s.element_size()
-
-
-def _check_apart(states, out, W):
+def _check_apart(rows, out, B, N, W):
+    """That outputs overlap with nothing, but for one that is its state itself (the same place for every hypothesis)."""
     taken = []
+    ends = [_end(row, B, N) for row in rows]
     for i, o in enumerate(out):
-        mine = _extent(o)
-        if mine is None:
+        mine = _row(o)
+        begin, end = mine[0], _end(mine, B, W)
+        if begin == end:
             continue
-        row = _row_numbers(o)
-        sizes = sorted((k, n) for n, k in zip(o.shape[:2], o.stride()[:2]) if n > 1)
-        reach = row
-        for k, n in sizes:   # rows of `o` that share memory
-            if k < reach:
+        reach = mine[3]
+        for step, n in sorted(((mine[1], B), (mine[2], W))):   # rows of `o` that share memory
+            if n > 1 and step < reach:
                 raise ValueError("out must not overlap with itself")
-            reach = k * (n - 1) + reach
-        for j, s in enumerate(states):
-            other = _extent(s)
-            if other is None or mine[1] <= other[0] or other[1] <= mine[0]:
+            reach += step * (n - 1)
+        for j, row in enumerate(rows):
+            if end <= row[0] or ends[j] <= begin:
                 continue
-            if i != j or not _same_place(s, o):
+            if i != j or begin != row[0] or (B > 1 and mine[1] != row[1]) or (min(N, W) > 1 and mine[2] != row[2]):
                 raise ValueError("out must be a state itself or not overlap with the states")
             if W > MAX_REORDERED_WIDTH:
                 raise ValueError("at most %d hypotheses are reordered in place" % MAX_REORDERED_WIDTH)
         for other in taken:
-            if mine[0] < other[1] and other[0] < mine[1]:
+            if begin < other[1] and other[0] < end:
                 raise ValueError("outputs must not overlap with each other")
-        taken.append(mine)
-
-
-def _same_place(s, o):
-    """Whether hypothesis n of utterance b lies at the same address in both."""
-    if s.data_ptr() != o.data_ptr():
-        return False
-    same_b = s.shape[0] == 1 or s.stride(0) == o.stride(0)
-    same_n = min(s.shape[1], o.shape[1]) == 1 or s.stride(1) == o.stride(1)
-    return same_b and same_n
+        taken.append((begin, end))

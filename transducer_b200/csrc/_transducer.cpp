@@ -263,14 +263,14 @@ PYBIND11_MODULE(_transducer, m) {
         },
         "scores"_a, "frames"_a, "positions"_a, "beam_scores"_a, "out_scores"_a, "parents"_a, "words"_a, "sizes"_a,
         "width"_a, "workspace"_a, "workspace_bytes"_a);
-  // `states`: of each tensor (from, to, their strides in bytes by utterance and by hypothesis, bytes of a row)
-  using Moved = std::tuple<addr, addr, long long, long long, long long, long long, long long>;
+  // `states`: of each tensor from, to, their strides in bytes by utterance and by hypothesis, bytes of a row
   m.def("reorder_states",
-        [](const std::vector<Moved>& states, addr parents, int B, int N, int W, bool kept) {
+        [](const std::vector<long long>& states, addr parents, int B, int N, int W, bool kept) {
           std::vector<tb200_states> all;
-          for (const Moved& s : states)
-            all.push_back(tb200_states{at<const void>(std::get<0>(s)), at<void>(std::get<1>(s)), std::get<2>(s),
-                                       std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s)});
+          for (size_t i = 0; i + 7 <= states.size(); i += 7) {
+            const long long* s = &states[i];
+            all.push_back(tb200_states{at<const void>((addr)s[0]), at<void>((addr)s[1]), s[2], s[3], s[4], s[5], s[6]});
+          }
           check(tb200_reorder_states(all.data(), (int)all.size(), at<const int>(parents), B, N, W, kept));
         },
         "states"_a, "parents"_a, "batch_size"_a, "hypotheses"_a, "width"_a, "kept"_a);

@@ -8,7 +8,7 @@ import torch
 
 from . import _transducer
 from .nodes import OnDevice, check_device, check_no_tangents
-from .torch_binding import _workspace, check_contiguous, check_dim, check_type
+from .torch_binding import check_contiguous, check_dim, check_type
 
 
 class WordEmbedding(torch.autograd.Function):
@@ -16,35 +16,29 @@ class WordEmbedding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, words, scale, dropout, seed, validate_words):
-        if table.stride(1) != 1 and table.shape[1] != 1:
-            table = table.contiguous()
+        rows = _rows_of(table, words, scale, dropout, seed, validate_words)
         R, H = table.shape
-        device = table.device
-        bf16 = table.dtype is torch.bfloat16
         numbers, place = _seed(seed)
-        with OnDevice(device):
-            rows = torch.empty(tuple(words.shape) + (H,), device=device, dtype=table.dtype)
-            _transducer.embed_words(table.data_ptr(), bf16, table.stride(0), words.data_ptr(), words.numel(),
-                                    rows.data_ptr(), R, H, scale, dropout, numbers, place)
-            if validate_words:
-                certify_words(words, R)
-        ctx.save_for_backward(words, seed if place else None)
-        ctx.rest = (R, H, bf16, scale, dropout, numbers)
+        if place:
+            ctx.save_for_backward(words, seed)
+        else:
+            ctx.save_for_backward(words)
+        ctx.rest = (R, H, table.dtype is torch.bfloat16, scale, dropout, numbers, place)
         return rows
 
     @staticmethod
     def backward(ctx, deltas):
-        words, seed = ctx.saved_tensors
-        R, H, bf16, scale, dropout, numbers = ctx.rest
-        deltas = deltas.contiguous()
-        device = deltas.device
-        with OnDevice(device):
-            grad = torch.empty((R, H), device=device, dtype=deltas.dtype)
-            nbytes = _transducer.embed_backward_workspace_bytes(words.numel(), R, H)
-            ws = _workspace(nbytes, device)
-            _transducer.embed_backward(deltas.data_ptr(), bf16, words.data_ptr(), words.numel(), grad.data_ptr(),
-                                       R, H, scale, dropout, numbers, 0 if seed is None else seed.data_ptr(),
-                                       ws.data_ptr(), nbytes)
+        words = ctx.saved_tensors[0]   # (refuses words, and a seed on the device, that were written since)
+        R, H, bf16, scale, dropout, numbers, place = ctx.rest
+        if not deltas.is_contiguous():
+            deltas = deltas.contiguous()
+        count = words.numel()
+        with OnDevice(deltas.device):
+            grad = deltas.new_empty((R, H))
+            nbytes = _transducer.embed_backward_workspace_bytes(count, R, H)
+            ws = words.new_empty((nbytes + 3) // 4)
+            _transducer.embed_backward(deltas.data_ptr(), bf16, words.data_ptr(), count, grad.data_ptr(), R, H, scale,
+                                       dropout, numbers, place, ws.data_ptr(), nbytes)
         if torch.is_grad_enabled():   # (somebody wants to differentiate it)
             grad = Once.apply(grad, deltas)
         return (grad,) + (None,) * 5
@@ -67,6 +61,20 @@ def _seed(seed):
     if isinstance(seed, torch.Tensor):
         return 0, seed.data_ptr()
     return 0 if seed is None else seed, 0
+
+
+def _rows_of(table, words, scale, dropout, seed, validate_words):
+    if table.stride(1) != 1 and table.shape[1] != 1:
+        table = table.contiguous()
+    R, H = table.shape
+    numbers, place = _seed(seed)
+    with OnDevice(table.device):
+        rows = table.new_empty(words.shape + (H,))
+        _transducer.embed_words(table.data_ptr(), table.dtype is torch.bfloat16, table.stride(0), words.data_ptr(),
+                                words.numel(), rows.data_ptr(), R, H, scale, dropout, numbers, place)
+        if validate_words:
+            certify_words(words, R)
+    return rows
 
 
 def certify_words(words, R):
@@ -120,4 +128,6 @@ def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=
         check_device(table, seed)
     elif seed is not None and not -2 ** 63 <= seed < 2 ** 63:
         raise ValueError("seed must fit 64 bits")
+    if not (table.requires_grad and torch.is_grad_enabled()):
+        return _rows_of(table, words, scale, dropout, seed, validate_words)
     return WordEmbedding.apply(table, words, scale, dropout, seed, validate_words)
