@@ -15,11 +15,11 @@ namespace tb200 {
 namespace {
 
 constexpr int kTile = 1024, kChunk = 32;
-constexpr int kScanWarps = 4, kPickThreads = 1024, kPickWarps = kPickThreads / 32;
-constexpr int kTilesListed = 1024, kChunksListed = 8192, kWordsListed = 8192;
+constexpr int kScanWarps = 4;
 
-// A row's log-sum-exp is off by 6e-6 at most: exponents (z - m) log2(e) are rounded three times, 3 * 2^-24 |z - m|, whose
-// mean under the softmax is ln V < 20 at most; ex2.approx 2^-22; sums of 32 words and 32 lanes 2^-24 (32 + 5).
+// A row's log-sum-exp is off by 6e-6 at most: exponents z - m times log2(e) are rounded three times, which is 3 * 2^-24
+// |z - m|, on average under the softmax less than 3 * 2^-24 * 20 (ln V); ex2.approx twice 2^-22; 23 additions and
+// products one after the other 2^-24 each.
 constexpr float kLseError = 6e-6f;
 
 struct ExtendScratch {
@@ -48,21 +48,32 @@ __device__ __forceinline__ float warp_greatest(float x) {
   return y;
 }
 
-// A warp goes through one tile of the rows of up to 32 hypotheses that follow each other; the frame's words stay in
-// registers as long as the frame is the same.
+// A warp goes through one tile of the rows of up to 32 hypotheses that follow each other, frame by frame, so that a
+// frame's words stay in registers.  The rows of the hypotheses come through a ring in shared memory, from which every lane
+// reads what it has copied itself (single bf16 words, which no asynchronous copy moves, come through registers).
+constexpr int kScanStages = 2;
+template <typename TIn, int VEC>
+constexpr bool kScanRing = VEC * sizeof(TIn) >= 4;
+template <typename TIn, int VEC>
+constexpr int kScanSmem = kScanRing<TIn, VEC> ? kScanWarps * kScanStages * kTile * (int)sizeof(TIn) : 0;
+
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a, const float* __restrict__ scores,
                                                                       int tiles, int perWarp, int groups,
                                                                       ExtendScratch out) {
   constexpr int J = kChunk / VEC;
-  const int lane = threadIdx.x & 31;
-  const i64 id = (i64)blockIdx.x * kScanWarps + (threadIdx.x >> 5);
-  const int tile = (int)(id % tiles);
-  const i64 rest = id / tiles;
-  const i64 b = rest / groups;
+  constexpr bool RING = kScanRing<TIn, VEC>;
+  using Raw = RawWords<TIn, VEC>;
+  extern __shared__ __align__(16) char shared[];
+  __shared__ unsigned char order[kScanWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   cudaTriggerProgrammaticLaunchCompletion();
-  if (b >= a.B) return;
-  const int first = (int)(rest % groups) * perWarp, count = min(perWarp, a.N - first);
+  // (x: tiles, groups of hypotheses; y, z: utterances)
+  const unsigned id = blockIdx.x * kScanWarps + warp;
+  const int tile = id % (unsigned)tiles, group = id / (unsigned)tiles;
+  const i64 b = (i64)blockIdx.z * gridDim.y + blockIdx.y;
+  if (group >= groups || b >= a.B) return;
+  const int first = group * perWarp, count = min(perWarp, a.N - first);
   int frame = -1, position = -1;
   if (lane < count) {
     const i64 node = b * a.N + first + lane;
@@ -70,40 +81,75 @@ __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a
     if ((unsigned)frame >= (unsigned)a.T || (unsigned)position >= (unsigned)a.U || scores[node] == neg_inf())
       frame = -1;
   }
+  // hypotheses in the order of their frames
+  const int live = __popc(__ballot_sync(0xffffffffu, frame >= 0));
+  int place = 0;
+  for (int i = 0; i < count; ++i) {
+    const int t = __shfl_sync(0xffffffffu, frame, i);
+    place += t >= 0 && (t < frame || (t == frame && i < lane)) ? 1 : 0;
+  }
+  if (frame >= 0) order[warp][place] = lane;
+  __syncwarp();
   const TIn* const E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
   const TIn* const P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
   const int at = chunk_word<VEC>(tile, lane, 0);
-  RawWords<TIn, VEC> e[J], p[J];
+  Raw* const ring = reinterpret_cast<Raw*>(shared) + warp * kScanStages * J * 32 + lane;
+  // the i-th hypothesis' row: to the ring, and from there (or from memory)
+  auto row_of = [&](int i) { return P + __shfl_sync(0xffffffffu, position, order[warp][i]) * a.pStrideU; };
+  auto send = [&](int i) {
+    if constexpr (RING) {
+      if (i < live) {
+        const TIn* row = row_of(i);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (at + 32 * VEC * j < a.V)
+            copy_async<VEC * sizeof(TIn)>(ring + (i % kScanStages * J + j) * 32, row + at + 32 * VEC * j);
+      }
+      commit_copies();
+    }
+  };
+  if (live == 0) return;
+#pragma unroll
+  for (int i = 0; i < kScanStages - 1; ++i) send(i);
+  Raw e[J];
   int held = -1;
 #pragma unroll 1
-  for (int n = 0; n < count; ++n) {
-    const int t = __shfl_sync(0xffffffffu, frame, n), u = __shfl_sync(0xffffffffu, position, n);
-    if (t < 0) continue;
+  for (int i = 0; i < live; ++i) {
+    const int n = order[warp][i], t = __shfl_sync(0xffffffffu, frame, n);
     if (t != held) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
         if (at + 32 * VEC * j < a.V) e[j].load(E + t * a.eStrideT + at + 32 * VEC * j);
       held = t;
     }
+    Raw p[J];
+    if constexpr (RING) {
+      send(i + kScanStages - 1);
+      wait_copies<kScanStages - 1>();
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (at + 32 * VEC * j < a.V) p[j].load(P + u * a.pStrideU + at + 32 * VEC * j);
+      for (int j = 0; j < J; ++j) p[j] = ring[(i % kScanStages * J + j) * 32];
+    } else {
+      const TIn* row = row_of(i);
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (at + 32 * VEC * j < a.V) p[j].load(row + at + 32 * VEC * j);
+    }
     float z[kChunk];
     float top = neg_inf();
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const Words<VEC> x = e[j].words(), y = p[j].words();
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        z[VEC * j + i] = at + 32 * VEC * j < a.V ? x.x[i] + y.x[i] : neg_inf();
-        top = fmaxf(top, z[VEC * j + i]);
+      for (int k = 0; k < VEC; ++k) {
+        z[VEC * j + k] = at + 32 * VEC * j < a.V ? x.x[k] + y.x[k] : neg_inf();
+        top = fmaxf(top, z[VEC * j + k]);
       }
     }
     const float most = warp_greatest(top);
     const float ref = most == neg_inf() ? 0.0f : most;   // (+inf and NaN: the sum is NaN)
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) sum[i % 4] += ex2((z[i] - ref) * 1.4426950408889634f);
+    for (int k = 0; k < kChunk; ++k) sum[k % 4] += ex2((z[k] - ref) * 1.4426950408889634f);
     const float all = warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
     const i64 row = (b * a.N + first + n) * tiles + tile;
     out.best[row * 32 + lane] = top;
@@ -111,31 +157,100 @@ __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a
   }
 }
 
-struct Picked {   // extensions that may be among the best
-  double d[kWordsListed];
-  int parent[kWordsListed], word[kWordsListed];
-  int chunk[kChunksListed];
-  i64 tile[kTilesListed];
-  double2 scratch[64];
-  int count[4], flag, close;
-  unsigned char again[kWordsListed];
+// ---- what is picked of them ---------------------------------------------------------------------
+// A CTA per utterance: of 256 threads where up to 64 extensions are wanted of so many rows and tiles as shared memory
+// holds, else of 1024, whose own maxima tell 256 extensions, and which read what is not held from memory again.
+
+constexpr int kRowsHeld = 256, kTilesHeld = 4096;
+inline bool all_held(int W, i64 N, i64 tiles) { return W <= 64 && N <= kRowsHeld && N * tiles + N <= kTilesHeld; }
+enum Kind : unsigned char { kNotThere, kFinished, kExtended };
+
+// An extension's parent and word: of equal extensions the lower one comes first.
+using Place = unsigned long long;
+__device__ __forceinline__ Place place_of(int parent, int word) { return (Place)parent << 32 | (unsigned)(word + 1); }
+__device__ __forceinline__ int parent_of(Place x) { return (int)(x >> 32); }
+__device__ __forceinline__ int word_of(Place x) { return (int)(unsigned)x - 1; }
+
+// A tile that is looked at again: its hypothesis, which tile of its row (-1: the hypothesis is finished, its score is row.y),
+// its row (see ExtendScratch), and where the rows of the frame and of the position begin.
+struct ListedTile {
+  int n, tile;
+  double2 row;
+  i64 e, p;
 };
 
-// A key that `W` of the items' greatest reach, and hardly more than W, from the threads' own (0: none); 0 if there are
-// fewer.  All threads.
-__device__ __forceinline__ unsigned reached_by(unsigned mine, int W, Group<kPickThreads>& g) {
-  const int n = __syncthreads_count(mine != 0);
-  if (n < W) return 0;
-  unsigned from = g.min(mine ? mine : ~0u), to = g.max(mine) + 1;
-  int reached = n;
+template <int T>
+struct PickRoom {
+  static constexpr int kTiles = T == 256 ? 128 : 512;       // listed; where there are more: general_pick
+  static constexpr int kChunks = T == 256 ? 4096 : 8192;
+  static constexpr int kWords = T == 256 ? 2048 : 8192;
+  double2 row[kRowsHeld];
+  i64 e[kRowsHeld], p[kRowsHeld];   // where the rows begin
+  union {
+    unsigned chunkKey[kTiles * 32];
+    struct {   // extensions that may be among the best
+      double d[kWords];
+      Place place[kWords];
+    };
+  };
+  double2 scratch[64];
+  ListedTile tile[kTiles];
+  unsigned key[T];
+  union {
+    float top[kTilesHeld];          // of tiles
+    unsigned tileKey[kTilesHeld];   // of their greatest extensions
+  };
+  int chunk[kChunks];
+  float score[kRowsHeld];
+  int count[4];
+  unsigned reached;
+  int close;
+  Kind kind[kRowsHeld];
+  unsigned char again[kWords];
+};
+
+// A key that `W` of the threads' keys reach (0: none), the W-th of them or a little less; 0 if there are fewer.
+template <int T>
+__device__ __forceinline__ unsigned reached_by(unsigned mine, int W, PickRoom<T>& r, Group<T>& g) {
+  if constexpr (T == 256) {   // (by one warp: no barriers in between)
+    r.key[g.tid] = mine;
+    if (__syncthreads_count(mine != 0) < W) return 0;
+    if (g.warp == 0) {
+      const uint4 x = reinterpret_cast<const uint4*>(r.key)[2 * g.lane], y = reinterpret_cast<const uint4*>(r.key)[2 * g.lane + 1];
+      const unsigned k[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      unsigned least = ~0u, most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) least = min(least, k[i] ? k[i] : ~0u), most = max(most, k[i]);
+      unsigned from = __reduce_min_sync(0xffffffffu, least), to = __reduce_max_sync(0xffffffffu, most) + 1;
+      int reached = T;
 #pragma unroll 1
-  while (to - from > 1 && reached > W + W / 8) {
-    const unsigned mid = from + (to - from) / 2;
-    const int c = __syncthreads_count(mine >= mid);
-    if (c >= W) from = mid, reached = c;
-    else to = mid;
+      while (to - from > 1 && reached > W + W / 8) {
+        const unsigned mid = from + (to - from) / 2;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c += k[i] >= mid ? 1 : 0;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= W) from = mid, reached = c;
+        else to = mid;
+      }
+      if (g.lane == 0) r.reached = from;
+    }
+    __syncthreads();
+    return r.reached;
+  } else {
+    const int n = __syncthreads_count(mine != 0);
+    if (n < W) return 0;
+    unsigned from = g.min(mine ? mine : ~0u), to = g.max(mine) + 1;
+    int reached = n;
+#pragma unroll 1
+    while (to - from > 1 && reached > W + W / 8) {
+      const unsigned mid = from + (to - from) / 2;
+      const int c = __syncthreads_count(mine >= mid);
+      if (c >= W) from = mid, reached = c;
+      else to = mid;
+    }
+    return from;
   }
-  return from;
 }
 
 // The key from which on words are looked at, given one that W of them reach: as much lower as two rows' errors and the
@@ -153,75 +268,140 @@ __device__ __forceinline__ unsigned long long wide_key(double x) {
   return u ^ ((unsigned long long)((long long)u >> 63) | 0x8000000000000000ull);
 }
 
-template <typename TIn, int VEC>
+// The key of an extension's score; above 0 for all that are extensions.
+__device__ __forceinline__ unsigned extension_key(double d) {
+  const unsigned lowest = score_key(neg_inf());
+  return d > -1.0 / 0.0 ? max(score_key((float)d), lowest + 1) : 0u;
+}
+
+template <typename TIn, int VEC, int T>
 struct Utterance {
   const NodeArgs& a;
-  const float* scores;
+  const float* scores;   // of the utterance
   const ExtendScratch& s;
   i64 first;   // node
   int tiles;
+  PickRoom<T>& room;
 
-  __device__ __forceinline__ NodeScores<TIn> node(int n) const { return node_scores<TIn>(a, first + n); }
-  // a hypothesis that is kept as it is
-  __device__ __forceinline__ bool finished(int n) const {
-    return scores[first + n] > neg_inf() && !node(n).here;
+  __device__ __forceinline__ i64 all_tiles() const { return (i64)a.N * tiles; }
+  // A hypothesis, from memory: what it is, and its rows.
+  __device__ __forceinline__ Kind look(int n, float& score, i64& e, i64& p) const {
+    const int t = a.frames[first + n], u = a.positions[first + n];
+    score = scores[n];
+    const bool here = (unsigned)t < (unsigned)a.T && (unsigned)u < (unsigned)a.U;
+    e = here ? t * a.eStrideT : 0, p = here ? u * a.pStrideU : 0;
+    return score == neg_inf() ? kNotThere : here ? kExtended : kFinished;
   }
-  __device__ __forceinline__ double2 at_row(int n) const { return s.row[first + n]; }
-  __device__ __forceinline__ bool has_words(int n) const { return at_row(n).y != -1.0 / 0.0; }
+  __device__ __forceinline__ void hold(int n) const {
+    room.kind[n] = look(n, room.score[n], room.e[n], room.p[n]);
+  }
+  static __device__ __forceinline__ bool held(int n) { return T == 256 || n < kRowsHeld; }
+  __device__ __forceinline__ Kind kind(int n) const {
+    if (held(n)) return room.kind[n];
+    float score;
+    i64 e, p;
+    return look(n, score, e, p);
+  }
+  __device__ __forceinline__ float score(int n) const { return held(n) ? room.score[n] : scores[n]; }
+  __device__ __forceinline__ void begins(int n, i64& e, i64& p) const {
+    float score;
+    if (held(n)) e = room.e[n], p = room.p[n];
+    else look(n, score, e, p);
+  }
+  __device__ __forceinline__ const TIn* frame_at(i64 e) const {
+    return static_cast<const TIn*>(a.E) + blockIdx.x * a.eStrideB + e;
+  }
+  __device__ __forceinline__ const TIn* position_at(i64 p) const {
+    return static_cast<const TIn*>(a.P) + blockIdx.x * a.pStrideB + p;
+  }
+  __device__ __forceinline__ NodeScores<TIn> rows(int n) const {
+    i64 e, p;
+    begins(n, e, p);
+    return {frame_at(e), position_at(p), 0, 0, true};
+  }
+  // Its greatest score m and score - log sum exp(z - m); the latter -inf if it has no words.
+  __device__ __forceinline__ double2 row(int n) const { return held(n) ? room.row[n] : s.row[first + n]; }
+  __device__ __forceinline__ void set_row(int n, double2 x) const {
+    if (held(n)) room.row[n] = x;
+    else s.row[first + n] = x;
+  }
   // An extension's score: z - m loses nothing, however large the two are.
   static __device__ __forceinline__ double value(double2 row, float z) { return row.y + ((double)z - row.x); }
+  __device__ __forceinline__ float tile_top(i64 t) const {
+    return T == 256 || t < kTilesHeld ? room.top[t] : s.sums[first * tiles + t].x;
+  }
+  // the key of a tile's greatest extension; tiles from all_tiles() on: hypotheses that are finished
+  __device__ __forceinline__ unsigned tile_key(i64 t) const {
+    if (t >= all_tiles()) {
+      const int n = (int)(t - all_tiles());
+      return kind(n) == kFinished ? extension_key(score(n)) : 0u;
+    }
+    const int n = tiles == 1 ? (int)t : (int)((unsigned)t / (unsigned)tiles);
+    const double2 x = row(n);
+    return x.y > -1.0 / 0.0 ? extension_key(value(x, tile_top(t))) : 0u;
+  }
+  __device__ __forceinline__ ListedTile listed(i64 t) const {
+    ListedTile x;
+    if (t >= all_tiles()) {
+      x.n = (int)(t - all_tiles()), x.tile = -1;
+      x.row = make_double2(0.0, score(x.n));
+      x.e = x.p = 0;
+    } else {
+      x.n = (int)((unsigned)t / (unsigned)tiles), x.tile = (int)((unsigned)t % (unsigned)tiles);
+      x.row = row(x.n);
+      begins(x.n, x.e, x.p);
+    }
+    return x;
+  }
 
-  // at_row(n), its sum in 64 bits, by the CTA
-  __device__ __noinline__ double2 exact_row(int n, Group<kPickThreads>& g) const {
-    const NodeScores<TIn> row = node(n);
-    float m = neg_inf();
-    each_score<TIn, VEC, kPickThreads>(row, a.V, g.tid, [&](float z, int) { m = fmaxf(m, z); });
-    m = g.max(m);
+  // log sum exp(z - m) of a row in 64 bits, by the CTA
+  __device__ __noinline__ double2 exact_row(int n, Group<T>& g) const {
+    const NodeScores<TIn> r = rows(n);
+    const float m = (float)row(n).x;
     double sum = 0.0;
-    if (m > neg_inf())
-      each_score<TIn, VEC, kPickThreads>(row, a.V, g.tid, [&](float z, int) { sum += exp((double)z - (double)m); });
+    each_score<TIn, VEC, T>(r, a.V, g.tid, [&](float z, int) { sum += exp((double)z - (double)m); });
     sum = g.sum(sum);
-    return make_double2(m, (double)scores[first + n] - log(sum));
+    return make_double2(m, (double)score(n) - log(sum));
   }
 
   // f(value, parent, word) for every extension of at least `least`, in any order, by the CTA
   template <typename F>
   __device__ __forceinline__ void each(double least, int tid, F f) const {
     const int lane = tid & 31;
-    const i64 all = (i64)a.N * tiles;
 #pragma unroll 1
-    for (i64 t = tid >> 5; t < all; t += kPickWarps) {
-      const int n = (int)(t / tiles), tile = (int)(t % tiles);
-      const double2 at = at_row(n);
-      if (at.y == -1.0 / 0.0) continue;
-      const float top = s.best[(first * tiles + t) * 32 + lane];
-      if (!(value(at, top) >= least)) continue;
-      const NodeScores<TIn> row = node(n);
+    for (i64 t = tid >> 5; t < all_tiles(); t += T / 32) {
+      const int n = (int)((unsigned)t / (unsigned)tiles), tile = (int)((unsigned)t % (unsigned)tiles);
+      const double2 x = row(n);
+      if (x.y == -1.0 / 0.0) continue;
+      if (!(value(x, s.best[(first * tiles + t) * 32 + lane]) >= least)) continue;
+      const NodeScores<TIn> r = rows(n);
 #pragma unroll 1
       for (int i = 0; i < kChunk; ++i) {
         const int v = chunk_word<VEC>(tile, lane, i);
         if (v >= a.V) break;
-        const float z = to_f32(row.e[v]) + to_f32(row.p[v]);
-        if (z > neg_inf() && value(at, z) >= least) f(value(at, z), n, v);
+        const float z = to_f32(r.e[v]) + to_f32(r.p[v]);
+        if (z > neg_inf() && value(x, z) >= least) f(value(x, z), n, v);
       }
     }
 #pragma unroll 1
-    for (int n = tid; n < a.N; n += kPickThreads)
-      if (finished(n) && scores[first + n] >= least) f((double)scores[first + n], n, -1);
+    for (int n = tid; n < a.N; n += T)
+      if (kind(n) == kFinished && score(n) >= least) f((double)score(n), n, -1);
   }
 };
 
 // Where equal scores make the lists too long: the W-th value by a search over 64-bit keys, a pass over the chunks that reach
 // it for each bit, then the place up to which its equals belong to the best.  Leaves the list.
-template <typename TIn, int VEC>
-__device__ __noinline__ int general_pick(const Utterance<TIn, VEC>& at, int W, Picked& p, Group<kPickThreads>& g) {
+template <typename TIn, int VEC, int T>
+__device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W, Group<T>& g) {
   const NodeArgs& a = at.a;
+  PickRoom<T>& p = at.room;
+  __syncthreads();
 #pragma unroll 1
   for (int n = 0; n < a.N; ++n) {
-    if (!at.has_words(n)) continue;   // (the same for all threads)
+    if (at.row(n).y == -1.0 / 0.0) continue;   // (the same for all threads)
     const double2 row = at.exact_row(n, g);
     __syncthreads();
-    if (g.tid == 0) at.s.row[at.first + n] = row;
+    if (g.tid == 0) at.set_row(n, row);
     __syncthreads();
   }
   const double lowest = -1.7976931348623157e308;
@@ -247,13 +427,11 @@ __device__ __noinline__ int general_pick(const Utterance<TIn, VEC>& at, int W, P
   key = max(key, wide_key(lowest));
   const double cut = value(key);
   const int above = count(cut, [&](double d, int, int) { return wide_key(d) > key; });
-  // (the place of an extension in the order of equals)
-  auto place = [&](int n, int v) { return (i64)n * (a.V + 1ll) + v + 1; };
-  i64 lo = 0, hi = (i64)a.N * (a.V + 1ll) - 1;
+  i64 lo = 0, hi = (i64)place_of(a.N, 0);
 #pragma unroll 1
   while (lo < hi) {
     const i64 mid = lo + (hi - lo) / 2;
-    if (count(cut, [&](double d, int n, int v) { return wide_key(d) == key && place(n, v) <= mid; }) >= W - above)
+    if (count(cut, [&](double d, int n, int v) { return wide_key(d) == key && (i64)place_of(n, v) <= mid; }) >= W - above)
       hi = mid;
     else lo = mid + 1;
   }
@@ -261,201 +439,268 @@ __device__ __noinline__ int general_pick(const Utterance<TIn, VEC>& at, int W, P
   if (g.tid == 0) p.count[2] = 0;
   __syncthreads();
   at.each(cut, g.tid, [&](double d, int n, int v) {
-    if (wide_key(d) == key && place(n, v) > lo) return;
+    if (wide_key(d) == key && (i64)place_of(n, v) > lo) return;
     const int i = atomicAdd(&p.count[2], 1);
-    if (i < kWordsListed) p.d[i] = d, p.parent[i] = n, p.word[i] = v;
+    if (i < p.kWords) p.d[i] = d, p.place[i] = place_of(n, v);
   });
   __syncthreads();
   return min(p.count[2], W);
 }
 
-template <typename TIn, int VEC>
-__global__ void __launch_bounds__(kPickThreads) extend_pick_kernel(NodeArgs a, const float* __restrict__ scores,
-                                                                   float* __restrict__ outScores,
-                                                                   int* __restrict__ parents, int* __restrict__ words,
-                                                                   int W, int tiles, ExtendScratch s) {
+template <typename TIn, int VEC, int T>
+__global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float* __restrict__ scores,
+                                                        float* __restrict__ outScores, int* __restrict__ parents,
+                                                        int* __restrict__ words, int W, int tiles, ExtendScratch s) {
+  constexpr int kWarps = T / 32;
   extern __shared__ __align__(16) char shared[];
-  Picked& p = *reinterpret_cast<Picked*>(shared);
+  PickRoom<T>& r = *reinterpret_cast<PickRoom<T>*>(shared);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const i64 first = (i64)blockIdx.x * a.N;
   outScores += (i64)blockIdx.x * W;
   parents += (i64)blockIdx.x * W;
   words += (i64)blockIdx.x * W;
-  Group<kPickThreads> g(tid, p.scratch);
-  const Utterance<TIn, VEC> at{a, scores, s, first, tiles};
+  Group<T> g(tid, r.scratch);
+  const Utterance<TIn, VEC, T> at{a, scores + first, s, first, tiles, r};
+  // (what the scan does not write may be read before it ends)
+  for (int n = tid; n < min(a.N, kRowsHeld); n += T) at.hold(n);
+  if (tid < 4) r.count[tid] = 0;
+  if (tid == 4) r.close = 0;
+  __syncthreads();
   cudaGridDependencySynchronize();
 
-  // log-sum-exp of every row, a warp each
-  bool bad = false;
+  // every row's greatest score and sum, a warp each, four rows at a time
+  constexpr int kRows = 4;
 #pragma unroll 1
-  for (int n = warp; n < a.N; n += kPickWarps) {
-    const float score = scores[first + n];
-    double2 row = make_double2(0.0, -1.0 / 0.0);
-    if (score != neg_inf()) {
-      bad |= !(score < pos_inf());
-      if (at.node(n).here) {
-        const float2* t = s.sums + (first + n) * tiles;
-        float m = neg_inf();
-        for (int i = lane; i < tiles; i += 32) m = fmaxf(m, t[i].x);
-        m = warp_greatest(m);
-        double sum = 0.0;
-        for (int i = lane; i < tiles; i += 32) {
-          const float2 x = t[i];
-          // (no word: 0, or NaN where there is one)
-          sum += x.x > neg_inf() ? (double)x.y * exp((double)x.x - (double)m) : (double)x.y;
-        }
+  for (int n0 = warp; n0 < a.N; n0 += kRows * kWarps) {
+    float2 x[kRows];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        bad |= !(sum < 1.0 / 0.0);
-        if (m > neg_inf()) row = make_double2(m, (double)score - log(sum));
+    for (int k = 0; k < kRows; ++k) {
+      const int n = n0 + k * kWarps;
+      x[k] = make_float2(neg_inf(), 0.0f);
+      if (n < a.N && lane < tiles && at.kind(n) == kExtended) x[k] = s.sums[(first + n) * tiles + lane];
+    }
+    float m[kRows], sum[kRows];
+    // (no word: 0, or NaN where there is one)
+    auto weight = [](float2 y, float most) {
+      return y.x > neg_inf() ? y.y * ex2((y.x - most) * 1.4426950408889634f) : y.y;
+    };
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      m[k] = x[k].x;
+      if (tiles > 32) {
+        const int n = min(n0 + k * kWarps, a.N - 1);
+        const float2* t = s.sums + (first + n) * tiles;
+        double all = 0.0;
+        if (n == n0 + k * kWarps && at.kind(n) == kExtended) {
+          for (int i = lane + 32; i < tiles; i += 32) m[k] = fmaxf(m[k], t[i].x);
+          m[k] = warp_greatest(m[k]);
+          for (int i = lane; i < tiles; i += 32) {
+            all += weight(t[i], m[k]);
+            if (T == 256 || (i64)n * tiles + i < kTilesHeld) r.top[n * tiles + i] = t[i].x;
+          }
+        }
+        sum[k] = (float)all;
+      } else {
+        m[k] = warp_greatest(m[k]);
+        sum[k] = weight(x[k], m[k]);
+        const i64 t = (i64)(n0 + k * kWarps) * tiles + lane;
+        if (n0 + k * kWarps < a.N && lane < tiles && (T == 256 || t < kTilesHeld)) r.top[t] = x[k].x;
       }
     }
-    if (lane == 0) s.row[first + n] = row;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      sum[k] = warp_sum(sum[k]);
+      if (lane == 0 && n0 + k * kWarps < a.N) at.set_row(n0 + k * kWarps, make_double2(m[k], sum[k]));
+    }
   }
-  if (tid < 4) p.count[tid] = 0;
-  if (tid == 4) p.close = 0;
+  __syncthreads();
+  bool bad = false;
+#pragma unroll 1
+  for (int n = tid; n < a.N; n += T) {
+    const Kind kind = at.kind(n);
+    double2 row = at.row(n);
+    if (kind != kNotThere) bad |= !(at.score(n) < pos_inf());
+    if (kind == kExtended) bad |= !(row.y < 1.0 / 0.0);
+    row.y = kind == kExtended && row.x > -1.0 / 0.0 ? (double)at.score(n) - log(row.y) : -1.0 / 0.0;
+    at.set_row(n, row);
+  }
   if (__syncthreads_or(bad)) {
-    for (int i = tid; i < W; i += kPickThreads)
-      outScores[i] = __int_as_float(0x7fffffff), parents[i] = -1, words[i] = -1;
+    for (int i = tid; i < W; i += T) outScores[i] = __int_as_float(0x7fffffff), parents[i] = -1, words[i] = -1;
     return;
   }
 
-  // tiles: [0, N * tiles), then the hypotheses that are finished
-  const i64 rowTiles = (i64)a.N * tiles, allTiles = rowTiles + a.N;
-  auto tile_key = [&](i64 t) {
-    double d;
-    if (t < rowTiles) {
-      const double2 row = at.at_row((int)(t / tiles));
-      if (row.y == -1.0 / 0.0) return 0u;
-      d = at.value(row, s.sums[first * tiles + t].x);
-    } else {
-      const int n = (int)(t - rowTiles);
-      if (!at.finished(n)) return 0u;
-      d = scores[first + n];
+  // tiles, and the hypotheses that are finished; all of them where they are few
+  const i64 rowTiles = at.all_tiles(), allTiles = rowTiles + a.N;
+  unsigned least = with_slack(0), mine = 0;
+  if (allTiles > r.kTiles) {
+#pragma unroll 1
+    for (i64 t = tid; t < allTiles; t += T) {
+      const unsigned key = at.tile_key(t);
+      if (T == 256 || t < kTilesHeld) r.tileKey[t] = key;   // (in the place of what it comes from)
+      mine = max(mine, key);
     }
-    const float x = (float)d;
-    return x > neg_inf() ? score_key(x) : d > -1.0 / 0.0 ? score_key(neg_inf()) + 1 : 0u;
-  };
-  unsigned mine = 0;
+    least = with_slack(reached_by<T>(mine, W, r, g));
+  }
 #pragma unroll 1
-  for (i64 t = tid; t < allTiles; t += kPickThreads) mine = max(mine, tile_key(t));
-  unsigned least = with_slack(reached_by(mine, W, g));
-#pragma unroll 1
-  for (i64 t = tid; t < allTiles; t += kPickThreads)
-    if (tile_key(t) >= least) {
-      const int i = atomicAdd(&p.count[0], 1);
-      if (i < kTilesListed) p.tile[i] = t;
+  for (i64 t = tid; t < allTiles; t += T)
+    if ((allTiles > r.kTiles && (T == 256 || t < kTilesHeld) ? r.tileKey[t] : at.tile_key(t)) >= least) {
+      const int i = atomicAdd(&r.count[0], 1);
+      if (i < r.kTiles) r.tile[i] = at.listed(t);
     }
   __syncthreads();
-  bool many = p.count[0] > kTilesListed;
-  const int listed = min(p.count[0], kTilesListed);
+  bool many = r.count[0] > r.kTiles;
 
   // their chunks
-  auto chunk_key = [&](i64 t) {
-    if (t >= rowTiles) return lane == 0 ? tile_key(t) : 0u;
-    const float top = s.best[(first * tiles + t) * 32 + lane];
-    if (top == neg_inf()) return 0u;
-    return max(score_key((float)at.value(at.at_row((int)(t / tiles)), top)), score_key(neg_inf()) + 1);
-  };
   if (!many) {
+    const int listed = r.count[0];
     mine = 0;
+    constexpr int kBatch = 8;
 #pragma unroll 1
-    for (int i = warp; i < listed; i += kPickWarps) mine = max(mine, chunk_key(p.tile[i]));
-    least = max(least, with_slack(reached_by(mine, W, g)));
+    for (int i0 = warp; i0 < listed; i0 += kBatch * kWarps) {
+      float top[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const ListedTile& t = r.tile[min(i0 + j * kWarps, listed - 1)];
+        const i64 place = ((first + t.n) * tiles + max(t.tile, 0)) * 32 + lane;
+        top[j] = t.tile >= 0 ? s.best[place] : lane == 0 ? 0.0f : neg_inf();
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kWarps;
+        if (i >= listed) break;
+        const unsigned key = extension_key(at.value(r.tile[i].row, top[j]));
+        r.chunkKey[i * 32 + lane] = key;
+        mine = max(mine, key);
+      }
+    }
+    least = max(least, with_slack(reached_by<T>(mine, W, r, g)));
 #pragma unroll 1
-    for (int i = warp; i < listed; i += kPickWarps)
-      if (chunk_key(p.tile[i]) >= least) {
-        const int k = atomicAdd(&p.count[1], 1);
-        if (k < kChunksListed) p.chunk[k] = i * 32 + lane;
+    for (int i = warp; i < listed; i += kWarps)
+      if (r.chunkKey[i * 32 + lane] >= least) {
+        const int k = atomicAdd(&r.count[1], 1);
+        if (k < r.kChunks) r.chunk[k] = i * 32 + lane;
       }
     __syncthreads();
-    many = p.count[1] > kChunksListed;
+    many = r.count[1] > r.kChunks;
   }
 
   // their words
   int c = 0;
   if (!many) {
-    const int chunks = p.count[1];
+    const int chunks = r.count[1];
+    constexpr int kBatch = 8;   // chunks on their way at a time
 #pragma unroll 1
-    for (int k = warp; k < chunks; k += kPickWarps) {
-      const i64 t = p.tile[p.chunk[k] >> 5];
-      int n = (int)(t - rowTiles), v = -1;
-      double d;
-      bool in;
-      if (t >= rowTiles) {
-        d = scores[first + n];
-        in = lane == 0;
-      } else {
-        n = (int)(t / tiles);
-        v = chunk_word<VEC>((int)(t % tiles), p.chunk[k] & 31, lane);
-        in = v < a.V;
-        const NodeScores<TIn> row = at.node(n);
-        const float z = in ? to_f32(row.e[v]) + to_f32(row.p[v]) : neg_inf();
-        d = at.value(at.at_row(n), z);
-        in = z > neg_inf() && max(score_key((float)d), score_key(neg_inf()) + 1) >= least;
+    for (int k0 = warp; k0 < chunks; k0 += kBatch * kWarps) {
+      float z[kBatch];
+      TIn e[kBatch], p[kBatch];
+      unsigned words = 0;   // bit j: this lane has a word of the j-th chunk
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int k = min(k0 + j * kWarps, chunks - 1), chunk = r.chunk[k];
+        const ListedTile& t = r.tile[chunk >> 5];
+        const int v = chunk_word<VEC>(t.tile, chunk & 31, lane);
+        const bool in = t.tile >= 0 && v < a.V;
+        words |= in ? 1u << j : 0u;
+        if (in) e[j] = at.frame_at(t.e)[v];
+        if (in) p[j] = at.position_at(t.p)[v];
       }
-      if (in) {
-        const int i = atomicAdd(&p.count[2], 1);
-        if (i < kWordsListed) p.d[i] = d, p.parent[i] = n, p.word[i] = v;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) z[j] = words >> j & 1 ? to_f32(e[j]) + to_f32(p[j]) : neg_inf();
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int k = k0 + j * kWarps;
+        if (k >= chunks) break;
+        const ListedTile& t = r.tile[r.chunk[k] >> 5];
+        if (t.tile < 0 && lane == 0) z[j] = 0.0f;
+        const double d = at.value(t.row, z[j]);
+        if (extension_key(d) < least) continue;
+        const int v = t.tile < 0 ? -1 : chunk_word<VEC>(t.tile, r.chunk[k] & 31, lane);
+        const int i = atomicAdd(&r.count[2], 1);
+        if (i < r.kWords) r.d[i] = d, r.place[i] = place_of(t.n, v);
       }
     }
     __syncthreads();
-    c = p.count[2];
-    many = c > kWordsListed;
+    c = r.count[2];
+    many = c > r.kWords;
   }
   const bool exact = many;
-  if (many) c = general_pick<TIn, VEC>(at, W, p, g);
+  if (many) c = general_pick<TIn, VEC, T>(at, W, g);
+
+  // of many words those that can be among the best
+  if (c > 2 * W + 64) {
+    mine = 0;
+    for (int i = tid; i < c; i += T) mine = max(mine, extension_key(r.d[i]));
+    least = with_slack(reached_by<T>(mine, W, r, g));
+#pragma unroll 1
+    for (int i0 = 0; i0 < c; i0 += T) {   // (in place: what is written lies before what is read)
+      const int i = i0 + tid;
+      const bool in = i < c && extension_key(r.d[i]) >= least;
+      const double d = in ? r.d[i] : 0.0;
+      const Place place = in ? r.place[i] : 0;
+      __syncthreads();
+      if (in) {
+        const int k = atomicAdd(&r.count[3], 1);
+        r.d[k] = d, r.place[k] = place;
+      }
+      __syncthreads();
+    }
+    c = r.count[3];
+  }
 
   // where each is in the order, and whether what it rests on is closer than the sums' errors
-  auto before = [&](int i, int j) {   // extension j comes before i
-    if (p.d[j] != p.d[i]) return p.d[j] > p.d[i];
-    return p.parent[j] != p.parent[i] ? p.parent[j] < p.parent[i] : p.word[j] < p.word[i];
-  };
-  for (int i = tid; i < c; i += kPickThreads) p.again[i] = 0;
+  for (int i = tid; i < c; i += T) r.again[i] = 0;
   __syncthreads();
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
+    constexpr int kShare = 4;   // threads that look at a quarter of the others each
 #pragma unroll 1
-    for (int i = tid; i < c; i += kPickThreads) {
+    for (int i0 = 0; i0 < c; i0 += T / kShare) {
+      const int i = i0 + tid / kShare;
+      const double d = r.d[min(i, c - 1)];
+      const Place place = r.place[min(i, c - 1)];
+      const int parent = parent_of(place);
       int rank = 0;
       bool close = false;
-#pragma unroll 1
-      for (int j = 0; j < c; ++j) {
-        rank += before(i, j) ? 1 : 0;
-        close |= p.parent[i] != p.parent[j] && fabs(p.d[i] - p.d[j]) <= 2.0 * kLseError;
+#pragma unroll 4
+      for (int j = tid % kShare; j < c; j += kShare) {
+        const double other = r.d[j];
+        const Place at = r.place[j];
+        rank += (other > d) | ((other == d) & (at < place));
+        close |= (parent_of(at) != parent) & (fabs(d - other) <= 2.0 * kLseError);
       }
+      rank += close ? 1 << 20 : 0;
+#pragma unroll
+      for (int o = 1; o < kShare; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      close = rank >= 1 << 20;
+      rank &= (1 << 20) - 1;
+      if (i >= c || tid % kShare != 0) continue;
       if (pass == 0 && !exact && close && rank < W) {
-        p.close = p.again[i] = 1;
+        r.close = r.again[i] = 1;
 #pragma unroll 1
         for (int j = 0; j < c; ++j)
-          if (p.parent[i] != p.parent[j] && fabs(p.d[i] - p.d[j]) <= 2.0 * kLseError) p.again[j] = 1;
+          if (parent_of(r.place[j]) != parent && fabs(d - r.d[j]) <= 2.0 * kLseError) r.again[j] = 1;
       }
-      if (rank < W) {
-        outScores[rank] = (float)p.d[i];
-        parents[rank] = p.parent[i];
-        words[rank] = p.word[i];
-      }
+      if (rank < W) outScores[rank] = (float)d, parents[rank] = parent, words[rank] = word_of(place);
     }
     __syncthreads();
-    if (pass > 0 || !p.close) break;
+    if (pass > 0 || !r.close) break;
     // 64 bits for the rows in question
 #pragma unroll 1
     for (int n = 0; n < a.N; ++n) {
       bool inQuestion = false;
-      for (int i = tid; i < c; i += kPickThreads)
-        inQuestion |= p.again[i] && p.parent[i] == n && p.word[i] >= 0;
+      for (int i = tid; i < c; i += T) inQuestion |= r.again[i] && parent_of(r.place[i]) == n && word_of(r.place[i]) >= 0;
       if (!__syncthreads_or(inQuestion)) continue;
       const double2 exactly = at.exact_row(n, g);
-      const NodeScores<TIn> row = at.node(n);
-      for (int i = tid; i < c; i += kPickThreads)
-        if (p.parent[i] == n && p.word[i] >= 0) {
-          const int v = p.word[i];
-          p.d[i] = at.value(exactly, to_f32(row.e[v]) + to_f32(row.p[v]));
+      const NodeScores<TIn> rows = at.rows(n);
+      for (int i = tid; i < c; i += T)
+        if (parent_of(r.place[i]) == n && word_of(r.place[i]) >= 0) {
+          const int v = word_of(r.place[i]);
+          r.d[i] = at.value(exactly, to_f32(rows.e[v]) + to_f32(rows.p[v]));
         }
       __syncthreads();
     }
   }
-  for (int i = c + tid; i < W; i += kPickThreads) outScores[i] = neg_inf(), parents[i] = -1, words[i] = -1;
+  for (int i = c + tid; i < W; i += T) outScores[i] = neg_inf(), parents[i] = -1, words[i] = -1;
 }
 
 }  // namespace
@@ -470,32 +715,43 @@ void launch_extend_beams(const NodeArgs& a, const float* scores, float* outScore
                          void* workspace, cudaStream_t stream) {
   if (a.B == 0) return;
   const int tiles = div_up(a.V, kTile);
+  if ((i64)a.N * tiles >= 0x7fff0000LL) throw std::invalid_argument("too many words and hypotheses");
   const ExtendScratch s = scratch_at(workspace, (i64)a.B * a.N, tiles);
   with_type(a.dtype, node_rows_aligned(a), [&](auto type, auto vec) {
     using TIn = decltype(type);
     constexpr int VEC = decltype(vec)::value;
     if (a.N > 0) {
-      // hypotheses per warp: as many as leave 20 warps per SM
+      // hypotheses per warp: as many as leave 64 warps per SM
       const i64 most = (i64)a.B * tiles * a.N;
-      const int perWarp = (int)std::max<i64>(1, std::min<i64>(std::min(a.N, 32), most / (148 * 20)));
-      const int groups = div_up(a.N, perWarp);
-      const i64 ctas = div_up64((i64)a.B * tiles * groups, kScanWarps);
-      if (ctas > 0x7fffffffLL) throw std::invalid_argument("too many words and hypotheses");
+      const int fewest = (int)std::max<i64>(1, std::min<i64>(std::min(a.N, 32), most / (148 * 64)));
+      const int groups = div_up(a.N, fewest), perWarp = div_up(a.N, groups);
+      const i64 warps = (i64)tiles * groups;
+      const int rows = std::min(a.B, 65535), layers = div_up(a.B, rows);
+      if (warps > 0x7fff0000LL || layers > 65535) throw std::invalid_argument("too many words and hypotheses");
       ScopedKernel prof("extend_scan", stream);
-      extend_scan_kernel<TIn, VEC><<<(unsigned)ctas, 32 * kScanWarps, 0, stream>>>(a, scores, tiles, perWarp, groups, s);
+      auto kernel = extend_scan_kernel<TIn, VEC>;
+      constexpr int smem = kScanSmem<TIn, VEC>;
+      if (smem > 40 * 1024) allow_dyn_smem(kernel, smem);
+      kernel<<<dim3((unsigned)div_up64(warps, kScanWarps), rows, layers), 32 * kScanWarps, smem, stream>>>(
+          a, scores, tiles, perWarp, groups, s);
       TB200_CHECK_LAUNCH();
     }
-    auto kernel = extend_pick_kernel<TIn, VEC>;
-    allow_dyn_smem(kernel, sizeof(Picked));
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(a.B), config.blockDim = dim3(kPickThreads);
-    config.dynamicSmemBytes = sizeof(Picked), config.stream = stream;
-    cudaLaunchAttribute early;   // (its launch overlaps the scan; it waits for the scan's end before it reads)
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early, config.numAttrs = 1;
-    ScopedKernel prof("extend_pick", stream);
-    TB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, scores, outScores, parents, words, W, tiles, s));
+    auto pick = [&](auto threads) {
+      constexpr int T = decltype(threads)::value;
+      auto kernel = extend_pick_kernel<TIn, VEC, T>;
+      allow_dyn_smem(kernel, sizeof(PickRoom<T>));
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(a.B), config.blockDim = dim3(T);
+      config.dynamicSmemBytes = sizeof(PickRoom<T>), config.stream = stream;
+      cudaLaunchAttribute early;   // (its launch overlaps the scan; it waits for the scan's end before it reads its results)
+      early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      early.val.programmaticStreamSerializationAllowed = a.N > 0;
+      config.attrs = &early, config.numAttrs = 1;
+      ScopedKernel prof("extend_pick", stream);
+      TB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, scores, outScores, parents, words, W, tiles, s));
+    };
+    if (all_held(W, a.N, tiles)) pick(std::integral_constant<int, 256>{});
+    else pick(std::integral_constant<int, 1024>{});
   });
 }
 
