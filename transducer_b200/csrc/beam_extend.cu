@@ -476,8 +476,12 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
       const int n = n0 + k * kWarps;
-      x[k] = make_float2(neg_inf(), 0.0f);
-      if (n < a.N && lane < tiles && at.kind(n) == kExtended) x[k] = s.sums[(first + n) * tiles + lane];
+      x[k] = s.sums[(first + min(n, a.N - 1)) * tiles + min(lane, tiles - 1)];   // (whether or not it was written)
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int n = n0 + k * kWarps;
+      if (!(n < a.N && lane < tiles && at.kind(n) == kExtended)) x[k] = make_float2(neg_inf(), 0.0f);
     }
     float m[kRows], sum[kRows];
     // (no word: 0, or NaN where there is one)
@@ -533,11 +537,26 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
   const i64 rowTiles = at.all_tiles(), allTiles = rowTiles + a.N;
   unsigned least = with_slack(0), mine = 0;
   if (allTiles > r.kTiles) {
-#pragma unroll 1
-    for (i64 t = tid; t < allTiles; t += T) {
+    auto take = [&](i64 t) {
       const unsigned key = at.tile_key(t);
       if (T == 256 || t < kTilesHeld) r.tileKey[t] = key;   // (in the place of what it comes from)
       mine = max(mine, key);
+    };
+    if constexpr (T == 256) {   // (a warp a row: nothing is divided)
+#pragma unroll 2
+      for (int n = warp; n < a.N; n += kWarps) {
+        const double2 row = at.row(n);
+        for (int i = lane; i < tiles; i += 32) {
+          const int t = n * tiles + i;
+          const unsigned key = row.y > -1.0 / 0.0 ? extension_key(at.value(row, r.top[t])) : 0u;
+          r.tileKey[t] = key;
+          mine = max(mine, key);
+        }
+      }
+      for (i64 t = rowTiles + tid; t < allTiles; t += T) take(t);
+    } else {
+#pragma unroll 1
+      for (i64 t = tid; t < allTiles; t += T) take(t);
     }
     least = with_slack(reached_by<T>(mine, W, r, g));
   }
@@ -562,13 +581,14 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
       for (int j = 0; j < kBatch; ++j) {
         const ListedTile& t = r.tile[min(i0 + j * kWarps, listed - 1)];
         const i64 place = ((first + t.n) * tiles + max(t.tile, 0)) * 32 + lane;
-        top[j] = t.tile >= 0 ? s.best[place] : lane == 0 ? 0.0f : neg_inf();
+        top[j] = s.best[place];   // (whether or not it was written)
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int i = i0 + j * kWarps;
         if (i >= listed) break;
-        const unsigned key = extension_key(at.value(r.tile[i].row, top[j]));
+        const bool extends = r.tile[i].tile >= 0;
+        const unsigned key = extension_key(at.value(r.tile[i].row, extends ? top[j] : lane == 0 ? 0.0f : neg_inf()));
         r.chunkKey[i * 32 + lane] = key;
         mine = max(mine, key);
       }
