@@ -398,12 +398,20 @@ int tb200_distill_backward(const void* emissions, const void* predictions, int b
 /* ---- a beam search's step, and the words' embeddings that it goes on with ----
  * No counterpart in the reference, which decodes given transcripts only. */
 
+/* What a checked call wants to know of its indices: calls that take `beyond` (host memory that the device
+ * can write, device memory, or NULL) set beyond[0] to 1 where a frame, parent or word, and beyond[1]
+ * where a position is not below the size of its tensor, and else leave them alone.  tb200_flags_take:
+ * two such numbers, 0, in host memory; tb200_flags_wait waits for the calling thread's stream, copies
+ * them to values[2] (host memory) and takes them back. */
+int tb200_flags_take(int** flags);
+int tb200_flags_wait(int* flags, int* values);
+
 /* The best extensions of every utterance's hypotheses.  Hypothesis n < N of utterance b has the score
  * scores[b,n] (a log-probability) and is at the node frames[b,n], positions[b,n]; word v, the blank like
  * any other, extends it to
  *   d(n, v) = scores[b,n] + (z[v] - log sum exp(z)),   z[v] = E[b, frame, v] + P[b, position, v].
  * A hypothesis without a node is finished: it stays as it is, d(n, -1) = scores[b,n].  One with a score of
- * -inf is not there, and nothing is read for it; words whose z is -inf are no extensions.  The `width`
+ * -inf is not there, and nothing is read for it, whatever its node; words whose z is -inf are no extensions.  The `width`
  * (1 to 256) greatest are returned in order, of equal ones the lower parent, then the lower word
  * first: outScores, parents, words [B, width]; where there are fewer: -inf, -1, -1.  The order is
  * that of 64-bit arithmetic on z.  An utterance one of whose hypotheses has a score of NaN or +inf, or
@@ -413,7 +421,7 @@ int tb200_extend_beams(const void* emissions, const void* predictions, int bf16,
                        long long eStrideT, long long pStrideB, long long pStrideU, const int* frames,
                        const int* positions, const float* scores, float* outScores, int* parents,
                        int* words, int batchSize, int maxInputLength, int maxLabelLength,
-                       int alphabetSize, int nodes, int width, void* workspace,
+                       int alphabetSize, int nodes, int width, int* beyond, void* workspace,
                        size_t workspaceBytes);
 
 /* States that follow their hypotheses.  In each of `count` tensors (host array) the rowBytes bytes at
@@ -428,7 +436,7 @@ typedef struct {
   long long fromStrideB, fromStrideN, toStrideB, toStrideN, rowBytes;
 } tb200_states;
 int tb200_reorder_states(const tb200_states* states, int count, const int* parents, int batchSize,
-                         int hypotheses, int width, int kept);
+                         int hypotheses, int width, int kept, int* beyond);
 
 /* Rows of a table [R, H] (`stride` elements from one row to the next) for words [count]:
  *   rows[n,h] = factor * table[words[n], h] where number (n, h) stays, else 0,
@@ -442,7 +450,7 @@ int tb200_reorder_states(const tb200_states* states, int count, const int* paren
  * count is below 2^31 - 1, R 2^28 and H 2^23 at most. */
 int tb200_embed_words(const void* table, int bf16, long long stride, const int* words, long long count,
                       void* rows, int R, int H, double scale, double dropout, long long seed,
-                      const long long* seedAt);
+                      const long long* seedAt, int* beyond);
 size_t tb200_embed_backward_workspace_bytes(long long count, int R, int H);
 int tb200_embed_backward(const void* deltas, int bf16, const int* words, long long count, void* grad, int R,
                          int H, double scale, double dropout, long long seed, const long long* seedAt,

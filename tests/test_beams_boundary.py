@@ -156,7 +156,7 @@ def refused(rc, message):
 
 
 def extend_abi(B=1, T=2, U=2, V=8, N=2, width=2, strides=(16, 8, 16, 8), ws=P, nbytes=1 << 20):
-    return lib.tb200_extend_beams(P, P, 0, *strides, P, P, P, P, P, P, B, T, U, V, N, width, ws, nbytes)
+    return lib.tb200_extend_beams(P, P, 0, *strides, P, P, P, P, P, P, B, T, U, V, N, width, None, ws, nbytes)
 
 
 @pytest.mark.parametrize("change,message", [
@@ -182,7 +182,7 @@ class Moved(ctypes.Structure):
     ((64, 128, 16, 8, 16, 8, 8), (1 << 16, 1 << 15, 2), "too many hypotheses"),
     ((64, 128, 16, 8, 16, 8, 1 << 50), (1, 2, 2), "too large")])
 def test_abi_refuses_to_reorder(state, sizes, message):
-    refused(lib.tb200_reorder_states(ctypes.byref(Moved(*state)), 1, P, *sizes, 0), message)
+    refused(lib.tb200_reorder_states(ctypes.byref(Moved(*state)), 1, P, *sizes, 0, None), message)
 
 
 @pytest.mark.parametrize("change,message", [
@@ -194,7 +194,7 @@ def test_abi_refuses_to_embed(change, message):
     a = dict(stride=4, count=2, R=3, H=4, scale=1.0, dropout=0.0)
     a.update(change)
     refused(lib.tb200_embed_words(P, 0, a["stride"], P, a["count"], P, a["R"], a["H"], a["scale"], a["dropout"], 0,
-                                  None), message)
+                                  None, None), message)
     if "stride" not in change:
         refused(lib.tb200_embed_backward(P, 0, P, a["count"], P, a["R"], a["H"], a["scale"], a["dropout"], 0, None,
                                          P, 1 << 40), message)

@@ -236,6 +236,45 @@ def test_indices_beyond():
         extend_beams(E, P, frames, positions, scores, 2)
 
 
+def test_nodes_of_hypotheses_that_are_not_there():
+    """They are not looked at, nor checked; and a refused call leaves nothing behind for the next one."""
+    E, P, frames, positions, scores = hypotheses(2, 3, 4, 20, 3, done=0.0, gone=0.0)
+    for _ in range(3):
+        frames[0, 1], positions[0, 1], scores[0, 1] = 2 ** 30, 2 ** 31 - 1, -INF
+        check_extend([E, P, frames, positions, scores], 8)
+        scores[0, 1] = -1.0
+        with pytest.raises(ValueError, match="Frame index mismatch"):
+            extend_beams(E, P, frames, positions, scores, 2)
+
+
+def test_checked_calls_of_many_threads():
+    """Each sees its own indices."""
+    import threading
+    E, P, frames, positions, scores = hypotheses(2, 3, 4, 200, 3, done=0.0, gone=0.0)
+    bad = frames.clone()
+    bad[1, 1] = 3
+    wrong = []
+
+    def call(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for k in range(30):
+                refused = False
+                try:
+                    extend_beams(E, P, bad if (i + k) % 3 == 0 else frames, positions, scores, 2)
+                except ValueError:
+                    refused = True
+                if refused != ((i + k) % 3 == 0):
+                    wrong.append((i, k))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_results_are_detached_and_the_same_from_run_to_run():
     args = hypotheses(4, 3, 4, 5000, 12, seed=11)
     args[0].requires_grad_(True)
@@ -390,6 +429,10 @@ def test_parents_beyond():
     with pytest.raises(ValueError, match="Parent index mismatch"):
         reorder_states(s, parents)
     assert reorder_states(s, parents, validate_parents=False).tolist() == [[[0.0, 1.0], [0.0, 0.0]]]
+    with pytest.raises(ValueError, match="Parent index mismatch"):
+        reorder_states([s[..., :0]], parents)
+    with pytest.raises(ValueError, match="Parent index mismatch"):
+        reorder_states(s, parents, out=s[:, :2])
     assert reorder_states(s, parents[:, :0]).shape == (1, 0, 2)
     assert not reorder_states(s[:, :0], torch.full((1, 2), -1, dtype=torch.int32).cuda()).any()
 
@@ -503,6 +546,10 @@ def test_words_beyond():
     words[1, 1], words[0, 2] = 6, 2 ** 31 - 1
     with pytest.raises(ValueError, match="Word index mismatch"):
         embed_words(table, words)
+    with pytest.raises(ValueError, match="Word index mismatch"):
+        embed_words(table[:, :0], words)
+    with pytest.raises(ValueError, match="Word index mismatch"):
+        embed_words(table.detach().requires_grad_(True), words)
     words[0, 3] = -2 ** 31
     rows = embed_words(table.requires_grad_(True), words, validate_words=False)
     grad, = torch.autograd.grad(rows.sum(), table)

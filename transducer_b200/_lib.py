@@ -76,9 +76,11 @@ SIGNATURES = {
     "tb200_distill_backward": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 4 + [_z] + [_p] * 3 + [_i] * 6
                                + [_d, _p, _z]),
     "tb200_extend_beams_workspace_bytes": (_z, [_i] * 3),
-    "tb200_extend_beams": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 6 + [_i] * 6 + [_p, _z]),
-    "tb200_reorder_states": (_i, [_p, _i, _p] + [_i] * 4),
-    "tb200_embed_words": (_i, [_p, _i, _l, _p, _l, _p, _i, _i, _d, _d, _l, _p]),
+    "tb200_extend_beams": (_i, [_p] * 2 + [_i] + [_l] * 4 + [_p] * 6 + [_i] * 6 + [_p, _p, _z]),
+    "tb200_reorder_states": (_i, [_p, _i, _p] + [_i] * 4 + [_p]),
+    "tb200_flags_take": (_i, [ctypes.POINTER(_p)]),
+    "tb200_flags_wait": (_i, [_p, ctypes.POINTER(_i)]),
+    "tb200_embed_words": (_i, [_p, _i, _l, _p, _l, _p, _i, _i, _d, _d, _l, _p, _p]),
     "tb200_embed_backward_workspace_bytes": (_z, [_l, _i, _i]),
     "tb200_embed_backward": (_i, [_p, _i, _p, _l, _p, _i, _i, _d, _d, _l, _p, _p, _z]),
     "tb200_loss_sum_exchange": (_i, [_p, _p, _i, _i, ctypes.c_uint, _p, ctypes.c_uint]),

@@ -12,8 +12,7 @@ CUDA tensors only, like `TransducerLoss`; the work is enqueued on torch's curren
 import torch
 
 from . import _transducer
-from .nodes import (MAX_LISTED_WORDS, OnDevice, _describe, _rows, certify_indices, certify_nodes, check_device,
-                    check_no_tangents)
+from .nodes import (MAX_LISTED_WORDS, OnDevice, _describe, _rows, certify_nodes, check_device, check_no_tangents)
 from .torch_binding import check_contiguous, check_dim, check_type
 
 MAX_REORDERED_WIDTH = 8192
@@ -31,7 +30,8 @@ def extend_beams(emissions, predictions, frames, positions, scores, width, valid
     equal ones the lower parent, then the lower word; -inf, -1, -1 where there are fewer (words whose z is
     -inf are none).  The order is that of 64-bit arithmetic.  An utterance with a hypothesis whose score is
     NaN or +inf, or that has such a z, gets NaN, -1, -1.  The results are detached from the inputs' graph.
-    ``validate_nodes``: see `top_words`; an index beyond its tensor is taken for no node."""
+    ``validate_nodes=False`` skips the check that no node of a hypothesis lies beyond its tensor (an index that does
+    is taken for none), which waits for the kernels, so that the call only enqueues work."""
     certify_nodes(emissions, predictions, frames, positions)
     check_no_tangents(emissions, predictions, scores)
     check_dim(scores, 2, "scores")
@@ -52,11 +52,11 @@ def extend_beams(emissions, predictions, frames, positions, scores, width, valid
         described, sizes = _describe(emissions, predictions, frames)
         nbytes = _transducer.extend_beams_workspace_bytes(B, sizes[3], N)
         ws = frames.new_empty((nbytes + 3) // 4)
-        _transducer.extend_beams(described, frames.data_ptr(), positions.data_ptr(), scores.data_ptr(),
-                                 best.data_ptr(), parents.data_ptr(), words.data_ptr(), sizes, width,
-                                 ws.data_ptr(), nbytes)
-        if validate_nodes:
-            certify_indices(emissions, predictions, frames, positions)
+        beyond = _transducer.extend_beams(described, frames.data_ptr(), positions.data_ptr(), scores.data_ptr(),
+                                          best.data_ptr(), parents.data_ptr(), words.data_ptr(), sizes, width,
+                                          validate_nodes, ws.data_ptr(), nbytes)
+    if beyond:
+        raise ValueError("Frame index mismatch" if beyond & 1 else "Position index mismatch")
     return best, parents, words
 
 
@@ -120,12 +120,13 @@ def reorder_states(states, parents, out=None, validate_parents=True):
                 moved += at, to, from_b, from_n, to_b, to_n, size
         if not made:
             _check_apart(rows, out, B, N, W)
+        beyond = 0
         if B * W:
-            _transducer.reorder_states(moved, parents.data_ptr(), B, N, W, not made)
+            beyond = _transducer.reorder_states(moved, parents.data_ptr(), B, N, W, not made, validate_parents)
             if not made:   # (written behind autograd's back)
                 torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
-            if validate_parents:
-                certify_parents(parents, N)
+    if beyond:
+        raise ValueError("Parent index mismatch")
     return out[0] if single else list(out)
 
 
@@ -142,14 +143,6 @@ def _check_outputs(states, out, parents):
         if o.requires_grad:
             raise ValueError("out must not require gradients")
     check_device(parents, *out)
-
-
-def certify_parents(parents, N):
-    """That no parent lies beyond the N hypotheses; see nodes.certify_indices."""
-    scratch = torch.empty(_transducer.node_summary_scratch_bytes, dtype=torch.uint8, device=parents.device)
-    most = _transducer.node_summary(0, 0, 0, parents.data_ptr(), parents.numel(), scratch.data_ptr())[2]
-    if most >= N:
-        raise ValueError("Parent index mismatch")
 
 
 def _row(s):

@@ -34,6 +34,31 @@ void check(int rc) {
   throw std::runtime_error(tb200_last_error());
 }
 
+// Which indices of a checked call are beyond their tensors: bit 0 frames, parents or words, bit 1 positions.
+class Beyond {
+ public:
+  explicit Beyond(bool wanted) {
+    if (wanted) check(tb200_flags_take(&flags_));
+  }
+  Beyond(const Beyond&) = delete;
+  Beyond& operator=(const Beyond&) = delete;
+  ~Beyond() {   // (the call has failed; kernels of it may still run)
+    int values[2];
+    if (flags_) tb200_flags_wait(flags_, values);
+  }
+  int* flags() const { return flags_; }
+  int wait() {
+    if (!flags_) return 0;
+    int values[2], *flags = flags_;
+    flags_ = nullptr;
+    check(tb200_flags_wait(flags, values));
+    return (values[0] ? 1 : 0) | (values[1] ? 2 : 0);
+  }
+
+ private:
+  int* flags_ = nullptr;
+};
+
 }  // namespace
 
 PYBIND11_MODULE(_transducer, m) {
@@ -253,35 +278,42 @@ PYBIND11_MODULE(_transducer, m) {
   m.def("extend_beams_workspace_bytes", &tb200_extend_beams_workspace_bytes);
   m.def("extend_beams",
         [](const Scores& s, addr frames, addr positions, addr scores, addr out_scores, addr parents, addr words,
-           const Sizes& n, int width, addr ws, size_t ws_bytes) {
+           const Sizes& n, int width, bool validate, addr ws, size_t ws_bytes) {
+          Beyond beyond(validate);
           check(tb200_extend_beams(at<const void>(std::get<0>(s)), at<const void>(std::get<1>(s)), std::get<2>(s),
                                    std::get<3>(s), std::get<4>(s), std::get<5>(s), std::get<6>(s),
                                    at<const int>(frames), at<const int>(positions), at<const float>(scores),
                                    at<float>(out_scores), at<int>(parents), at<int>(words), std::get<0>(n),
                                    std::get<1>(n), std::get<2>(n), std::get<3>(n), std::get<4>(n), width,
-                                   at<void>(ws), ws_bytes));
+                                   beyond.flags(), at<void>(ws), ws_bytes));
+          return beyond.wait();
         },
         "scores"_a, "frames"_a, "positions"_a, "beam_scores"_a, "out_scores"_a, "parents"_a, "words"_a, "sizes"_a,
-        "width"_a, "workspace"_a, "workspace_bytes"_a);
+        "width"_a, "validate"_a, "workspace"_a, "workspace_bytes"_a);
   // `states`: of each tensor from, to, their strides in bytes by utterance and by hypothesis, bytes of a row
   m.def("reorder_states",
-        [](const std::vector<long long>& states, addr parents, int B, int N, int W, bool kept) {
+        [](const std::vector<long long>& states, addr parents, int B, int N, int W, bool kept, bool validate) {
+          Beyond beyond(validate);
           std::vector<tb200_states> all;
           for (size_t i = 0; i + 7 <= states.size(); i += 7) {
             const long long* s = &states[i];
             all.push_back(tb200_states{at<const void>((addr)s[0]), at<void>((addr)s[1]), s[2], s[3], s[4], s[5], s[6]});
           }
-          check(tb200_reorder_states(all.data(), (int)all.size(), at<const int>(parents), B, N, W, kept));
+          check(tb200_reorder_states(all.data(), (int)all.size(), at<const int>(parents), B, N, W, kept,
+                                     beyond.flags()));
+          return beyond.wait();
         },
-        "states"_a, "parents"_a, "batch_size"_a, "hypotheses"_a, "width"_a, "kept"_a);
+        "states"_a, "parents"_a, "batch_size"_a, "hypotheses"_a, "width"_a, "kept"_a, "validate"_a);
   m.def("embed_words",
         [](addr table, bool bf16, long long stride, addr words, long long count, addr rows, int R, int H, double scale,
-           double dropout, long long seed, addr seed_at) {
+           double dropout, long long seed, addr seed_at, bool validate) {
+          Beyond beyond(validate);
           check(tb200_embed_words(at<const void>(table), bf16, stride, at<const int>(words), count, at<void>(rows), R, H,
-                                  scale, dropout, seed, at<const long long>(seed_at)));
+                                  scale, dropout, seed, at<const long long>(seed_at), beyond.flags()));
+          return beyond.wait();
         },
         "table"_a, "bf16"_a, "stride"_a, "words"_a, "count"_a, "rows"_a, "R"_a, "H"_a, "scale"_a, "dropout"_a, "seed"_a,
-        "seed_at"_a);
+        "seed_at"_a, "validate"_a);
   m.def("embed_backward_workspace_bytes", &tb200_embed_backward_workspace_bytes);
   m.def("embed_backward",
         [](addr deltas, bool bf16, addr words, long long count, addr grad, int R, int H, double scale, double dropout,

@@ -1,7 +1,9 @@
 // C ABI of the states that follow a beam search's hypotheses and of words' embeddings (include/transducer_b200.h, last
-// part).
+// part), and the flags that checked calls read.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
+#include <vector>
 
 #include "api_guard.h"
 #include "kernels.h"
@@ -21,6 +23,26 @@ EmbedArgs embed_args(const void* table, int bf16, long long stride, const int* w
   return EmbedArgs{table, stride, words, count, R, H, bf16 ? kDtypeBf16 : kDtypeF32, (float)factor, dropped, seed, seedAt};
 }
 
+// Flags that no call uses at present, all 0.  A call's kernels write its own in host memory, only where an index is
+// beyond its tensor: to read them takes the wait for the stream and no copy.
+std::mutex g_flags;
+std::vector<int*> g_free;
+constexpr int kFlagsAtOnce = 64, kFlagInts = 16;   // (64 bytes each)
+
+int* take_flags() {
+  std::lock_guard<std::mutex> lock(g_flags);
+  if (g_free.empty()) {
+    int* p = nullptr;
+    const unsigned how = cudaHostAllocPortable | cudaHostAllocMapped;
+    TB200_CUDA_CHECK(cudaHostAlloc(&p, kFlagsAtOnce * kFlagInts * sizeof(int), how));
+    std::fill(p, p + kFlagsAtOnce * kFlagInts, 0);
+    for (int i = 0; i < kFlagsAtOnce; ++i) g_free.push_back(p + i * kFlagInts);
+  }
+  int* flags = g_free.back();
+  g_free.pop_back();
+  return flags;
+}
+
 }  // namespace
 }  // namespace tb200
 
@@ -28,7 +50,28 @@ using namespace tb200;
 
 extern "C" {
 
-int tb200_reorder_states(const tb200_states* states, int count, const int* parents, int B, int N, int W, int kept) {
+int tb200_flags_take(int** flags) {
+  return guarded([&] {
+    check(flags != nullptr, "null pointer");
+    *flags = take_flags();
+  });
+}
+
+int tb200_flags_wait(int* flags, int* values) {
+  return guarded([&] {
+    check(flags && values, "null pointer");
+    TB200_CUDA_CHECK(cudaStreamSynchronize(api_stream()));   // (where this fails the flags are not used again)
+    for (int i = 0; i < 2; ++i) {
+      values[i] = *static_cast<volatile int*>(flags + i);
+      flags[i] = 0;
+    }
+    std::lock_guard<std::mutex> lock(g_flags);
+    g_free.push_back(flags);
+  });
+}
+
+int tb200_reorder_states(const tb200_states* states, int count, const int* parents, int B, int N, int W, int kept,
+                         int* beyond) {
   return guarded([&] {
     check(count >= 0 && B >= 0 && N >= 0 && W >= 0, "negative number of states, utterances or hypotheses");
     check((long long)B * N < 0x7fffffffLL && (long long)B * W < 0x7fffffffLL,
@@ -41,19 +84,21 @@ int tb200_reorder_states(const tb200_states* states, int count, const int* paren
             "negative size or stride");
       check(s.rowBytes <= 1ll << 40, "the states are too large");
       if (s.from == s.to && s.from) {
-        check(s.fromStrideB == s.toStrideB && s.fromStrideN == s.toStrideN,
+        check((B <= 1 || s.fromStrideB == s.toStrideB) && (std::min(N, W) <= 1 || s.fromStrideN == s.toStrideN),
               "states that are reordered in place must keep their strides");
         check(W <= kMaxReorderedWidth, "at most 8192 hypotheses are reordered in place");
       }
     }
-    launch_reorder_states(reinterpret_cast<const States*>(states), count, parents, B, N, W, kept != 0, api_stream());
+    launch_reorder_states(reinterpret_cast<const States*>(states), count, parents, B, N, W, kept != 0, beyond,
+                          api_stream());
   });
 }
 
 int tb200_embed_words(const void* table, int bf16, long long stride, const int* words, long long count, void* rows,
-                      int R, int H, double scale, double dropout, long long seed, const long long* seedAt) {
+                      int R, int H, double scale, double dropout, long long seed, const long long* seedAt,
+                      int* beyond) {
   return guarded([&] {
-    launch_embed_words(embed_args(table, bf16, stride, words, count, R, H, scale, dropout, seed, seedAt), rows,
+    launch_embed_words(embed_args(table, bf16, stride, words, count, R, H, scale, dropout, seed, seedAt), rows, beyond,
                        api_stream());
   });
 }

@@ -450,7 +450,8 @@ __device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W
 template <typename TIn, int VEC, int T>
 __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float* __restrict__ scores,
                                                         float* __restrict__ outScores, int* __restrict__ parents,
-                                                        int* __restrict__ words, int W, int tiles, ExtendScratch s) {
+                                                        int* __restrict__ words, int W, int tiles, ExtendScratch s,
+                                                        int* beyond) {
   constexpr int kWarps = T / 32;
   extern __shared__ __align__(16) char shared[];
   PickRoom<T>& r = *reinterpret_cast<PickRoom<T>*>(shared);
@@ -462,7 +463,13 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
   Group<T> g(tid, r.scratch);
   const Utterance<TIn, VEC, T> at{a, scores + first, s, first, tiles, r};
   // (what the scan does not write may be read before it ends)
-  for (int n = tid; n < min(a.N, kRowsHeld); n += T) at.hold(n);
+  for (int n = tid; n < (beyond ? a.N : min(a.N, kRowsHeld)); n += T) {
+    if (n < kRowsHeld) at.hold(n);
+    if (beyond && scores[first + n] != neg_inf()) {
+      if (a.frames[first + n] >= a.T) beyond[0] = 1;
+      if (a.positions[first + n] >= a.U) beyond[1] = 1;
+    }
+  }
   if (tid < 4) r.count[tid] = 0;
   if (tid == 4) r.close = 0;
   __syncthreads();
@@ -732,7 +739,7 @@ size_t extend_workspace_bytes(int B, int V, int N) {
 }
 
 void launch_extend_beams(const NodeArgs& a, const float* scores, float* outScores, int* parents, int* words, int W,
-                         void* workspace, cudaStream_t stream) {
+                         int* beyond, void* workspace, cudaStream_t stream) {
   if (a.B == 0) return;
   const int tiles = div_up(a.V, kTile);
   if ((i64)a.N * tiles >= 0x7fff0000LL) throw std::invalid_argument("too many words and hypotheses");
@@ -768,7 +775,7 @@ void launch_extend_beams(const NodeArgs& a, const float* scores, float* outScore
       early.val.programmaticStreamSerializationAllowed = a.N > 0;
       config.attrs = &early, config.numAttrs = 1;
       ScopedKernel prof("extend_pick", stream);
-      TB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, scores, outScores, parents, words, W, tiles, s));
+      TB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, scores, outScores, parents, words, W, tiles, s, beyond));
     };
     if (all_held(W, a.N, tiles)) pick(std::integral_constant<int, 256>{});
     else pick(std::integral_constant<int, 1024>{});

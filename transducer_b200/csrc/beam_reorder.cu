@@ -38,7 +38,7 @@ __device__ __forceinline__ void move_row(const char* from, char* to, i64 bytes, 
 
 __global__ void __launch_bounds__(32 * kWarps) reorder_kernel(const __grid_constant__ Batch batch,
                                                               const int* __restrict__ parents, int N, int W,
-                                                              bool kept, i64 warps) {
+                                                              bool kept, i64 warps, int* beyond) {
   const i64 id = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (id >= warps) return;
@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(32 * kWarps) reorder_kernel(const __grid_const
   const i64 b = row / W, w = row % W;
   const int n = parents[row];
   const bool here = (unsigned)n < (unsigned)N;
+  if (beyond && n >= N) *beyond = 1;
   if (!here && kept) return;
   const i64 piece = 32ll * kBatch * it.bytes, at = (id - it.firstWarp) % it.pieces * piece;
   const i64 bytes = min(piece, it.s.rowBytes - at);
@@ -82,7 +83,7 @@ __device__ __forceinline__ void move_in_place(const States& s, const int* parent
 
 __global__ void __launch_bounds__(256) reorder_in_place_kernel(const __grid_constant__ Batch batch,
                                                                const int* __restrict__ parents, int N, int W,
-                                                               int held) {
+                                                               int held, int* beyond) {
   extern __shared__ __align__(16) char room[];
   const i64 id = blockIdx.x;
   int k = 0;
@@ -91,6 +92,9 @@ __global__ void __launch_bounds__(256) reorder_in_place_kernel(const __grid_cons
   const i64 b = (id - it.firstWarp) / it.pieces, at = (id - it.firstWarp) % it.pieces * held;
   const int units = (int)(min((i64)held, it.s.rowBytes - at) / it.bytes);
   parents += b * W;
+  if (beyond)
+    for (int w = threadIdx.x; w < W; w += blockDim.x)
+      if (parents[w] >= N) *beyond = 1;
   switch (it.bytes) {
     case 16: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<uint4*>(room)); break;
     case 8: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<uint2*>(room)); break;
@@ -111,7 +115,7 @@ int vector_bytes(const States& s) {
 }  // namespace
 
 void launch_reorder_states(const States* states, int count, const int* parents, int B, int N, int W, bool kept,
-                           cudaStream_t stream) {
+                           int* beyond, cudaStream_t stream) {
   if ((i64)B * W == 0) return;
   std::vector<Item> apart, inPlace;
   for (int i = 0; i < count; ++i) {
@@ -119,6 +123,8 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
     Item it{states[i], 0, 0, vector_bytes(states[i])};
     (states[i].from == states[i].to ? inPlace : apart).push_back(it);
   }
+  // (nothing is to be moved, but the parents are to be looked at)
+  if (beyond && count > 0 && apart.empty() && inPlace.empty()) apart.push_back(Item{states[0], 0, 0, 1});
   // a piece of a row in place: with W of them 32 KB, a vector at least
   const int held = std::max(16, 32 * 1024 / std::max(W, 1) / 16 * 16);
   for (size_t first = 0; first < apart.size(); first += kMostStates) {
@@ -127,12 +133,12 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
     for (size_t i = first; i < apart.size() && batch.count < kMostStates; ++i) {
       Item& it = batch.item[batch.count++] = apart[i];
       it.firstWarp = warps;
-      it.pieces = (int)div_up64(it.s.rowBytes, 32ll * kBatch * it.bytes);
+      it.pieces = (int)std::max<i64>(1, div_up64(it.s.rowBytes, 32ll * kBatch * it.bytes));
       warps += (i64)B * W * it.pieces;
     }
     if (div_up64(warps, kWarps) > 0x7fffffffLL) throw std::invalid_argument("the states are too large");
     ScopedKernel prof("reorder_states", stream);
-    reorder_kernel<<<(unsigned)div_up64(warps, kWarps), 32 * kWarps, 0, stream>>>(batch, parents, N, W, kept, warps);
+    reorder_kernel<<<(unsigned)div_up64(warps, kWarps), 32 * kWarps, 0, stream>>>(batch, parents, N, W, kept, warps, beyond);
     TB200_CHECK_LAUNCH();
   }
   for (size_t first = 0; first < inPlace.size(); first += kMostStates) {
@@ -147,7 +153,7 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
     if (ctas > 0x7fffffffLL) throw std::invalid_argument("the states are too large");
     allow_dyn_smem(reorder_in_place_kernel, 16 * kMaxReorderedWidth);
     ScopedKernel prof("reorder_in_place", stream);
-    reorder_in_place_kernel<<<(unsigned)ctas, 256, held * W, stream>>>(batch, parents, N, W, held);
+    reorder_in_place_kernel<<<(unsigned)ctas, 256, held * W, stream>>>(batch, parents, N, W, held, beyond);
     TB200_CHECK_LAUNCH();
   }
 }

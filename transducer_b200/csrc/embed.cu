@@ -120,13 +120,18 @@ __device__ __forceinline__ void stays(Stays<VEC> (&out)[K], N place, int first, 
 
 // A warp writes 256 numbers of each of ROWS rows that follow each other.
 template <typename T, int VEC, bool DROP, int ROWS>
-__global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __restrict__ rows) {
+__global__ void __launch_bounds__(32 * kWarps) embed_kernel(EmbedArgs a, T* __restrict__ rows, int* beyond) {
   const int lane = threadIdx.x & 31, first = blockIdx.y * 32 * kGroup;
   const i64 n0 = ((i64)blockIdx.x * kWarps + (threadIdx.x >> 5)) * ROWS;
   if (n0 >= a.N) return;
   int r[ROWS];
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) r[k] = n0 + k < a.N ? a.words[n0 + k] : -1;
+  if (beyond) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (r[k] >= a.R) *beyond = 1;
+  }
   Numbers<T, VEC> x[ROWS];
 #pragma unroll
   for (int k = 0; k < ROWS; ++k)
@@ -499,19 +504,19 @@ void launch_early(void (*kernel)(P...), dim3 ctas, int threads, cudaStream_t str
 
 }  // namespace
 
-void launch_embed_words(const EmbedArgs& a, void* rows, cudaStream_t stream) {
-  if (a.N == 0 || a.H == 0) return;
-  const int pieces = div_up(a.H, 32 * kGroup);
+void launch_embed_words(const EmbedArgs& a, void* rows, int* beyond, cudaStream_t stream) {
+  if (a.N == 0 || (a.H == 0 && !beyond)) return;
+  const int pieces = std::max(1, div_up(a.H, 32 * kGroup));   // (rows of nothing have words to look at)
   with_variant(a, aligned(a, rows), [&](auto type, auto vec, auto drop) {
     using T = decltype(type);
     constexpr int VEC = decltype(vec)::value;
     constexpr bool DROP = decltype(drop)::value;
     ScopedKernel prof("embed_words", stream);
     if (a.N * pieces <= 148 * 64)   // (a row per warp fits the chip at once)
-      embed_kernel<T, VEC, DROP, 1><<<dim3(ctas(a.N), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows));
+      embed_kernel<T, VEC, DROP, 1><<<dim3(ctas(a.N), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows), beyond);
     else
       embed_kernel<T, VEC, DROP, 4>
-          <<<dim3(ctas(div_up64(a.N, 4)), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows));
+          <<<dim3(ctas(div_up64(a.N, 4)), pieces), 32 * kWarps, 0, stream>>>(a, static_cast<T*>(rows), beyond);
     TB200_CHECK_LAUNCH();
   });
 }

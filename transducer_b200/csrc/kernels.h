@@ -311,10 +311,12 @@ void launch_distill_backward(const NodeArgs& a, const int* words, DistillSaved s
                              void* workspace, cudaStream_t stream);
 
 // ---- beam_extend.cu, beam_reorder.cu, embed.cu: a beam search's step, words' embeddings -------
+// beyond (may be null; host or device memory): a kernel sets [0] to 1 where a frame, parent or word, [1] where a position
+// is beyond its tensor.
 // scores, see tb200_extend_beams, for hypotheses at the nodes of `a`.
 size_t extend_workspace_bytes(int B, int V, int N);
 void launch_extend_beams(const NodeArgs& a, const float* scores, float* outScores, int* parents, int* words, int W,
-                         void* workspace, cudaStream_t stream);
+                         int* beyond, void* workspace, cudaStream_t stream);
 
 // One tensor of states: hypothesis n of utterance b has rowBytes bytes at from + b * fromB + n * fromN, and
 // hypothesis w of the next step gets them at to + b * toB + w * toW.  Strides in bytes.
@@ -326,7 +328,7 @@ struct States {
 constexpr int kMaxReorderedWidth = 8192;   // of hypotheses that are reordered in place
 // kept: rows without a parent stay as they are (else they become 0).
 void launch_reorder_states(const States* states, int count, const int* parents, int B, int N, int W, bool kept,
-                           cudaStream_t stream);
+                           int* beyond, cudaStream_t stream);
 
 // Rows of a table [R, H], `stride` elements from one to the next, for words [N].
 struct EmbedArgs {
@@ -341,7 +343,7 @@ struct EmbedArgs {
   i64 seed;
   const i64* seedAt;     // the seed is there (device memory), if not null
 };
-void launch_embed_words(const EmbedArgs& a, void* rows, cudaStream_t stream);
+void launch_embed_words(const EmbedArgs& a, void* rows, int* beyond, cudaStream_t stream);
 size_t embed_backward_workspace_bytes(i64 N, int R, int H);
 void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, void* workspace, cudaStream_t stream);
 

@@ -99,13 +99,13 @@ size_t tb200_extend_beams_workspace_bytes(int B, int V, int N) { return extend_w
 int tb200_extend_beams(const void* E, const void* P, int bf16, long long eStrideB, long long eStrideT,
                        long long pStrideB, long long pStrideU, const int* frames, const int* positions,
                        const float* scores, float* outScores, int* parents, int* words, int B, int maxT, int maxU,
-                       int V, int N, int width, void* workspace, size_t workspaceBytes) {
+                       int V, int N, int width, int* beyond, void* workspace, size_t workspaceBytes) {
   return guarded([&] {
     const NodeArgs a = node_args(E, P, bf16, eStrideB, eStrideT, pStrideB, pStrideU, frames, positions, B, maxT,
                                  maxU, V, N);
     check(width >= 1 && width <= kMaxListedWords, "the number of extensions must be between 1 and 256");
     need(workspaceBytes, extend_workspace_bytes(B, V, N), workspace, "workspace");
-    launch_extend_beams(a, scores, outScores, parents, words, width, workspace, api_stream());
+    launch_extend_beams(a, scores, outScores, parents, words, width, beyond, workspace, api_stream());
   });
 }
 

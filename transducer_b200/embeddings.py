@@ -70,21 +70,12 @@ def _rows_of(table, words, scale, dropout, seed, validate_words):
     numbers, place = _seed(seed)
     with OnDevice(table.device):
         rows = table.new_empty(words.shape + (H,))
-        _transducer.embed_words(table.data_ptr(), table.dtype is torch.bfloat16, table.stride(0), words.data_ptr(),
-                                words.numel(), rows.data_ptr(), R, H, scale, dropout, numbers, place)
-        if validate_words:
-            certify_words(words, R)
-    return rows
-
-
-def certify_words(words, R):
-    """That no word lies beyond the table; see nodes.certify_indices."""
-    if words.numel() == 0:
-        return
-    scratch = torch.empty(_transducer.node_summary_scratch_bytes, dtype=torch.uint8, device=words.device)
-    most = _transducer.node_summary(0, 0, 0, words.data_ptr(), words.numel(), scratch.data_ptr())[2]
-    if most >= R:
+        beyond = _transducer.embed_words(table.data_ptr(), table.dtype is torch.bfloat16, table.stride(0),
+                                         words.data_ptr(), words.numel(), rows.data_ptr(), R, H, scale, dropout,
+                                         numbers, place, validate_words)
+    if beyond:
         raise ValueError("Word index mismatch")
+    return rows
 
 
 def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=True):
