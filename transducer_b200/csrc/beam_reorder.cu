@@ -1,6 +1,7 @@
 // States that follow their hypotheses: row w of an utterance becomes what row parents[w] was, in every tensor of a
 // list at once.
 #include <algorithm>
+#include <cstdlib>
 #include <vector>
 
 #include "kernels.h"
@@ -10,12 +11,13 @@ namespace tb200 {
 namespace {
 
 constexpr int kMostStates = 24;        // of a launch (they travel as kernel arguments)
+constexpr int kShifted = -16, kShiftedRow = 64;   // rows that long are moved in vectors whatever their alignment
 constexpr int kWarps = 8, kBatch = 8;  // a warp moves kBatch vectors per lane at a time
 
 struct Item {
   States s;
-  i64 firstWarp;      // of the launch
-  int pieces, bytes;  // of a row; bytes of a vector
+  unsigned firstWarp;   // of the launch
+  int pieces, bytes;    // of a row; bytes of a vector (kShifted: see move_shifted)
 };
 struct Batch {
   Item item[kMostStates];
@@ -36,26 +38,57 @@ __device__ __forceinline__ void move_row(const char* from, char* to, i64 bytes, 
     if (lane + 32 * j < n) t[lane + 32 * j] = x[j];
 }
 
+// Bytes of any alignment: stored in 16-byte vectors, loaded as the aligned words that hold them.
+__device__ __forceinline__ void move_shifted(const char* from, char* to, int bytes, int lane) {
+  const int head = min(bytes, (int)(-(uintptr_t)to & 15)), vectors = (bytes - head) / 16, tail = head + 16 * vectors;
+  const char* at = from + head;
+  const int shift = (int)((uintptr_t)at & 3);
+  const unsigned* words = reinterpret_cast<const unsigned*>(at - shift);
+  unsigned x[kBatch][5];
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) {
+    const int v = lane + 32 * j;
+    if (v < vectors) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j][i] = from ? words[4 * v + i] : 0u;
+      x[j][4] = from && shift ? words[4 * v + 4] : 0u;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) {
+    const int v = lane + 32 * j;
+    if (v < vectors) {
+      uint4 y;
+      y.x = __funnelshift_r(x[j][0], x[j][1], 8 * shift), y.y = __funnelshift_r(x[j][1], x[j][2], 8 * shift);
+      y.z = __funnelshift_r(x[j][2], x[j][3], 8 * shift), y.w = __funnelshift_r(x[j][3], x[j][4], 8 * shift);
+      reinterpret_cast<uint4*>(to + head)[v] = y;
+    }
+  }
+  if (lane < head) to[lane] = from ? from[lane] : 0;
+  if (tail + lane < bytes) to[tail + lane] = from ? from[tail + lane] : 0;
+}
+
 __global__ void __launch_bounds__(32 * kWarps) reorder_kernel(const __grid_constant__ Batch batch,
                                                               const int* __restrict__ parents, int N, int W,
-                                                              bool kept, i64 warps, int* beyond) {
-  const i64 id = (i64)blockIdx.x * kWarps + (threadIdx.x >> 5);
+                                                              bool kept, unsigned warps, int* beyond) {
+  const unsigned id = blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (id >= warps) return;
   int k = 0;
   while (k + 1 < batch.count && batch.item[k + 1].firstWarp <= id) ++k;
   const Item& it = batch.item[k];
-  const i64 row = (id - it.firstWarp) / it.pieces;
-  const i64 b = row / W, w = row % W;
+  const unsigned row = (id - it.firstWarp) / (unsigned)it.pieces;
   const int n = parents[row];
+  const int b = row / (unsigned)W, w = row % (unsigned)W;
   const bool here = (unsigned)n < (unsigned)N;
   if (beyond && n >= N) *beyond = 1;
   if (!here && kept) return;
-  const i64 piece = 32ll * kBatch * it.bytes, at = (id - it.firstWarp) % it.pieces * piece;
+  const i64 piece = 32ll * kBatch * abs(it.bytes), at = (id - it.firstWarp) % (unsigned)it.pieces * piece;
   const i64 bytes = min(piece, it.s.rowBytes - at);
   const char* from = here ? it.s.from + b * it.s.fromB + n * it.s.fromN + at : nullptr;
   char* to = it.s.to + b * it.s.toB + w * it.s.toW + at;
   switch (it.bytes) {
+    case kShifted: move_shifted(from, to, (int)bytes, lane); break;
     case 16: move_row<uint4>(from, to, bytes, lane); break;
     case 8: move_row<uint2>(from, to, bytes, lane); break;
     case 4: move_row<unsigned>(from, to, bytes, lane); break;
@@ -85,11 +118,11 @@ __global__ void __launch_bounds__(256) reorder_in_place_kernel(const __grid_cons
                                                                const int* __restrict__ parents, int N, int W,
                                                                int held, int* beyond) {
   extern __shared__ __align__(16) char room[];
-  const i64 id = blockIdx.x;
+  const unsigned id = blockIdx.x;
   int k = 0;
   while (k + 1 < batch.count && batch.item[k + 1].firstWarp <= id) ++k;   // (CTAs here)
   const Item& it = batch.item[k];
-  const i64 b = (id - it.firstWarp) / it.pieces, at = (id - it.firstWarp) % it.pieces * held;
+  const i64 b = (id - it.firstWarp) / (unsigned)it.pieces, at = (id - it.firstWarp) % (unsigned)it.pieces * (i64)held;
   const int units = (int)(min((i64)held, it.s.rowBytes - at) / it.bytes);
   parents += b * W;
   if (beyond)
@@ -127,18 +160,25 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
   if (beyond && count > 0 && apart.empty() && inPlace.empty()) apart.push_back(Item{states[0], 0, 0, 1});
   // a piece of a row in place: with W of them 32 KB, a vector at least
   const int held = std::max(16, 32 * 1024 / std::max(W, 1) / 16 * 16);
-  for (size_t first = 0; first < apart.size(); first += kMostStates) {
+  for (size_t i = 0; i < apart.size();) {
     Batch batch{};
     i64 warps = 0;
-    for (size_t i = first; i < apart.size() && batch.count < kMostStates; ++i) {
-      Item& it = batch.item[batch.count++] = apart[i];
-      it.firstWarp = warps;
-      it.pieces = (int)std::max<i64>(1, div_up64(it.s.rowBytes, 32ll * kBatch * it.bytes));
-      warps += (i64)B * W * it.pieces;
+    for (; i < apart.size() && batch.count < kMostStates; ++i) {
+      Item it = apart[i];
+      if (it.bytes < 16 && it.s.rowBytes >= kShiftedRow) it.bytes = kShifted;
+      it.firstWarp = (unsigned)warps;
+      it.pieces = (int)std::max<i64>(1, div_up64(it.s.rowBytes, 32ll * kBatch * std::abs(it.bytes)));
+      const i64 more = (i64)B * W * it.pieces;
+      if (warps + more > 0xfffffff0LL) {
+        if (batch.count == 0) throw std::invalid_argument("the states are too large");
+        break;
+      }
+      batch.item[batch.count++] = it;
+      warps += more;
     }
-    if (div_up64(warps, kWarps) > 0x7fffffffLL) throw std::invalid_argument("the states are too large");
     ScopedKernel prof("reorder_states", stream);
-    reorder_kernel<<<(unsigned)div_up64(warps, kWarps), 32 * kWarps, 0, stream>>>(batch, parents, N, W, kept, warps, beyond);
+    reorder_kernel<<<(unsigned)div_up64(warps, kWarps), 32 * kWarps, 0, stream>>>(batch, parents, N, W, kept,
+                                                                                 (unsigned)warps, beyond);
     TB200_CHECK_LAUNCH();
   }
   for (size_t first = 0; first < inPlace.size(); first += kMostStates) {
@@ -146,7 +186,7 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
     i64 ctas = 0;
     for (size_t i = first; i < inPlace.size() && batch.count < kMostStates; ++i) {
       Item& it = batch.item[batch.count++] = inPlace[i];
-      it.firstWarp = ctas;
+      it.firstWarp = (unsigned)ctas;
       it.pieces = (int)div_up64(it.s.rowBytes, held);
       ctas += (i64)B * it.pieces;
     }

@@ -294,6 +294,68 @@ struct Parts {
   }
 };
 
+// Adds up 256 numbers of the rows of `count` places that follow each other, at(i) the i-th place and its word; `before` and
+// `behind` are the words next to them.  Rows that lie within are written to the gradient, the shares of others to
+// part(slot): 0 where the row is the first, 1 where it is a later one.
+template <typename T, int VEC, bool DROP, typename At, typename Part>
+__device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, int count, At at, int before, int behind,
+                                           int first, int lane, T* grad, Part part) {
+  constexpr int kBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows on their way while as many are added (more: registers)
+  const Seed seed(a);
+  float sum[kGroup] = {};
+  int row = at(0).y;
+  bool begins = true;   // the present row is the first
+  auto finish = [&](bool ends) {   // `ends`: it is the last
+    if (!(begins && row == before) && !(ends && row == behind)) {
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) sum[k] *= a.factor;
+      Numbers<T, VEC>::store(grad + (i64)row * a.H, first, lane, a.H, sum);
+    } else {
+      float4* p = part(begins ? 0 : 1, row);
+      p[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      p[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+    }
+  };
+  Numbers<T, VEC> next[kBatch];
+  auto bring = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int n = at(min(i + j, count - 1)).x;
+      if (i + j < count) next[j].load(deltas + (i64)n * a.H, first, lane, a.H);
+    }
+  };
+  bring(0);
+#pragma unroll 2
+  for (int i = 0; i < count; i += kBatch) {
+    Numbers<T, VEC> x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = next[j];
+    bring(i + kBatch);
+    Stays<VEC> stay[kBatch];
+    if constexpr (DROP)
+      stays<VEC, kBatch>(stay, [&](int k) { return at(min(i + k, count - 1)).x; }, first, lane, seed, a.dropped);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (i + j >= count) break;
+      const int r = at(i + j).y;
+      if (r != row) {
+        finish(false);
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) sum[k] = 0.0f;
+        row = r, begins = false;
+      }
+      float y[kGroup];
+      bool keep[kGroup] = {true, true, true, true, true, true, true, true};
+      x[j].get(y);
+      if constexpr (DROP) stay[j].get(keep, a.dropped);
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k)
+        if (keep[k]) sum[k] += y[k];
+    }
+  }
+  finish(true);
+}
+
 constexpr int kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
 
 // CTAs (x, piece): the warps of the first sumCtas add up 256 numbers of an item's rows each; the others fill rows that
@@ -301,7 +363,6 @@ constexpr int kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills 
 template <typename T, int VEC, bool DROP>
 __global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
                                                                  Parts parts, T* __restrict__ grad, int sumCtas) {
-  constexpr int kBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows on their way while as many are added (more: registers)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
@@ -322,64 +383,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a,
   if (item >= parts.items || item * (i64)parts.part >= all) return;
   const int from = item * parts.part;
   const int to = (int)min((i64)from + parts.part, (i64)all);
-  // lane i: the item's place i; the rows before it and behind it
+  // lane i: the item's place i
   const int2 mine = lane < to - from ? s.order[from + lane] : make_int2(0, -1);
+  auto at = [&](int i) {
+    return make_int2(__shfl_sync(0xffffffffu, mine.x, i & 31), __shfl_sync(0xffffffffu, mine.y, i & 31));
+  };
   const int before = from > 0 ? s.order[from - 1].y : -1, behind = to < all ? s.order[to].y : -1;
-  const Seed seed(a);
-  float sum[kGroup] = {};
-  int row = __shfl_sync(0xffffffffu, mine.y, 0);
-  bool begins = true;   // the present row is the item's first
-  auto finish = [&](bool ends) {   // `ends`: it is the item's last
-    const bool whole = !(begins && row == before) && !(ends && row == behind);
-    if (whole) {
-#pragma unroll
-      for (int k = 0; k < kGroup; ++k) sum[k] *= a.factor;
-      Numbers<T, VEC>::store(grad + (i64)row * a.H, first, lane, a.H, sum);
-    } else {
-      float4* p = parts.at(item, begins ? 0 : 1, piece, lane);
-      p[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
-      p[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
-    }
-  };
-  Numbers<T, VEC> next[kBatch];
-  auto bring = [&](int i) {
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int n = __shfl_sync(0xffffffffu, mine.x, (i + j) & 31);
-      if (i + j < to - from) next[j].load(deltas + (i64)n * a.H, first, lane, a.H);
-    }
-  };
-  bring(0);
-#pragma unroll 2
-  for (int i = 0; i < to - from; i += kBatch) {
-    Numbers<T, VEC> x[kBatch];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = next[j];
-    bring(i + kBatch);
-    Stays<VEC> stay[kBatch];
-    if constexpr (DROP)
-      stays<VEC, kBatch>(stay, [&](int k) { return __shfl_sync(0xffffffffu, mine.x, i + k); }, first, lane, seed,
-                         a.dropped);
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (i + j >= to - from) break;
-      const int r = __shfl_sync(0xffffffffu, mine.y, i + j);
-      if (r != row) {
-        finish(false);
-#pragma unroll
-        for (int k = 0; k < kGroup; ++k) sum[k] = 0.0f;
-        row = r, begins = false;
-      }
-      float y[kGroup];
-      bool keep[kGroup] = {true, true, true, true, true, true, true, true};
-      x[j].get(y);
-      if constexpr (DROP) stay[j].get(keep, a.dropped);
-#pragma unroll
-      for (int k = 0; k < kGroup; ++k)
-        if (keep[k]) sum[k] += y[k];
-    }
-  }
-  finish(true);
+  add_places<T, VEC, DROP>(a, deltas, to - from, at, before, behind, first, lane, grad,
+                           [&](int slot, int) { return parts.at(item, slot, piece, lane); });
 }
 
 constexpr int kJoinWarps = 16;
@@ -466,6 +477,119 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArg
   }
 }
 
+// ---- few words: all in one launch ---------------------------------------------------------------
+
+constexpr int kDirectWords = 4096, kDirectWarps = 8;
+
+struct DirectRoom {
+  int count[kDirectWarps][kSortRows];
+  int start[kSortRows + 1];
+  unsigned order[kDirectWords];   // (place, row of the CTA's)
+  float4 share[kDirectWarps][2][32][2];
+};
+
+// CTA (c, piece) of 2^bits has 256 numbers of the rows r with r mod 2^bits = c: it sorts its words as sort_words_kernel does,
+// adds them up, an eighth of the places per warp, and joins what lies with several warps.
+template <typename T, int VEC, bool DROP>
+__global__ void __launch_bounds__(32 * kDirectWarps, 2) embed_direct_kernel(EmbedArgs a, const T* __restrict__ deltas,
+                                                                            T* __restrict__ grad, int bits) {
+  constexpr int kOwn = kDirectWords / kDirectWarps / 32;   // words of a lane
+  extern __shared__ __align__(16) char shared[];
+  DirectRoom& room = *reinterpret_cast<DirectRoom*>(shared);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cta = blockIdx.x, low = (1 << bits) - 1, first = blockIdx.y * 32 * kGroup, N = (int)a.N;
+  const int seg = (div_up(N, kDirectWarps) + 31) / 32 * 32, from = warp * seg;
+  int r[kOwn], rank[kOwn];
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    const int i = 32 * j + lane;
+    r[j] = i < seg && from + i < N ? a.words[from + i] : -1;
+  }
+  for (int i = tid; i < kDirectWarps * kSortRows; i += 32 * kDirectWarps) (&room.count[0][0])[i] = 0;
+  __syncthreads();
+  int* const count = room.count[warp];
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    const bool in = (unsigned)r[j] < (unsigned)a.R && (r[j] & low) == cta;
+    const unsigned any = __ballot_sync(0xffffffffu, in);
+    rank[j] = -1;
+    if (in) {
+      const unsigned same = __match_any_sync(any, r[j]);
+      const int base = count[r[j] >> bits];
+      rank[j] = base + __popc(same & ((1u << lane) - 1));
+      __syncwarp(any);
+      if ((same & ((1u << lane) - 1)) == 0) count[r[j] >> bits] = base + __popc(same);
+      __syncwarp(any);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  {   // (thread i: row i of the CTA's)
+    int mine = 0;
+#pragma unroll
+    for (int w = 0; w < kDirectWarps; ++w) {
+      const int c = room.count[w][tid];
+      room.count[w][tid] = mine;
+      mine += c;
+    }
+    room.start[tid] = mine;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int sum[kSortRows / 32], all = 0;
+#pragma unroll
+    for (int i = 0; i < kSortRows / 32; ++i) sum[i] = all, all += room.start[lane * (kSortRows / 32) + i];
+    int upto = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+#pragma unroll
+    for (int i = 0; i < kSortRows / 32; ++i) room.start[lane * (kSortRows / 32) + i] = upto - all + sum[i];
+    if (lane == 31) room.start[kSortRows] = upto;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j)
+    if (rank[j] >= 0) {
+      const int row = r[j] >> bits;
+      room.order[room.start[row] + count[row] + rank[j]] = (unsigned)row << 16 | (unsigned)(from + 32 * j + lane);
+    }
+  __syncthreads();
+  const int all = room.start[kSortRows], part = div_up(all, kDirectWarps);
+  const int begin = warp * part, end = min(all, begin + part);
+  auto word = [&](int i) { return (int)(room.order[i] >> 16) << bits | cta; };
+  if (begin < end) {
+    auto at = [&](int i) { return make_int2((int)(room.order[begin + i] & 0xffffu), word(begin + i)); };
+    add_places<T, VEC, DROP>(a, deltas, end - begin, at, begin > 0 ? word(begin - 1) : -1, end < all ? word(end) : -1, first,
+                             lane, grad, [&](int slot, int) { return room.share[warp][slot][lane]; });
+  }
+  // rows that no word has
+  const float zero[kGroup] = {};
+#pragma unroll 1
+  for (int row = warp; row < kSortRows && (((i64)row << bits) | cta) < a.R; row += kDirectWarps)
+    if (room.start[row] == room.start[row + 1])
+      Numbers<T, VEC>::store(grad + (((i64)row << bits) | cta) * a.H, first, lane, a.H, zero);
+  __syncthreads();
+  // rows that lie with several warps, by the first of them
+  if (begin < end) {
+    const int row = room.order[end - 1] >> 16, last = (room.start[row + 1] - 1) / part;
+    if (room.start[row] / part == warp && last > warp) {
+      float sum[kGroup] = {};
+      for (int w = warp; w <= last; ++w) {
+        const float4* p = room.share[w][w == warp && room.start[row] != begin ? 1 : 0][lane];
+        const float4 x = p[0], y = p[1];
+        sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
+        sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
+      }
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) sum[k] *= a.factor;
+      Numbers<T, VEC>::store(grad + ((i64)row << bits | cta) * a.H, first, lane, a.H, sum);
+    }
+  }
+}
+
 // Places per item: few where there are few warps, so that the rows are read at once; their shares then weigh more.
 int places_per_item(i64 N, int pieces) { return N * pieces <= 32 * 148 * 16 ? 8 : kMostPart; }
 
@@ -488,6 +612,16 @@ unsigned ctas(i64 warps, int ofCta = kWarps) {
   const i64 n = div_up64(warps, ofCta);
   if (n > 0x7fffffffLL) throw std::invalid_argument("too many rows");
   return (unsigned)n;
+}
+
+// Whether the gradient is made in one launch.  A frequent word is one CTA's there, for every 256 numbers: of 4096 words in a
+// table of 30 rows it takes 23 us instead of 16 in three launches, in one of 1025 rows 16 instead of 17.
+bool in_one_launch(i64 N, int R) { return N <= kDirectWords && N <= 32ll * R && R <= 128 * kSortRows; }
+// CTAs that the rows are shared between, as a power of two: up to 128, and no more than 256 rows each.
+int row_bits(int R) {
+  int bits = 0;
+  while ((bits < 7 && 2 << bits <= R) || (i64)kSortRows << bits < R) ++bits;
+  return bits;
 }
 
 // The launches of one call: each begins while the one before it ends, and waits for its results.
@@ -524,6 +658,7 @@ void launch_embed_words(const EmbedArgs& a, void* rows, int* beyond, cudaStream_
 size_t embed_backward_workspace_bytes(i64 N, int R, int H) {
   if (N <= 0 || R <= 0 || H <= 0) return 0;
   const int pieces = div_up(H, 32 * kGroup);
+  if (in_one_launch(N, R)) return 0;
   return (size_t)(round_up64(N * 8, 16) + round_up64((R + 1ll) * 8, 16) +
                   div_up64(N, places_per_item(N, pieces)) * 2 * pieces * 32 * kGroup * 4);
 }
@@ -536,6 +671,21 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     return;
   }
   const int pieces = div_up(a.H, 32 * kGroup), part = places_per_item(a.N, pieces);
+  EmbedArgs d = a;
+  d.table = deltas, d.stride = a.H;
+  const bool wide = aligned(d, grad);
+  if (in_one_launch(a.N, a.R)) {
+    with_variant(a, wide, [&](auto type, auto vec, auto drop) {
+      using T = decltype(type);
+      auto kernel = embed_direct_kernel<T, decltype(vec)::value, decltype(drop)::value>;
+      const int bits = row_bits(a.R);
+      ScopedKernel prof("embed_direct", stream);
+      kernel<<<dim3(1u << bits, pieces), 32 * kDirectWarps, sizeof(DirectRoom), stream>>>(
+          a, static_cast<const T*>(deltas), static_cast<T*>(grad), bits);
+      TB200_CHECK_LAUNCH();
+    });
+    return;
+  }
   char* at = static_cast<char*>(workspace);
   Sorted s;
   s.order = reinterpret_cast<int2*>(at), at += round_up64(a.N * 8, 16);
@@ -543,8 +693,7 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
   s.R = a.R;
   const Parts parts{reinterpret_cast<float*>(at), part, pieces, (int)div_up64(a.N, part)};
   {
-    int bits = 0;   // CTAs: up to 128, and no more than 256 rows each
-    while ((bits < 7 && 2 << bits <= a.R) || (i64)kSortRows << bits < a.R) ++bits;
+    const int bits = row_bits(a.R);
     ScopedKernel prof("embed_sort", stream);
     auto sort = [&](auto warps) {
       constexpr int WARPS = decltype(warps)::value;
@@ -552,12 +701,10 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
       sort_words_kernel<WARPS><<<1u << bits, 32 * WARPS, sizeof(SortRoom<WARPS>), stream>>>(a.words, (int)a.N, bits, s);
       TB200_CHECK_LAUNCH();
     };
-    if (a.N <= 4096) sort(std::integral_constant<int, 8>{});
+    if (a.N <= 4096) sort(std::integral_constant<int, 8>{});   // (of tables beyond what one launch does)
     else sort(std::integral_constant<int, 32>{});
   }
-  EmbedArgs d = a;
-  d.table = deltas, d.stride = a.H;
-  with_variant(a, aligned(d, grad), [&](auto type, auto vec, auto drop) {
+  with_variant(a, wide, [&](auto type, auto vec, auto drop) {
     using T = decltype(type);
     constexpr int VEC = decltype(vec)::value;
     constexpr bool DROP = decltype(drop)::value;
