@@ -359,7 +359,7 @@ def test_states(B, N, W):
         assert torch.equal(a.cpu(), b)
 
 
-@pytest.mark.parametrize("B,N,W", [(1, 1, 1), (2, 3, 3), (3, 8, 5), (4, 5, 12), (2, 64, 64), (2, 3000, 3000)])
+@pytest.mark.parametrize("B,N,W", [(1, 1, 1), (2, 3, 3), (3, 8, 5), (4, 5, 12), (2, 64, 64), (2, 3000, 3000), (1, 4096, 4096)])
 def test_states_in_place(B, N, W):
     """The state itself, its first hypotheses, or more room than there were; identical rows are left alone."""
     g = torch.Generator().manual_seed(N + W)

@@ -15,7 +15,7 @@ from . import _transducer
 from .nodes import (MAX_LISTED_WORDS, OnDevice, _describe, _rows, certify_nodes, check_device, check_no_tangents)
 from .torch_binding import check_contiguous, check_dim, check_type
 
-MAX_REORDERED_WIDTH = 8192
+MAX_REORDERED_WIDTH = 4096
 
 
 def extend_beams(emissions, predictions, frames, positions, scores, width, validate_nodes=True):
@@ -67,7 +67,7 @@ def reorder_states(states, parents, out=None, validate_parents=True):
                  far, keys and values); what follows the second dimension has to be contiguous, or is copied
     ``parents``  int32 [B, W], as from `extend_beams`: a negative one says that there is no hypothesis
     ``out``      tensors [B, W, ...] to write, else they are made; any of them may be its state itself (or
-                 its first W hypotheses), which is then reordered in place (at most 8192 hypotheses).  It
+                 its first W hypotheses), which is then reordered in place (at most 4096 hypotheses).  It
                  must not overlap with others.
 
     Returns the new states as they came: a tensor, or a list.  Rows without a hypothesis are left as they were

@@ -86,7 +86,7 @@ int tb200_reorder_states(const tb200_states* states, int count, const int* paren
       if (s.from == s.to && s.from) {
         check((B <= 1 || s.fromStrideB == s.toStrideB) && (std::min(N, W) <= 1 || s.fromStrideN == s.toStrideN),
               "states that are reordered in place must keep their strides");
-        check(W <= kMaxReorderedWidth, "at most 8192 hypotheses are reordered in place");
+        check(W <= kMaxReorderedWidth, "at most 4096 hypotheses are reordered in place");
       }
     }
     launch_reorder_states(reinterpret_cast<const States*>(states), count, parents, B, N, W, kept != 0, beyond,

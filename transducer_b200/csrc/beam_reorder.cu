@@ -5,6 +5,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "node_rows.cuh"
 #include "profile.h"
 
 namespace tb200 {
@@ -97,43 +98,65 @@ __global__ void __launch_bounds__(32 * kWarps) reorder_kernel(const __grid_const
   }
 }
 
-// In place: a CTA has a piece of the rows of all hypotheses of an utterance and reads it whole before it writes.
-template <typename T>
-__device__ __forceinline__ void move_in_place(const States& s, const int* parents, i64 b, i64 at, int units, int N, int W,
-                                              T* held) {
-  for (int i = threadIdx.x; i < W * units; i += blockDim.x) {
-    const int w = i / units, n = parents[w];
-    if ((unsigned)n < (unsigned)N && n != w)
-      held[i] = reinterpret_cast<const T*>(s.from + b * s.fromB + n * s.fromN + at)[i % units];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < W * units; i += blockDim.x) {
-    const int w = i / units, n = parents[w];
-    if ((unsigned)n < (unsigned)N && n != w)
-      reinterpret_cast<T*>(s.to + b * s.toB + w * s.toW + at)[i % units] = held[i];
-  }
-}
-
-__global__ void __launch_bounds__(256) reorder_in_place_kernel(const __grid_constant__ Batch batch,
-                                                               const int* __restrict__ parents, int N, int W,
-                                                               int held, int* beyond) {
-  extern __shared__ __align__(16) char room[];
+// In place: a CTA has a piece of the rows of all hypotheses of an utterance and has read what moves before it writes any of
+// it.  The rows are brought as the aligned 16-byte vectors that hold them (of which others may be writing the bytes of
+// other rows; those are not looked at).
+__global__ void __launch_bounds__(32 * kWarps) reorder_in_place_kernel(const __grid_constant__ Batch batch,
+                                                                       const int* __restrict__ parents, int N, int W,
+                                                                       int held, int* beyond) {
+  extern __shared__ __align__(16) char room[];   // W rows of held + 32 bytes, then the hypotheses that move
+  __shared__ int moved;
+  int* const list = reinterpret_cast<int*>(room + (size_t)W * (held + 32));
   const unsigned id = blockIdx.x;
   int k = 0;
   while (k + 1 < batch.count && batch.item[k + 1].firstWarp <= id) ++k;   // (CTAs here)
   const Item& it = batch.item[k];
   const i64 b = (id - it.firstWarp) / (unsigned)it.pieces, at = (id - it.firstWarp) % (unsigned)it.pieces * (i64)held;
-  const int units = (int)(min((i64)held, it.s.rowBytes - at) / it.bytes);
+  const int bytes = (int)min((i64)held, it.s.rowBytes - at);
   parents += b * W;
-  if (beyond)
-    for (int w = threadIdx.x; w < W; w += blockDim.x)
-      if (parents[w] >= N) *beyond = 1;
-  switch (it.bytes) {
-    case 16: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<uint4*>(room)); break;
-    case 8: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<uint2*>(room)); break;
-    case 4: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<unsigned*>(room)); break;
-    case 2: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<unsigned short*>(room)); break;
-    default: move_in_place(it.s, parents, b, at, units, N, W, reinterpret_cast<unsigned char*>(room));
+  if (threadIdx.x == 0) moved = 0;
+  __syncthreads();
+  for (int w = threadIdx.x; w < W; w += blockDim.x) {
+    const int n = parents[w];
+    if (beyond && n >= N) *beyond = 1;
+    if ((unsigned)n < (unsigned)N && n != w) list[atomicAdd(&moved, 1)] = w;
+  }
+  __syncthreads();
+  const int moves = moved;
+  const int stride = held + 32;
+  const unsigned lanes = min(32, held / 16 + 1);   // that a row takes, at most 32 vectors at a time
+  auto from_of = [&](int w) { return it.s.from + b * it.s.fromB + parents[w] * it.s.fromN + at; };
+  for (unsigned i = threadIdx.x; i < moves * lanes; i += blockDim.x) {
+    const unsigned m = i / lanes;
+    const char* from = from_of(list[m]);
+    const int before = (int)((uintptr_t)from & 15);
+    for (unsigned v = i % lanes; 16 * v < before + bytes; v += lanes)
+      copy_async<16>(room + m * stride + 16 * v, from - before + 16 * v);
+  }
+  commit_copies();
+  wait_copies<0>();
+  __syncthreads();
+  for (unsigned i = threadIdx.x; i < moves * lanes; i += blockDim.x) {
+    const unsigned m = i / lanes, lane = i % lanes;
+    const int w = list[m];
+    const char* from = room + m * stride + ((uintptr_t)from_of(w) & 15);
+    char* to = it.s.to + b * it.s.toB + w * it.s.toW + at;
+    const int head = min(bytes, (int)(-(uintptr_t)to & 15)), vectors = (bytes - head) / 16, tail = head + 16 * vectors;
+    const int shift = (int)((uintptr_t)(from + head) & 15);
+    const unsigned* words = reinterpret_cast<const unsigned*>(from + head - (shift & 3));
+    uint4* vec = reinterpret_cast<uint4*>(to + head);
+    for (int v = lane; v < vectors; v += lanes) {
+      if (shift == 0) {
+        vec[v] = reinterpret_cast<const uint4*>(words)[v];
+      } else {
+        const unsigned x[5] = {words[4 * v], words[4 * v + 1], words[4 * v + 2], words[4 * v + 3], words[4 * v + 4]};
+        const int s = 8 * (shift & 3);
+        vec[v] = make_uint4(__funnelshift_r(x[0], x[1], s), __funnelshift_r(x[1], x[2], s), __funnelshift_r(x[2], x[3], s),
+                            __funnelshift_r(x[3], x[4], s));
+      }
+    }
+    for (int j = lane; j < head; j += lanes) to[j] = from[j];
+    for (int j = tail + lane; j < bytes; j += lanes) to[j] = from[j];
   }
 }
 
@@ -158,8 +181,8 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
   }
   // (nothing is to be moved, but the parents are to be looked at)
   if (beyond && count > 0 && apart.empty() && inPlace.empty()) apart.push_back(Item{states[0], 0, 0, 1});
-  // a piece of a row in place: with W of them 32 KB, a vector at least
-  const int held = std::max(16, 32 * 1024 / std::max(W, 1) / 16 * 16);
+  // a piece of a row in place: with W of them 48 KB, a vector at least
+  const int held = std::min(4096, std::max(16, (48 * 1024 / std::max(W, 1) - 32) / 16 * 16));
   for (size_t i = 0; i < apart.size();) {
     Batch batch{};
     i64 warps = 0;
@@ -191,9 +214,9 @@ void launch_reorder_states(const States* states, int count, const int* parents, 
       ctas += (i64)B * it.pieces;
     }
     if (ctas > 0x7fffffffLL) throw std::invalid_argument("the states are too large");
-    allow_dyn_smem(reorder_in_place_kernel, 16 * kMaxReorderedWidth);
+    allow_dyn_smem(reorder_in_place_kernel, 52 * kMaxReorderedWidth);
     ScopedKernel prof("reorder_in_place", stream);
-    reorder_in_place_kernel<<<(unsigned)ctas, 256, held * W, stream>>>(batch, parents, N, W, held, beyond);
+    reorder_in_place_kernel<<<(unsigned)ctas, 32 * kWarps, (held + 36) * W, stream>>>(batch, parents, N, W, held, beyond);
     TB200_CHECK_LAUNCH();
   }
 }

@@ -325,7 +325,7 @@ struct States {
   char* to;
   i64 fromB, fromN, toB, toW, rowBytes;
 };
-constexpr int kMaxReorderedWidth = 8192;   // of hypotheses that are reordered in place
+constexpr int kMaxReorderedWidth = 4096;   // of hypotheses that are reordered in place
 // kept: rows without a parent stay as they are (else they become 0).
 void launch_reorder_states(const States* states, int count, const int* parents, int B, int N, int W, bool kept,
                            int* beyond, cudaStream_t stream);
