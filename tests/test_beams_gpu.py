@@ -106,6 +106,29 @@ def test_two_values():
         check_extend([x.cuda() for x in (E, P, frames, positions, scores)], width)
 
 
+@pytest.mark.parametrize("width", [1, 40, 64, 256])
+def test_scores_that_lists_are_not_made_for(width):
+    """Few values, values next to each other, values that rise, and good hypotheses a multiple of 8 apart."""
+    V, N = 3000, 40
+    E, P, frames, positions, scores = hypotheses(2, 4, N, V, N, seed=20, done=0.05, gone=0.0)
+    positions[positions >= 0] = torch.arange(N, device="cuda").repeat(2, 1)[positions >= 0].int()
+    few = torch.randint(0, 3, E.shape, generator=torch.Generator().manual_seed(1)).float().cuda()
+    rising = torch.arange(V, device="cuda").expand_as(E).contiguous()
+    flat = torch.full_like(scores, -5.0)
+    for e, p, s in ((few, 0 * P, flat), (1e-7 * E, 1e-7 * P, flat), (few, 1e-7 * P, flat), (1e-6 * rising, 0 * P, flat),
+                    (-1e-6 * rising, 0 * P, flat), (1e-3 * rising, 0 * P, flat), (0 * E, P, flat), (E, 0 * P, flat)):
+        check_extend([e, p, frames, positions, s], width)
+    check_extend([few, 0 * P, frames, positions, scores], width)
+    ahead = scores.clone()
+    ahead[:, ::8] += 30.0
+    check_extend([E, P, frames, positions, ahead], width)
+    ahead[:, 1:] -= 60.0
+    check_extend([E, P, frames, positions, ahead], width)
+    lowest = torch.full_like(P, torch.finfo(torch.float32).min)
+    lowest[:, :, 5] = 0.0
+    check_extend([E, lowest, frames, positions, scores], width)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_equal_hypotheses(dtype):
     """The same node and score more than once: the lower parent first."""

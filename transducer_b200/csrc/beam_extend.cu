@@ -17,10 +17,10 @@ namespace {
 constexpr int kTile = 1024, kChunk = 32;
 constexpr int kScanWarps = 4;
 
-// A row's log-sum-exp is off by 6e-6 at most: exponents z - m times log2(e) are rounded three times, which is 3 * 2^-24
-// |z - m|, on average under the softmax less than 3 * 2^-24 * 20 (ln V); ex2.approx twice 2^-22; 23 additions and
-// products one after the other 2^-24 each.
-constexpr float kLseError = 6e-6f;
+// What the logarithm of a row's sum S = sum exp(z - m) is off by at most: exponents z - m times log2(e) are rounded three
+// times, which is 3 * 2^-24 |z - m|, under the softmax on average at most 3 * 2^-24 (ln V - ln S) (its entropy is at most
+// ln V); ex2.approx twice 2^-22; 23 additions and products one after the other 2^-24 each.
+constexpr float kSumError = 1.9e-6f, kExponentError = 1.8e-7f;
 
 struct ExtendScratch {
   double2* row;   // [B*N] a row's greatest score m, and scores - log sum exp(z - m); the latter -inf: it has no words
@@ -49,20 +49,17 @@ __device__ __forceinline__ float warp_greatest(float x) {
 }
 
 // A warp goes through one tile of the rows of up to 32 hypotheses that follow each other, frame by frame, so that a
-// frame's words stay in registers.  The rows of the hypotheses come through a ring in shared memory, from which every lane
-// reads what it has copied itself (single bf16 words, which no asynchronous copy moves, come through registers).
+// frame's words stay in registers.  The rows of the hypotheses come through a ring in shared memory, as 16-byte vectors:
+// where rows begin anywhere, as the aligned vectors that hold the tile's words.
 constexpr int kScanStages = 2;
 template <typename TIn, int VEC>
-constexpr bool kScanRing = VEC * sizeof(TIn) >= 4;
-template <typename TIn, int VEC>
-constexpr int kScanSmem = kScanRing<TIn, VEC> ? kScanWarps * kScanStages * kTile * (int)sizeof(TIn) : 0;
+constexpr int kStageBytes = kTile * (int)sizeof(TIn) + (VEC == 1 ? 16 : 0);
 
 template <typename TIn, int VEC>
 __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a, const float* __restrict__ scores,
                                                                       int tiles, int perWarp, int groups,
                                                                       ExtendScratch out) {
   constexpr int J = kChunk / VEC;
-  constexpr bool RING = kScanRing<TIn, VEC>;
   using Raw = RawWords<TIn, VEC>;
   extern __shared__ __align__(16) char shared[];
   __shared__ unsigned char order[kScanWarps][32];
@@ -93,20 +90,26 @@ __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a
   const TIn* const E = static_cast<const TIn*>(a.E) + b * a.eStrideB;
   const TIn* const P = static_cast<const TIn*>(a.P) + b * a.pStrideB;
   const int at = chunk_word<VEC>(tile, lane, 0);
-  Raw* const ring = reinterpret_cast<Raw*>(shared) + warp * kScanStages * J * 32 + lane;
-  // the i-th hypothesis' row: to the ring, and from there (or from memory)
+  constexpr int kStage = kStageBytes<TIn, VEC>;
+  char* const ring = shared + warp * kScanStages * kStage;
+  // the i-th hypothesis' row, to the ring
   auto row_of = [&](int i) { return P + __shfl_sync(0xffffffffu, position, order[warp][i]) * a.pStrideU; };
   auto send = [&](int i) {
-    if constexpr (RING) {
-      if (i < live) {
-        const TIn* row = row_of(i);
+    if (i < live) {
+      const TIn* row = row_of(i);
+      if constexpr (VEC > 1) {   // (every lane what it reads itself)
 #pragma unroll
         for (int j = 0; j < J; ++j)
           if (at + 32 * VEC * j < a.V)
-            copy_async<VEC * sizeof(TIn)>(ring + (i % kScanStages * J + j) * 32, row + at + 32 * VEC * j);
+            copy_async<16>(ring + i % kScanStages * kStage + (32 * j + lane) * 16, row + at + 32 * VEC * j);
+      } else {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(row + tile * kTile), begin = from & ~(uintptr_t)15;
+        const uintptr_t end = from + min(kTile, a.V - tile * kTile) * sizeof(TIn);
+        for (int j = lane; begin + 16 * j < end; j += 32)
+          copy_async<16>(ring + i % kScanStages * kStage + 16 * j, reinterpret_cast<const char*>(begin + 16 * j));
       }
-      commit_copies();
     }
+    commit_copies();
   };
   if (live == 0) return;
 #pragma unroll
@@ -123,16 +126,18 @@ __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a
       held = t;
     }
     Raw p[J];
-    if constexpr (RING) {
-      send(i + kScanStages - 1);
-      wait_copies<kScanStages - 1>();
+    if constexpr (VEC == 1) __syncwarp();   // (all have read what the next row takes the place of)
+    send(i + kScanStages - 1);
+    wait_copies<kScanStages - 1>();
+    const char* stage = ring + i % kScanStages * kStage;
+    if constexpr (VEC > 1) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) p[j] = ring[(i % kScanStages * J + j) * 32];
+      for (int j = 0; j < J; ++j) p[j].load(reinterpret_cast<const TIn*>(stage + (32 * j + lane) * 16));
     } else {
-      const TIn* row = row_of(i);
+      __syncwarp();
+      const TIn* words = reinterpret_cast<const TIn*>(stage + (reinterpret_cast<uintptr_t>(row_of(i) + tile * kTile) & 15));
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (at + 32 * VEC * j < a.V) p[j].load(row + at + 32 * VEC * j);
+      for (int j = 0; j < J; ++j) p[j].load(words + 32 * j + lane);   // (beyond the row: anything)
     }
     float z[kChunk];
     float top = neg_inf();
@@ -183,7 +188,7 @@ template <int T>
 struct PickRoom {
   static constexpr int kTiles = T == 256 ? 128 : 512;       // listed; where there are more: general_pick
   static constexpr int kChunks = T == 256 ? 4096 : 8192;
-  static constexpr int kWords = T == 256 ? 2048 : 8192;
+  static constexpr int kWords = T == 256 ? 2560 : 8192;
   double2 row[kRowsHeld];
   i64 e[kRowsHeld], p[kRowsHeld];   // where the rows begin
   union {
@@ -205,6 +210,9 @@ struct PickRoom {
   int count[4];
   unsigned reached;
   int close;
+  unsigned spread;   // the greatest ln V - ln S of the rows
+  double cutValue;   // general_pick: extensions that come before this one may be among the best
+  Place cutPlace;
   Kind kind[kRowsHeld];
   unsigned char again[kWords];
 };
@@ -255,17 +263,11 @@ __device__ __forceinline__ unsigned reached_by(unsigned mine, int W, PickRoom<T>
 
 // The key from which on words are looked at, given one that W of them reach: as much lower as two rows' errors and the
 // rounding of the keys' values to 32 bits may come to.
-__device__ __forceinline__ unsigned with_slack(unsigned key) {
+__device__ __forceinline__ unsigned with_slack(unsigned key, float error) {
   const unsigned lowest = score_key(neg_inf()) + 1;
   if (key <= lowest) return lowest;
   const float x = fminf(key_score(key), 3.4028234e38f);
-  return max(lowest, score_key(x - (2.5f * kLseError + fabsf(x) * 3e-7f)));
-}
-
-// Order of doubles as of whole numbers.
-__device__ __forceinline__ unsigned long long wide_key(double x) {
-  const unsigned long long u = (unsigned long long)__double_as_longlong(x + 0.0);
-  return u ^ ((unsigned long long)((long long)u >> 63) | 0x8000000000000000ull);
+  return max(lowest, score_key(x - (2.5f * error + fabsf(x) * 3e-7f)));
 }
 
 // The key of an extension's score; above 0 for all that are extensions.
@@ -358,43 +360,42 @@ struct Utterance {
   __device__ __noinline__ double2 exact_row(int n, Group<T>& g) const {
     const NodeScores<TIn> r = rows(n);
     const float m = (float)row(n).x;
+    constexpr int kBatch = (VEC == 1 ? 2048 : 1024) / T;   // vectors on their way at a time
     double sum = 0.0;
-    each_score<TIn, VEC, T>(r, a.V, g.tid, [&](float z, int) { sum += exp((double)z - (double)m); });
+#pragma unroll 1
+    for (int v = g.tid * VEC; v < a.V; v += T * VEC * kBatch) {
+      RawWords<TIn, VEC> e[kBatch], p[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (v + j * T * VEC < a.V) e[j].load(r.e + v + j * T * VEC), p[j].load(r.p + v + j * T * VEC);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (v + j * T * VEC >= a.V) break;
+        const Words<VEC> x = e[j].words(), y = p[j].words();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum += exp((double)(x.x[i] + y.x[i]) - (double)m);
+      }
+    }
     sum = g.sum(sum);
     return make_double2(m, (double)score(n) - log(sum));
   }
-
-  // f(value, parent, word) for every extension of at least `least`, in any order, by the CTA
-  template <typename F>
-  __device__ __forceinline__ void each(double least, int tid, F f) const {
-    const int lane = tid & 31;
-#pragma unroll 1
-    for (i64 t = tid >> 5; t < all_tiles(); t += T / 32) {
-      const int n = (int)((unsigned)t / (unsigned)tiles), tile = (int)((unsigned)t % (unsigned)tiles);
-      const double2 x = row(n);
-      if (x.y == -1.0 / 0.0) continue;
-      if (!(value(x, s.best[(first * tiles + t) * 32 + lane]) >= least)) continue;
-      const NodeScores<TIn> r = rows(n);
-#pragma unroll 1
-      for (int i = 0; i < kChunk; ++i) {
-        const int v = chunk_word<VEC>(tile, lane, i);
-        if (v >= a.V) break;
-        const float z = to_f32(r.e[v]) + to_f32(r.p[v]);
-        if (z > neg_inf() && value(x, z) >= least) f(value(x, z), n, v);
-      }
-    }
-#pragma unroll 1
-    for (int n = tid; n < a.N; n += T)
-      if (kind(n) == kFinished && score(n) >= least) f((double)score(n), n, -1);
-  }
 };
 
-// Where equal scores make the lists too long: the W-th value by a search over 64-bit keys, a pass over the chunks that reach
-// it for each bit, then the place up to which its equals belong to the best.  Leaves the list.
+// Where equal scores make the lists too long: all rows' sums in 64 bits, then one way through everything that may be among
+// the best, the best W so far in a list that is put in order and cut whenever it is full.  Leaves the list.
 template <typename TIn, int VEC, int T>
-__device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W, Group<T>& g) {
+__device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W, unsigned least, float error, Group<T>& g) {
+  constexpr int kRoom = 2 * T;   // of the list
   const NodeArgs& a = at.a;
   PickRoom<T>& p = at.room;
+  static_assert(kRoom <= PickRoom<T>::kWords);
+  int& count = p.count[2];
+  __syncthreads();
+  if (g.tid == 0) {
+    count = 0;
+    p.cutValue = least <= score_key(neg_inf()) + 1 ? -1.0 / 0.0 : (double)key_score(with_slack(least, error));
+    p.cutPlace = 0;
+  }
   __syncthreads();
 #pragma unroll 1
   for (int n = 0; n < a.N; ++n) {
@@ -404,47 +405,85 @@ __device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W
     if (g.tid == 0) at.set_row(n, row);
     __syncthreads();
   }
-  const double lowest = -1.7976931348623157e308;
-  auto count = [&](double least, auto pick) {
-    int c = 0;
-    at.each(least, g.tid, [&](double d, int n, int v) { c += pick(d, n, v) ? 1 : 0; });
-    return g.sum(min(c, 1 << 20));
-  };
-  auto value = [](unsigned long long k) {
-    return __longlong_as_double((long long)(k ^ ((unsigned long long)((long long)~k >> 63) | 0x8000000000000000ull)));
-  };
-  unsigned long long key = 0;
-#pragma unroll 1
-  for (int bit = 63; bit >= 0; --bit) {
-    const unsigned long long t = key | (1ull << bit);
-    if (t <= wide_key(lowest)) {   // (all reach it)
-      key = t;
-      continue;
+  auto cut = [&] {   // the first W of the list, in order
+    double d[2];
+    Place place[2];
+    int rank[2];
+    const int c = count;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = g.tid + k * T;
+      d[k] = i < c ? p.d[i] : 0.0, place[k] = i < c ? p.place[i] : 0, rank[k] = i < c ? 0 : W;
     }
-    if (t > wide_key(1.7976931348623157e308)) continue;
-    if (count(value(t), [&](double d, int, int) { return wide_key(d) >= t; }) >= W) key = t;
-  }
-  key = max(key, wide_key(lowest));
-  const double cut = value(key);
-  const int above = count(cut, [&](double d, int, int) { return wide_key(d) > key; });
-  i64 lo = 0, hi = (i64)place_of(a.N, 0);
+#pragma unroll 4
+    for (int j = 0; j < c; ++j) {
+      const double other = p.d[j];
+      const Place from = p.place[j];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) rank[k] += (other > d[k]) | ((other == d[k]) & (from < place[k]));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (rank[k] >= W) continue;
+      p.d[rank[k]] = d[k], p.place[rank[k]] = place[k];
+      if (rank[k] == W - 1) p.cutValue = d[k], p.cutPlace = place[k];
+    }
+    if (g.tid == 0) count = min(c, W);
+    __syncthreads();
+  };
+  auto better = [&](double d, Place place) {
+    return d > p.cutValue || (d == p.cutValue && place < p.cutPlace);
+  };
+  auto push = [&](bool has, double d, Place place) {   // by all threads; between two of these the cut does not change
+    if (has) {
+      const int i = atomicAdd(&count, 1);
+      p.d[i] = d, p.place[i] = place;
+    }
+    __syncthreads();
+    const int c = count;
+    __syncthreads();
+    if (c > kRoom - T) cut();
+  };
 #pragma unroll 1
-  while (lo < hi) {
-    const i64 mid = lo + (hi - lo) / 2;
-    if (count(cut, [&](double d, int n, int v) { return wide_key(d) == key && (i64)place_of(n, v) <= mid; }) >= W - above)
-      hi = mid;
-    else lo = mid + 1;
+  for (int n0 = 0; n0 < a.N; n0 += T) {
+    const int n = n0 + g.tid;
+    const bool has = n < a.N && at.kind(n) == kFinished;
+    const double d = has ? (double)at.score(n) : 0.0;
+    push(has && better(d, place_of(n, -1)), d, place_of(n, -1));
   }
-  __syncthreads();
-  if (g.tid == 0) p.count[2] = 0;
-  __syncthreads();
-  at.each(cut, g.tid, [&](double d, int n, int v) {
-    if (wide_key(d) == key && (i64)place_of(n, v) > lo) return;
-    const int i = atomicAdd(&p.count[2], 1);
-    if (i < p.kWords) p.d[i] = d, p.place[i] = place_of(n, v);
-  });
-  __syncthreads();
-  return min(p.count[2], W);
+#pragma unroll 1
+  for (i64 t0 = 0; t0 < at.all_tiles(); t0 += T / 32) {   // a warp a tile, a lane a chunk
+    const i64 t = t0 + g.warp;
+    unsigned left = 0;   // of its words
+    double2 row = make_double2(0.0, -1.0 / 0.0);
+    NodeScores<TIn> r{};
+    int n = 0, tile = 0;
+    if (t < at.all_tiles()) {
+      n = (int)((unsigned)t / (unsigned)at.tiles), tile = (int)((unsigned)t % (unsigned)at.tiles);
+      row = at.row(n);
+    }
+    auto value = [&](int i) {
+      const int v = chunk_word<VEC>(tile, g.lane, i);
+      return v < a.V ? at.value(row, to_f32(r.e[v]) + to_f32(r.p[v])) : -1.0 / 0.0;
+    };
+    auto place = [&](int i) { return place_of(n, chunk_word<VEC>(tile, g.lane, i)); };
+    auto counts = [&](int i, double d) { return d > -1.0 / 0.0 && better(d, place(i)); };
+    if (row.y > -1.0 / 0.0 && at.value(row, at.s.best[(at.first * at.tiles + t) * 32 + g.lane]) >= p.cutValue) {
+      r = at.rows(n);
+#pragma unroll 8
+      for (int i = 0; i < kChunk; ++i) left |= counts(i, value(i)) ? 1u << i : 0u;
+    }
+    while (__syncthreads_or(left != 0)) {   // (one word of every lane at a time)
+      const int i = __ffs(left) - 1;
+      const double d = i >= 0 ? value(i) : 0.0;
+      const bool has = i >= 0 && counts(i, d);
+      left &= left - 1;
+      push(has, d, i >= 0 ? place(i) : 0);
+    }
+  }
+  cut();
+  return count;
 }
 
 template <typename TIn, int VEC, int T>
@@ -471,7 +510,7 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
     }
   }
   if (tid < 4) r.count[tid] = 0;
-  if (tid == 4) r.close = 0;
+  if (tid == 4) r.close = 0, r.spread = 0;
   __syncthreads();
   cudaGridDependencySynchronize();
 
@@ -532,7 +571,10 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
     double2 row = at.row(n);
     if (kind != kNotThere) bad |= !(at.score(n) < pos_inf());
     if (kind == kExtended) bad |= !(row.y < 1.0 / 0.0);
-    row.y = kind == kExtended && row.x > -1.0 / 0.0 ? (double)at.score(n) - log(row.y) : -1.0 / 0.0;
+    const bool extends = kind == kExtended && row.x > -1.0 / 0.0;
+    const double log_sum = extends ? log(row.y) : 0.0;
+    if (extends) atomicMax(&r.spread, __float_as_uint(fmaxf(0.0f, logf((float)a.V) - (float)log_sum)));
+    row.y = extends ? (double)at.score(n) - log_sum : -1.0 / 0.0;
     at.set_row(n, row);
   }
   if (__syncthreads_or(bad)) {
@@ -542,38 +584,63 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
 
   // tiles, and the hypotheses that are finished; all of them where they are few
   const i64 rowTiles = at.all_tiles(), allTiles = rowTiles + a.N;
-  unsigned least = with_slack(0), mine = 0;
+  const float error = kSumError + kExponentError * __uint_as_float(r.spread);
+  unsigned least = with_slack(0, error), mine = 0;
+  // The greatest key that W of `count` items reach, which they do from `from` on: the threads' own maxima have told one that
+  // too many do.
+  auto exactly = [&](auto key_of, i64 count, unsigned from) {
+    unsigned to = score_key(pos_inf()) + 1;
+#pragma unroll 1
+    while (to - from > 1) {
+      const unsigned mid = from + (to - from) / 2;
+      int c = 0;
+      for (i64 i = tid; i < count; i += T) c += key_of(i) >= mid ? 1 : 0;
+      if (g.sum(c) >= W) from = mid;
+      else to = mid;
+    }
+    return from;
+  };
   if (allTiles > r.kTiles) {
     auto take = [&](i64 t) {
       const unsigned key = at.tile_key(t);
       if (T == 256 || t < kTilesHeld) r.tileKey[t] = key;   // (in the place of what it comes from)
       mine = max(mine, key);
     };
-    if constexpr (T == 256) {   // (a warp a row: nothing is divided)
-#pragma unroll 2
-      for (int n = warp; n < a.N; n += kWarps) {
-        const double2 row = at.row(n);
-        for (int i = lane; i < tiles; i += 32) {
-          const int t = n * tiles + i;
-          const unsigned key = row.y > -1.0 / 0.0 ? extension_key(at.value(row, r.top[t])) : 0u;
-          r.tileKey[t] = key;
-          mine = max(mine, key);
-        }
+    if constexpr (T == 256) {   // (t / tiles: fewer than 2^12 tiles, off by less than half of one)
+      const float per = 1.0f / (float)tiles;
+      for (int t = tid; t < rowTiles; t += T) {
+        const double2 row = at.row((int)(((float)t + 0.5f) * per));
+        const unsigned key = row.y > -1.0 / 0.0 ? extension_key(at.value(row, r.top[t])) : 0u;
+        r.tileKey[t] = key;
+        mine = max(mine, key);
       }
       for (i64 t = rowTiles + tid; t < allTiles; t += T) take(t);
     } else {
 #pragma unroll 1
       for (i64 t = tid; t < allTiles; t += T) take(t);
     }
-    least = with_slack(reached_by<T>(mine, W, r, g));
+    least = with_slack(reached_by<T>(mine, W, r, g), error);
   }
+  auto listed_key = [&](i64 t) {
+    return allTiles > r.kTiles && (T == 256 || t < kTilesHeld) ? r.tileKey[t] : at.tile_key(t);
+  };
+  auto list_tiles = [&] {
 #pragma unroll 1
-  for (i64 t = tid; t < allTiles; t += T)
-    if ((allTiles > r.kTiles && (T == 256 || t < kTilesHeld) ? r.tileKey[t] : at.tile_key(t)) >= least) {
-      const int i = atomicAdd(&r.count[0], 1);
-      if (i < r.kTiles) r.tile[i] = at.listed(t);
-    }
-  __syncthreads();
+    for (i64 t = tid; t < allTiles; t += T)
+      if (listed_key(t) >= least) {
+        const int i = atomicAdd(&r.count[0], 1);
+        if (i < r.kTiles) r.tile[i] = at.listed(t);
+      }
+    __syncthreads();
+  };
+  list_tiles();
+  if (r.count[0] > r.kTiles) {
+    least = with_slack(exactly(listed_key, allTiles, least), error);
+    __syncthreads();
+    if (tid == 0) r.count[0] = 0;
+    __syncthreads();
+    list_tiles();
+  }
   bool many = r.count[0] > r.kTiles;
 
   // their chunks
@@ -600,14 +667,24 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
         mine = max(mine, key);
       }
     }
-    least = max(least, with_slack(reached_by<T>(mine, W, r, g)));
+    least = max(least, with_slack(reached_by<T>(mine, W, r, g), error));
+    auto list_chunks = [&] {
 #pragma unroll 1
-    for (int i = warp; i < listed; i += kWarps)
-      if (r.chunkKey[i * 32 + lane] >= least) {
-        const int k = atomicAdd(&r.count[1], 1);
-        if (k < r.kChunks) r.chunk[k] = i * 32 + lane;
-      }
-    __syncthreads();
+      for (int i = tid; i < 32 * listed; i += T)
+        if (r.chunkKey[i] >= least) {
+          const int k = atomicAdd(&r.count[1], 1);
+          if (k < r.kChunks) r.chunk[k] = i;
+        }
+      __syncthreads();
+    };
+    list_chunks();
+    if (r.count[1] > r.kWords / 32) {   // (more words than there is room for)
+      least = max(least, with_slack(exactly([&](i64 i) { return r.chunkKey[i]; }, 32 * listed, least), error));
+      __syncthreads();
+      if (tid == 0) r.count[1] = 0;
+      __syncthreads();
+      list_chunks();
+    }
     many = r.count[1] > r.kChunks;
   }
 
@@ -651,13 +728,13 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
     many = c > r.kWords;
   }
   const bool exact = many;
-  if (many) c = general_pick<TIn, VEC, T>(at, W, g);
+  if (many) c = general_pick<TIn, VEC, T>(at, W, least, error, g);
 
   // of many words those that can be among the best
   if (c > 2 * W + 64) {
     mine = 0;
     for (int i = tid; i < c; i += T) mine = max(mine, extension_key(r.d[i]));
-    least = with_slack(reached_by<T>(mine, W, r, g));
+    least = with_slack(reached_by<T>(mine, W, r, g), error);
 #pragma unroll 1
     for (int i0 = 0; i0 < c; i0 += T) {   // (in place: what is written lies before what is read)
       const int i = i0 + tid;
@@ -693,7 +770,7 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
         const double other = r.d[j];
         const Place at = r.place[j];
         rank += (other > d) | ((other == d) & (at < place));
-        close |= (parent_of(at) != parent) & (fabs(d - other) <= 2.0 * kLseError);
+        close |= (parent_of(at) != parent) & (fabs(d - other) <= 2.0f * error);
       }
       rank += close ? 1 << 20 : 0;
 #pragma unroll
@@ -705,7 +782,7 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
         r.close = r.again[i] = 1;
 #pragma unroll 1
         for (int j = 0; j < c; ++j)
-          if (parent_of(r.place[j]) != parent && fabs(d - r.d[j]) <= 2.0 * kLseError) r.again[j] = 1;
+          if (parent_of(r.place[j]) != parent && fabs(d - r.d[j]) <= 2.0f * error) r.again[j] = 1;
       }
       if (rank < W) outScores[rank] = (float)d, parents[rank] = parent, words[rank] = word_of(place);
     }
@@ -757,7 +834,7 @@ void launch_extend_beams(const NodeArgs& a, const float* scores, float* outScore
       if (warps > 0x7fff0000LL || layers > 65535) throw std::invalid_argument("too many words and hypotheses");
       ScopedKernel prof("extend_scan", stream);
       auto kernel = extend_scan_kernel<TIn, VEC>;
-      constexpr int smem = kScanSmem<TIn, VEC>;
+      constexpr int smem = kScanWarps * kScanStages * kStageBytes<TIn, VEC>;
       if (smem > 40 * 1024) allow_dyn_smem(kernel, smem);
       kernel<<<dim3((unsigned)div_up64(warps, kScanWarps), rows, layers), 32 * kScanWarps, smem, stream>>>(
           a, scores, tiles, perWarp, groups, s);
