@@ -163,10 +163,12 @@ __global__ void __launch_bounds__(32 * kScanWarps) extend_scan_kernel(NodeArgs a
 }
 
 // ---- what is picked of them ---------------------------------------------------------------------
-// A CTA per utterance: of 256 threads where up to 64 extensions are wanted of so many rows and tiles as shared memory
-// holds, else of 1024, whose own maxima tell 256 extensions, and which read what is not held from memory again.
+// A CTA per utterance: of kSmall threads where up to 64 extensions are wanted of so many rows and tiles as shared memory
+// holds, else of kLarge, whose own maxima tell 256 extensions, and which read what is not held from memory again.
 
 constexpr int kRowsHeld = 256, kTilesHeld = 4096;
+constexpr int kSmall = 256, kLarge = 1024;   // threads
+constexpr int kRoots = 32;   // of 2, for exp64
 inline bool all_held(int W, i64 N, i64 tiles) { return W <= 64 && N <= kRowsHeld && N * tiles + N <= kTilesHeld; }
 enum Kind : unsigned char { kNotThere, kFinished, kExtended };
 
@@ -186,9 +188,9 @@ struct ListedTile {
 
 template <int T>
 struct PickRoom {
-  static constexpr int kTiles = T == 256 ? 128 : 512;       // listed; where there are more: general_pick
-  static constexpr int kChunks = T == 256 ? 4096 : 8192;
-  static constexpr int kWords = T == 256 ? 2560 : 8192;
+  static constexpr int kTiles = T == kSmall ? 128 : 384;       // listed; where there are more: general_pick
+  static constexpr int kChunks = 4096;
+  static constexpr int kWords = T == kSmall ? 4096 : 9216;
   double2 row[kRowsHeld];
   i64 e[kRowsHeld], p[kRowsHeld];   // where the rows begin
   union {
@@ -205,12 +207,16 @@ struct PickRoom {
     float top[kTilesHeld];          // of tiles
     unsigned tileKey[kTilesHeld];   // of their greatest extensions
   };
-  int chunk[kChunks];
+  union {
+    int chunk[kChunks];
+    float z[kChunks];   // exact_row: words that are added up next
+  };
   float score[kRowsHeld];
   int count[4];
   unsigned reached;
   int close;
   unsigned spread;   // the greatest ln V - ln S of the rows
+  double root[kRoots];   // kRoot
   double cutValue;   // general_pick: extensions that come before this one may be among the best
   Place cutPlace;
   Kind kind[kRowsHeld];
@@ -220,15 +226,17 @@ struct PickRoom {
 // A key that `W` of the threads' keys reach (0: none), the W-th of them or a little less; 0 if there are fewer.
 template <int T>
 __device__ __forceinline__ unsigned reached_by(unsigned mine, int W, PickRoom<T>& r, Group<T>& g) {
-  if constexpr (T == 256) {   // (by one warp: no barriers in between)
+  if constexpr (T == kSmall) {   // (by one warp: no barriers in between)
     r.key[g.tid] = mine;
     if (__syncthreads_count(mine != 0) < W) return 0;
     if (g.warp == 0) {
-      const uint4 x = reinterpret_cast<const uint4*>(r.key)[2 * g.lane], y = reinterpret_cast<const uint4*>(r.key)[2 * g.lane + 1];
-      const unsigned k[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      constexpr int kKeys = T / 32;
+      unsigned k[kKeys];
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) k[i] = r.key[32 * i + g.lane];
       unsigned least = ~0u, most = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) least = min(least, k[i] ? k[i] : ~0u), most = max(most, k[i]);
+      for (int i = 0; i < kKeys; ++i) least = min(least, k[i] ? k[i] : ~0u), most = max(most, k[i]);
       unsigned from = __reduce_min_sync(0xffffffffu, least), to = __reduce_max_sync(0xffffffffu, most) + 1;
       int reached = T;
 #pragma unroll 1
@@ -236,7 +244,7 @@ __device__ __forceinline__ unsigned reached_by(unsigned mine, int W, PickRoom<T>
         const unsigned mid = from + (to - from) / 2;
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c += k[i] >= mid ? 1 : 0;
+        for (int i = 0; i < kKeys; ++i) c += k[i] >= mid ? 1 : 0;
         c = __reduce_add_sync(0xffffffffu, c);
         if (c >= W) from = mid, reached = c;
         else to = mid;
@@ -276,6 +284,31 @@ __device__ __forceinline__ unsigned extension_key(double d) {
   return d > -1.0 / 0.0 ? max(score_key((float)d), lowest + 1) : 0u;
 }
 
+// exp(z - m) for z <= m in 64 bits, 2^(n + j/32) times the Taylor series of exp(r), |r| <= log(2) / 64, whose seventh power
+// weighs less than 2^-57 (P. T. P. Tang: Table-driven implementation of the exponential function in IEEE floating-point
+// arithmetic, 1989).  Below exp(-100) it is that: next to the row's greatest weight, 1, nothing.
+__device__ const double kRoot[kRoots] = {   // 2^(j/32)
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+__device__ __forceinline__ double exp64(const double* roots, float z, float m) {
+  const float about = fmaxf(z - m, -100.0f);
+  const double x = fmax((double)z - (double)m, -100.0);
+  const float shifted = fmaf(about, 46.166241f, 12582912.0f);   // 32 / log(2); 3 * 2^22: the sum is rounded to a whole number
+  const int n = __float_as_int(shifted) - __float_as_int(12582912.0f);
+  const double k = (double)(shifted - 12582912.0f);
+  constexpr double high = 0x1.62e42fefa39efp-6, low = 0x1.abc9e3b39803fp-61;   // log(2) / 32
+  const double r = fma(k, -low, fma(k, -high, x)), r2 = r * r;
+  const double p = fma(fma(fma(r, 1.0 / 720, 1.0 / 120), r2, fma(r, 1.0 / 24, 1.0 / 6)), r2 * r, fma(r2, 1.0 / 2, r));
+  const double root = roots[n & (kRoots - 1)], y = fma(root, p, root);
+  return __hiloint2double(__double2hiint(y) + (n >> 5 << 20), __double2loint(y));
+}
+
 template <typename TIn, int VEC, int T>
 struct Utterance {
   const NodeArgs& a;
@@ -297,7 +330,7 @@ struct Utterance {
   __device__ __forceinline__ void hold(int n) const {
     room.kind[n] = look(n, room.score[n], room.e[n], room.p[n]);
   }
-  static __device__ __forceinline__ bool held(int n) { return T == 256 || n < kRowsHeld; }
+  static __device__ __forceinline__ bool held(int n) { return T == kSmall || n < kRowsHeld; }
   __device__ __forceinline__ Kind kind(int n) const {
     if (held(n)) return room.kind[n];
     float score;
@@ -330,7 +363,7 @@ struct Utterance {
   // An extension's score: z - m loses nothing, however large the two are.
   static __device__ __forceinline__ double value(double2 row, float z) { return row.y + ((double)z - row.x); }
   __device__ __forceinline__ float tile_top(i64 t) const {
-    return T == 256 || t < kTilesHeld ? room.top[t] : s.sums[first * tiles + t].x;
+    return T == kSmall || t < kTilesHeld ? room.top[t] : s.sums[first * tiles + t].x;
   }
   // the key of a tile's greatest extension; tiles from all_tiles() on: hypotheses that are finished
   __device__ __forceinline__ unsigned tile_key(i64 t) const {
@@ -356,27 +389,46 @@ struct Utterance {
     return x;
   }
 
-  // log sum exp(z - m) of a row in 64 bits, by the CTA
+  // Its sum in 64 bits, by the CTA.  (Little code: where it is needed it has to be brought first.)
   __device__ __noinline__ double2 exact_row(int n, Group<T>& g) const {
+    constexpr int kWords = PickRoom<T>::kChunks / T, kBatch = kWords > VEC ? kWords / VEC : 1;   // of a thread at a time
+    static_assert(VEC <= kWords || T == kLarge);
     const NodeScores<TIn> r = rows(n);
     const float m = (float)row(n).x;
-    constexpr int kBatch = (VEC == 1 ? 2048 : 1024) / T;   // vectors on their way at a time
-    double sum = 0.0;
-#pragma unroll 1
-    for (int v = g.tid * VEC; v < a.V; v += T * VEC * kBatch) {
-      RawWords<TIn, VEC> e[kBatch], p[kBatch];
+    double part[4] = {0.0, 0.0, 0.0, 0.0};
+    if (g.tid < kRoots) room.root[g.tid] = kRoot[g.tid];
+    __syncthreads();
+    constexpr int kStep = VEC < kWords ? VEC : kWords;   // words of a vector that are added at once
+    RawWords<TIn, VEC> x[kBatch], y[kBatch];
+    auto bring = [&](int v) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
-        if (v + j * T * VEC < a.V) e[j].load(r.e + v + j * T * VEC), p[j].load(r.p + v + j * T * VEC);
+        if (v + j * T * VEC < a.V) x[j].load(r.e + v + j * T * VEC), y[j].load(r.p + v + j * T * VEC);
+    };
+    bring(g.tid * VEC);
+#pragma unroll 1
+    for (int v = g.tid * VEC; v < a.V; v += T * VEC * kBatch) {
+      Words<VEC> xs[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        if (v + j * T * VEC >= a.V) break;
-        const Words<VEC> x = e[j].words(), y = p[j].words();
+        const Words<VEC> es = x[j].words(), ps = y[j].words();
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum += exp((double)(x.x[i] + y.x[i]) - (double)m);
+        for (int i = 0; i < VEC; ++i) xs[j].x[i] = v + j * T * VEC < a.V ? es.x[i] + ps.x[i] : neg_inf();
+      }
+      bring(v + T * VEC * kBatch);
+#pragma unroll
+      for (int h = 0; h < VEC / kStep; ++h) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+          for (int i = 0; i < kStep; ++i) room.z[(kStep * j + i) * T + g.tid] = xs[j].x[kStep * h + i];
+#pragma unroll 1
+        for (int i = 0; i < kBatch * kStep; i += 4)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) part[k] += exp64(room.root, room.z[(i + k) * T + g.tid], m);
       }
     }
-    sum = g.sum(sum);
+    const double sum = g.sum((part[0] + part[1]) + (part[2] + part[3]));
     return make_double2(m, (double)score(n) - log(sum));
   }
 };
@@ -546,7 +598,7 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
           m[k] = warp_greatest(m[k]);
           for (int i = lane; i < tiles; i += 32) {
             all += weight(t[i], m[k]);
-            if (T == 256 || (i64)n * tiles + i < kTilesHeld) r.top[n * tiles + i] = t[i].x;
+            if (T == kSmall || (i64)n * tiles + i < kTilesHeld) r.top[n * tiles + i] = t[i].x;
           }
         }
         sum[k] = (float)all;
@@ -554,7 +606,7 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
         m[k] = warp_greatest(m[k]);
         sum[k] = weight(x[k], m[k]);
         const i64 t = (i64)(n0 + k * kWarps) * tiles + lane;
-        if (n0 + k * kWarps < a.N && lane < tiles && (T == 256 || t < kTilesHeld)) r.top[t] = x[k].x;
+        if (n0 + k * kWarps < a.N && lane < tiles && (T == kSmall || t < kTilesHeld)) r.top[t] = x[k].x;
       }
     }
 #pragma unroll
@@ -586,16 +638,21 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
   const i64 rowTiles = at.all_tiles(), allTiles = rowTiles + a.N;
   const float error = kSumError + kExponentError * __uint_as_float(r.spread);
   unsigned least = with_slack(0, error), mine = 0;
-  // The greatest key that W of `count` items reach, which they do from `from` on: the threads' own maxima have told one that
+  // A key that W of `count` items reach, as they do `from`, and hardly more than W: the threads' own maxima have told one that
   // too many do.
   auto exactly = [&](auto key_of, i64 count, unsigned from) {
-    unsigned to = score_key(pos_inf()) + 1;
+    unsigned to = 0;
+    for (i64 i = tid; i < count; i += T) to = max(to, key_of(i));
+    to = g.max(to) + 1;
+    int reached = 0x7fffffff;
 #pragma unroll 1
-    while (to - from > 1) {
+    while (to - from > 1 && reached > W + W / 8) {
       const unsigned mid = from + (to - from) / 2;
       int c = 0;
+#pragma unroll 4
       for (i64 i = tid; i < count; i += T) c += key_of(i) >= mid ? 1 : 0;
-      if (g.sum(c) >= W) from = mid;
+      c = g.sum(c);
+      if (c >= W) from = mid, reached = c;
       else to = mid;
     }
     return from;
@@ -603,10 +660,10 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
   if (allTiles > r.kTiles) {
     auto take = [&](i64 t) {
       const unsigned key = at.tile_key(t);
-      if (T == 256 || t < kTilesHeld) r.tileKey[t] = key;   // (in the place of what it comes from)
+      if (T == kSmall || t < kTilesHeld) r.tileKey[t] = key;   // (in the place of what it comes from)
       mine = max(mine, key);
     };
-    if constexpr (T == 256) {   // (t / tiles: fewer than 2^12 tiles, off by less than half of one)
+    if constexpr (T == kSmall) {   // (t / tiles: fewer than 2^12 tiles, off by less than half of one)
       const float per = 1.0f / (float)tiles;
       for (int t = tid; t < rowTiles; t += T) {
         const double2 row = at.row((int)(((float)t + 0.5f) * per));
@@ -622,7 +679,7 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
     least = with_slack(reached_by<T>(mine, W, r, g), error);
   }
   auto listed_key = [&](i64 t) {
-    return allTiles > r.kTiles && (T == 256 || t < kTilesHeld) ? r.tileKey[t] : at.tile_key(t);
+    return allTiles > r.kTiles && (T == kSmall || t < kTilesHeld) ? r.tileKey[t] : at.tile_key(t);
   };
   auto list_tiles = [&] {
 #pragma unroll 1
@@ -790,16 +847,17 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
     if (pass > 0 || !r.close) break;
     // 64 bits for the rows in question
 #pragma unroll 1
-    for (int n = 0; n < a.N; ++n) {
-      bool inQuestion = false;
-      for (int i = tid; i < c; i += T) inQuestion |= r.again[i] && parent_of(r.place[i]) == n && word_of(r.place[i]) >= 0;
-      if (!__syncthreads_or(inQuestion)) continue;
+    for (int k = 0; k < c; ++k) {
+      if (!r.again[k] || word_of(r.place[k]) < 0) continue;   // (the same for all threads)
+      const int n = parent_of(r.place[k]);
       const double2 exactly = at.exact_row(n, g);
       const NodeScores<TIn> rows = at.rows(n);
+      __syncthreads();
       for (int i = tid; i < c; i += T)
         if (parent_of(r.place[i]) == n && word_of(r.place[i]) >= 0) {
           const int v = word_of(r.place[i]);
           r.d[i] = at.value(exactly, to_f32(rows.e[v]) + to_f32(rows.p[v]));
+          r.again[i] = 0;
         }
       __syncthreads();
     }
@@ -854,8 +912,8 @@ void launch_extend_beams(const NodeArgs& a, const float* scores, float* outScore
       ScopedKernel prof("extend_pick", stream);
       TB200_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, scores, outScores, parents, words, W, tiles, s, beyond));
     };
-    if (all_held(W, a.N, tiles)) pick(std::integral_constant<int, 256>{});
-    else pick(std::integral_constant<int, 1024>{});
+    if (all_held(W, a.N, tiles)) pick(std::integral_constant<int, kSmall>{});
+    else pick(std::integral_constant<int, kLarge>{});
   });
 }
 
