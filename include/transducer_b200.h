@@ -441,7 +441,8 @@ int tb200_reorder_states(const tb200_states* states, int count, const int* paren
 /* Rows of a table [R, H] (`stride` elements from one row to the next) for words [count]:
  *   rows[n,h] = factor * table[words[n], h] where number (n, h) stays, else 0,
  * in fp32, rounded once (bf16 = 1: table, rows, deltas and grad are bfloat16); a row of zeros where the
- * word is not in [0, R).  Of 65536 numbers k = round(65536 * dropout), 65535 at most, are dropped, and
+ * word is not in [0, R).  Of 65536 numbers k = round(65536 * dropout), of two next ones the even one and 65535
+ * at most, are dropped, and
  * factor = scale * 65536 / (65536 - k).  Number (n, h) is dropped if 16 bits of Philox4x32-10 are below
  * k: counter (n mod 2^32, n / 2^32, h / 8, 0), key (seed mod 2^32, seed / 2^32), of its four numbers x the low
  * (h even) or high half of x[h % 8 / 2].  seedAt (device memory): the seed is there instead, if not NULL.

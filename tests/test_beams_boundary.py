@@ -91,8 +91,10 @@ def test_bad_parents_and_states():
 
 
 def test_outputs_that_overlap():
+    parents = torch.zeros(2, 4, dtype=torch.int32)
+
     def accept(states, out, W):
-        _check_apart([_row(s) for s in states], out, states[0].shape[0], states[0].shape[1], W)
+        _check_apart([_row(s) for s in states], out, states[0].shape[0], states[0].shape[1], W, parents)
 
     def refuse(states, out, message):
         with pytest.raises(ValueError, match=message):
@@ -113,6 +115,7 @@ def test_outputs_that_overlap():
     refuse([s], [torch.zeros(2, 1, 5).expand(2, 4, 5)], "with itself")
     refuse([s], [torch.zeros(1, 4, 5).expand(2, 4, 5)], "with itself")
     refuse([s], [torch.zeros(32).as_strided((2, 4, 5), (15, 4, 1))], "with itself")
+    refuse([parents], [parents], "with parents")
     big = torch.zeros(1, 4097, 1)
     refuse([big], [big], "at most 4096")
 

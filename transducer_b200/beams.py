@@ -119,7 +119,7 @@ def reorder_states(states, parents, out=None, validate_parents=True):
                 rows.append(row)
                 moved += at, to, from_b, from_n, to_b, to_n, size
         if not made:
-            _check_apart(rows, out, B, N, W)
+            _check_apart(rows, out, B, N, W, parents)
         beyond = 0
         if B * W:
             beyond = _transducer.reorder_states(moved, parents.data_ptr(), B, N, W, not made, validate_parents)
@@ -167,9 +167,9 @@ def _end(row, B, N):
     return row[0] + ((B - 1) * row[1] + (N - 1) * row[2] + row[3] if B * N * row[3] else 0)
 
 
-def _check_apart(rows, out, B, N, W):
+def _check_apart(rows, out, B, N, W, parents):
     """That outputs overlap with nothing, but for one that is its state itself (the same place for every hypothesis)."""
-    taken = []
+    taken = [(parents.data_ptr(), parents.data_ptr() + parents.nbytes)]
     ends = [_end(row, B, N) for row in rows]
     for i, o in enumerate(out):
         mine = _row(o)
@@ -190,5 +190,5 @@ def _check_apart(rows, out, B, N, W):
                 raise ValueError("at most %d hypotheses are reordered in place" % MAX_REORDERED_WIDTH)
         for other in taken:
             if begin < other[1] and other[0] < end:
-                raise ValueError("outputs must not overlap with each other")
+                raise ValueError("outputs must not overlap with each other or with parents")
         taken.append((begin, end))

@@ -17,7 +17,7 @@ EmbedArgs embed_args(const void* table, int bf16, long long stride, const int* w
   check(count < 0x7fffffffLL, "too many words (there must be fewer than 2^31 - 1)");
   check(R <= 1 << 28 && H <= 1 << 23, "the table must have at most 2^28 rows of 2^23 numbers");
   check(dropout >= 0.0 && dropout < 1.0, "dropout must be at least 0 and below 1");
-  const unsigned dropped = std::min(65535u, (unsigned)std::lround(dropout * 65536.0));
+  const unsigned dropped = std::min(65535u, (unsigned)std::nearbyint(dropout * 65536.0));
   const double factor = scale * 65536.0 / (65536.0 - dropped);
   check(std::isfinite((float)factor), "scale must be finite");
   return EmbedArgs{table, stride, words, count, R, H, bf16 ? kDtypeBf16 : kDtypeF32, (float)factor, dropped, seed, seedAt};

@@ -40,14 +40,14 @@ __device__ __forceinline__ void philox(uint4 (&c)[K], Seed key) {
   }
 }
 
-// The numbers of a row that a lane of a warp has, of 256 that begin at `first`: eight that follow each other where rows
-// can be moved in 16-byte vectors, else every 32nd.
+// The numbers of a row that a lane of a warp has, of 256 that begin at `first`: vectors of 16 bytes, the lanes' side by
+// side, where rows can be moved so, else every 32nd.
 template <typename T, int VEC>
 struct Numbers {
   static constexpr int kMoves = VEC == 1 ? kGroup : kGroup / VEC;
   RawWords<T, VEC> raw[kMoves];
   static __device__ __forceinline__ int at(int first, int lane, int move) {
-    return first + (VEC == 1 ? 32 * move + lane : kGroup * lane + VEC * move);
+    return first + 32 * VEC * move + VEC * lane;
   }
   __device__ __forceinline__ void load(const T* row, int first, int lane, int H) {
 #pragma unroll
@@ -78,9 +78,9 @@ struct Numbers {
 // number of row n and 256 that begin at `first`.  All lanes: each makes the bits of a whole counter.
 template <int VEC>
 struct Stays {
-  uint4 bits;   // VEC == 1: bit i of x for number i
+  uint4 bits;   // VEC < 8: bit i of x for number i
   __device__ __forceinline__ void get(bool (&stay)[kGroup], unsigned dropped) const {
-    if constexpr (VEC == 1) {
+    if constexpr (VEC < kGroup) {
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) stay[i] = bits.x >> i & 1;
     } else {
@@ -101,16 +101,19 @@ __device__ __forceinline__ void stays(Stays<VEC> (&out)[K], N place, int first, 
   philox(c, seed);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if constexpr (VEC == 1) {
-      const Stays<2> whole{c[k]};
+    if constexpr (VEC < kGroup) {   // (the bits of a counter are several lanes')
+      const Stays<kGroup> whole{c[k]};
       bool stay[kGroup];
       whole.get(stay, dropped);
       unsigned mine = 0, bits = 0;
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) mine |= stay[i] ? 1u << i : 0u;
+      constexpr int kLanes = kGroup / VEC;   // to a counter
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i)
-        bits |= (__shfl_sync(0xffffffffu, mine, 4 * i + lane / kGroup) >> lane % kGroup & 1) << i;
+      for (int i = 0; i < kLanes; ++i) {
+        const unsigned theirs = __shfl_sync(0xffffffffu, mine, 32 / kLanes * i + lane / kLanes);
+        bits |= (theirs >> lane % kLanes * VEC & ((1u << VEC) - 1)) << VEC * i;
+      }
       out[k].bits.x = bits;
     } else {
       out[k].bits = c[k];
@@ -296,11 +299,18 @@ struct Parts {
 
 // Adds up 256 numbers of the rows of `count` places that follow each other, at(i) the i-th place and its word; `before` and
 // `behind` are the words next to them.  Rows that lie within are written to the gradient, the shares of others to
-// part(slot): 0 where the row is the first, 1 where it is a later one.
+// part(slot): 0 where the row is the first, 1 where it is a later one.  Rows of vectors come through `ring`, the warp's shared
+// memory, from which every lane reads what it has copied itself.
+template <typename T, int VEC>
+constexpr int kAddBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows that are added at a time
+constexpr int kAddBatches = 3;                                  // in the ring
+template <typename T, int VEC>
+constexpr int kAddRing = VEC > 1 ? kAddBatches * kAddBatch<T, VEC> * 32 * kGroup * (int)sizeof(T) : 0;   // bytes of a warp
+
 template <typename T, int VEC, bool DROP, typename At, typename Part>
 __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, int count, At at, int before, int behind,
-                                           int first, int lane, T* grad, Part part) {
-  constexpr int kBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows on their way while as many are added (more: registers)
+                                           int first, int lane, T* grad, char* ring, Part part) {
+  constexpr int kBatch = kAddBatch<T, VEC>, kMoves = Numbers<T, VEC>::kMoves;
   const Seed seed(a);
   float sum[kGroup] = {};
   int row = at(0).y;
@@ -316,21 +326,45 @@ __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, 
       p[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
     }
   };
-  Numbers<T, VEC> next[kBatch];
+  Numbers<T, VEC> next[kBatch];   // (of single words: the next batch)
+  auto place = [&](int i, int j) { return ring + ((i / kBatch % kAddBatches * kBatch + j) * kMoves * 32 + lane) * 16; };
   auto bring = [&](int i) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int n = at(min(i + j, count - 1)).x;
-      if (i + j < count) next[j].load(deltas + (i64)n * a.H, first, lane, a.H);
+      const T* row = deltas + (i64)at(min(i + j, count - 1)).x * a.H;
+      if (i + j >= count) break;
+      if constexpr (VEC > 1) {
+#pragma unroll
+        for (int k = 0; k < kMoves; ++k)
+          if (Numbers<T, VEC>::at(first, lane, k) < a.H)
+            copy_async<16>(place(i, j) + 32 * 16 * k, row + Numbers<T, VEC>::at(first, lane, k));
+      } else {
+        next[j].load(row, first, lane, a.H);
+      }
     }
+    if constexpr (VEC > 1) commit_copies();
   };
-  bring(0);
-#pragma unroll 2
+  if constexpr (VEC > 1) {
+#pragma unroll
+    for (int k = 0; k < kAddBatches - 1; ++k) bring(kBatch * k);
+  } else {
+    bring(0);
+  }
+#pragma unroll 1
   for (int i = 0; i < count; i += kBatch) {
     Numbers<T, VEC> x[kBatch];
+    if constexpr (VEC > 1) {
+      bring(i + kBatch * (kAddBatches - 1));
+      wait_copies<kAddBatches - 1>();
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = next[j];
-    bring(i + kBatch);
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int k = 0; k < kMoves; ++k) x[j].raw[k].load(reinterpret_cast<const T*>(place(i, j) + 32 * 16 * k));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) x[j] = next[j];
+      bring(i + kBatch);
+    }
     Stays<VEC> stay[kBatch];
     if constexpr (DROP)
       stays<VEC, kBatch>(stay, [&](int k) { return at(min(i + k, count - 1)).x; }, first, lane, seed, a.dropped);
@@ -361,7 +395,7 @@ constexpr int kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills 
 // CTAs (x, piece): the warps of the first sumCtas add up 256 numbers of an item's rows each; the others fill rows that
 // no word has.
 template <typename T, int VEC, bool DROP>
-__global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
+__global__ void __launch_bounds__(32 * kWarps, 3) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
                                                                  Parts parts, T* __restrict__ grad, int sumCtas) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   cudaTriggerProgrammaticLaunchCompletion();
@@ -389,7 +423,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) embed_sums_kernel(EmbedArgs a,
     return make_int2(__shfl_sync(0xffffffffu, mine.x, i & 31), __shfl_sync(0xffffffffu, mine.y, i & 31));
   };
   const int before = from > 0 ? s.order[from - 1].y : -1, behind = to < all ? s.order[to].y : -1;
-  add_places<T, VEC, DROP>(a, deltas, to - from, at, before, behind, first, lane, grad,
+  extern __shared__ __align__(16) char rings[];
+  add_places<T, VEC, DROP>(a, deltas, to - from, at, before, behind, first, lane, grad, rings + warp * kAddRing<T, VEC>,
                            [&](int slot, int) { return parts.at(item, slot, piece, lane); });
 }
 
@@ -496,6 +531,7 @@ __global__ void __launch_bounds__(32 * kDirectWarps, 2) embed_direct_kernel(Embe
   constexpr int kOwn = kDirectWords / kDirectWarps / 32;   // words of a lane
   extern __shared__ __align__(16) char shared[];
   DirectRoom& room = *reinterpret_cast<DirectRoom*>(shared);
+  char* const ring = shared + sizeof(DirectRoom);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cta = blockIdx.x, low = (1 << bits) - 1, first = blockIdx.y * 32 * kGroup, N = (int)a.N;
   const int seg = (div_up(N, kDirectWarps) + 31) / 32 * 32, from = warp * seg;
@@ -563,7 +599,8 @@ __global__ void __launch_bounds__(32 * kDirectWarps, 2) embed_direct_kernel(Embe
   if (begin < end) {
     auto at = [&](int i) { return make_int2((int)(room.order[begin + i] & 0xffffu), word(begin + i)); };
     add_places<T, VEC, DROP>(a, deltas, end - begin, at, begin > 0 ? word(begin - 1) : -1, end < all ? word(end) : -1, first,
-                             lane, grad, [&](int slot, int) { return room.share[warp][slot][lane]; });
+                             lane, grad, ring + warp * kAddRing<T, VEC>,
+                             [&](int slot, int) { return room.share[warp][slot][lane]; });
   }
   // rows that no word has
   const float zero[kGroup] = {};
@@ -626,9 +663,10 @@ int row_bits(int R) {
 
 // The launches of one call: each begins while the one before it ends, and waits for its results.
 template <typename... P, typename... A>
-void launch_early(void (*kernel)(P...), dim3 ctas, int threads, cudaStream_t stream, A... args) {
+void launch_early(void (*kernel)(P...), dim3 ctas, int threads, int smem, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = ctas, config.blockDim = dim3(threads), config.stream = stream;
+  config.gridDim = ctas, config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem, config.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
@@ -678,9 +716,11 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     with_variant(a, wide, [&](auto type, auto vec, auto drop) {
       using T = decltype(type);
       auto kernel = embed_direct_kernel<T, decltype(vec)::value, decltype(drop)::value>;
+      constexpr int smem = sizeof(DirectRoom) + kDirectWarps * kAddRing<T, decltype(vec)::value>;
+      allow_dyn_smem(kernel, smem);
       const int bits = row_bits(a.R);
       ScopedKernel prof("embed_direct", stream);
-      kernel<<<dim3(1u << bits, pieces), 32 * kDirectWarps, sizeof(DirectRoom), stream>>>(
+      kernel<<<dim3(1u << bits, pieces), 32 * kDirectWarps, smem, stream>>>(
           a, static_cast<const T*>(deltas), static_cast<T*>(grad), bits);
       TB200_CHECK_LAUNCH();
     });
@@ -710,13 +750,14 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     constexpr bool DROP = decltype(drop)::value;
     {
       ScopedKernel prof("embed_sums", stream);
+      allow_dyn_smem(embed_sums_kernel<T, VEC, DROP>, kWarps * kAddRing<T, VEC>);
       const int sumCtas = div_up(parts.items, kWarps), filled = kFilled * kWarps * pieces;
-      launch_early(embed_sums_kernel<T, VEC, DROP>, dim3(sumCtas + div_up(a.R, filled), pieces), 32 * kWarps, stream, a,
-                   static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad), sumCtas);
+      launch_early(embed_sums_kernel<T, VEC, DROP>, dim3(sumCtas + div_up(a.R, filled), pieces), 32 * kWarps,
+                   kWarps * kAddRing<T, VEC>, stream, a, static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad), sumCtas);
     }
     if (parts.items > 1) {
       ScopedKernel prof("embed_join", stream);
-      launch_early(embed_join_kernel<T, VEC>, dim3(ctas(parts.items, kJoinWarps), pieces), 32 * kJoinWarps, stream, a, s, parts,
+      launch_early(embed_join_kernel<T, VEC>, dim3(ctas(parts.items, kJoinWarps), pieces), 32 * kJoinWarps, 0, stream, a, s, parts,
                    static_cast<T*>(grad));
     }
   });
