@@ -303,11 +303,10 @@ struct Parts {
 // memory, from which every lane reads what it has copied itself.
 template <typename T, int VEC>
 constexpr int kAddBatch = sizeof(T) == 2 && VEC > 1 ? 4 : 2;   // rows that are added at a time
-constexpr int kAddBatches = 3;                                  // in the ring
-template <typename T, int VEC>
-constexpr int kAddRing = VEC > 1 ? kAddBatches * kAddBatch<T, VEC> * 32 * kGroup * (int)sizeof(T) : 0;   // bytes of a warp
+template <typename T, int VEC, int BATCHES>
+constexpr int kAddRing = VEC > 1 ? BATCHES * kAddBatch<T, VEC> * 32 * kGroup * (int)sizeof(T) : 0;   // bytes of a warp
 
-template <typename T, int VEC, bool DROP, typename At, typename Part>
+template <typename T, int VEC, bool DROP, int BATCHES, typename At, typename Part>
 __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, int count, At at, int before, int behind,
                                            int first, int lane, T* grad, char* ring, Part part) {
   constexpr int kBatch = kAddBatch<T, VEC>, kMoves = Numbers<T, VEC>::kMoves;
@@ -327,7 +326,7 @@ __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, 
     }
   };
   Numbers<T, VEC> next[kBatch];   // (of single words: the next batch)
-  auto place = [&](int i, int j) { return ring + ((i / kBatch % kAddBatches * kBatch + j) * kMoves * 32 + lane) * 16; };
+  auto place = [&](int i, int j) { return ring + ((i / kBatch % BATCHES * kBatch + j) * kMoves * 32 + lane) * 16; };
   auto bring = [&](int i) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
@@ -346,7 +345,7 @@ __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, 
   };
   if constexpr (VEC > 1) {
 #pragma unroll
-    for (int k = 0; k < kAddBatches - 1; ++k) bring(kBatch * k);
+    for (int k = 0; k < BATCHES - 1; ++k) bring(kBatch * k);
   } else {
     bring(0);
   }
@@ -354,8 +353,8 @@ __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, 
   for (int i = 0; i < count; i += kBatch) {
     Numbers<T, VEC> x[kBatch];
     if constexpr (VEC > 1) {
-      bring(i + kBatch * (kAddBatches - 1));
-      wait_copies<kAddBatches - 1>();
+      bring(i + kBatch * (BATCHES - 1));
+      wait_copies<BATCHES - 1>();
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
 #pragma unroll
@@ -390,7 +389,7 @@ __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, 
   finish(true);
 }
 
-constexpr int kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
+constexpr int kSumBatches = 3, kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
 
 // CTAs (x, piece): the warps of the first sumCtas add up 256 numbers of an item's rows each; the others fill rows that
 // no word has.
@@ -424,7 +423,8 @@ __global__ void __launch_bounds__(32 * kWarps, 3) embed_sums_kernel(EmbedArgs a,
   };
   const int before = from > 0 ? s.order[from - 1].y : -1, behind = to < all ? s.order[to].y : -1;
   extern __shared__ __align__(16) char rings[];
-  add_places<T, VEC, DROP>(a, deltas, to - from, at, before, behind, first, lane, grad, rings + warp * kAddRing<T, VEC>,
+  add_places<T, VEC, DROP, kSumBatches>(a, deltas, to - from, at, before, behind, first, lane, grad,
+                                        rings + warp * kAddRing<T, VEC, kSumBatches>,
                            [&](int slot, int) { return parts.at(item, slot, piece, lane); });
 }
 
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArg
 
 // ---- few words: all in one launch ---------------------------------------------------------------
 
-constexpr int kDirectWords = 4096, kDirectWarps = 8;
+constexpr int kDirectWords = 4096, kDirectWarps = 8, kDirectBatches = 4;
 
 struct DirectRoom {
   int count[kDirectWarps][kSortRows];
@@ -598,8 +598,8 @@ __global__ void __launch_bounds__(32 * kDirectWarps, 2) embed_direct_kernel(Embe
   auto word = [&](int i) { return (int)(room.order[i] >> 16) << bits | cta; };
   if (begin < end) {
     auto at = [&](int i) { return make_int2((int)(room.order[begin + i] & 0xffffu), word(begin + i)); };
-    add_places<T, VEC, DROP>(a, deltas, end - begin, at, begin > 0 ? word(begin - 1) : -1, end < all ? word(end) : -1, first,
-                             lane, grad, ring + warp * kAddRing<T, VEC>,
+    add_places<T, VEC, DROP, kDirectBatches>(a, deltas, end - begin, at, begin > 0 ? word(begin - 1) : -1, end < all ? word(end) : -1, first,
+                             lane, grad, ring + warp * kAddRing<T, VEC, kDirectBatches>,
                              [&](int slot, int) { return room.share[warp][slot][lane]; });
   }
   // rows that no word has
@@ -654,10 +654,10 @@ unsigned ctas(i64 warps, int ofCta = kWarps) {
 // Whether the gradient is made in one launch.  A frequent word is one CTA's there, for every 256 numbers: of 4096 words in a
 // table of 30 rows it takes 23 us instead of 16 in three launches, in one of 1025 rows 16 instead of 17.
 bool in_one_launch(i64 N, int R) { return N <= kDirectWords && N <= 32ll * R && R <= 128 * kSortRows; }
-// CTAs that the rows are shared between, as a power of two: up to 128, and no more than 256 rows each.
-int row_bits(int R) {
+// CTAs that the rows are shared between, as a power of two: up to `most`, and no more than 256 rows each.
+int row_bits(int R, int most) {
   int bits = 0;
-  while ((bits < 7 && 2 << bits <= R) || (i64)kSortRows << bits < R) ++bits;
+  while ((2 << bits <= std::min(R, most)) || (i64)kSortRows << bits < R) ++bits;
   return bits;
 }
 
@@ -716,9 +716,9 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     with_variant(a, wide, [&](auto type, auto vec, auto drop) {
       using T = decltype(type);
       auto kernel = embed_direct_kernel<T, decltype(vec)::value, decltype(drop)::value>;
-      constexpr int smem = sizeof(DirectRoom) + kDirectWarps * kAddRing<T, decltype(vec)::value>;
+      constexpr int smem = sizeof(DirectRoom) + kDirectWarps * kAddRing<T, decltype(vec)::value, kDirectBatches>;
       allow_dyn_smem(kernel, smem);
-      const int bits = row_bits(a.R);
+      const int bits = row_bits(a.R, std::min(128, 2 * 148 / pieces));   // (two CTAs per SM at once)
       ScopedKernel prof("embed_direct", stream);
       kernel<<<dim3(1u << bits, pieces), 32 * kDirectWarps, smem, stream>>>(
           a, static_cast<const T*>(deltas), static_cast<T*>(grad), bits);
@@ -733,7 +733,7 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
   s.R = a.R;
   const Parts parts{reinterpret_cast<float*>(at), part, pieces, (int)div_up64(a.N, part)};
   {
-    const int bits = row_bits(a.R);
+    const int bits = row_bits(a.R, 128);
     ScopedKernel prof("embed_sort", stream);
     auto sort = [&](auto warps) {
       constexpr int WARPS = decltype(warps)::value;
@@ -750,10 +750,10 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     constexpr bool DROP = decltype(drop)::value;
     {
       ScopedKernel prof("embed_sums", stream);
-      allow_dyn_smem(embed_sums_kernel<T, VEC, DROP>, kWarps * kAddRing<T, VEC>);
+      allow_dyn_smem(embed_sums_kernel<T, VEC, DROP>, kWarps * kAddRing<T, VEC, kSumBatches>);
       const int sumCtas = div_up(parts.items, kWarps), filled = kFilled * kWarps * pieces;
       launch_early(embed_sums_kernel<T, VEC, DROP>, dim3(sumCtas + div_up(a.R, filled), pieces), 32 * kWarps,
-                   kWarps * kAddRing<T, VEC>, stream, a, static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad), sumCtas);
+                   kWarps * kAddRing<T, VEC, kSumBatches>, stream, a, static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad), sumCtas);
     }
     if (parts.items > 1) {
       ScopedKernel prof("embed_join", stream);
