@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
 
 // ---- the gradient -------------------------------------------------------------------------------
 
-// An item is `part` places of the order that follow each other.  Rows that lie within one item are its sums; of the
-// others every item leaves its share: slot 0 if it begins with the item, else slot 1.
+// An item is `part` places of the order that follow each other, a CTA's.  Rows that lie within one item are its sums; of the
+// others every item leaves its share: slot 0 if it begins with the item or before it, else slot 1.
 struct Parts {
   float* sums;   // [items, 2, pieces, 32 lanes, 8]
   int part, pieces;
@@ -389,10 +389,10 @@ __device__ __forceinline__ void add_places(const EmbedArgs& a, const T* deltas, 
   finish(true);
 }
 
-constexpr int kSumBatches = 3, kMostPart = 32, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
+constexpr int kSumBatches = 3, kFilled = 8;   // kFilled: rows that a warp fills where no word has them
 
-// CTAs (x, piece): the warps of the first sumCtas add up 256 numbers of an item's rows each; the others fill rows that
-// no word has.
+// CTAs (x, piece): the first sumCtas add up 256 numbers of an item's rows, an eighth of its places per warp; the others
+// fill rows that no word has.
 template <typename T, int VEC, bool DROP>
 __global__ void __launch_bounds__(32 * kWarps, 3) embed_sums_kernel(EmbedArgs a, const T* __restrict__ deltas, Sorted s,
                                                                  Parts parts, T* __restrict__ grad, int sumCtas) {
@@ -411,30 +411,62 @@ __global__ void __launch_bounds__(32 * kWarps, 3) embed_sums_kernel(EmbedArgs a,
         Numbers<T, VEC>::store(grad + (fill * kFilled + __ffs(empty) - 1) * a.H, first, lane, a.H, zero);
     return;
   }
-  const int item = blockIdx.x * kWarps + warp, piece = blockIdx.y, first = piece * 32 * kGroup;
-  const int all = s.all();
-  if (item >= parts.items || item * (i64)parts.part >= all) return;
-  const int from = item * parts.part;
-  const int to = (int)min((i64)from + parts.part, (i64)all);
-  // lane i: the item's place i
+  extern __shared__ __align__(16) char rings[];
+  __shared__ float4 share[kWarps][2][32][2];   // what the warps leave, as the items do
+  __shared__ int firstRow[kWarps], lastRow[kWarps];   // -1: the warp has no places
+  const int item = blockIdx.x, piece = blockIdx.y, first = piece * 32 * kGroup, all = s.all(), own = parts.part / kWarps;
+  if ((i64)item * parts.part >= all) return;
+  const int end = (int)min((i64)(item + 1) * parts.part, (i64)all);   // of the item
+  const int from = (int)min((i64)item * parts.part + warp * own, (i64)end), to = from + min(own, end - from);
+  // lane i: the warp's place i
   const int2 mine = lane < to - from ? s.order[from + lane] : make_int2(0, -1);
   auto at = [&](int i) {
     return make_int2(__shfl_sync(0xffffffffu, mine.x, i & 31), __shfl_sync(0xffffffffu, mine.y, i & 31));
   };
   const int before = from > 0 ? s.order[from - 1].y : -1, behind = to < all ? s.order[to].y : -1;
-  extern __shared__ __align__(16) char rings[];
-  add_places<T, VEC, DROP, kSumBatches>(a, deltas, to - from, at, before, behind, first, lane, grad,
-                                        rings + warp * kAddRing<T, VEC, kSumBatches>,
-                           [&](int slot, int) { return parts.at(item, slot, piece, lane); });
+  const int behindAll = end < all ? s.order[end].y : -1;
+  const int begins = at(0).y, ends = at(to - from - 1).y;
+  if (lane == 0) firstRow[warp] = from < to ? begins : -1, lastRow[warp] = from < to ? ends : -1;
+  if (from < to)
+    add_places<T, VEC, DROP, kSumBatches>(a, deltas, to - from, at, before, behind, first, lane, grad,
+                                          rings + warp * kAddRing<T, VEC, kSumBatches>,
+                                          [&](int slot, int) { return share[warp][slot][lane]; });
+  __syncthreads();
+  if (from >= to) return;
+  // rows that the warp is the first of the item to have and has not written
+  const bool single = begins == ends;
+#pragma unroll 1
+  for (int slot = 0; slot < 2; ++slot) {
+    const int row = slot == 0 ? begins : ends;
+    const bool onward = (slot == 1 || single) && ends == behind;
+    if (slot == 0 ? !(begins == before || onward) || (warp > 0 && begins == before) : single || !onward) continue;
+    float4 x = share[warp][slot][lane][0], y = share[warp][slot][lane][1];
+    bool more = onward;   // the row goes on behind what has been added
+    for (int w = warp + 1; more && w < kWarps && firstRow[w] >= 0; ++w) {
+      const float4 u = share[w][0][lane][0], v = share[w][0][lane][1];
+      x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
+      y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+      more = lastRow[w] == row && (w + 1 < kWarps && firstRow[w + 1] >= 0 ? firstRow[w + 1] : behindAll) == row;
+    }
+    const bool start = warp == 0 && slot == 0;
+    if (more || (start && begins == before)) {
+      float4* p = parts.at(item, start ? 0 : 1, piece, lane);
+      p[0] = x, p[1] = y;
+    } else {
+      const float sum[kGroup] = {x.x * a.factor, x.y * a.factor, x.z * a.factor, x.w * a.factor,
+                                 y.x * a.factor, y.y * a.factor, y.z * a.factor, y.w * a.factor};
+      Numbers<T, VEC>::store(grad + (i64)row * a.H, first, lane, a.H, sum);
+    }
+  }
 }
 
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 8;
 
 // Rows that lie in several items, each by the warp (or, of many items, the CTA) that has the first of them.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kJoinWarps, 2) embed_join_kernel(EmbedArgs a, Sorted s, Parts parts,
                                                                  T* __restrict__ grad) {
-  constexpr int kMany = 32;   // items from which on the CTA adds them up together
+  constexpr int kMany = 16;   // items from which on the CTA adds them up together
   __shared__ float4 shares[kJoinWarps][32][2];
   struct Row {
     int row, slot;   // -1: none begins in the item
@@ -627,8 +659,9 @@ __global__ void __launch_bounds__(32 * kDirectWarps, 2) embed_direct_kernel(Embe
   }
 }
 
-// Places per item: few where there are few warps, so that the rows are read at once; their shares then weigh more.
-int places_per_item(i64 N, int pieces) { return N * pieces <= 32 * 148 * 16 ? 8 : kMostPart; }
+// Places per item: 8 to a warp while those warps fit the chip at once, so that their rows are read at once, else 32 (64 x 101
+// words, rows of 256 numbers: 21 us with 8, 25 with 32; 256 x 201 words, rows of 1024: 96 with 8, 82 with 32).
+int places_per_item(i64 N, int pieces) { return kWarps * (N * pieces <= 32 * 148 * 16 ? 8 : 32); }
 
 bool aligned(const EmbedArgs& a, const void* rows) {
   const int size = a.dtype == kDtypeBf16 ? 2 : 4;
@@ -751,7 +784,7 @@ void launch_embed_backward(const EmbedArgs& a, const void* deltas, void* grad, v
     {
       ScopedKernel prof("embed_sums", stream);
       allow_dyn_smem(embed_sums_kernel<T, VEC, DROP>, kWarps * kAddRing<T, VEC, kSumBatches>);
-      const int sumCtas = div_up(parts.items, kWarps), filled = kFilled * kWarps * pieces;
+      const int sumCtas = parts.items, filled = kFilled * kWarps * pieces;
       launch_early(embed_sums_kernel<T, VEC, DROP>, dim3(sumCtas + div_up(a.R, filled), pieces), 32 * kWarps,
                    kWarps * kAddRing<T, VEC, kSumBatches>, stream, a, static_cast<const T*>(deltas), s, parts, static_cast<T*>(grad), sumCtas);
     }
