@@ -447,7 +447,8 @@ int tb200_reorder_states(const tb200_states* states, int count, const int* paren
  * k: counter (n mod 2^32, n / 2^32, h / 8, 0), key (seed mod 2^32, seed / 2^32), of its four numbers x the low
  * (h even) or high half of x[h % 8 / 2].  seedAt (device memory): the seed is there instead, if not NULL.
  * The backward call writes grad [R, H] whole: the sums of factor * deltas[n,h] over the numbers that stay
- * of the rows that are a word's, in fp32, rounded once; the same bits from run to run.
+ * of the rows that are a word's, in fp32, in an order that follows from the words alone, rounded once: the same bits from run to
+ * run.
  * count is below 2^31 - 1, R 2^28 and H 2^23 at most. */
 int tb200_embed_words(const void* table, int bf16, long long stride, const int* words, long long count,
                       void* rows, int R, int H, double scale, double dropout, long long seed,

