@@ -1,7 +1,7 @@
 // States that follow their hypotheses: row w of an utterance becomes what row parents[w] was, in every tensor of a
 // list at once.  Copies, bound by HBM: 32 x 16 hypotheses with 410 KB each (339 MB read and written, parents that
-// have several successors read once) take 55 us, 52 at the measured copy rate; in place, where a third of them stays as it is,
-// 64 us; 4 x 8 hypotheses with 10 KB 4 us, latency.  A warp has 4 KB of a row, eight vectors a lane on their way.
+// have several successors read once) take 55 us, 52 at the measured copy rate; in place 64; 4 x 8 hypotheses with
+// 10 KB 4 us, latency.  A warp has 4 KB of a row, eight vectors a lane on their way.
 #include <algorithm>
 #include <cstdlib>
 #include <vector>
