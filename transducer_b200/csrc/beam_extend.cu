@@ -531,7 +531,8 @@ __device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W
     };
     auto place = [&](int i) { return place_of(n, chunk_word<VEC>(tile, g.lane, i)); };
     auto counts = [&](int i, double d) { return d > -1.0 / 0.0 && better(d, place(i)); };
-    if (row.y > -1.0 / 0.0 && at.value(row, at.s.best[(at.first * at.tiles + t) * 32 + g.lane]) >= p.cutValue) {
+    // (the chunk's first word is the first of equals)
+    if (row.y > -1.0 / 0.0 && counts(0, at.value(row, at.s.best[(at.first * at.tiles + t) * 32 + g.lane]))) {
       r = at.rows(n);
 #pragma unroll 8
       for (int i = 0; i < kChunk; ++i) left |= counts(i, value(i)) ? 1u << i : 0u;
@@ -794,11 +795,9 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
     c = r.count[2];
     many = c > r.kWords;
   }
-  const bool exact = many;
-  if (many) c = general_pick<TIn, VEC, T>(at, W, least, error, g);
 
   // of many words those that can be among the best
-  if (c > 2 * W + 64) {
+  if (!many && c > 2 * W + 64) {
     mine = 0;
     for (int i = tid; i < c; i += T) mine = max(mine, extension_key(r.d[i]));
     least = with_slack(reached_by<T>(mine, W, r, g), error);
@@ -816,7 +815,10 @@ __global__ void __launch_bounds__(T) extend_pick_kernel(NodeArgs a, const float*
       __syncthreads();
     }
     c = r.count[3];
+    many = c > 2 * T;   // (to compare each with all others takes as long as the way through the rows)
   }
+  const bool exact = many;
+  if (many) c = general_pick<TIn, VEC, T>(at, W, least, error, g);
 
   // where each is in the order, and whether what it rests on is closer than the sums' errors
   for (int i = tid; i < c; i += T) r.again[i] = 0;
