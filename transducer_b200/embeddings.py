@@ -16,29 +16,27 @@ class WordEmbedding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, words, scale, dropout, seed, validate_words):
-        rows = _rows_of(table, words, scale, dropout, seed, validate_words)
-        R, H = table.shape
-        numbers, place = _seed(seed)
+        rows, numbers, place = _rows_of(table, words, scale, dropout, seed, validate_words)
         if place:
             ctx.save_for_backward(words, seed)
         else:
             ctx.save_for_backward(words)
-        ctx.rest = (R, H, table.dtype is torch.bfloat16, scale, dropout, numbers, place)
+        count, (R, H) = words.numel(), table.shape
+        ctx.rest = (count, R, H, table.dtype is torch.bfloat16, scale, dropout, numbers, place,
+                    _transducer.embed_backward_workspace_bytes(count, R, H))
         return rows
 
     @staticmethod
     def backward(ctx, deltas):
         words = ctx.saved_tensors[0]   # (refuses words, and a seed on the device, that were written since)
-        R, H, bf16, scale, dropout, numbers, place = ctx.rest
+        count, R, H, bf16, scale, dropout, numbers, place, nbytes = ctx.rest
         if not deltas.is_contiguous():
             deltas = deltas.contiguous()
-        count = words.numel()
         with OnDevice(deltas.device):
             grad = deltas.new_empty((R, H))
-            nbytes = _transducer.embed_backward_workspace_bytes(count, R, H)
-            ws = words.new_empty((nbytes + 3) // 4)
+            ws = words.new_empty(nbytes // 4 + 1) if nbytes else None   # (few words need none)
             _transducer.embed_backward(deltas.data_ptr(), bf16, words.data_ptr(), count, grad.data_ptr(), R, H, scale,
-                                       dropout, numbers, place, ws.data_ptr(), nbytes)
+                                       dropout, numbers, place, ws.data_ptr() if nbytes else 0, nbytes)
         if torch.is_grad_enabled():   # (somebody wants to differentiate it)
             grad = Once.apply(grad, deltas)
         return (grad,) + (None,) * 5
@@ -64,6 +62,7 @@ def _seed(seed):
 
 
 def _rows_of(table, words, scale, dropout, seed, validate_words):
+    """The rows, and the seed as `_seed` has it."""
     if table.stride(1) != 1 and table.shape[1] != 1:
         table = table.contiguous()
     R, H = table.shape
@@ -75,7 +74,7 @@ def _rows_of(table, words, scale, dropout, seed, validate_words):
                                          numbers, place, validate_words)
     if beyond:
         raise ValueError("Word index mismatch")
-    return rows
+    return rows, numbers, place
 
 
 def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=True):
@@ -120,5 +119,5 @@ def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=
     elif seed is not None and not -2 ** 63 <= seed < 2 ** 63:
         raise ValueError("seed must fit 64 bits")
     if not (table.requires_grad and torch.is_grad_enabled()):
-        return _rows_of(table, words, scale, dropout, seed, validate_words)
+        return _rows_of(table, words, scale, dropout, seed, validate_words)[0]
     return WordEmbedding.apply(table, words, scale, dropout, seed, validate_words)
