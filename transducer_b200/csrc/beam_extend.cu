@@ -397,9 +397,10 @@ struct Utterance {
     return x;
   }
 
-  // Its sum in 64 bits, by the CTA.  (Little code: where it is needed it has to be brought first.)  Bound by the 64-bit units, 1
+  // Its sum in 64 bits, by the CTA.  (Little code: where it is needed it has to be brought first.)  One CTA's loads and sums, 1
   // word a cycle: 32000 words take 17 us.  Of calls with 64 x 32 hypotheses of N(0, 1.5) scores a sixth needs two rows' (60 ->
-  // 98 us); clusters of four CTAs that share a row took 12 us more in every call.
+  // 98 us).  Exponentials in two 32-bit terms, and 64 bits only where those are too close as well, took 13 us a row and
+  // 97 a call; clusters of four CTAs that share a row 12 us more in every call.
   __device__ __noinline__ double2 exact_row(int n, Group<T>& g) const {
     constexpr int kWords = PickRoom<T>::kChunks / T, kBatch = kWords > VEC ? kWords / VEC : 1;   // of a thread at a time
     static_assert(VEC <= kWords || T == kLarge);
