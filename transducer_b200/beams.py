@@ -104,10 +104,12 @@ def reorder_states(states, parents, out=None, validate_parents=True):
         if made:
             out = []
         rows, moved = [], []
+        copies = []   # (which have to live until the kernels are enqueued: `moved` has addresses)
         for i, s in enumerate(states):
             row = _row(s)
             if row is None:
                 s = s.detach().contiguous()
+                copies.append(s)
                 row = _row(s)
             at, from_b, from_n, size = row
             if made:
