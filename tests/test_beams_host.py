@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from transducer_b200 import beams, reorder_states
+from transducer_b200 import beams, embed_words, embeddings, reorder_states
 
 
 class Anywhere(object):
@@ -93,3 +93,127 @@ def test_states_that_are_copied_live_until_the_kernels_are_enqueued(mover, copie
     got = reorder_states(states, PARENTS, out=out)
     assert mover.calls == 1
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- the seed of embed_words --------------------------------------------------------------------
+
+class Embedder(object):
+    """embed_words and its gradient on the host, with a mask that shows which seed was read: number (n, h) is dropped where
+    bit (n + h) mod 64 of the seed is set."""
+
+    @staticmethod
+    def _masked(rows, words, seed, seed_at):
+        if seed_at:
+            seed = ctypes.c_int64.from_address(seed_at).value
+        n, h = torch.arange(rows.shape[0])[:, None], torch.arange(rows.shape[1])
+        dropped = torch.tensor([(seed >> i) & 1 for i in range(64)], dtype=torch.bool)[(n + h) % 64]
+        return torch.where(dropped, 0.0, rows)
+
+    @staticmethod
+    def _tensor(address, kind, dtype, *shape):
+        count = 1
+        for n in shape:
+            count *= n
+        return torch.frombuffer((kind * count).from_address(address), dtype=dtype).view(shape)
+
+    def embed_words(self, table, bf16, stride, words, count, rows, R, H, scale, dropout, seed, seed_at, validate):
+        words = self._tensor(words, ctypes.c_int, torch.int32, count)
+        table = self._tensor(table, ctypes.c_float, torch.float32, R, H)
+        self._tensor(rows, ctypes.c_float, torch.float32, count, H).copy_(
+            self._masked(table[words.long()], words, seed, seed_at))
+        return 0
+
+    def embed_backward_workspace_bytes(self, count, R, H):
+        return 0
+
+    def embed_backward(self, deltas, bf16, words, count, grad, R, H, scale, dropout, seed, seed_at, ws, nbytes):
+        words = self._tensor(words, ctypes.c_int, torch.int32, count)
+        deltas = self._tensor(deltas, ctypes.c_float, torch.float32, count, H)
+        grad = self._tensor(grad, ctypes.c_float, torch.float32, R, H)
+        grad.zero_().index_add_(0, words.long(), self._masked(deltas, words, seed, seed_at))
+
+
+@pytest.fixture
+def embedder(monkeypatch):
+    monkeypatch.setattr(embeddings, "_transducer", Embedder())
+    monkeypatch.setattr(embeddings, "OnDevice", Anywhere)
+
+
+def fresh_seed(value):
+    return torch.tensor([value], dtype=torch.int64)
+
+
+def others():
+    """Numbers that take the place of a seed that was freed."""
+    return [fresh_seed(-1) for _ in range(200)]
+
+
+def held_to(grad, table, words, rows, deltas):
+    """The gradient has the rows' mask (no number of the table is 0)."""
+    kept = rows.detach().flatten(0, -2) != 0
+    want = torch.zeros_like(table).index_add_(0, words.flatten().long(), deltas.flatten(0, -2) * kept)
+    assert 0.2 < kept.float().mean() < 0.8
+    assert torch.equal(grad, want)
+
+
+SEED = 0x5a5a33cc0f1e6978
+
+
+def embed_case():
+    g = torch.Generator().manual_seed(2)
+    table = torch.rand(6, 40, generator=g) + 1.0
+    words = torch.randint(0, 6, (5, 7), generator=g).int()
+    deltas = torch.randint(1, 9, (5, 7, 40), generator=g).float()   # (sums that are exact)
+    return table.requires_grad_(True), words, deltas
+
+
+@pytest.mark.parametrize("copied", [False, True])
+def test_seed_that_goes_through_hooks(embedder, copied):
+    """Saved tensors that a hook has copied, as when they are moved to the host: the seed itself is gone by then."""
+    table, words, deltas = embed_case()
+    pack = (lambda x: x.clone()) if copied else (lambda x: x)
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda x: x.clone()):
+        rows = embed_words(table, words, dropout=0.5, seed=fresh_seed(SEED))
+    held = others()
+    grad, = torch.autograd.grad(rows, table, deltas)
+    held_to(grad, table, words, rows, deltas)
+    del held
+
+
+def test_seed_of_a_recomputed_call(embedder):
+    """Checkpointing makes the call again when the gradient is wanted, its seed with it."""
+    from torch.utils.checkpoint import checkpoint
+    table, words, deltas = embed_case()
+    rows = checkpoint(lambda t: embed_words(t, words, dropout=0.5, seed=fresh_seed(SEED)), table, use_reentrant=False)
+    held = others()
+    grad, = torch.autograd.grad(rows, table, deltas)
+    held_to(grad, table, words, rows, deltas)
+    del held
+
+
+def test_seeds_without_hooks(embedder):
+    table, words, deltas = embed_case()
+    for seed in (SEED, fresh_seed(SEED)):
+        rows = embed_words(table, words, dropout=0.5, seed=seed)
+        grad, = torch.autograd.grad(rows, table, deltas)
+        held_to(grad, table, words, rows, deltas)
+    place = fresh_seed(SEED)
+    rows = embed_words(table, words, dropout=0.5, seed=place)
+    place += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(rows, table, deltas)
+
+
+def test_saved_words_that_come_back_elsewhere(embedder):
+    """A hook that leaves them on another device, or not one after the other."""
+    table, words, deltas = embed_case()
+    for unpack, kind, message in [(lambda x: x.to("meta"), ValueError, "same device"),
+                                  (lambda x: x.t().contiguous().t() if x.dim() == 2 else x, None, None)]:
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack):
+            rows = embed_words(table, words, dropout=0.5, seed=fresh_seed(SEED))
+        if kind is None:
+            grad, = torch.autograd.grad(rows, table, deltas)
+            held_to(grad, table, words, rows, deltas)
+        else:
+            with pytest.raises(kind, match=message):
+                torch.autograd.grad(rows, table, deltas)

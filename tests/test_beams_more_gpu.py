@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import test_beams_gpu as base
-from transducer_b200 import reorder_states
+from transducer_b200 import embed_words, reorder_states
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,29 @@ def test_several_states_that_are_copied(shape, given):
     for _ in range(3):   # (the allocator has blocks of this size by then)
         got = reorder_states(states, parents, out=out)
         assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
+# ---- embeddings -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("how", ["host", "hooks", "checkpoint"])
+@pytest.mark.parametrize("shape", [(4, 9), (70, 80)])
+def test_seeds_that_the_call_does_not_keep(how, shape):
+    """Saved tensors moved to the host, copied by hooks, or made again: the gradient has the rows' own mask."""
+    from torch.utils.checkpoint import checkpoint
+    seed = 2 ** 50 + 3
+    table, words, deltas = base.table_and_words(40, 100, shape)
+    table.requires_grad_(True)
+
+    def embed(t):
+        return embed_words(t, words, dropout=0.25, seed=torch.tensor([seed]).cuda())
+    if how == "checkpoint":
+        rows = checkpoint(embed, table, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu() if how == "host" else \
+                torch.autograd.graph.saved_tensors_hooks(lambda x: x.clone(), lambda x: x.clone()):
+            rows = embed(table)
+    others = [torch.tensor([-1]).cuda() for _ in range(200)]   # (in the seed's place)
+    grad, = torch.autograd.grad(rows, table, deltas)
+    here = base.check_rows(rows, table, words, 1.0, 0.25, seed)
+    base.check_grad(grad, 40, words, deltas, here, 1.0, 0.25)
+    del others

@@ -22,14 +22,19 @@ class WordEmbedding(torch.autograd.Function):
         else:
             ctx.save_for_backward(words)
         count, (R, H) = words.numel(), table.shape
-        ctx.rest = (count, R, H, table.dtype is torch.bfloat16, scale, dropout, numbers, place,
+        ctx.rest = (count, R, H, table.dtype is torch.bfloat16, scale, dropout, numbers,
                     _transducer.embed_backward_workspace_bytes(count, R, H))
         return rows
 
     @staticmethod
     def backward(ctx, deltas):
-        words = ctx.saved_tensors[0]   # (refuses words, and a seed on the device, that were written since)
-        count, R, H, bf16, scale, dropout, numbers, place, nbytes = ctx.rest
+        # (refuses words, and a seed on the device, that were written since; hooks may bring them back as other tensors)
+        words, *seed = ctx.saved_tensors
+        count, R, H, bf16, scale, dropout, numbers, nbytes = ctx.rest
+        check_device(deltas, words, *seed)
+        place = seed[0].data_ptr() if seed else 0
+        if not words.is_contiguous():
+            words = words.contiguous()
         if not deltas.is_contiguous():
             deltas = deltas.contiguous()
         with OnDevice(deltas.device):
