@@ -217,3 +217,35 @@ def test_saved_words_that_come_back_elsewhere(embedder):
         else:
             with pytest.raises(kind, match=message):
                 torch.autograd.grad(rows, table, deltas)
+
+
+# ---- tensors that are conjugated or negated when they are read ----------------------------------
+
+def lazy(kind, *shape):
+    z = torch.complex(*torch.randn(2, *shape, generator=torch.Generator().manual_seed(4)))
+    return {"conj": z.conj(), "neg": z.conj().imag, "both": torch.complex(z.imag, z.real).conj()._neg_view(),
+            "column": z.conj().imag[..., 0], "plain": z}[kind]
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("kind", ["conj", "neg", "both", "column", "plain"])
+def test_states_that_are_read_lazily(mover, kind, given):
+    states = [lazy(kind, 2, 3, 5) for _ in range(2)]
+    out = [torch.full((2, 3) + s.shape[2:], 7.0, dtype=s.dtype) for s in states] if given else None
+    want = plain(states, PARENTS, out)
+    got = reorder_states(states, PARENTS, out=out)
+    assert all(torch.equal(a, b) and not a.is_conj() and not a.is_neg() for a, b in zip(got, want))
+
+
+def test_lazy_states_in_place_and_as_outputs(mover):
+    x = lazy("plain", 2, 3, 5)
+    want = plain([x.conj()], PARENTS, [x])[0]
+    got = reorder_states(x.conj(), PARENTS, out=x)   # (the same memory, other numbers)
+    assert got is x and torch.equal(x, want)
+    lazily = lazy("conj", 2, 3, 5)
+    want = plain([lazily], PARENTS, [lazily])[0]
+    assert torch.equal(reorder_states(lazily, PARENTS, out=lazily), want)   # in place
+    with pytest.raises(ValueError, match="lazily"):
+        reorder_states(x, PARENTS, out=torch.zeros_like(x).conj())
+    with pytest.raises(ValueError, match="lazily"):
+        reorder_states(x.real.contiguous(), PARENTS, out=torch.zeros(2, 3, 5)._neg_view())

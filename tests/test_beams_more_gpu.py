@@ -26,6 +26,20 @@ def test_several_states_that_are_copied(shape, given):
         assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
 
 
+def test_states_that_are_read_lazily():
+    """Conjugated or negated when they are read: the numbers are moved, not the bytes."""
+    g = torch.Generator().manual_seed(2)
+    z = torch.complex(*torch.randn(2, 3, 5, 7, generator=g)).cuda()
+    parents = base.some_parents(3, 5, 5, g)
+    states = [z.conj(), z.conj().imag, z.conj().imag[..., 0], z]
+    out = [torch.zeros(s.shape, dtype=s.dtype, device="cuda") for s in states]
+    want = base.plain_reorder(states, parents)
+    for got in reorder_states(states, parents), reorder_states(states, parents, out=out):
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+    want = base.plain_reorder([z.conj()], parents, [z])[0]
+    assert torch.equal(reorder_states(z.conj(), parents, out=z).cpu(), want)
+
+
 # ---- embeddings -------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("how", ["host", "hooks", "checkpoint"])

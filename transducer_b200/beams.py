@@ -64,7 +64,8 @@ def reorder_states(states, parents, out=None, validate_parents=True):
     """What belongs to hypotheses, for those that follow them: ``states[b, parents[b, w]]`` for every w.
 
     ``states``   a tensor [B, N, ...] of any type, or a list or tuple of them (predictor states, words so
-                 far, keys and values); what follows the second dimension has to be contiguous, or is copied
+                 far, keys and values); what follows the second dimension has to be contiguous, and nothing
+                 lazily conjugated or negated, or is copied
     ``parents``  int32 [B, W], as from `extend_beams`: a negative one says that there is no hypothesis
     ``out``      tensors [B, W, ...] to write, else they are made; any of them may be its state itself (or
                  its first W hypotheses), which is then reordered in place (at most 4096 hypotheses).  It
@@ -106,6 +107,9 @@ def reorder_states(states, parents, out=None, validate_parents=True):
         rows, moved = [], []
         copies = []   # (which have to live until the kernels are enqueued: `moved` has addresses)
         for i, s in enumerate(states):
+            if (s.is_conj() or s.is_neg()) and (made or not _alike(s, out[i])):
+                s = s.detach().resolve_conj().resolve_neg()
+                copies.append(s)
             row = _row(s)
             if row is None:
                 s = s.detach().contiguous()
@@ -144,7 +148,14 @@ def _check_outputs(states, out, parents):
             raise ValueError("out must be contiguous behind its second dimension")
         if o.requires_grad:
             raise ValueError("out must not require gradients")
+        if (o.is_conj() or o.is_neg()) and not _alike(s, o):
+            raise ValueError("out must not be lazily conjugated or negated where its state is not")
     check_device(parents, *out)
+
+
+def _alike(s, o):
+    """Whether the same bytes are the same numbers: tensors may be conjugated or negated when they are read."""
+    return s.is_conj() == o.is_conj() and s.is_neg() == o.is_neg()
 
 
 def _row(s):
