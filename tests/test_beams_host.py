@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from transducer_b200 import beams, embed_words, embeddings, reorder_states
+from transducer_b200 import beams, embed_words, embeddings, extend_beams, reorder_states
 
 
 class Anywhere(object):
@@ -118,7 +118,7 @@ class Embedder(object):
 
     def embed_words(self, table, bf16, stride, words, count, rows, R, H, scale, dropout, seed, seed_at, validate):
         words = self._tensor(words, ctypes.c_int, torch.int32, count)
-        table = self._tensor(table, ctypes.c_float, torch.float32, R, H)
+        table = self._tensor(table, ctypes.c_float, torch.float32, (R - 1) * stride + H).as_strided((R, H), (stride, 1))
         self._tensor(rows, ctypes.c_float, torch.float32, count, H).copy_(
             self._masked(table[words.long()], words, seed, seed_at))
         return 0
@@ -249,3 +249,43 @@ def test_lazy_states_in_place_and_as_outputs(mover):
         reorder_states(x, PARENTS, out=torch.zeros_like(x).conj())
     with pytest.raises(ValueError, match="lazily"):
         reorder_states(x.real.contiguous(), PARENTS, out=torch.zeros(2, 3, 5)._neg_view())
+
+
+def negated(*shape):
+    """A negative number throughout, from memory that holds a positive one."""
+    return torch.complex(torch.ones(shape), torch.full(shape, 3.0)).conj().imag
+
+
+@pytest.mark.parametrize("R,H", [(1, 1), (4, 1), (4, 5)])
+def test_embeddings_that_are_read_lazily(embedder, R, H):
+    words = torch.zeros(1, dtype=torch.int32)
+    table = negated(R, H)
+    assert torch.equal(embed_words(table, words), table[:1])
+    table = table.detach().requires_grad_(True)
+    rows = embed_words(table, words)
+    assert torch.equal(rows, table[:1])
+    grad, = torch.autograd.grad(rows, table, negated(1, H))
+    assert torch.equal(grad, torch.cat((negated(1, H), torch.zeros(R - 1, H))))
+
+
+class Extender(object):
+    """Reads what extend_beams hands on of one hypothesis at one node."""
+
+    def extend_beams_workspace_bytes(self, B, V, N):
+        return 0
+
+    def extend_beams(self, described, frames, positions, scores, *rest):
+        e, p = described[:2]
+        self.seen = [ctypes.c_float.from_address(x).value for x in (e, p, scores)]
+        return 0
+
+
+def test_scores_that_are_read_lazily(monkeypatch):
+    extender = Extender()
+    monkeypatch.setattr(beams, "_transducer", extender)
+    monkeypatch.setattr(beams, "OnDevice", Anywhere)
+    node = torch.zeros(1, 1, dtype=torch.int32)
+    extend_beams(negated(1, 1, 1), negated(1, 1, 1), node, node, negated(1, 1), 1)
+    assert extender.seen == [-3.0] * 3
+    extend_beams(negated(1, 1, 6), negated(1, 1, 6), node, node, negated(1, 1), 1)
+    assert extender.seen == [-3.0] * 3
