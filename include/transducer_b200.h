@@ -428,8 +428,8 @@ int tb200_extend_beams(const void* emissions, const void* predictions, int bf16,
  * to + b * toStrideB + w * toStrideN become those at from + b * fromStrideB + n * fromStrideN with
  * n = parents[b,w] (strides in bytes, rows of any alignment).  Where n is not in [0, hypotheses) the row
  * is set to zeros, or left as it is if `kept`.  from == to with equal strides: in place (rows without a
- * parent are left as they are, at most 4096 of them per utterance); else the two must not overlap, nor
- * may the rows that are written. */
+ * parent are left as they are, at most 4096 of them per utterance; no two of the batchSize x hypotheses
+ * rows may overlap); else the two must not overlap, nor may the rows that are written. */
 typedef struct {
   const void* from;
   void* to;

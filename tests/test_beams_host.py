@@ -289,3 +289,47 @@ def test_scores_that_are_read_lazily(monkeypatch):
     assert extender.seen == [-3.0] * 3
     extend_beams(negated(1, 1, 6), negated(1, 1, 6), node, node, negated(1, 1), 1)
     assert extender.seen == [-3.0] * 3
+
+
+# ---- states in place whose other rows are utterances' of their own ------------------------------
+
+def shared_bytes(row, B, N):
+    """Rows that share memory, by looking at each with each."""
+    _, by_b, by_n, size = row
+    at = sorted(b * by_b + n * by_n for b in range(B) for n in range(N))
+    return size > 0 and any(y - x < size for x, y in zip(at, at[1:]))
+
+
+def test_rows_in_place_that_are_another_utterances():
+    """Only the first W hypotheses are written, but all N may be read."""
+    room = torch.zeros(400)
+    refused = accepted = 0
+    for B, N, W in [(2, 4, 2), (3, 4, 1), (2, 3, 3), (4, 7, 2), (1, 5, 2), (2, 2, 4)]:
+        parents = torch.zeros(B, W, dtype=torch.int32)
+        for by_b in range(0, 41):
+            for by_n in (0, 1, 2, 3, 5, 9, 10):
+                for size in (1, 2, 5):
+                    whole = room.as_strided((B, max(N, W), size), (by_b, by_n, 1))
+                    s, out = whole[:, :N], whole[:, :W]
+                    try:
+                        beams._check_apart([beams._row(s)], [out], B, N, W, parents)
+                    except ValueError:
+                        refused += 1
+                        # (nothing is refused for the rows that are only read, unless they do share memory)
+                        try:
+                            beams._check_apart([beams._row(out)], [out], B, W, W, parents)
+                        except ValueError:
+                            continue
+                        assert shared_bytes(beams._row(whole), B, max(N, W))
+                    else:
+                        accepted += 1
+                        assert not shared_bytes(beams._row(whole), B, max(N, W))
+    assert refused > 100 and accepted > 100
+
+
+def test_example_of_such_rows(mover):
+    s = torch.zeros(30).as_strided((2, 4, 5), (10, 5, 1))
+    parents = torch.tensor([[2, 3], [0, 1]], dtype=torch.int32)
+    with pytest.raises(ValueError, match="rows of a state"):
+        reorder_states(s, parents, out=s[:, :2])
+    assert mover.calls == 0

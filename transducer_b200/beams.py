@@ -180,6 +180,21 @@ def _end(row, B, N):
     return row[0] + ((B - 1) * row[1] + (N - 1) * row[2] + row[3] if B * N * row[3] else 0)
 
 
+def _shared(row, B, N):
+    """Whether rows of a tensor of B utterances and N hypotheses share memory."""
+    _, by_b, by_n, size = row
+    if by_b >= by_n * (N - 1) + size and by_n >= size:   # (one utterance behind the other)
+        return False
+    for n in range(N):   # rows n hypotheses and b utterances apart begin b * by_b + n * by_n bytes apart
+        if by_b == 0:
+            least, most = (1 - B, B - 1) if n * by_n < size else (1, 0)
+        else:
+            least, most = max(1 - B, -((size - 1 + n * by_n) // by_b)), min(B - 1, (size - 1 - n * by_n) // by_b)
+        if least <= most and (n > 0 or most > 0):
+            return True
+    return False
+
+
 def _check_apart(rows, out, B, N, W, parents):
     """That outputs overlap with nothing, but for one that is its state itself (the same place for every hypothesis)."""
     taken = [(parents.data_ptr(), parents.data_ptr() + parents.nbytes)]
@@ -201,6 +216,8 @@ def _check_apart(rows, out, B, N, W, parents):
                 raise ValueError("out must be a state itself or not overlap with the states")
             if W > MAX_REORDERED_WIDTH:
                 raise ValueError("at most %d hypotheses are reordered in place" % MAX_REORDERED_WIDTH)
+            if N > W and _shared(row, B, N):
+                raise ValueError("rows of a state that is reordered in place must not be another utterance's")
         for other in taken:
             if begin < other[1] and other[0] < end:
                 raise ValueError("outputs must not overlap with each other or with parents")
