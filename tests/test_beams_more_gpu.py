@@ -64,3 +64,30 @@ def test_seeds_that_the_call_does_not_keep(how, shape):
     here = base.check_rows(rows, table, words, 1.0, 0.25, seed)
     base.check_grad(grad, 40, words, deltas, here, 1.0, 0.25)
     del others
+
+
+def test_as_many_words_as_there_may_be():
+    """2^31 - 2 of them, with numbers whose sums are exact in 32 bits."""
+    N, R = 2 ** 31 - 2, 1000
+    torch.cuda.empty_cache()
+    words = torch.arange(R, dtype=torch.int32, device="cuda").repeat(N // R + 1)[:N]
+    counts = torch.full((R,), N // R, dtype=torch.int64)
+    counts[:N % R] += 1
+    for part, word in ((slice(0, 40), 9), (slice(N - 40, N), 7)):
+        counts -= torch.bincount(words[part].cpu(), minlength=R)
+        counts[word] += 40
+        words[part] = word
+    words[-1] = -1
+    counts[7] -= 1
+    table = torch.randn(R, 1, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_(True)
+    rows = embed_words(table, words)
+    for begin in range(0, N, 2 ** 28):
+        some = words[begin:min(N, begin + 2 ** 28)]
+        want = table.detach()[:, 0].index_select(0, some.clamp(min=0))
+        assert torch.equal(rows.detach()[begin:begin + 2 ** 28, 0], want.mul_(some >= 0))
+        del some, want
+    deltas = torch.ones_like(rows)
+    grad, = torch.autograd.grad(rows, table, deltas)
+    assert torch.equal(grad[:, 0].cpu().double(), counts.double())
+    del rows, deltas, words
+    torch.cuda.empty_cache()

@@ -202,13 +202,13 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
   for (int i = tid; i < WARPS * kSortRows; i += 32 * WARPS) (&count[0][0])[i] = 0;
   if (tid == 0) below = 0;
   __syncthreads();
-  const int seg = (int)round_up64(div_up(N, WARPS), 32);
+  const int seg = (int)round_up64(div_up64(N, WARPS), 32);
   const int first = (int)min((i64)N, (i64)warp * seg), end = (int)min((i64)N, (i64)first + seg);
   // f(word or -1, place of the first) for the warp's words, 32 that follow each other at a time, in order
   auto each = [&](auto f) {
-    int n = first;
+    unsigned n = first, last = end;   // (the step behind the last word may pass 31 bits)
 #pragma unroll 1
-    for (; end - n >= 32 * kBatch; n += 32 * kBatch) {
+    for (; last - n >= 32 * kBatch; n += 32 * kBatch) {
       int r[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) r[j] = words[n + 32 * j + lane];
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
       for (int j = 0; j < kBatch; ++j) f(r[j], n + 32 * j);
     }
 #pragma unroll 4
-    for (; n < end; n += 32) f(lane < end - n ? words[n + lane] : -1, n);
+    for (; n < last; n += 32) f((unsigned)lane < last - n ? words[n + lane] : -1, n);
   };
   const unsigned before = (1u << lane) - 1;
   int lower = 0, found = 0;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
       put((int)(x & 255) << bits | cta, first + (int)(x >> 8), i + lane < found);
     }
   } else {
-    each([&](int r, int n) { put(r, n + lane, (unsigned)r < (unsigned)out.R && (r & low) == cta); });
+    each([&](int r, unsigned n) { put(r, (int)(n + lane), (unsigned)r < (unsigned)out.R && (r & low) == cta); });
   }
 }
 
