@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import test_beams_gpu as base
-from transducer_b200 import embed_words, reorder_states
+from transducer_b200 import TransducerLoss, embed_words, extend_beams, reorder_states, top_words
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,50 @@ def test_as_many_words_as_there_may_be():
     assert torch.equal(grad[:, 0].cpu().double(), counts.double())
     del rows, deltas, words
     torch.cuda.empty_cache()
+
+
+# ---- calls that wait --------------------------------------------------------------------------
+
+def checked_calls():
+    E, P, frames, positions, scores = base.hypotheses(2, 3, 4, 200, 3, done=0.0, gone=0.0)
+    parents = torch.zeros(2, 3, dtype=torch.int32).cuda()
+    labels = torch.ones(2, 3, dtype=torch.int32).cuda()
+    lens = torch.full((2,), 3, dtype=torch.int32).cuda()
+    return {"extend": lambda: extend_beams(E, P, frames, positions, scores, 2),
+            "reorder": lambda: reorder_states(scores, parents),
+            "embed": lambda: embed_words(E[0], parents),
+            "top": lambda: top_words(E, P, frames, positions, 2),
+            "loss": lambda: TransducerLoss(blank=0)(E, P, labels, lens, lens)}
+
+
+@pytest.mark.parametrize("which", ["extend", "reorder", "embed", "top", "loss"])
+def test_other_threads_go_on_while_a_call_waits(which):
+    """The stream is busy for a while; another thread counts meanwhile, which takes the interpreter's lock."""
+    import threading
+    import time
+    call = checked_calls()[which]
+    call()
+    a = torch.randn(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    begins, ends = torch.cuda.Event(), []
+    called, done = threading.Event(), threading.Event()
+
+    def work():
+        b = a
+        for _ in range(60):   # (some 20 ms each)
+            b = a @ b * 1e-3
+        begins.record()
+        called.set()
+        call()
+        ends.append(begins.query())
+        done.set()
+    thread = threading.Thread(target=work)
+    thread.start()
+    called.wait()
+    counted = 0
+    while not done.is_set() and not begins.query():   # (as long as the stream has not come to the call)
+        counted += 1
+        time.sleep(1e-3)
+    thread.join()
+    assert ends == [True]   # (it did wait)
+    assert counted >= 50

@@ -34,6 +34,13 @@ void check(int rc) {
   throw std::runtime_error(tb200_last_error());
 }
 
+// A call that waits for the stream: other threads of the interpreter go on meanwhile (what is waited for may need them).
+template <typename F>
+int waiting(F&& call) {
+  py::gil_scoped_release released;
+  return call();
+}
+
 // Which indices of a checked call are beyond their tensors: bit 0 frames, parents or words, bit 1 positions.
 class Beyond {
  public:
@@ -44,14 +51,14 @@ class Beyond {
   Beyond& operator=(const Beyond&) = delete;
   ~Beyond() {   // (the call has failed; kernels of it may still run)
     int values[2];
-    if (flags_) tb200_flags_wait(flags_, values);
+    if (flags_) waiting([&] { return tb200_flags_wait(flags_, values); });
   }
   int* flags() const { return flags_; }
   int wait() {
     if (!flags_) return 0;
     int values[2], *flags = flags_;
     flags_ = nullptr;
-    check(tb200_flags_wait(flags, values));
+    check(waiting([&] { return tb200_flags_wait(flags, values); }));
     return (values[0] ? 1 : 0) | (values[1] ? 2 : 0);
   }
 
@@ -219,8 +226,10 @@ PYBIND11_MODULE(_transducer, m) {
   m.def("node_summary",
         [](addr frames, addr positions, long long nodes, addr words, long long word_count, addr scratch) {
           int most[3];
-          check(tb200_node_summary(at<const int>(frames), at<const int>(positions), nodes, at<const int>(words),
-                                   word_count, at<void>(scratch), most));
+          check(waiting([&] {
+            return tb200_node_summary(at<const int>(frames), at<const int>(positions), nodes, at<const int>(words),
+                                      word_count, at<void>(scratch), most);
+          }));
           return py::make_tuple(most[0], most[1], most[2]);
         },
         "frames"_a, "positions"_a, "nodes"_a, "words"_a, "word_count"_a, "scratch"_a);
@@ -327,14 +336,16 @@ PYBIND11_MODULE(_transducer, m) {
   // ---- device status (bounded waits that ran out) -----------------------------------
   // Returns the code of tb200_check_status (0, or 5 = a kernel gave up) without throwing, so the
   // Python layer can raise its own exception type; the text is in last_error().
-  m.def("check_status", []() { return tb200_check_status(); });
+  m.def("check_status", []() { return waiting([] { return tb200_check_status(); }); });
   // (code as check_status, longest input length, longest label length), after one synchronisation;
   // the status word is left for check_status to clear
   m.def("call_summary",
         [](addr ilen, addr llen, int B, bool withStatus, addr scratch) {
           int maxLens[2] = {0, 0};
-          const int rc = tb200_call_summary(at<const int>(ilen), at<const int>(llen), B,
-                                            withStatus ? 2 : 0, at<void>(scratch), maxLens);
+          const int rc = waiting([&] {
+            return tb200_call_summary(at<const int>(ilen), at<const int>(llen), B, withStatus ? 2 : 0,
+                                      at<void>(scratch), maxLens);
+          });
           return py::make_tuple(rc, maxLens[0], maxLens[1]);
         },
         "input_lengths"_a, "label_lengths"_a, "batch_size"_a, "with_status"_a, "scratch"_a);
