@@ -1,7 +1,9 @@
 """reorder_states, extend_beams and embed_words on a GPU: calls beside those of test_beams_gpu.py."""
+import numpy as np
 import pytest
 import torch
 
+import beam_reference as ref
 import test_beams_gpu as base
 from transducer_b200 import TransducerLoss, embed_words, extend_beams, reorder_states, top_words
 
@@ -138,3 +140,77 @@ def test_other_threads_go_on_while_a_call_waits(which):
     thread.join()
     assert ends == [True]   # (it did wait)
     assert counted >= 50
+
+
+# ---- ways through the kernels that take many words, rows or numbers -------------------------------
+
+@pytest.mark.parametrize("width", [5, 64, 256])
+@pytest.mark.parametrize("N,V", [(300, 1200), (257, 2049), (700, 40)])
+def test_equal_scores_of_many_hypotheses(N, V, width):
+    """More than are held in shared memory, and more words next to each other than there are lists for."""
+    E, P, frames, positions, scores = base.hypotheses(2, 3, N, V, N, seed=N, done=0.05, gone=0.05)
+    positions[positions >= 0] = torch.arange(N, device="cuda").repeat(2, 1)[positions >= 0].int()
+    flat = torch.where(scores == -base.INF, scores, -5.0)
+    few = torch.randint(0, 3, E.shape, generator=torch.Generator().manual_seed(1)).float().cuda()
+    for e, p, s in ((0 * E, 0 * P, flat), (few, 0 * P, flat), (1e-7 * E, 1e-7 * P, flat), (few, 0 * P, scores),
+                    (E, 1e-7 * P, flat)):
+        base.check_extend([e, p, frames, positions, s], width)
+
+
+@pytest.mark.parametrize("dtype", base.TYPES)
+@pytest.mark.parametrize("R,H,count,skew", [
+    (3, 40, 70001, 20.0),         # most are one word: more of a warp's than are listed
+    (500, 9, 100003, 9.0), (40000, 5, 150000, 30.0),
+    (2000, 24, 100003, 3.0),      # 32 places to a warp
+    (100, 700, 40000, 3.0), (300, 1030, 16000, 1.0)])
+def test_many_words(R, H, count, skew, dtype):
+    base.check_embed(R, H, (count,), dtype, skew=skew, none=0.05)
+    base.check_embed(R, H, (count,), dtype, skew=skew, none=0.0, scale=0.25, dropout=0.1, seed=77)
+
+
+def test_one_word_throughout():
+    count = 80000
+    table, words, deltas = base.table_and_words(4, 16, (count,))
+    words[:] = 2
+    rows = embed_words(table.requires_grad_(True), words)
+    grad, = torch.autograd.grad(rows, table, deltas)
+    base.check_grad(grad, 4, words, deltas, torch.ones(count, 16, dtype=torch.bool), 1.0, 0.0)
+
+
+@pytest.mark.parametrize("dropout", [0.0, 0.5])
+def test_embeddings_beyond_32_bit_offsets(dropout):
+    """More than 2^31 numbers in the table, in the rows and in the gradient."""
+    R = N = 66000
+    H, seed = 32776, 12345
+    g = torch.Generator().manual_seed(8)
+    torch.cuda.empty_cache()
+    table = torch.zeros(R, H, dtype=torch.bfloat16, device="cuda")
+    some = [0, 1, 65535, R - 2, R - 1]
+    table[some] = torch.randn(len(some), H, generator=g).bfloat16().cuda()
+    words = torch.randint(2, 65535, (N,), generator=g).int().cuda()
+    places = [0, 3, 40000, N - 2, N - 1]
+    words[places] = torch.tensor([R - 1, 0, R - 2, 65535, R - 1], dtype=torch.int32).cuda()
+    rows = embed_words(table.requires_grad_(True), words, dropout=dropout, seed=seed)
+    deltas = torch.zeros_like(rows)
+    deltas[places] = torch.randn(len(places), H, generator=g).bfloat16().cuda()
+    grad, = torch.autograd.grad(rows, table, deltas)
+    groups = H // 8
+    counter = np.zeros((len(places), groups, 4), np.uint64)
+    counter[..., 0] = np.array(places)[:, None]
+    counter[..., 2] = np.arange(groups)
+    x = ref.philox(counter, (seed, 0))
+    halves = np.stack((x & np.uint64(0xffff), x >> np.uint64(16)), -1).reshape(len(places), H)
+    stays = torch.from_numpy(halves >= round(dropout * 65536))
+    factor = ref.factor(1.0, dropout)
+    # (factors are powers of 2: products are exact, and a sum of two is rounded in 32 bits and to the type)
+    want = torch.where(stays, table.detach()[words[places].long()].cpu().double() * factor, 0.0)
+    assert torch.equal(rows.detach()[places].cpu().double(), want)
+    d = torch.where(stays, deltas[places].cpu().double() * factor, 0.0)
+    want = torch.stack((d[1], torch.zeros(H, dtype=torch.float64), d[3], d[2], d[0] + d[4]))
+    bound = (base.half_step(torch.bfloat16) + base.UNIT) * 1.01 * want.abs() + base.UNIT * (d[0].abs() + d[4].abs())
+    assert ((grad[some].cpu().double() - want).abs() <= bound).all()
+    rest = torch.ones(R, dtype=torch.bool, device="cuda")
+    rest[some] = False
+    assert all(not grad[begin:begin + 8192][rest[begin:begin + 8192]].any() for begin in range(0, R, 8192))
+    del rows, deltas, grad, table
+    torch.cuda.empty_cache()
