@@ -42,7 +42,9 @@ def extend_beams(emissions, predictions, frames, positions, scores, width, valid
     check_device(emissions, scores)
     if not 1 <= width <= MAX_LISTED_WORDS:
         raise ValueError("width must be between 1 and %d" % MAX_LISTED_WORDS)
-    emissions, predictions, scores = _rows(emissions), _rows(predictions), scores.resolve_neg()
+    emissions, predictions = _rows(emissions), _rows(predictions)
+    if scores.is_neg():
+        scores = scores.resolve_neg()
     B, N = frames.shape
     device = emissions.device
     with OnDevice(device):

@@ -35,7 +35,8 @@ class WordEmbedding(torch.autograd.Function):
         place = seed[0].data_ptr() if seed else 0
         if not words.is_contiguous():
             words = words.contiguous()
-        deltas = deltas.resolve_neg()
+        if deltas.is_neg():
+            deltas = deltas.resolve_neg()
         if not deltas.is_contiguous():
             deltas = deltas.contiguous()
         with OnDevice(deltas.device):
@@ -69,7 +70,8 @@ def _seed(seed):
 
 def _rows_of(table, words, scale, dropout, seed, validate_words):
     """The rows, and the seed as `_seed` has it."""
-    table = table.resolve_neg()   # (as for scores, see nodes.py)
+    if table.is_neg():   # (as for scores, see nodes.py)
+        table = table.resolve_neg()
     if table.stride(1) != 1 and table.shape[1] != 1:
         table = table.contiguous()
     R, H = table.shape

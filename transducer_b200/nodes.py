@@ -116,7 +116,8 @@ def check_temperature(temperature):
 
 def _rows(scores):
     """`scores` with the words of a row next to each other: itself wherever it is so laid out."""
-    scores = scores.resolve_neg()   # (of numbers that are negated when they are read the kernels would see others)
+    if scores.is_neg():   # (of numbers that are negated when they are read the kernels would see others)
+        scores = scores.resolve_neg()
     return scores if scores.stride(2) == 1 or scores.shape[2] == 1 else scores.contiguous()
 
 
