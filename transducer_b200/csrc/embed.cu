@@ -206,9 +206,9 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
   const int first = (int)min((i64)N, (i64)warp * seg), end = (int)min((i64)N, (i64)first + seg);
   // f(word or -1, place of the first) for the warp's words, 32 that follow each other at a time, in order
   auto each = [&](auto f) {
-    unsigned n = first, last = end;   // (the step behind the last word may pass 31 bits)
+    int n = first;
 #pragma unroll 1
-    for (; last - n >= 32 * kBatch; n += 32 * kBatch) {
+    for (; end - n >= 32 * kBatch; n += 32 * kBatch) {
       int r[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) r[j] = words[n + 32 * j + lane];
@@ -216,7 +216,9 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
       for (int j = 0; j < kBatch; ++j) f(r[j], n + 32 * j);
     }
 #pragma unroll 4
-    for (; n < last; n += 32) f((unsigned)lane < last - n ? words[n + lane] : -1, n);
+    for (int left = end - n; left > 0; left -= 32) {   // (n + 32 may pass 31 bits behind the last word)
+      f(lane < left ? words[end - left + lane] : -1, end - left);
+    }
   };
   const unsigned before = (1u << lane) - 1;
   int lower = 0, found = 0;
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(32 * WARPS) sort_words_kernel(const int* __res
       put((int)(x & 255) << bits | cta, first + (int)(x >> 8), i + lane < found);
     }
   } else {
-    each([&](int r, unsigned n) { put(r, (int)(n + lane), (unsigned)r < (unsigned)out.R && (r & low) == cta); });
+    each([&](int r, int n) { put(r, (int)((unsigned)n + lane), (unsigned)r < (unsigned)out.R && (r & low) == cta); });
   }
 }
 
