@@ -415,7 +415,8 @@ int tb200_flags_wait(int* flags, int* values);
  * (1 to 256) greatest are returned in order, of equal ones the lower parent, then the lower word
  * first: outScores, parents, words [B, width]; where there are fewer: -inf, -1, -1.  The order is
  * that of 64-bit arithmetic on z.  An utterance one of whose hypotheses has a score of NaN or +inf, or
- * such a z, gets NaN, -1, -1 throughout.  workspace: 16-byte aligned. */
+ * such a z, gets NaN, -1, -1 throughout.  workspace: 16-byte aligned.  Rows that do not begin and end on 16
+ * bytes are read as the aligned 16-byte vectors that hold them; what else is in the first and the last is not used. */
 size_t tb200_extend_beams_workspace_bytes(int batchSize, int alphabetSize, int nodes);
 int tb200_extend_beams(const void* emissions, const void* predictions, int bf16, long long eStrideB,
                        long long eStrideT, long long pStrideB, long long pStrideU, const int* frames,
@@ -429,7 +430,8 @@ int tb200_extend_beams(const void* emissions, const void* predictions, int bf16,
  * n = parents[b,w] (strides in bytes, rows of any alignment).  Where n is not in [0, hypotheses) the row
  * is set to zeros, or left as it is if `kept`.  from == to with equal strides: in place (rows without a
  * parent are left as they are, at most 4096 of them per utterance; no two of the batchSize x hypotheses
- * rows may overlap); else the two must not overlap, nor may the rows that are written. */
+ * rows may overlap); else the two must not overlap, nor may the rows that are written.  Rows are read as the aligned
+ * vectors of 4 or, in place, 16 bytes that hold them; what else is in the first and the last is not used. */
 typedef struct {
   const void* from;
   void* to;

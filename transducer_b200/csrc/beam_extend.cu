@@ -56,7 +56,9 @@ __device__ __forceinline__ float warp_greatest(float x) {
 // where rows begin anywhere, as the aligned vectors that hold the tile's words.  Bound by HBM; 16 warps an SM without a ring,
 // the next row in registers, took 67 us where this takes 58 (events around 64 x 32 rows of 32000 words), a ring of three rows
 // with fewer warps 62.  fp32 rows of 31999 words take as long as those of 32000, bf16 ones 52 us instead of 32: half a word
-// of shared memory per load.
+// of shared memory per load.  bf16 rows of 32000 words take 46 us a call where their bytes take 18: the scan executes 11.7
+// instructions per 32 words in fp32, by its code no fewer in bf16, 21 us of the issue slots at best.  Of the aligned vectors up to
+// 15 bytes in front of and behind a row are read with it, also where those are another tensor's; they are not used.
 constexpr int kScanStages = 2;
 template <typename TIn, int VEC>
 constexpr int kStageBytes = kTile * (int)sizeof(TIn) + (VEC == 1 ? 16 : 0);
@@ -398,7 +400,7 @@ struct Utterance {
   }
 
   // Its sum in 64 bits, by the CTA.  (Little code: where it is needed it has to be brought first.)  One CTA's loads and sums, 1
-  // word a cycle: 32000 words take 17 us.  Of calls with 64 x 32 hypotheses of N(0, 1.5) scores a sixth needs two rows' (60 ->
+  // word a cycle: 32000 words take 17 us.  Of 240 inputs of 64 x 32 hypotheses of N(0, 1.5) scores a tenth needs two rows' (60 ->
   // 98 us).  Exponentials in two 32-bit terms, and 64 bits only where those are too close as well, took 13 us a row and
   // 97 a call; clusters of four CTAs that share a row 12 us more in every call.
   __device__ __noinline__ double2 exact_row(int n, Group<T>& g) const {
@@ -444,7 +446,8 @@ struct Utterance {
   }
 };
 
-// Where equal scores make the lists too long: all rows' sums in 64 bits, then one way through everything that may be among
+// Where equal scores make the lists too long, as in the first steps of an untrained model: all rows' sums in 64 bits, one after
+// the other by the utterance's CTA (64 x 64 rows of 10000 words: 700 us), then one way through everything that may be among
 // the best, the best W so far in a list that is put in order and cut whenever it is full.  Leaves the list.
 template <typename TIn, int VEC, int T>
 __device__ __noinline__ int general_pick(const Utterance<TIn, VEC, T>& at, int W, unsigned least, float error, Group<T>& g) {

@@ -6,8 +6,9 @@
 // rows that are r's, in an order that follows from the words alone, in fp32: the words' places are sorted by word first,
 // so that no sum needs atomics and the bits are the same from run to run.
 //
-// The bound is HBM without dropout and integer arithmetic with it: eight numbers take 18 products of 32 x 32 bits and 20 logical
-// operations.  256 x 201 words, rows of 1024 bf16 numbers, a table of 32000: rows 22 us without dropout and 38 with it (105 MB
+// The bound is HBM without dropout.  With it no single unit is: of the 138 instructions (163 in the gradient's sums) that a warp
+// executes per 256 numbers the generator needs 38 (18 products of 32 x 32 bits, 20 logical operations); issue slots are 71 % busy, the
+// integer and the product pipe 63 to 64 %.  Rows of words that are none get their bits as well.  256 x 201 words, rows of 1024 bf16 numbers, a table of 32000: rows 22 us without dropout and 38 with it (105 MB
 // written, 30 read: 21 us at the measured copy rate), the gradient's launches 12 + 30 + 4 and 12 + 46 + 4 (170 MB: 26 us).
 #include <algorithm>
 

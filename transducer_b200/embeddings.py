@@ -99,7 +99,8 @@ def embed_words(table, words, scale=1.0, dropout=0.0, seed=None, validate_words=
     Differentiable once w.r.t. the table: the gradient is dense, its sums are made in fp32 in an order that follows
     from the words alone and are the same bits from run to run.  ``validate_words=False`` skips the check that no word is R or
     more (such ones have rows of zeros), which waits for the kernels, so that the call only enqueues work and
-    can be captured in a CUDA graph (its backward pass by torch.autograd.grad).
+    can be captured in a CUDA graph (its backward pass by torch.autograd.grad, when no earlier graph of the
+    table, such as rows of a call before, lives any more: torch would make the capture wait for that one's stream).
 
     Previous words of transcripts, as a prediction network takes them (0: the start symbol)::
 

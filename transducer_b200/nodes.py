@@ -279,7 +279,8 @@ class NodeDistillationLoss(torch.nn.Module):
             for the forward kernels and reads three numbers back).  Pass False for a call that only
             enqueues work and can be captured in a CUDA graph (with its backward pass by
             torch.autograd.grad: `Tensor.backward` adds to a leaf on the stream on which the leaf
-            was first used, which the capture does not see).
+            was first used, which the capture does not see; and when no earlier graph of the same
+            leaves, such as costs of a call before, lives any more).
         reduction (str, optional): "none" (default), "sum" or "mean", the latter over the nodes
             that there are.
     """
